@@ -64,6 +64,18 @@ SIGNATURES = {
                                           _I32P, _P, _I64, _P, _P, _P]),
     "aq_decode_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float,
                                            ctypes.c_float, _P, _P, _P, _I64, _P, _P]),
+    "aq_window_decode_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                                  ctypes.c_float, ctypes.c_float, _P, _P, _I64, _P, _I64, _P, _P]),
+    "aq_window_attention": (ctypes.c_int, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
+                                           ctypes.c_float, _P, _P, _P]),
+    "aq_kv4_store": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64,
+                                    _P]),
+    "aq_kv4_load": (ctypes.c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "aq_kv4_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "aq_kv4_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                        ctypes.c_float, ctypes.c_float, _P, _P, _I64, _P, _I64, _P, _P]),
+    "aq_sample": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_float,
+                                 ctypes.c_int32, ctypes.c_float, ctypes.c_float, _P, _P]),
     "aq_qlinear_decode": (ctypes.c_int, [_P, _I64, _I64, ctypes.c_int, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                          _P, _P, ctypes.c_int,
                                          _P, _P, _P, ctypes.c_float, _P, _P, _P]),
@@ -123,6 +135,14 @@ def ptr(t) -> int | None:
     if t is None or t.numel() == 0:
         return None
     return t.data_ptr()
+
+
+def strided_rows(t):
+    """t, or a copy of it, as kernels read it by strides: the last dimension
+    contiguous, every row on a 16-byte boundary (2-byte elements)."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -160,6 +160,17 @@ inline Split split_of(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t L) {
 __host__ __device__ constexpr int numerators(int G, int D) { return D == 64 ? G * 32 : 0; }
 inline size_t attention_lds(int G, int D, int64_t nw) { return (size_t)nw * (numerators(G, D) + G * D + 2 * G) * 4; }
 
+// How positions map to slots: one position for all sequences (pos_stride 0) or
+// one each (1); positions run up to max_pos; sinks < 0: position = slot.
+struct Ring {
+  int pos_stride, sinks;
+  int64_t max_pos;
+};
+
+__device__ __forceinline__ int64_t ring_slot(int64_t pos, int L, int sinks) {
+  return pos < L ? pos : sinks + (int64_t)((uint32_t)(pos - sinks) % (uint32_t)(L - sinks));
+}
+
 // Workgroup (j, b, z) takes key/value head j of batch row b (query heads
 // j G .. j G + G - 1) and cache positions z span .. z span + span - 1
 // (span = 64 nt); q [B, H, D], k_new / v_new [B, Hkv, D], k_cache and
@@ -187,7 +198,15 @@ inline size_t attention_lds(int G, int D, int64_t nw) { return (size_t)nw * (num
 // 4 queries, 131 MB) take 30.0 us and one of 700 11.5; a wave per 64 positions,
 // a key row per lane and no loads ahead took 39.8 and 13.3.
 // Position pos's key and value come from k_new / v_new (the cache's copy is
-// this kernel's own store); positions past pos read as zero and weigh zero.  Before use the queries are multiplied by q_scale (rounded to fp16;
+// this kernel's own store); positions past pos read as zero and weigh zero.
+// RING: the position is the sequence's own (pos_p[b pos_stride]); one past a
+// cache with sinks >= 0 takes slot sinks + (pos - sinks) mod (L - sinks), so
+// that the slots hold the first `sinks` positions and the last L - sinks.  What
+// the slot held is read with the rest and replaced in registers.  Softmax does
+// not ask for an order and cached keys are rotated.  Its scores stay in f32
+// (rounded to fp16 as the plain step's are, they were three quarters of its
+// error: 8.3e-4 of the result, 2.1e-4 without).
+// Before use the queries are multiplied by q_scale (rounded to fp16;
 // skipped for 1) and, given rcos / rsin (fp16 [L, D] tables), the queries
 // and the new key are rotated at position pos in the rotate-half form:
 // x' = fp16(fp16(x c) + fp16(r s)), r = (-x[D/2:], x[:D/2]) -- the order
@@ -203,12 +222,12 @@ inline size_t attention_lds(int G, int D, int64_t nw) { return (size_t)nw * (num
 // span's XCD; the kernel boundary orders the slots for free.)
 // (Registers: up to 128, four waves a SIMD, for G <= 2; one more and 1024
 // workgroups, G = 2, D = 64, come in two rounds.)
-template <int D, int G>
+template <int D, int G, bool RING>
 __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new,
     uint16_t* __restrict__ k_cache, uint16_t* __restrict__ v_cache, const int64_t* __restrict__ pos_p, int H, int Hkv,
     int L, float scale, float q_scale, const uint16_t* __restrict__ rcos, const uint16_t* __restrict__ rsin, int nt,
-    int ns, float* __restrict__ part, uint16_t* __restrict__ out) {
+    int ns, float* __restrict__ part, uint16_t* __restrict__ out, Ring ring) {
   constexpr int KV = D / 8;     // 16-byte chunks of a row
   constexpr int RPW = 64 / KV;  // rows one wave-wide load covers
   constexpr int NS = 4;         // loads of keys, and of values, a step
@@ -218,11 +237,15 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
   const int j = blockIdx.x, b = blockIdx.y, z = blockIdx.z, t = threadIdx.x;
   const int nw = blockDim.x >> 6, ln = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int64_t pos = *pos_p;
-  if (pos < 0 || pos >= L) return;  // the caller guards this; no access outside the cache
+  const int64_t pos = pos_p[RING ? b * ring.pos_stride : 0];
+  if (pos < 0 || pos >= (RING ? ring.max_pos : L)) return;  // the caller guards this; no access outside the cache
+  // the slot that pos takes, the last slot in use, the slots read from the cache
+  const int64_t slot = RING ? ring_slot(pos, L, ring.sinks) : pos;
+  const int64_t last_slot = RING ? min(pos, (int64_t)L - 1) : pos;
+  const int64_t filled = RING ? min(pos, (int64_t)L) : pos;
   const int64_t span = (int64_t)kChunk * nt, z0 = (int64_t)z * span;
-  if (z0 > pos) return;  // no cached position in this span yet
-  const int nact = (int)(pos / span) + 1;
+  if (z0 > last_slot) return;  // no cached position in this span yet
+  const int nact = (int)(last_slot / span) + 1;
   const int64_t kv = (int64_t)b * Hkv + j;
   uint16_t* Kc = k_cache + kv * L * D;
   uint16_t* Vc = v_cache + kv * L * D;
@@ -235,7 +258,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
   // the span's rows below pos: the rest read as zero without touching memory,
   // so no load has a condition, and waiting for one step's rows leaves the
   // next step's in flight
-  const int bytes = (int)((min(pos, z0 + span) - z0) * D * 2);
+  const int bytes = (int)((min(filled, z0 + span) - z0) * D * 2);
   const __amdgpu_buffer_rsrc_t kbuf = __builtin_amdgcn_make_buffer_rsrc(Kc + z0 * D, (short)0, bytes, 0x00020000);
   const __amdgpu_buffer_rsrc_t vbuf = __builtin_amdgcn_make_buffer_rsrc(Vc + z0 * D, (short)0, bytes, 0x00020000);
   struct Rows {
@@ -270,7 +293,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
     if (cs) v = rope_h(v, scale_h(bits_to_h(qb[i - d + (d + D / 2) % D]), q_scale), d < D / 2, cs[d], sn[d]);
     reinterpret_cast<uint16_t*>(&qs[0][0])[i] = h_to_bits(v);
   }
-  const bool last = z == nact - 1;  // the span holding pos
+  const bool last = RING ? slot >= z0 && slot < z0 + span : z == nact - 1;  // the span holding pos's slot
   if (last) {
     const uint16_t* kb = k_new + kv * D;
     for (int d = t; d < D; d += 64 * nw) {
@@ -281,8 +304,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
   }
   __syncthreads();
   if (last && t < KV) {
-    reinterpret_cast<uint4*>(Kc + pos * D)[t] = krot[t];
-    reinterpret_cast<uint4*>(Vc + pos * D)[t] = vn[t];
+    reinterpret_cast<uint4*>(Kc + slot * D)[t] = krot[t];
+    reinterpret_cast<uint4*>(Vc + slot * D)[t] = vn[t];
   }
 
   uint4 qv[G];  // this lane's chunk of the queries
@@ -300,11 +323,11 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
   const int nrow = ch >> (KV == 16 ? 2 : 1);  // the row (of four per rs) whose score this lane holds
   const bool first = (ch & (KV == 16 ? 3 : 1)) == 0;  // one of the lanes holding it
   auto step = [&](Rows& r, int64_t t0) {
-    const bool valid = t0 + RPW * nrow + rs <= pos;
+    const bool valid = t0 + RPW * nrow + rs <= last_slot;
     if (last) {  // position pos: its key as cached and its value
 #pragma unroll
       for (int n = 0; n < NS; n++)
-        if (t0 + RPW * n + rs == pos) {
+        if (t0 + RPW * n + rs == slot) {
           r.k[n] = krot[ch];
           r.v[n] = vn[ch];
         }
@@ -317,7 +340,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
 #pragma unroll
       for (int n = 0; n < NS; n++) v[n] = dot8(r.k[n], qv[g], 0.0f);
       const float dot = reduce4<KV>(v, ln);  // every lane takes part, whether its own row is valid or not
-      const float sg = valid ? (float)rn_h(dot) * scale : -INFINITY;
+      const float sg = valid ? (RING ? dot : (float)rn_h(dot)) * scale : -INFINITY;
       mn[g] = fmaxf(m[g], max4<KV>(sg));  // the same in every lane of a row group
       grows = grows || mn[g] != m[g];
       // a score of -inf (an fp16 overflow) weighs nothing, also while its row
@@ -363,18 +386,18 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
       asm volatile("" ::: "memory");
     }
   };
-  for (int i = wave; i < nsteps && t0 <= pos; i += 2 * nw) {
+  for (int i = wave; i < nsteps && t0 <= last_slot; i += 2 * nw) {
     load(rb, t0 + hop);
     __builtin_amdgcn_sched_barrier(0);
     step(ra, t0);
     load(ra, t0 + 2 * hop);
     __builtin_amdgcn_sched_barrier(0);
-    if (i + nw < nsteps && t0 + hop <= pos) step(rb, t0 + hop);
+    if (i + nw < nsteps && t0 + hop <= last_slot) step(rb, t0 + hop);
     t0 += 2 * hop;
   }
 
   // waves whose first step lies past pos have nothing to add
-  const int na = (int)min((int64_t)nw, (pos - z0) / PS + 1);
+  const int na = (int)min((int64_t)nw, (last_slot - z0) / PS + 1);
   if (wave < na) {
     // the wave's sums: the row groups' maxima meet, then the lanes' denominators
     // and the RPW row groups' outputs
@@ -452,14 +475,14 @@ __global__ __launch_bounds__(64 * kMaxWaves, G <= 2 ? 4 : 2) void decode_attenti
 template <int D, int G>
 __global__ __launch_bounds__(256) void decode_combine_kernel(const int64_t* __restrict__ pos_p, int H, int Hkv, int L,
                                                              int nt, int ns, const float* __restrict__ part,
-                                                             uint16_t* __restrict__ out) {
+                                                             uint16_t* __restrict__ out, Ring ring) {
   constexpr int PF = G * D + 2 * G;
   constexpr int NG = 256 / D;
   const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
   const int j = h / G, g = h % G;
-  const int64_t pos = *pos_p;
-  if (pos < 0 || pos >= L) return;
-  const int nact = (int)(pos / ((int64_t)kChunk * nt)) + 1;
+  const int64_t pos = pos_p[b * ring.pos_stride];
+  if (pos < 0 || pos >= ring.max_pos) return;
+  const int nact = (int)(min(pos, (int64_t)L - 1) / ((int64_t)kChunk * nt)) + 1;
   if (nact == 1) return;
   const float* pk = part + ((int64_t)b * Hkv + j) * ns * PF;
   const int grp = t / D, d = t % D;
@@ -511,39 +534,47 @@ extern "C" int64_t aq_decode_attention_workspace(int64_t B, int64_t H, int64_t H
   return split_of(B, Hkv, H / Hkv, D, L).bytes;
 }
 
-extern "C" int aq_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
-                                   const int64_t* pos, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t L,
-                                   float scale, float q_scale, const void* rope_cos, const void* rope_sin,
-                                   void* workspace, int64_t ws_bytes, void* out, void* stream) {
-  AQ_CHECK_ARG(q && k_new && v_new && k_cache && v_cache && pos && out && workspace,
-               "aq_decode_attention: null pointer");
-  AQ_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr),
-               "aq_decode_attention: rope_cos and rope_sin come together");
+namespace {
+
+int check_decode(const char* what, const void* q, const void* k_new, const void* v_new, const void* k_cache,
+                 const void* v_cache, const int64_t* pos, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t L,
+                 const void* rope_cos, const void* rope_sin, const void* workspace, int64_t ws_bytes, const void* out) {
+  AQ_CHECK_ARG(q && k_new && v_new && k_cache && v_cache && pos && out && workspace, "%s: null pointer", what);
+  AQ_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr), "%s: rope_cos and rope_sin come together", what);
   AQ_CHECK_ARG(B > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 &&
                    (H / Hkv == 1 || H / Hkv == 2 || H / Hkv == 4 || H / Hkv == 8),
-               "aq_decode_attention: H (%lld) must be 1, 2, 4 or 8 times Hkv (%lld)", (long long)H, (long long)Hkv);
-  AQ_CHECK_ARG(D == 64 || D == 128, "aq_decode_attention: head dim %lld (64 or 128 supported)", (long long)D);
+               "%s: H (%lld) must be 1, 2, 4 or 8 times Hkv (%lld)", what, (long long)H, (long long)Hkv);
+  AQ_CHECK_ARG(D == 64 || D == 128, "%s: head dim %lld (64 or 128 supported)", what, (long long)D);
   AQ_CHECK_ARG((uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0 && (uintptr_t)k_new % 16 == 0 &&
                    (uintptr_t)v_new % 16 == 0 && (uintptr_t)workspace % 16 == 0,
-               "aq_decode_attention: k_new, v_new, the caches and the workspace must be 16-byte aligned");
-  AQ_CHECK_ARG(L > 0 && L <= (1 << 24) && B <= 65535 && Hkv <= 65535, "aq_decode_attention: sizes out of range");
+               "%s: k_new, v_new, the caches and the workspace must be 16-byte aligned", what);
+  AQ_CHECK_ARG(L > 0 && L <= (1 << 24) && B <= 65535 && Hkv <= 65535, "%s: sizes out of range", what);
+  const int64_t need = split_of(B, Hkv, H / Hkv, D, L).bytes;
+  AQ_CHECK_ARG(ws_bytes >= need, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes,
+               (long long)need);
+  return AQ_OK;
+}
+
+template <bool RING>
+void launch_decode(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                   const int64_t* pos, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t L, float scale,
+                   float q_scale, const void* rope_cos, const void* rope_sin, void* workspace, void* out, Ring ring,
+                   void* stream) {
   const Split sp = split_of(B, Hkv, H / Hkv, D, L);
-  AQ_CHECK_ARG(ws_bytes >= sp.bytes, "aq_decode_attention: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
-               (long long)sp.bytes);
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)Hkv, (unsigned)B, (unsigned)sp.ns);  // spans past pos exit at once
   const int G = (int)(H / Hkv);
   float* part = (float*)workspace;
 #define AQ_DECODE_LAUNCH(DD, GG)                                                                                     \
   do {                                                                                                               \
-    hipLaunchKernelGGL((decode_attention_kernel<DD, GG>), grid, dim3(64 * (unsigned)sp.nw),                       \
+    hipLaunchKernelGGL((decode_attention_kernel<DD, GG, RING>), grid, dim3(64 * (unsigned)sp.nw),                    \
                        attention_lds(GG, DD, sp.nw), s, (const uint16_t*)q,                                          \
                        (const uint16_t*)k_new, (const uint16_t*)v_new, (uint16_t*)k_cache, (uint16_t*)v_cache, pos, \
                        (int)H, (int)Hkv, (int)L, scale, q_scale, (const uint16_t*)rope_cos,                        \
-                       (const uint16_t*)rope_sin, (int)sp.nt, (int)sp.ns, part, (uint16_t*)out);                    \
+                       (const uint16_t*)rope_sin, (int)sp.nt, (int)sp.ns, part, (uint16_t*)out, ring);              \
     if (sp.ns > 1)                                                                                                   \
       hipLaunchKernelGGL((decode_combine_kernel<DD, GG>), dim3((unsigned)H, (unsigned)B), dim3(256), 0, s, pos,     \
-                         (int)H, (int)Hkv, (int)L, (int)sp.nt, (int)sp.ns, part, (uint16_t*)out);                  \
+                         (int)H, (int)Hkv, (int)L, (int)sp.nt, (int)sp.ns, part, (uint16_t*)out, ring);             \
   } while (0)
   if (D == 64) {
     if (G == 1) AQ_DECODE_LAUNCH(64, 1);
@@ -557,7 +588,41 @@ extern "C" int aq_decode_attention(const void* q, const void* k_new, const void*
     else AQ_DECODE_LAUNCH(128, 8);
   }
 #undef AQ_DECODE_LAUNCH
+}
+
+}  // namespace
+
+extern "C" int aq_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                                   const int64_t* pos, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t L,
+                                   float scale, float q_scale, const void* rope_cos, const void* rope_sin,
+                                   void* workspace, int64_t ws_bytes, void* out, void* stream) {
+  if (const int rc = check_decode("aq_decode_attention", q, k_new, v_new, k_cache, v_cache, pos, B, H, Hkv, D, L,
+                                  rope_cos, rope_sin, workspace, ws_bytes, out))
+    return rc;
+  launch_decode<false>(q, k_new, v_new, k_cache, v_cache, pos, B, H, Hkv, D, L, scale, q_scale, rope_cos, rope_sin,
+                       workspace, out, Ring{0, -1, L}, stream);
   AQ_LAUNCH_CHECK("aq_decode_attention");
+  return AQ_OK;
+}
+
+extern "C" int aq_window_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_cache,
+                                          void* v_cache, const int64_t* pos, int64_t pos_stride, int64_t B, int64_t H,
+                                          int64_t Hkv, int64_t D, int64_t L, int64_t sinks, float scale, float q_scale,
+                                          const void* rope_cos, const void* rope_sin, int64_t rope_rows,
+                                          void* workspace, int64_t ws_bytes, void* out, void* stream) {
+  if (const int rc = check_decode("aq_window_decode_attention", q, k_new, v_new, k_cache, v_cache, pos, B, H, Hkv, D,
+                                  L, rope_cos, rope_sin, workspace, ws_bytes, out))
+    return rc;
+  AQ_CHECK_ARG(pos_stride == 0 || pos_stride == 1, "aq_window_decode_attention: pos_stride %lld (0 or 1)",
+               (long long)pos_stride);
+  AQ_CHECK_ARG(sinks >= -1 && sinks < L, "aq_window_decode_attention: %lld sinks in %lld slots", (long long)sinks,
+               (long long)L);
+  AQ_CHECK_ARG(!rope_cos || rope_rows > 0, "aq_window_decode_attention: %lld rows of rope_cos", (long long)rope_rows);
+  int64_t max_pos = sinks < 0 ? L : INT32_MAX;
+  if (rope_cos) max_pos = std::min(max_pos, rope_rows);
+  launch_decode<true>(q, k_new, v_new, k_cache, v_cache, pos, B, H, Hkv, D, L, scale, q_scale, rope_cos, rope_sin,
+                      workspace, out, Ring{(int)pos_stride, (int)sinks, max_pos}, stream);
+  AQ_LAUNCH_CHECK("aq_window_decode_attention");
   return AQ_OK;
 }
 

@@ -1,0 +1,675 @@
+// aq_kv4.hip -- a key/value cache held in 4 bits: rows written (a prompt, or
+// the step's own row inside the attention), read back, and attended to by a
+// decode step.
+//
+// A row of D elements is cut into groups of 32; a group has its minimum m and
+// a scale s = fp16((max - m) / 15), an element x the code
+// c = min(rint((x - m) / s), 15) and the value s c + m: 5 bits an element, 5/16
+// of an fp16 cache's bytes, which is what bounds a decode step at long
+// contexts.  s is taken one step less where m + 15 s would round past the
+// largest fp16 number; a group with an infinity or NaN reads as NaN.
+//
+// Layout (c = slots rounded up to 32):
+//   k_codes  [B, Hkv, c, D / 2]         element d in nibble d % 8 of word d / 8
+//   k_params [B, Hkv, c, D / 32, 2]     (s, m) fp16
+//   v_codes  [B, Hkv, c / 32, 16 D]     per block of 32 slots the words [D / 64]
+//            [r: 4][l: 16][e: 4], slot 16 t + 4 r + i of element 64 a + 16 e + l
+//            in nibble 4 t + i of word (a, r, l, e)
+//   v_params [B, Hkv, c / 32, D / 32, r: 4, i: 4, 4]   (s of t = 0, 1, m of t = 0, 1)
+// so that both products of the attention find their operands where a lane of
+// the 16 x 16 x 32 matrix instruction needs them: a lane has a piece of one key
+// row (the contraction runs over its elements) and, of the values, eight slots
+// of one element (the contraction runs over slots).
+#include "aq_common.h"
+
+namespace {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr int kSlotBlock = 32;
+constexpr uint16_t kNaN16 = 0x7E00;
+
+struct Cache4 {
+  uint8_t* kc;
+  uint16_t* kp;
+  uint8_t* vc;
+  uint16_t* vp;
+};
+
+// Slot of position p: p itself while the cache has room; then, with sinks, the
+// slots behind the first `sinks` are used over and over.
+__device__ __forceinline__ int slot_of(int64_t p, int slots, int sinks) {
+  if (p < slots) return (int)p;
+  return sinks + (int)((uint32_t)(p - sinks) % (uint32_t)(slots - sinks));
+}
+
+// Offset (in fp16) of a block's parameters of (group, r, i).
+__device__ __forceinline__ int v_param(int g, int r, int i) { return ((g * 4 + r) * 4 + i) * 4; }
+
+// Eight consecutive elements of a group of 32 in four neighbouring lanes:
+// the group's (s, m) as fp16 bits, and the lane's codes as eight nibbles.
+__device__ __forceinline__ uint32_t quantize8(const uint16_t (&h)[8], uint16_t* s_bits, uint16_t* m_bits) {
+  float x[8], lo = INFINITY, hi = -INFINITY, bad = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    x[i] = (float)bits_to_h(h[i]);
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    if ((h[i] & 0x7C00) == 0x7C00) bad = 1.0f;
+  }
+  lo = -xlane_level_max_f32<2>(xlane_level_max_f32<1>(-lo));
+  hi = xlane_level_max_f32<2>(xlane_level_max_f32<1>(hi));
+  bad = xlane_level_max_f32<2>(xlane_level_max_f32<1>(bad));
+  f16 s16 = rn_h((hi - lo) / 15.0f);
+  if (lo + 15.0f * (float)s16 >= 65520.0f) s16 = bits_to_h(h_to_bits(s16) - 1);
+  const float s = (float)s16;
+  // a / s as IEEE division gives it: one correction of a * RN(1 / s) (s has 11
+  // significant bits, so RN(1 / s) is never the exception of that theorem)
+  const float r = s > 0.0f ? 1.0f / s : 0.0f;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const float a = x[i] - lo, q0 = a * r;
+    const float q = fmaf(fmaf(-q0, s, a), r, q0);
+    w |= (uint32_t)fminf(rintf(q), 15.0f) << (4 * i);
+  }
+  *s_bits = bad != 0.0f ? kNaN16 : h_to_bits(s16);
+  *m_bits = bad != 0.0f ? kNaN16 : h_to_bits(rn_h(lo));
+  return bad != 0.0f ? 0 : w;
+}
+
+// ---------------------------------------------------------------- a prompt
+
+// One workgroup per block of 32 slots of a sequence's head, 256 threads: 8
+// elements a thread and step, keys first.  A slot takes the newest of the
+// given positions that belongs to it; slots without one keep what they hold.
+// The codes of the values are turned in LDS.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_store_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
+                                                        int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
+                                                        int64_t vss, int S, int64_t start,
+                                                        const int64_t* __restrict__ lengths, Cache4 c, int Hkv,
+                                                        int slots, int sinks, int first_block) {
+  constexpr int TPR = D / 8;        // threads a row
+  constexpr int RPS = 256 / TPR;    // rows a step
+  const int t = threadIdx.x, j = blockIdx.y, b = blockIdx.z;
+  const int blk = first_block + blockIdx.x, nblk = (slots + kSlotBlock - 1) / kSlotBlock;
+  const int64_t len = lengths ? lengths[b] : S;
+  const int64_t end = start + max((int64_t)0, min(len, (int64_t)S));  // positions [start, end)
+  // the position (relative to start) that a slot takes, or -1
+  auto source = [&](int slot) -> int64_t {
+    if (slot >= slots || slot >= end) return -1;
+    int64_t p = slot;
+    if (sinks >= 0 && slot >= sinks) {
+      const uint32_t W = slots - sinks;
+      p += (int64_t)((uint32_t)(end - 1 - slot) / W) * W;
+    }
+    return p >= start ? p - start : -1;
+  };
+  __shared__ uint8_t codes[kSlotBlock][D];
+  __shared__ uint8_t has[kSlotBlock];
+  const int64_t head = (int64_t)b * Hkv + j;
+  uint8_t* kc = c.kc + (head * nblk + blk) * (kSlotBlock * D / 2);
+  uint16_t* kp = c.kp + (head * nblk + blk) * (kSlotBlock * (D / 32) * 2);
+  uint8_t* vc = c.vc + (head * nblk + blk) * (16 * D);
+  uint16_t* vp = c.vp + (head * nblk + blk) * ((D / 32) * 64);
+  const uint16_t* kb = k + b * ksb + j * ksh;
+  const uint16_t* vb = v + b * vsb + j * vsh;
+  const int d = t % TPR * 8;
+#pragma unroll
+  for (int n = 0; n < kSlotBlock / RPS; n++) {
+    const int r = n * RPS + t / TPR;
+    const int64_t p = source(blk * kSlotBlock + r);
+    uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+    if (p >= 0) {
+      kx = *reinterpret_cast<const uint4*>(kb + p * kss + d);
+      vx = *reinterpret_cast<const uint4*>(vb + p * vss + d);
+    }
+    uint16_t sb, mb;
+    uint32_t w = quantize8(reinterpret_cast<const uint16_t(&)[8]>(kx), &sb, &mb);
+    if (p >= 0) {
+      *reinterpret_cast<uint32_t*>(kc + r * (D / 2) + d / 2) = w;
+      if ((t & 3) == 0)
+        *reinterpret_cast<uint32_t*>(kp + (r * (D / 32) + d / 32) * 2) = (uint32_t)sb | (uint32_t)mb << 16;
+    }
+    w = quantize8(reinterpret_cast<const uint16_t(&)[8]>(vx), &sb, &mb);
+    if (p >= 0 && (t & 3) == 0) {
+      uint16_t* q = vp + v_param(d / 32, (r & 15) >> 2, r & 3) + (r >> 4);
+      q[0] = sb;
+      q[2] = mb;
+    }
+    uint2 by;  // a code a byte
+    by.x = (w & 0xF) | (w & 0xF0) << 4 | (w & 0xF00) << 8 | (w & 0xF000) << 12;
+    w >>= 16;
+    by.y = (w & 0xF) | (w & 0xF0) << 4 | (w & 0xF00) << 8 | (w & 0xF000) << 12;
+    *reinterpret_cast<uint2*>(&codes[r][d]) = by;
+    if (t % TPR == 0) has[r] = p >= 0;
+  }
+  __syncthreads();
+  for (int i = t; i < 4 * D; i += 256) {
+    // word i of the block: (a, r, l, e)
+    const int e = i & 3, l = (i >> 2) & 15, r = (i >> 6) & 3, a = i >> 8;
+    const int el = a * 64 + e * 16 + l;
+    uint32_t w = 0, mask = 0;
+#pragma unroll
+    for (int n = 0; n < 8; n++) {
+      const int slot = 16 * (n >> 2) + 4 * r + (n & 3);
+      if (has[slot]) {
+        w |= (uint32_t)codes[slot][el] << (4 * n);
+        mask |= 0xFu << (4 * n);
+      }
+    }
+    uint32_t* q = reinterpret_cast<uint32_t*>(vc) + i;
+    if (mask == 0xFFFFFFFFu)
+      *q = w;
+    else if (mask)
+      *q = (*q & ~mask) | w;
+  }
+}
+
+// Slots [0, count) back in fp16: fp16(s c + m), the product exact in f32.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_load_kernel(Cache4 c, int slots, int count, uint16_t* __restrict__ k,
+                                                       uint16_t* __restrict__ v) {
+  constexpr int TPR = D / 8, RPS = 256 / TPR;
+  const int t = threadIdx.x, blk = blockIdx.x, nblk = (slots + kSlotBlock - 1) / kSlotBlock;
+  const int64_t head = blockIdx.y;
+  const uint8_t* kc = c.kc + (head * nblk + blk) * (kSlotBlock * D / 2);
+  const uint16_t* kp = c.kp + (head * nblk + blk) * (kSlotBlock * (D / 32) * 2);
+  const uint8_t* vc = c.vc + (head * nblk + blk) * (16 * D);
+  const uint16_t* vp = c.vp + (head * nblk + blk) * ((D / 32) * 64);
+  __shared__ uint8_t codes[kSlotBlock][D];
+  for (int i = t; i < 4 * D; i += 256) {
+    const int e = i & 3, l = (i >> 2) & 15, r = (i >> 6) & 3, a = i >> 8;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(vc)[i];
+#pragma unroll
+    for (int n = 0; n < 8; n++) codes[16 * (n >> 2) + 4 * r + (n & 3)][a * 64 + e * 16 + l] = (w >> (4 * n)) & 15;
+  }
+  __syncthreads();
+  const int d = t % TPR * 8;
+#pragma unroll
+  for (int n = 0; n < kSlotBlock / RPS; n++) {
+    const int r = n * RPS + t / TPR;
+    const int64_t slot = (int64_t)blk * kSlotBlock + r;
+    if (slot >= count) continue;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(kc + r * (D / 2) + d / 2);
+    const uint16_t* q = kp + (r * (D / 32) + d / 32) * 2;
+    float s = (float)bits_to_h(q[0]), m = (float)bits_to_h(q[1]);
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      o[i] = (uint32_t)h_to_bits(rn_h(s * (float)((w >> (8 * i)) & 15) + m)) |
+             (uint32_t)h_to_bits(rn_h(s * (float)((w >> (8 * i + 4)) & 15) + m)) << 16;
+    *reinterpret_cast<uint4*>(k + (head * count + slot) * D + d) = make_uint4(o[0], o[1], o[2], o[3]);
+    q = vp + v_param(d / 32, (r & 15) >> 2, r & 3) + (r >> 4);
+    s = (float)bits_to_h(q[0]);
+    m = (float)bits_to_h(q[2]);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      o[i] = (uint32_t)h_to_bits(rn_h(s * (float)codes[r][d + 2 * i] + m)) |
+             (uint32_t)h_to_bits(rn_h(s * (float)codes[r][d + 2 * i + 1] + m)) << 16;
+    *reinterpret_cast<uint4*>(v + (head * count + slot) * D + d) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ---------------------------------------------------------------- a decode step
+
+constexpr int kMaxWaves4 = 4;
+constexpr int64_t kMaxSpans4 = 64;
+constexpr int kHeads = 16;  // query heads a workgroup takes: a tile's columns
+
+struct Split4 {
+  int64_t nt, ns, nw, hb, part_floats, bytes;  // blocks a span, spans, waves, head tiles
+};
+
+inline Split4 split4_of(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t slots) {
+  Split4 sp;
+  const int64_t blocks = (slots + kSlotBlock - 1) / kSlotBlock;
+  sp.hb = (G + kHeads - 1) / kHeads;
+  sp.nt = 4;
+  auto spans = [&](int64_t nt) { return (blocks + nt - 1) / nt; };
+  while (sp.nt < blocks && (spans(sp.nt) > kMaxSpans4 || B * Hkv * sp.hb * spans(sp.nt) > 1024)) sp.nt *= 2;
+  sp.ns = spans(sp.nt);
+  sp.nw = std::min<int64_t>(kMaxWaves4, blocks);
+  sp.part_floats = kHeads * D + 2 * kHeads;
+  sp.bytes = sp.ns > 1 ? B * Hkv * sp.hb * sp.ns * sp.part_floats * 4 : 0;
+  return sp;
+}
+
+__device__ __forceinline__ f16 turned(f16 x, f16 partner, bool lo, uint16_t c, uint16_t s) {
+  const float r = lo ? -(float)partner : (float)partner;
+  const f16 a = rn_h((float)x * (float)bits_to_h(c));
+  const f16 b2 = rn_h(r * (float)bits_to_h(s));
+  return rn_h((float)a + (float)b2);
+}
+
+// Nibbles n and n + 4 of a word, n = 0 .. 3, as a pair of fp16 numbers 0 .. 15:
+// under the exponent of 1024 a nibble in the lowest bits counts 1 each, one
+// four bits up 16 each; taking the 1024 away again is exact.
+__device__ __forceinline__ half2v pair_of(uint32_t w, int n) {
+  const half2v big = {(f16)1024.0f, (f16)1024.0f}, sixteenth = {(f16)0.0625f, (f16)0.0625f}, off = {(f16)-64.0f, (f16)-64.0f};
+  if (n & 2) w >>= 8;
+  if (n & 1) return __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x64006400u), sixteenth, off);
+  return __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) - big;
+}
+
+__device__ __forceinline__ uint32_t splat_lo(uint32_t x) { return (x & 0xFFFF) | x << 16; }
+__device__ __forceinline__ uint32_t splat_hi(uint32_t x) { return (x >> 16) | (x & 0xFFFF0000u); }
+
+// The value of lane n of each row of 16 lanes, in the whole row.
+template <int N>
+__device__ __forceinline__ uint32_t row16_bcast(uint32_t x) {
+  return __builtin_amdgcn_mov_dpp(x, 0x150 + N, 0xF, 0xF, false);  // row_newbcast
+}
+
+__device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_f32<6>(xlane_level_max_f32<5>(x)); }
+
+// Workgroup (j, b, z) takes key/value head j (and head tile) of sequence b and
+// blocks z nt .. of its slots; wave w every nw-th of them.  One step is a block
+// of 32 slots: scores of 2 x 16 slots against up to 16 query heads
+// (mfma 16 x 16 x 32, keys as rows, so that a lane's results are 2 x 4 slots of
+// one head), the running softmax of a head in the four lanes that hold it, the
+// numerators rounded to fp16 as the second product's operand, which they are
+// without an exchange, and the values' rows.  The denominator is the product of
+// the same numerators with ones, so rounding them does not shift the mean.
+// Dequantized keys and values are rounded to fp16 once each (fma).
+template <int D>
+__global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, Cache4 c,
+    const int64_t* __restrict__ pos_p, int pos_stride, int H, int Hkv, int hb, int slots, int sinks, float scale2,
+    float q_scale, const uint16_t* __restrict__ rcos, const uint16_t* __restrict__ rsin, int64_t max_pos, int nt,
+    int ns, float* __restrict__ part, uint16_t* __restrict__ out) {
+  constexpr int NK = D / 32;   // k-steps of the scores, groups of a row
+  constexpr int ND = D / 16;   // row tiles of the output
+  const int t = threadIdx.x, ln = t & 63, nw = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int j = blockIdx.x / hb, h0 = blockIdx.x % hb * kHeads, b = blockIdx.y, z = blockIdx.z;
+  const int G = H / Hkv, heads = min(kHeads, G - h0);
+  const int64_t pos = pos_p[(int64_t)b * pos_stride];
+  if (pos < 0 || pos >= max_pos) return;
+  const int slot = slot_of(pos, slots, sinks);
+  const int last = (int)min(pos, (int64_t)slots - 1);  // the last slot in use
+  const int blk0 = z * nt;
+  if (blk0 * kSlotBlock > last) return;
+  const int blk1 = min(blk0 + nt, last / kSlotBlock + 1);
+  const int nact = last / (kSlotBlock * nt) + 1;
+  const int nblk = (slots + kSlotBlock - 1) / kSlotBlock;
+  const int64_t head = (int64_t)b * Hkv + j;
+  uint8_t* kc = c.kc + head * nblk * (kSlotBlock * D / 2);
+  uint16_t* kp = c.kp + head * nblk * (kSlotBlock * NK * 2);
+  uint8_t* vc = c.vc + head * nblk * (16 * D);
+  uint16_t* vp = c.vp + head * nblk * (NK * 64);
+  const bool owner = slot / (kSlotBlock * nt) == z && h0 == 0;  // writes the new row
+  const bool holds = slot / (kSlotBlock * nt) == z;
+
+  __shared__ uint16_t qs[kHeads][D];
+  __shared__ uint32_t new_k[D / 8], new_v[D / 8], new_kp[NK], new_vp[NK];
+  extern __shared__ float res[];  // [nw][kHeads][D + 2]
+
+  const uint16_t* cs = rcos ? rcos + pos * D : nullptr;
+  const uint16_t* sn = rsin ? rsin + pos * D : nullptr;
+  const uint16_t* qb = q + ((int64_t)b * H + (int64_t)j * G + h0) * D;
+  for (int i = t; i < kHeads * D; i += 64 * nw) {
+    const int g = i / D, d = i % D;
+    f16 x = (f16)0.0f;
+    if (g < heads) {
+      x = bits_to_h(qb[i]);
+      if (q_scale != 1.0f) x = rn_h((float)x * q_scale);
+      if (cs) {
+        f16 y = bits_to_h(qb[i - d + (d + D / 2) % D]);
+        if (q_scale != 1.0f) y = rn_h((float)y * q_scale);
+        x = turned(x, y, d < D / 2, cs[d], sn[d]);
+      }
+    }
+    qs[g][d] = h_to_bits(x);
+  }
+  if (holds && t < 64) {
+    // the step's own row, keys in the wave's lower half, values in its upper
+    const bool val = t >= 32;
+    const int d = (t & 31) * 8;
+    if (d < D) {
+      const uint16_t* src = (val ? v_new : k_new) + head * D;
+      uint16_t x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[i] = src[d + i];
+        if (!val && cs) x[i] = h_to_bits(turned(bits_to_h(x[i]), bits_to_h(src[(d + i + D / 2) % D]), d + i < D / 2, cs[d + i], sn[d + i]));
+      }
+      uint16_t sb, mb;
+      const uint32_t w = quantize8(x, &sb, &mb);
+      (val ? new_v : new_k)[d / 8] = w;
+      if ((t & 3) == 0) (val ? new_vp : new_kp)[d / 32] = (uint32_t)sb | (uint32_t)mb << 16;
+    }
+  }
+  __syncthreads();
+
+  const int l = ln & 15, r = ln >> 4;
+  // the queries as the scores' second operand: head l, elements
+  // (D / 4) r + 8 kk + the order in which pair_of gives a word's nibbles
+  half8v qv[NK];
+#pragma unroll
+  for (int kk = 0; kk < NK; kk++)
+#pragma unroll
+    for (int n = 0; n < 8; n++) qv[kk][n] = bits_to_h(qs[l][(D / 4) * r + 8 * kk + (n >> 1) + 4 * (n & 1)]);
+
+  float4v o[ND], den;
+#pragma unroll
+  for (int e = 0; e < ND; e++) o[e] = float4v{0, 0, 0, 0};
+  den = float4v{0, 0, 0, 0};
+  float m = -INFINITY;
+  half8v ones;
+#pragma unroll
+  for (int n = 0; n < 8; n++) ones[n] = (f16)1.0f;
+
+  for (int blk = blk0 + wave; blk < blk1; blk += nw) {
+    const int s0 = blk * kSlotBlock;
+    uint32_t kw[2][NK], kpar[2], vw[ND];
+    uint2 vpar;
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++) {
+      const int row = s0 + 16 * tt + l;
+#pragma unroll
+      for (int kk = 0; kk < NK; kk++) kw[tt][kk] = *reinterpret_cast<const uint32_t*>(kc + (int64_t)row * (D / 2) + r * (D / 8) + kk * 4);
+      kpar[tt] = *reinterpret_cast<const uint32_t*>(kp + ((int64_t)row * NK + (D == 128 ? r : r >> 1)) * 2);
+    }
+#pragma unroll
+    for (int e = 0; e < ND; e++)
+      vw[e] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)blk * (16 * D) + (e >> 2) * 1024 + ln * 16 + (e & 3) * 4);
+    vpar = *reinterpret_cast<const uint2*>(vp + (int64_t)blk * (NK * 64) + v_param((l >> 2) % NK, r, l & 3));
+    if (slot / kSlotBlock == blk) {
+      // the step's own row replaces what the slot held, here and in memory
+      const int at = slot % kSlotBlock, n = (at >> 4) * 4 + (at & 3);
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++)
+        if (16 * tt + l == at) {
+#pragma unroll
+          for (int kk = 0; kk < NK; kk++) {
+            kw[tt][kk] = new_k[r * (D / 32) + kk];
+            if (owner) *reinterpret_cast<uint32_t*>(kc + (int64_t)slot * (D / 2) + r * (D / 8) + kk * 4) = kw[tt][kk];
+          }
+          kpar[tt] = new_kp[D == 128 ? r : r >> 1];
+          if (owner && (D == 128 || (r & 1) == 0))
+            *reinterpret_cast<uint32_t*>(kp + ((int64_t)slot * NK + (D == 128 ? r : r >> 1)) * 2) = kpar[tt];
+        }
+      if (r == ((at & 15) >> 2)) {
+#pragma unroll
+        for (int e = 0; e < ND; e++) {
+          const int d = e * 16 + l;
+          const uint32_t code = (new_v[d / 8] >> (4 * (d & 7))) & 15;
+          vw[e] = (vw[e] & ~(15u << (4 * n))) | code << (4 * n);
+          if (owner) *reinterpret_cast<uint32_t*>(vc + (int64_t)blk * (16 * D) + (e >> 2) * 1024 + ln * 16 + (e & 3) * 4) = vw[e];
+        }
+        if ((l & 3) == (at & 3)) {
+          const uint32_t p = new_vp[(l >> 2) % NK];
+          const int sh = (at >> 4) * 16;
+          vpar.x = (vpar.x & ~(0xFFFFu << sh)) | (p & 0xFFFF) << sh;
+          vpar.y = (vpar.y & ~(0xFFFFu << sh)) | (p >> 16) << sh;
+          if (owner && l < 4 * NK)
+            *reinterpret_cast<uint2*>(vp + (int64_t)blk * (NK * 64) + v_param(l >> 2, r, l & 3)) = vpar;
+        }
+      }
+    }
+    const bool edge = s0 + kSlotBlock - 1 > last;
+    if (edge) {
+      // slots past the last in use: whatever they hold, their values count as 0
+      const int i = l & 3;
+      if (s0 + 4 * r + i > last) vpar.x &= 0xFFFF0000u, vpar.y &= 0xFFFF0000u;
+      if (s0 + 16 + 4 * r + i > last) vpar.x &= 0xFFFFu, vpar.y &= 0xFFFFu;
+    }
+    float x[8];
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++) {
+      const half2v s2 = __builtin_bit_cast(half2v, splat_lo(kpar[tt])), m2 = __builtin_bit_cast(half2v, splat_hi(kpar[tt]));
+      float4v acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int kk = 0; kk < NK; kk++) {
+        half8v a;
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const half2v v2 = __builtin_elementwise_fma(pair_of(kw[tt][kk], n), s2, m2);
+          a[2 * n] = v2.x;
+          a[2 * n + 1] = v2.y;
+        }
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qv[kk], acc, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[4 * tt + i] = acc[i] * scale2;
+    }
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < 8; n++)
+        if (s0 + 16 * (n >> 2) + 4 * r + (n & 3) > last) x[n] = -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int n = 1; n < 8; n++) mx = fmaxf(mx, x[n]);
+    mx = fmaxf(m, max_quarters(mx));
+    if (__ballot(mx != m)) {
+      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+#pragma unroll
+      for (int e = 0; e < ND; e++) o[e] *= f;
+      den *= f;
+      m = mx;
+    }
+    // numerators, slot pairs (t = 0, 1) as pair_of gives the values'
+    half8v pv;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      pv[2 * i] = rn_h(x[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m));
+      pv[2 * i + 1] = rn_h(x[4 + i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[4 + i] - m));
+    }
+    den = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pv, den, 0, 0, 0);
+    auto values = [&](auto gc) {
+      constexpr int g = decltype(gc)::value;
+      half2v s2[4], m2[4];
+      s2[0] = __builtin_bit_cast(half2v, row16_bcast<4 * g>(vpar.x));
+      s2[1] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 1>(vpar.x));
+      s2[2] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 2>(vpar.x));
+      s2[3] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 3>(vpar.x));
+      m2[0] = __builtin_bit_cast(half2v, row16_bcast<4 * g>(vpar.y));
+      m2[1] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 1>(vpar.y));
+      m2[2] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 2>(vpar.y));
+      m2[3] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 3>(vpar.y));
+#pragma unroll
+      for (int e = 2 * g; e < 2 * g + 2; e++) {
+        half8v a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const half2v v2 = __builtin_elementwise_fma(pair_of(vw[e], i), s2[i], m2[i]);
+          a[2 * i] = v2.x;
+          a[2 * i + 1] = v2.y;
+        }
+        o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pv, o[e], 0, 0, 0);
+      }
+    };
+    values(std::integral_constant<int, 0>{});
+    values(std::integral_constant<int, 1>{});
+    if constexpr (NK == 4) {
+      values(std::integral_constant<int, 2>{});
+      values(std::integral_constant<int, 3>{});
+    }
+  }
+
+  // the waves' sums meet: maximum over the waves, each scaled to it, in order
+  constexpr int RS = D + 2;
+  if (l < heads) {
+    float* w = res + (wave * kHeads + l) * RS;
+#pragma unroll
+    for (int e = 0; e < ND; e++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[16 * e + 4 * r + i] = o[e][i];
+    if (r == 0) {
+      w[D] = m;
+      w[D + 1] = den[0];
+    }
+  }
+  __syncthreads();
+  const int na = min(nw, blk1 - blk0);  // waves that had a block
+  uint16_t* ob = out + ((int64_t)b * H + (int64_t)j * G + h0) * D;
+  float* sp = part + (((int64_t)b * gridDim.x + blockIdx.x) * ns + z) * (kHeads * D + 2 * kHeads);
+  for (int i = t; i < heads * D; i += 64 * nw) {
+    const int g = i / D, d = i % D;
+    float mx = -INFINITY;
+    for (int w = 0; w < na; w++) mx = fmaxf(mx, res[(w * kHeads + g) * RS + D]);
+    float num = 0.0f, sum = 0.0f;
+    for (int w = 0; w < na; w++) {
+      const float* y = res + (w * kHeads + g) * RS;
+      const float f = y[D] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(y[D] - mx);
+      num = fmaf(y[d], f, num);
+      sum = fmaf(y[D + 1], f, sum);
+    }
+    if (nact == 1) {
+      ob[i] = h_to_bits(rn_h(num / sum));
+    } else {
+      sp[i] = num;
+      if (d == 0) {
+        sp[kHeads * D + g] = mx;
+        sp[kHeads * D + kHeads + g] = sum;
+      }
+    }
+  }
+}
+
+// Merges the spans' (maximum, denominator, sum) of one query head, in order.
+template <int D>
+__global__ __launch_bounds__(D) void kv4_combine_kernel(const int64_t* __restrict__ pos_p, int pos_stride, int H,
+                                                        int Hkv, int hb, int slots, int64_t max_pos, int nt, int ns,
+                                                        const float* __restrict__ part, uint16_t* __restrict__ out) {
+  constexpr int PF = kHeads * D + 2 * kHeads;
+  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+  const int G = H / Hkv, j = h / G, tile = h % G / kHeads, g = h % G % kHeads;
+  const int64_t pos = pos_p[(int64_t)b * pos_stride];
+  if (pos < 0 || pos >= max_pos) return;
+  const int nact = (int)min(pos, (int64_t)slots - 1) / (kSlotBlock * nt) + 1;
+  if (nact == 1) return;
+  const float* pk = part + (((int64_t)b * Hkv + j) * hb + tile) * ns * PF;
+  float mx = -INFINITY;
+  for (int z = 0; z < nact; z++) mx = fmaxf(mx, pk[(int64_t)z * PF + kHeads * D + g]);
+  float num = 0.0f, sum = 0.0f;
+  for (int z = 0; z < nact; z++) {
+    const float* y = pk + (int64_t)z * PF;
+    const float mz = y[kHeads * D + g], f = mz == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mz - mx);
+    num = fmaf(y[g * D + d], f, num);
+    sum = fmaf(y[kHeads * D + kHeads + g], f, sum);
+  }
+  out[((int64_t)b * H + h) * D + d] = h_to_bits(rn_h(num / sum));
+}
+
+int check_cache4(const char* what, const void* kc, const void* kp, const void* vc, const void* vp, int64_t B, int64_t Hkv,
+                 int64_t D, int64_t slots) {
+  AQ_CHECK_ARG(kc && kp && vc && vp, "%s: null pointer", what);
+  AQ_CHECK_ARG(D == 64 || D == 128, "%s: head dim %lld (64 or 128 supported)", what, (long long)D);
+  AQ_CHECK_ARG(B > 0 && B <= 65535 && Hkv > 0 && Hkv <= 65535 && slots > 0 && slots <= (1 << 24),
+               "%s: sizes out of range", what);
+  AQ_CHECK_ARG((uintptr_t)kc % 16 == 0 && (uintptr_t)kp % 16 == 0 && (uintptr_t)vc % 16 == 0 && (uintptr_t)vp % 16 == 0,
+               "%s: the cache's buffers must be 16-byte aligned", what);
+  return AQ_OK;
+}
+
+}  // namespace
+
+extern "C" int aq_kv4_store(const void* k, const void* v, int64_t B, int64_t Hkv, int64_t S, int64_t D,
+                            const int64_t* k_strides, const int64_t* v_strides, int64_t start, const int64_t* lengths,
+                            void* k_codes, void* k_params, void* v_codes, void* v_params, int64_t slots, int64_t sinks,
+                            void* stream) {
+  AQ_CHECK_ARG(k && v && k_strides && v_strides, "aq_kv4_store: null pointer");
+  if (const int rc = check_cache4("aq_kv4_store", k_codes, k_params, v_codes, v_params, B, Hkv, D, slots)) return rc;
+  AQ_CHECK_ARG(sinks >= -1 && sinks < slots, "aq_kv4_store: %lld sinks in %lld slots", (long long)sinks, (long long)slots);
+  AQ_CHECK_ARG(S > 0 && start >= 0 && S <= INT32_MAX && start <= INT32_MAX - S,
+               "aq_kv4_store: positions %lld .. +%lld out of range", (long long)start, (long long)S);
+  AQ_CHECK_ARG(sinks >= 0 || start + S <= slots, "aq_kv4_store: positions up to %lld in %lld slots",
+               (long long)(start + S), (long long)slots);
+  for (int i = 0; i < 3; i++)
+    AQ_CHECK_ARG(k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0, "aq_kv4_store: strides must be multiples of 8");
+  AQ_CHECK_ARG((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)lengths % 8 == 0,
+               "aq_kv4_store: k and v must be 16-byte aligned");
+  const int64_t nblk = aq::ceil_div(slots, kSlotBlock);
+  // blocks without one of the positions are left out, where no slot is used again
+  const int64_t first = start + S <= slots ? start / kSlotBlock : 0;
+  const int64_t end = start + S <= slots ? aq::ceil_div(start + S, kSlotBlock) : nblk;
+  const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
+  const dim3 grid((unsigned)(end - first), (unsigned)Hkv, (unsigned)B);
+#define AQ_KV4_STORE(DD)                                                                                              \
+  hipLaunchKernelGGL((kv4_store_kernel<DD>), grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t*)k,             \
+                     (const uint16_t*)v, k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1],        \
+                     v_strides[2], (int)S, start, lengths, c, (int)Hkv, (int)slots, (int)sinks, (int)first)
+  if (D == 64) AQ_KV4_STORE(64);
+  else AQ_KV4_STORE(128);
+#undef AQ_KV4_STORE
+  AQ_LAUNCH_CHECK("aq_kv4_store");
+  return AQ_OK;
+}
+
+extern "C" int aq_kv4_load(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                           int64_t B, int64_t Hkv, int64_t D, int64_t slots, int64_t count, void* k, void* v,
+                           void* stream) {
+  AQ_CHECK_ARG(k && v, "aq_kv4_load: null pointer");
+  if (const int rc = check_cache4("aq_kv4_load", k_codes, k_params, v_codes, v_params, B, Hkv, D, slots)) return rc;
+  AQ_CHECK_ARG(count > 0 && count <= slots, "aq_kv4_load: %lld of %lld slots", (long long)count, (long long)slots);
+  AQ_CHECK_ARG(B * Hkv <= 65535, "aq_kv4_load: %lld heads in all (at most 65535)", (long long)(B * Hkv));
+  AQ_CHECK_ARG((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "aq_kv4_load: k and v must be 16-byte aligned");
+  const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
+  const dim3 grid((unsigned)aq::ceil_div(count, kSlotBlock), (unsigned)(B * Hkv));
+  if (D == 64)
+    hipLaunchKernelGGL((kv4_load_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, c, (int)slots, (int)count, (uint16_t*)k, (uint16_t*)v);
+  else
+    hipLaunchKernelGGL((kv4_load_kernel<128>), grid, dim3(256), 0, (hipStream_t)stream, c, (int)slots, (int)count, (uint16_t*)k, (uint16_t*)v);
+  AQ_LAUNCH_CHECK("aq_kv4_load");
+  return AQ_OK;
+}
+
+extern "C" int64_t aq_kv4_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t slots) {
+  if (B <= 0 || Hkv <= 0 || H <= 0 || H % Hkv != 0 || (D != 64 && D != 128) || slots <= 0) return -1;
+  return split4_of(B, Hkv, H / Hkv, D, slots).bytes;
+}
+
+extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* k_codes, void* k_params,
+                                void* v_codes, void* v_params, const int64_t* pos, int64_t pos_stride, int64_t B,
+                                int64_t H, int64_t Hkv, int64_t D, int64_t slots, int64_t sinks, float scale,
+                                float q_scale, const void* rope_cos, const void* rope_sin, int64_t rope_rows,
+                                void* workspace, int64_t ws_bytes, void* out, void* stream) {
+  AQ_CHECK_ARG(q && k_new && v_new && pos && out, "aq_kv4_attention: null pointer");
+  if (const int rc = check_cache4("aq_kv4_attention", k_codes, k_params, v_codes, v_params, B, Hkv, D, slots)) return rc;
+  AQ_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr), "aq_kv4_attention: rope_cos and rope_sin come together");
+  AQ_CHECK_ARG(H > 0 && H % Hkv == 0, "aq_kv4_attention: H (%lld) must be a multiple of Hkv (%lld)", (long long)H,
+               (long long)Hkv);
+  AQ_CHECK_ARG(pos_stride == 0 || pos_stride == 1, "aq_kv4_attention: pos_stride %lld (0 or 1)", (long long)pos_stride);
+  AQ_CHECK_ARG(sinks >= -1 && sinks < slots, "aq_kv4_attention: %lld sinks in %lld slots", (long long)sinks,
+               (long long)slots);
+  AQ_CHECK_ARG(!rope_cos || rope_rows > 0, "aq_kv4_attention: %lld rows of rope_cos", (long long)rope_rows);
+  AQ_CHECK_ARG((uintptr_t)q % 2 == 0 && (uintptr_t)k_new % 2 == 0 && (uintptr_t)v_new % 2 == 0 && (uintptr_t)out % 2 == 0 &&
+                   (uintptr_t)pos % 8 == 0,
+               "aq_kv4_attention: misaligned buffer");
+  const Split4 sp = split4_of(B, Hkv, H / Hkv, D, slots);
+  AQ_CHECK_ARG(Hkv * sp.hb <= 65535 && H <= 65535, "aq_kv4_attention: sizes out of range");
+  AQ_CHECK_ARG(sp.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= sp.bytes),
+               "aq_kv4_attention: workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)ws_bytes,
+               (long long)sp.bytes);
+  // positions past the table, past a cache without sinks, or past 31 bits are not run
+  int64_t max_pos = sinks < 0 ? slots : INT32_MAX;
+  if (rope_cos) max_pos = std::min(max_pos, rope_rows);
+  const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
+  const float scale2 = scale * 1.44269504f;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)(Hkv * sp.hb), (unsigned)B, (unsigned)sp.ns);
+  const size_t lds = (size_t)sp.nw * kHeads * (D + 2) * 4;
+#define AQ_KV4_LAUNCH(DD)                                                                                             \
+  do {                                                                                                                \
+    hipLaunchKernelGGL((kv4_attention_kernel<DD>), grid, dim3(64 * (unsigned)sp.nw), lds, s, (const uint16_t*)q,      \
+                       (const uint16_t*)k_new, (const uint16_t*)v_new, c, pos, (int)pos_stride, (int)H, (int)Hkv,     \
+                       (int)sp.hb, (int)slots, (int)sinks, scale2, q_scale, (const uint16_t*)rope_cos,                \
+                       (const uint16_t*)rope_sin, max_pos, (int)sp.nt, (int)sp.ns, (float*)workspace,                 \
+                       (uint16_t*)out);                                                                               \
+    if (sp.ns > 1)                                                                                                    \
+      hipLaunchKernelGGL((kv4_combine_kernel<DD>), dim3((unsigned)H, (unsigned)B), dim3(DD), 0, s, pos,               \
+                         (int)pos_stride, (int)H, (int)Hkv, (int)sp.hb, (int)slots, max_pos, (int)sp.nt, (int)sp.ns,  \
+                         (const float*)workspace, (uint16_t*)out);                                                    \
+  } while (0)
+  if (D == 64) AQ_KV4_LAUNCH(64);
+  else AQ_KV4_LAUNCH(128);
+#undef AQ_KV4_LAUNCH
+  AQ_LAUNCH_CHECK("aq_kv4_attention");
+  return AQ_OK;
+}

@@ -1,0 +1,59 @@
+"""Attention of a prompt through a sliding window with sinks.
+
+``window_attention`` is the kernel's call (``aq_window_attention``);
+``use_window_attention`` makes an HF OPT / Llama / Mistral model's own forward
+use it, which ``GraphDecoder(window=...)`` does for its prompts.  No counterpart
+in the reference, whose attention (integration/atlas_wrappers.py:161-262) sees
+every position through torch's SDPA and a dense mask.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .. import _lib
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
+                     scale: Optional[float] = None, starts: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T) v in fp16 for the last M of N positions.
+
+    q [B, H, M, D], k and v [B, Hkv, N, D] (fp16 on a HIP device, any strides, H a
+    multiple of Hkv, D 64 or 128, M <= N); returns [B, M, H, D].  Query i stands
+    at position N - M + i and sees the keys j at or before it that are less than
+    ``window`` positions back (None: all) or among the first ``sinks``.
+    ``starts`` (int32 [B]): sequence b begins at that position (left padding):
+    earlier keys are not seen, and sinks count from there.  A query that sees
+    nothing gets zeros."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"window_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    B, H, M, D = q.shape
+    Hkv, N = k.shape[1], k.shape[2]
+    dev = q.device
+    if k.shape[0] != B or k.shape[3] != D or D not in (64, 128) or Hkv == 0 or H % Hkv or M > N:
+        raise ValueError(f"window_attention: q {tuple(q.shape)}, k {tuple(k.shape)} (D 64 or 128, H a multiple of "
+                         "Hkv, no more queries than keys)")
+    for t in (q, k, v):
+        if t.dtype != torch.float16 or t.device.type != "cuda" or t.device != dev:
+            raise ValueError("window_attention: q, k and v must be fp16 on one HIP device")
+    window = N if window is None else int(window)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window_attention: window {window}, {sinks} sinks")
+    if starts is not None and (starts.dtype != torch.int32 or starts.shape != (B,) or starts.device != dev
+                               or not starts.is_contiguous()):
+        raise ValueError(f"window_attention: starts must be contiguous int32 [{B}] on {dev}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise RuntimeError("window_attention records no gradients: call it under torch.no_grad()")
+    out = torch.empty(B, M, H, D, dtype=torch.float16, device=dev)
+    if out.numel() == 0:
+        return out
+    q, k, v = (_lib.strided_rows(t) for t in (q, k, v))
+    arr = [_lib.ptr_array(t.stride()[:3], ctypes.c_int64) for t in (q, k, v)]
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().aq_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), B, H, Hkv, M, N, D, *arr,
+                                                   window, int(sinks), D ** -0.5 if scale is None else scale,
+                                                   _lib.ptr(starts), out.data_ptr(), _lib.stream_of(dev)),
+                   "aq_window_attention")
+    return out

@@ -48,6 +48,7 @@ extern "C" {
 
 enum { AQ_FMT_INT8 = 0, AQ_FMT_E4M3 = 1 };
 enum { AQ_LAYOUT_FLAT = 0, AQ_LAYOUT_TILED = 1 };
+enum { AQ_F16 = 0, AQ_BF16 = 1, AQ_F32 = 2 };
 enum { AQ_OK = 0, AQ_EINVAL = -1, AQ_EHIP = -2, AQ_EUNSUPPORTED = -3, AQ_EWORKSPACE = -4 };
 
 /* ABI version of the loaded library (AQ_ABI_VERSION at build time). */
@@ -404,6 +405,124 @@ int aq_decode_attention(const void* q, const void* k_new, const void* v_new, voi
 /* Bytes of workspace aq_decode_attention needs for these sizes (-1 for
  * sizes it cannot take).  No counterpart in the reference. */
 int64_t aq_decode_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t L);
+
+/*
+ * aq_decode_attention over a cache that keeps a sliding window of positions
+ * and the first few (the attention of models with a window, and of endless
+ * generation; no counterpart in the reference, whose cache keeps every
+ * position).  The cache's L slots hold the first `sinks` positions and the last
+ * L - sinks (a window of L - sinks, the step's own position included): position
+ * p is in slot p while p < L, then in slot sinks + (p - sinks) mod (L - sinks).
+ * Keys are rotated at their position before they are cached, so the order of
+ * the slots does not matter.  sinks = -1: position = slot, no window.
+ *   pos         int64 [1] (pos_stride 0) or [B] (1: each sequence its own)
+ *   rope_cos, rope_sin  fp16 [rope_rows, D]
+ * A sequence whose position is negative, not below rope_rows (with rope_cos),
+ * not below L (with sinks = -1) or above 2^31 - 2 is not run: its row of out and
+ * its cache stay as they were.  Everything else as aq_decode_attention, with
+ * its workspace.
+ */
+int aq_window_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache,
+                               const int64_t* pos, int64_t pos_stride, int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                               int64_t L, int64_t sinks, float scale, float q_scale, const void* rope_cos,
+                               const void* rope_sin, int64_t rope_rows, void* workspace, int64_t ws_bytes, void* out,
+                               void* stream);
+
+/*
+ * Attention of a prompt, or of the last M of N positions, through a sliding
+ * window with sinks (no counterpart in the reference, which runs torch's SDPA
+ * over a dense mask).  Query i (0 .. M - 1) stands at position N - M + i; it sees
+ * key j when start <= j <= its position and (position - j < window or
+ * j - start < sinks), start = starts[b] (a left-padded batch) or 0.
+ *   out[b, i, h, :] = fp16(softmax(scale q . k) v)  (zeros where it sees nothing)
+ * Scores, softmax and sums in f32, the softmax's numerators rounded to fp16.
+ *   q      fp16 [B, H, M, D]    k, v  fp16 [B, Hkv, N, D], by strides
+ *          (elements, {batch, head, position}, multiples of 8; D contiguous)
+ *   starts int32 [B] or NULL    out   fp16 [B, M, H, D]
+ *   D = 64 or 128, H a multiple of Hkv, M <= N < 2^24, window >= 1 (N or more:
+ *   causal), sinks >= 0; q, k, v, out 16-byte aligned
+ * What a key or value that a query does not see holds, infinities and NaN
+ * included, does not reach its output.
+ */
+int aq_window_attention(const void* q, const void* k, const void* v, int64_t B, int64_t H, int64_t Hkv, int64_t M,
+                        int64_t N, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, int64_t window, int64_t sinks, float scale, const int32_t* starts,
+                        void* out, void* stream);
+
+/*
+ * A key/value cache in 4 bits (no counterpart in the reference, whose cache
+ * keeps fp16).  A row of D elements is cut into groups of 32 with minimum m and
+ * scale s = fp16((max - m) / 15), one fp16 step less where m + 15 s would be
+ * 65520 or more; element x has code min(rint((x - m) / s), 15) (differences and
+ * quotients rounded to f32, ties to even; 0 where s = 0) and stands for s c + m.
+ * A group with an infinity or NaN stands for NaN.  c = slots rounded up to 32:
+ *   k_codes  uint8 [B, Hkv, c, D / 2]       element d in nibble d % 2 of byte d / 2
+ *   k_params fp16  [B, Hkv, c, D / 32, 2]   s, m
+ *   v_codes  uint8 [B, Hkv, c / 32, 16 D]   blocks of 32 slots, as words
+ *            [D / 64][4][16][4]: slot 16 t + 4 r + i of element 64 a + 16 e + l
+ *            in nibble 4 t + i of word [a][r][l][e]
+ *   v_params fp16  [B, Hkv, c / 32, D / 32, 4, 4, 4]   [group][r][i]: s of slots
+ *            t = 0 and 1, then m of both
+ * all 16-byte aligned, D = 64 or 128, slots <= 2^24.  slots and sinks map
+ * positions to slots as in aq_window_decode_attention.
+ *
+ * aq_kv4_store writes positions start .. start + S - 1 (a prompt, or a piece of
+ * one) of k, v fp16 [B, Hkv, S, D] (by strides in elements, {batch, head,
+ * position}, multiples of 8; 16-byte aligned), of sequence b only the first
+ * lengths[b] of them if lengths (device int64 [B]) is given.  Of several
+ * positions that share a slot the newest is kept; other slots stay as they were.
+ * sinks = -1: start + S <= slots.
+ *
+ * aq_kv4_load reads slots 0 .. count - 1 back: k, v fp16 [B, Hkv, count, D],
+ * fp16(s c + m).
+ */
+int aq_kv4_store(const void* k, const void* v, int64_t B, int64_t Hkv, int64_t S, int64_t D, const int64_t* k_strides,
+                 const int64_t* v_strides, int64_t start, const int64_t* lengths, void* k_codes, void* k_params,
+                 void* v_codes, void* v_params, int64_t slots, int64_t sinks, void* stream);
+int aq_kv4_load(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, int64_t B,
+                int64_t Hkv, int64_t D, int64_t slots, int64_t count, void* k, void* v, void* stream);
+
+/*
+ * aq_window_decode_attention over a 4-bit cache: the step's key (rotated) and
+ * value are quantized into their slot as aq_kv4_store does it, then
+ *   out[b, h, :] = fp16(softmax(scale q . k) v)
+ * over the slots in use, as the values they stand for (each rounded to fp16;
+ * scores and sums in f32, the softmax's numerators rounded to fp16).  H any
+ * multiple of Hkv.  q, k_new, v_new, pos, q_scale, rope_* and which sequences
+ * are run: as there; workspace: aq_kv4_attention_workspace bytes (may be 0,
+ * then NULL will do; -1 for sizes it cannot take), 16-byte aligned, no initial
+ * contents; calls that overlap in time must not share one.
+ */
+int64_t aq_kv4_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t slots);
+int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* k_codes, void* k_params, void* v_codes,
+                     void* v_params, const int64_t* pos, int64_t pos_stride, int64_t B, int64_t H, int64_t Hkv,
+                     int64_t D, int64_t slots, int64_t sinks, float scale, float q_scale, const void* rope_cos,
+                     const void* rope_sin, int64_t rope_rows, void* workspace, int64_t ws_bytes, void* out,
+                     void* stream);
+
+/*
+ * The next token of every sequence from its logits and one random number
+ * (the sampling of HF generate, which the reference drives with do_sample;
+ * examples/run_atlas_inference.py:244-264).  Of the tokens of a row in the order
+ * of falling logit, equal ones by index, with w_i = exp((x_i - max) / T), those
+ * are kept
+ *   that are among the first top_k (top_k <= 0 or >= V: all),
+ *   before which less than top_p of the mass of these lies (top_p >= 1: all),
+ *   whose w is at least min(min_p, 1) (min_p <= 0: all),
+ * the first one always.  tokens[b] is the first kept token, by index, at which
+ * the running mass of the kept ones exceeds u[b] times their whole mass (u >= 1:
+ * the last).  temperature <= 0, or a row without a logit above -inf: the largest
+ * logit, the lowest index of equal ones.  NaN counts as -inf; logits of +inf
+ * share the whole mass.  Masses are sums of w rounded to 2^-45.
+ *   logits  dtype AQ_F16, AQ_BF16 or AQ_F32 [B, V], rows `stride` elements apart,
+ *           V <= 262144
+ *   u       f32 [B], in [0, 1)      tokens  int64 [B] (out)
+ *   temperature, top_p, min_p  f32 [B], top_k int32 [B]: one setting a row, or
+ *           NULL: temperature0, top_p0, min_p0, top_k0 for all rows
+ */
+int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t stride, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+              float temperature0, int32_t top_k0, float top_p0, float min_p0, int64_t* tokens, void* stream);
 
 /*
  * Residual add and normalisation of `rows` rows of n fp16 (n a multiple of
