@@ -9,6 +9,7 @@ every compute entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -135,6 +136,16 @@ def ptr(t) -> int | None:
     if t is None or t.numel() == 0:
         return None
     return t.data_ptr()
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context with ``device`` (a tensor's) as the current one, where kernels
+    are launched: nothing to do where it is already (a tenth of the cost of
+    torch.cuda.device, which matters on the per-token decode path)."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def strided_rows(t):

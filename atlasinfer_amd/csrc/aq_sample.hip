@@ -5,29 +5,47 @@
 // w_i = exp((x_i - max) / T).  Every filter keeps a beginning of that order:
 // the first k; of those the tokens before which less than p of their mass
 // lies; the tokens of w >= min_p.  So the kept set is known by one key (the
-// last logit kept) and the number of its ties kept, found by descending the
-// bits of the logits with histograms of counts and masses.  The token is the
-// first kept one, by index, whose running mass passes u times the kept mass.
+// last logit kept) and the number of its ties kept -- the cut -- and min_p.  The
+// token is the first kept one, by index, whose running mass passes u times the
+// kept mass.
 //
-// Masses are integers, w rounded to 2^-45 (V <= 2^18 of them stay below
-// 2^63): sums do not depend on their order, the same call gives the same
-// token on every run, and a border lies within V 2^-46 of its place (2^-28 of
-// the largest weight, were all the roundings one way).  The exponentials are
-// taken in 64 bits: a border between two of V tokens lies in an interval as
-// narrow as 1 / V, so an error of 2^-24 in the sums would choose another token
-// now and then.
+// Masses are whole numbers, w rounded to 2^-42 (V <= 2^18 of them stay below
+// 2^61): sums do not depend on their order, so the same call gives the same
+// token on every run, however the work is dealt.  The exponentials are taken in
+// 64 bits: with V tokens there are V borders a random number can fall beside,
+// and errors of 2^-24 in the sums would choose another token in one row of a
+// hundred where tens of thousands are kept.
+//
+// One workgroup takes a row.  A full sort is never made:
+//   max      one pass, 16 bytes a thread and load, packed maxima
+//   top-k    (k <= 512) of the 1024 threads' own maxima the k-th largest is a
+//            key that at least k tokens reach; the tokens that do (k and a few,
+//            for logits in any order) go to a list in LDS
+//   top-p    a histogram of masses in f32 brackets the key where the running mass
+//            reaches p; one exact pass sums what lies above the bracket and lists
+//            what lies inside
+//   the cut  by descending the keys' bits over the list (11 at a time, counts and
+//            masses in LDS); where list or bracket do not serve (more ties than
+//            the list has room for, large k) over the whole row
+//   token    kept masses by segments of 1 KiB, summed in the exact pass or from
+//            the list; one wave goes through the segment that the number falls in
+//
+// Passes are short loops over the row in memory (the L2 has it after the first):
+// with every element of a thread unrolled, and kept in registers, the kernel was
+// 20 000 instructions long, ran once through them and took 25 us for a greedy row
+// of 50272, most of it waiting for instructions.
 #include "aq_common.h"
 
 namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;  // 11 bits
 constexpr int64_t kMaxVocab = 1 << 18;
-constexpr int kTileShift = 13;  // 8192 elements: 8 a thread
-constexpr int kTile = 1 << kTileShift;
-constexpr int kMaxTiles = (int)(kMaxVocab >> kTileShift);
-constexpr double kOne = 35184372088832.0;  // 2^45
+constexpr double kOne = 4398046511104.0;  // 2^42
+constexpr int kList = 4096;
+constexpr int kMaxListK = 512;
+constexpr int kMaxSegments = 1024 + 16;  // 2^18 f32 and a misaligned start
 
 struct Settings {
   const float *t, *p, *m;
@@ -36,70 +54,85 @@ struct Settings {
   int k0;
 };
 
-// 16-bit or 32-bit keys whose order as integers is the logits' order: NaN as
-// -inf, -0 as 0.
+// A logit's key: its bits as a signed number (so that -0 and 0 are one), moved
+// up until -inf is the lowest and infinity the highest key there is; NaNs wrap
+// below -inf and are raised to it.
 template <int FMT>
-struct Logit;
-template <>
-struct Logit<AQ_F16> {
-  typedef uint16_t raw;
-  static constexpr int kBits = 16;
-  static __device__ float value(raw r) { return (float)bits_to_h(r); }
-};
-template <>
-struct Logit<AQ_BF16> {
-  typedef uint16_t raw;
-  static constexpr int kBits = 16;
-  static __device__ float value(raw r) { return __builtin_bit_cast(float, (uint32_t)r << 16); }
-};
-template <>
-struct Logit<AQ_F32> {
-  typedef uint32_t raw;
-  static constexpr int kBits = 32;
-  static __device__ float value(raw r) { return __builtin_bit_cast(float, r); }
-};
+struct Logit {
+  static constexpr int kBits = FMT == AQ_F32 ? 32 : 16;
+  static constexpr int kPer = FMT == AQ_F32 ? 4 : 8;  // elements of a 16-byte piece
+  static constexpr uint32_t kSign = 1u << (kBits - 1);
+  static constexpr uint32_t kInf = FMT == AQ_F16 ? 0x7C00u : FMT == AQ_BF16 ? 0x7F80u : 0x7F800000u;
+  static constexpr uint32_t kUp = kSign - 1 - kInf;
+  static constexpr uint32_t kLowest = 2 * kUp + 1;  // key of -inf
 
-template <int FMT>
-__device__ __forceinline__ float logit(typename Logit<FMT>::raw r) {
-  const float f = Logit<FMT>::value(r);
-  return f != f ? -INFINITY : f + 0.0f;
-}
-
-// Key of a logit: the sign bit flipped, every bit of negative numbers.
-template <int FMT>
-__device__ __forceinline__ uint32_t key_of(typename Logit<FMT>::raw r) {
-  constexpr int B = Logit<FMT>::kBits;
-  constexpr uint32_t sign = 1u << (B - 1), all = B == 32 ? 0xFFFFFFFFu : (1u << (B & 31)) - 1;
-  const float f = Logit<FMT>::value(r);
-  uint32_t b = r;
-  if (f == 0.0f) b = 0;
-  if (f != f) b = FMT == AQ_F16 ? 0xFC00u : FMT == AQ_BF16 ? 0xFF80u : 0xFF800000u;  // -inf
-  return b & sign ? ~b & all : b | sign;
-}
-
-template <int FMT>
-__device__ __forceinline__ float logit_of_key(uint32_t key) {
-  constexpr int B = Logit<FMT>::kBits;
-  constexpr uint32_t sign = 1u << (B - 1), all = B == 32 ? 0xFFFFFFFFu : (1u << (B & 31)) - 1;
-  const uint32_t b = key & sign ? key & ~sign : ~key & all;
-  return Logit<FMT>::value((typename Logit<FMT>::raw)b);
-}
-
-// exp((x - max) / T) with c = log2(e) / T; the largest logit weighs 1 also
-// where it is infinite or T so small that c is.
-__device__ __forceinline__ double weight(float x, float mx, double c) {
-  if (x == mx) return 1.0;
-  if (x == -INFINITY) return 0.0;
-  return exp2(((double)x - (double)mx) * c);
-}
-__device__ __forceinline__ uint64_t fixed(double w) { return (uint64_t)(w * kOne + 0.5); }
-
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t t = __shfl_up(v, d, 64);
-    if ((threadIdx.x & 63) >= d) v += t;
+  static __device__ __forceinline__ float value(uint32_t b) {
+    if (FMT == AQ_F16) return (float)bits_to_h((uint16_t)b);
+    return __builtin_bit_cast(float, FMT == AQ_BF16 ? b << 16 : b);
   }
+  static __device__ __forceinline__ uint32_t bits_of_key(uint32_t key) {
+    const int32_t s = (int32_t)(key - kSign - kUp);
+    return s >= 0 ? (uint32_t)s : kSign | (uint32_t)-s;
+  }
+  static __device__ __forceinline__ float value_of_key(uint32_t key) { return value(bits_of_key(key)); }
+};
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+
+// Keys of the two 16-bit logits of a word, or of one 32-bit logit.
+template <int FMT>
+__device__ __forceinline__ uint32_t keys_of_word(uint32_t w) {
+  typedef Logit<FMT> L;
+  if constexpr (FMT == AQ_F32) {
+    const uint32_t g = (uint32_t)((int32_t)w >> 31);
+    return max((((w & 0x7FFFFFFFu) ^ g) - g) + (L::kSign + L::kUp), L::kLowest);
+  } else {
+    const i16x2 g = __builtin_bit_cast(i16x2, w) >> 15;
+    const u16x2 gu = __builtin_bit_cast(u16x2, g);
+    u16x2 k = (__builtin_bit_cast(u16x2, w & 0x7FFF7FFFu) ^ gu) - gu;
+    k = k + (uint16_t)(L::kSign + L::kUp);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(k, (u16x2)((uint16_t)L::kLowest)));
+  }
+}
+
+// w = 2^(n / 64) 2^(r / 64), y = n + r, from a table of 2^(j / 64) and a
+// polynomial of degree 4 (|r| <= 1/2: relative error 4e-14).  y: 64 log2(e)
+// (x - max) / T; below -6400, and where it is not a number (x is not, or -inf at
+// T = inf), w is as good as 0.
+__device__ __forceinline__ double exp2_64th(double y, const double* table) {
+  y = fmin(fmax(y, -6400.0), 0.0);
+  const double n = rint(y), r = y - n;
+  constexpr double a = 0.010830424696249145;  // ln 2 / 64
+  constexpr double a2 = a * a / 2, a3 = a * a * a / 6, a4 = a * a * a * a / 24;
+  const double q = fma(r, fma(r, fma(r, fma(r, a4, a3), a2), a), 1.0);
+  const int i = (int)n;
+  return ldexp(table[i & 63] * q, i >> 6);
+}
+
+struct Weigh {
+  double mx, c;
+  const double* table;
+  __device__ __forceinline__ double operator()(float x) const { return exp2_64th(((double)x - mx) * c, table); }
+  __device__ __forceinline__ double whole(float x) const { return rint((*this)(x) * kOne); }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Inclusive prefix sum over the wave: row shifts within 16 lanes (zeros come
+// in), then lane 15 into rows 1 and 3, lane 31 into rows 2 and 3.
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += dpp_u64<0x111, 0xF>(v);
+  v += dpp_u64<0x112, 0xF>(v);
+  v += dpp_u64<0x114, 0xF>(v);
+  v += dpp_u64<0x118, 0xF>(v);
+  v += dpp_u64<0x142, 0xA>(v);
+  v += dpp_u64<0x143, 0xC>(v);
   return v;
 }
 
@@ -123,236 +156,450 @@ __device__ __forceinline__ uint64_t block_scan_u64(uint64_t v, uint64_t* lds, ui
 struct Shared {
   uint64_t mass[kBins];
   uint32_t count[kBins];
+  uint64_t seg_mass[kMaxSegments];
+  uint32_t seg_ties[kMaxSegments];
+  uint2 list[kList];  // (key, index)
+  double table[64];
   uint64_t red[kWaves];
-  uint64_t tile_mass[kMaxTiles];
-  uint32_t tile_ties[kMaxTiles];
-  uint64_t found_mass;
-  uint32_t found_bin, found_count, token;
+  uint64_t found_mass, total;
+  uint32_t found_bin, found_count, n_list, segment, seg_rank, token;
+  uint64_t seg_before;
 };
+
+struct Found {
+  uint32_t bin, count;
+  uint64_t mass;
+};
+
+// The bin, from the highest down, in which the running count (by_mass: the
+// running mass) reaches `most`, and what lies above it.  The caller knows that
+// one does.
+__device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t most) {
+  const int t = threadIdx.x;
+  const int b0 = kBins - 1 - 2 * t, b1 = b0 - 1;  // this thread's
+  const uint64_t m0 = s.mass[b0], m1 = s.mass[b1], c0 = s.count[b0], c1 = s.count[b1];
+  uint64_t all;
+  const uint64_t im = block_scan_u64(m0 + m1, s.red, &all), bm = im - m0 - m1;
+  const uint64_t ic = block_scan_u64(c0 + c1, s.red, &all), bc = ic - c0 - c1;
+  // a bin is the one if what lies above it does not reach `most` and with it does
+  auto take = [&](int bin, uint64_t mb, uint64_t cb, uint64_t m, uint64_t c) {
+    const uint64_t lo = by_mass ? mb : cb, hi = by_mass ? mb + m : cb + c;
+    if (lo < most && hi >= most) {
+      s.found_bin = bin;
+      s.found_count = (uint32_t)cb;
+      s.found_mass = mb;
+    }
+  };
+  take(b0, bm, bc, m0, c0);
+  take(b1, bm + m0, bc + c0, m1, c1);
+  __syncthreads();
+  const Found f = {s.found_bin, s.found_count, s.found_mass};
+  return f;
+}
 
 // A cut: keys above `key`, and the first `ties` of those equal to it.
 struct Cut {
   uint32_t key, ties;
 };
 
-// The bin, from the highest down, in which the running count (by_mass: the
-// running mass) reaches `most`, and what lies above it.  The caller knows that
-// one does.
-__device__ __forceinline__ void find_bin(Shared& s, bool by_mass, uint64_t most, uint32_t* bin,
-                                         uint32_t* count, uint64_t* mass) {
-  const int t = threadIdx.x;
-  // thread t has bins 2047 - 2t and 2046 - 2t
-  const int b0 = kBins - 1 - 2 * t, b1 = b0 - 1;
-  const uint64_t m0 = s.mass[b0], m1 = s.mass[b1], c0 = s.count[b0], c1 = s.count[b1];
-  uint64_t all_m, all_c;
-  const uint64_t im = block_scan_u64(m0 + m1, s.red, &all_m);
-  const uint64_t ic = block_scan_u64(c0 + c1, s.red, &all_c);
-  const uint64_t bm0 = im - m0 - m1, bc0 = ic - c0 - c1, bm1 = im - m1, bc1 = ic - c1;
-  // a bin is the one if the next one's first token is cut, and its own is not
-  auto cut = [&](uint64_t m, uint64_t c) { return (by_mass ? m : c) >= most; };
-  if (c0 && !cut(bm0, bc0) && cut(bm1, bc1)) {
-    s.found_bin = b0;
-    s.found_count = (uint32_t)bc0;
-    s.found_mass = bm0;
-  }
-  if (c1 && !cut(bm1, bc1) && cut(im, ic)) {
-    s.found_bin = b1;
-    s.found_count = (uint32_t)bc1;
-    s.found_mass = bm1;
-  }
-  __syncthreads();
-  *bin = s.found_bin;
-  *count = s.found_count;
-  *mass = s.found_mass;
-  __syncthreads();
-}
-
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const typename Logit<FMT>::raw* __restrict__ logits, int V,
-                                                          int64_t stride, const float* __restrict__ u, Settings set,
+__global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict__ logits, int V, int64_t stride,
+                                                          const float* __restrict__ u, Settings set,
                                                           int64_t* __restrict__ out) {
-  constexpr int B = Logit<FMT>::kBits;
+  typedef Logit<FMT> L;
+  constexpr int B = L::kBits, E = L::kPer;
   __shared__ Shared s;
-  const int t = threadIdx.x, row = blockIdx.x;
-  const typename Logit<FMT>::raw* x = logits + row * stride;
+  const int t = threadIdx.x, row = blockIdx.x, ln = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint8_t* x = (const uint8_t*)logits + (int64_t)row * stride * (B / 8);
   const float T = set.t ? set.t[row] : set.t0, p = set.p ? set.p[row] : set.p0, mp = set.m ? set.m[row] : set.m0;
   const int k = set.k ? set.k[row] : set.k0;
 
-  uint32_t best = 0;
-  for (int i = t; i < V; i += kThreads) best = max(best, key_of<FMT>(x[i]));
+  // the row as 16-byte pieces; `skip` elements of the first lie before it
+  const int skip = (int)((uintptr_t)x % 16) / (B / 8);
+  const uint4* pieces = reinterpret_cast<const uint4*>(x - skip * (B / 8));
+  const int np = (V + skip + E - 1) / E;
+  // pieces inside..outside - 1 lie in the row as a whole
+  const int inside = skip ? 1 : 0, outside = (V + skip) / E;
+  const uint4 none = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);  // NaNs, which count as -inf
+  auto load_edge = [&](int c) {  // the elements that there are
+    uint4 r = none;
+    const int i = c * E - skip;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if ((uint32_t)(i + e) < (uint32_t)V) {
+        if (FMT == AQ_F32)
+          (&r.x)[e] = reinterpret_cast<const uint32_t*>(x)[i + e];
+        else
+          reinterpret_cast<uint16_t*>(&r)[e] = reinterpret_cast<const uint16_t*>(x)[i + e];
+      }
+    return r;
+  };
+  auto piece = [&](int c) { return c >= inside && c < outside ? pieces[c] : c < np ? load_edge(c) : none; };
+  // the pieces that reach over the row's ends, in the threads that have them
+  uint4 head = none, tail = none;
+  if (skip && t == 0) head = load_edge(0);
+  if (outside < np && t == (np - 1) % kThreads) tail = load_edge(np - 1);
+  auto load = [&](int c) {
+    uint4 v = inside < outside ? pieces[min(max(c, inside), outside - 1)] : none;
+    if (c >= outside) v = c == np - 1 ? tail : none;
+    if (c < inside) v = head;
+    return v;
+  };
+  // f(piece, its 16 bytes) for every piece of the row, in order within a thread;
+  // the next one's load is on its way meanwhile.  The whole workgroup calls f
+  // together, for pieces past the end too.
+  auto each_piece = [&](auto f) {
+    uint4 next = load(t);
+#pragma unroll 1
+    for (int c = t; c - t < np; c += kThreads) {
+      const uint4 v = next;
+      next = load(c + kThreads);
+      f(c, v);
+    }
+  };
+  // the same in fours, for little work
+  auto each_four = [&](auto f) {
+#pragma unroll 1
+    for (int c = t; c - t < np; c += 4 * kThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int n = 0; n < 4; n++) v[n] = load(c + n * kThreads);
+#pragma unroll
+      for (int n = 0; n < 4; n++) f(c + n * kThreads, v[n]);
+    }
+  };
+  // f(index, bits, key) for the piece's elements
+  auto each_element = [&](int c, uint4 v, auto f) {
+    const int i0 = c * E - skip;
+#pragma unroll 1
+    for (int i = i0; i < i0 + E; i += E / 4) {
+      const uint32_t q = keys_of_word<FMT>(v.x);
+      f(i, FMT == AQ_F32 ? v.x : v.x & 0xFFFF, FMT == AQ_F32 ? q : q & 0xFFFF);
+      if (FMT != AQ_F32) f(i + 1, v.x >> 16, q >> 16);
+      v.x = v.y, v.y = v.z, v.z = v.w;
+    }
+  };
+  auto keys_of = [&](const uint4& v) {
+    return make_uint4(keys_of_word<FMT>(v.x), keys_of_word<FMT>(v.y), keys_of_word<FMT>(v.z), keys_of_word<FMT>(v.w));
+  };
+
+  // ---- the largest key, each thread's own on the way
+  if (t < 64) s.table[t] = exp2((double)t / 64.0);
+  if (t == 0) {
+    s.n_list = 0;
+    s.token = 0;
+  }
+  for (int i = t; i < kMaxSegments; i += kThreads) {
+    s.seg_mass[i] = 0;
+    s.seg_ties[i] = 0;
+  }
+  uint32_t own;
+  {
+    uint32_t acc = 0;
+    each_four([&](int, const uint4& v) {
+      const uint4 q = keys_of(v);
+      if constexpr (FMT == AQ_F32) {
+        acc = max(max(max(acc, q.x), q.y), max(q.z, q.w));
+      } else {
+        u16x2 a = __builtin_bit_cast(u16x2, acc);
+        a = __builtin_elementwise_max(a, __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.x), __builtin_bit_cast(u16x2, q.y)));
+        a = __builtin_elementwise_max(a, __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
+        acc = __builtin_bit_cast(uint32_t, a);
+      }
+    });
+    own = FMT == AQ_F32 ? acc : max(acc & 0xFFFF, acc >> 16);
+  }
+  uint32_t best = own;
 #pragma unroll
   for (int d = 32; d; d >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, d, 64));
-  if ((t & 63) == 0) s.red[t >> 6] = best;
+  if (ln == 0) s.red[wave] = best;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWaves; i++) best = max(best, (uint32_t)s.red[i]);
-  const float mx = logit_of_key<FMT>(best);
-  const double c = 1.4426950408889634 / (double)T;
-
-  // descends the keys' bits, 11 at a time, to the key at which the running
-  // count (by_mass: the running mass) reaches `most`
-  auto descend = [&](bool by_mass, uint64_t most, uint32_t* above, uint64_t* above_mass, uint64_t* each,
-                     uint32_t* ties) -> uint32_t {
-    uint32_t prefix = 0, cnt = 0;
-    uint64_t mass = 0;
-    int shift = B;
-    uint32_t bin_count = 0;
-    uint64_t bin_mass = 0;
-    while (shift > 0) {
-      const int bits = min(11, shift), next = shift - bits;
-      __syncthreads();
-      for (int i = t; i < kBins; i += kThreads) {
-        s.mass[i] = 0;
-        s.count[i] = 0;
-      }
-      __syncthreads();
-      for (int i = t; i < V; i += kThreads) {
-        const uint32_t key = key_of<FMT>(x[i]);
-        if (shift < 32 && shift < B && (key >> shift) != prefix) continue;
-        const uint32_t bin = (key >> next) & ((1u << bits) - 1);
-        atomicAdd(&s.count[bin], 1u);
-        const uint64_t w = fixed(weight(logit<FMT>(x[i]), mx, c));
-        if (w) atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)w);
-      }
-      __syncthreads();
-      uint32_t bin, bc;
-      uint64_t bm;
-      find_bin(s, by_mass, most - (by_mass ? mass : cnt), &bin, &bc, &bm);
-      cnt += bc;
-      mass += bm;
-      bin_count = s.count[bin];
-      bin_mass = s.mass[bin];
-      prefix = shift == B ? bin : (prefix << bits) | bin;
-      shift = next;
-      __syncthreads();
+  const float mx = L::value_of_key(best);
+  // 64 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
+  // the maximum would) and every number nothing
+  const bool endless = mx == INFINITY;
+  const Weigh weigh = {endless ? 1e39 : (double)mx, endless ? 1.0 : 92.33248261893425 / (double)T, s.table};
+  const bool greedy = !(T > 0.0f) || mx == -INFINITY;  // also a row without a token to choose: its first
+  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) : 0.0;
+  if (greedy) {
+    if (t == 0) s.token = 0xFFFFFFFFu;
+    __syncthreads();
+    if (own == best) {  // few threads
+      uint32_t i0 = 0xFFFFFFFFu;
+#pragma unroll 1
+      for (int c = t; c < np && i0 == 0xFFFFFFFFu; c += kThreads)
+        each_element(c, load(c), [&](int i, uint32_t, uint32_t key) {
+          if (key == best && (uint32_t)i < (uint32_t)V) i0 = min(i0, (uint32_t)i);
+        });
+      atomicMin(&s.token, i0);
     }
-    *above = cnt;
-    *above_mass = mass;
-    *ties = bin_count;
-    *each = bin_mass / bin_count;
-    return prefix;
+    __syncthreads();
+    if (t == 0) out[row] = s.token;
+    return;
+  }
+
+  auto clear_bins = [&] {
+    __syncthreads();
+    for (int i = t; i < kBins; i += kThreads) {
+      s.mass[i] = 0;
+      s.count[i] = 0;
+    }
+    __syncthreads();
+  };
+  auto append = [&](int i, uint32_t key) {
+    if ((uint32_t)i >= (uint32_t)V) return;
+    const uint32_t at = atomicAdd(&s.n_list, 1u);
+    if (at < kList) s.list[at] = make_uint2(key, (uint32_t)i);
   };
 
-  Cut cut = {0, (uint32_t)V};  // everything
-  const bool greedy = !(T > 0.0f) || mx == -INFINITY;  // also a row without a token to choose: its first
-  if (greedy) {
-    cut = {best, 1};
-  } else {
-    uint32_t above, ties;
-    uint64_t above_mass, each, mass = 0;
-    bool have_mass = false;
-    if (k > 0 && k < V) {
-      const uint32_t key = descend(false, (uint64_t)k, &above, &above_mass, &each, &ties);
-      cut = {key, (uint32_t)k - above};
-      mass = above_mass + cut.ties * each;
-      have_mass = true;
-    }
-    if (p < 1.0f) {
-      if (!have_mass) {
-        uint64_t part = 0;
-        for (int i = t; i < V; i += kThreads) part += fixed(weight(logit<FMT>(x[i]), mx, c));
-        block_scan_u64(part, s.red, &mass);
+  // One exact pass: masses of keys above `hi` by segment (of w >= wmin).  LISTING:
+  // keys from `lo` to `hi` go to the list, and the whole row's mass to s.total; else
+  // the keys equal to hi are counted by segment.  Returns the mass above hi,
+  // whatever its w.
+  auto exact_pass = [&](auto listing, uint32_t lo, uint32_t hi) -> uint64_t {
+    constexpr bool LISTING = decltype(listing)::value;
+    double all = 0.0, top = 0.0;
+    each_piece([&](int c, const uint4& v) {
+      double sum = 0.0;
+      uint32_t ties = 0;
+      each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
+        if (LISTING || __ballot(key > hi)) {  // the exponential only where a lane asks for it
+          const double w = weigh(L::value(bits)), n = rint(w * kOne), j = key > hi ? n : 0.0;
+          all += n;
+          top += j;
+          sum += w >= wmin ? j : 0.0;
+        }
+        if (LISTING) {
+          if (key >= lo && key <= hi) append(i, key);
+        } else {
+          ties += (uint32_t)__popcll(__ballot(key == hi && (uint32_t)i < (uint32_t)V));
+        }
+      });
+      sum = wave_group_sum_f64<64>(sum);
+      if (ln == 0) {  // 64 pieces are a segment
+        s.seg_mass[c >> 6] = (uint64_t)sum;
+        s.seg_ties[c >> 6] = ties;
       }
-      // a token stays while less than this lies before it; the first one always
-      const uint64_t most = min(mass, (uint64_t)fmax(ceil((double)p * (double)mass), 1.0));
-      const uint32_t key = descend(true, most, &above, &above_mass, &each, &ties);
+    });
+    // 2^8 tokens of up to 2^42: each thread's sum is exact in 64-bit floating point
+    uint64_t a = 0, b;
+    if (LISTING) block_scan_u64((uint64_t)all, s.red, &a);
+    block_scan_u64((uint64_t)top, s.red, &b);
+    if (LISTING && t == 0) s.total = a;
+    __syncthreads();
+    return b;
+  };
+
+  Cut cut = {0, 0};  // everything
+  bool from_list = false, summed = false;
+  const bool by_k = k > 0 && k < V, by_p = p < 1.0f;
+  uint64_t mass = 0;
+  // the cut of the first k, then that of the mass p of these
+#pragma unroll 1
+  for (int stage = 0; stage < 2; stage++) {
+    const bool by_mass = stage == 1;
+    if (by_mass ? !by_p : !by_k) continue;
+    uint64_t most = (uint64_t)k, start = 0;
+    // a token stays while less than this lies before it; the first one always
+    auto reach = [&](uint64_t m) { return min(m, (uint64_t)fmax(ceil((double)p * (double)m), 1.0)); };
+    if (!by_mass) {
+      if (k <= kMaxListK) {
+        clear_bins();
+        atomicAdd(&s.count[own >> (B - 11)], 1u);
+        __syncthreads();
+        const uint32_t least = find_bin(s, false, (uint64_t)k).bin << (B - 11);
+        if (own >= least) {  // a thread whose largest is less has none
+#pragma unroll 1
+          for (int c = t; c < np; c += kThreads) {
+            const uint4 v = load(c), q = keys_of(v);
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+            bool any = false;
+#pragma unroll
+            for (int n = 0; n < 4; n++) any = any || (FMT == AQ_F32 ? w[n] : max(w[n] & 0xFFFF, w[n] >> 16)) >= least;
+            if (any)
+              each_element(c, v, [&](int i, uint32_t, uint32_t key) {
+                if (key >= least) append(i, key);
+              });
+          }
+        }
+        __syncthreads();
+        from_list = s.n_list <= kList;
+      }
+    } else if (by_k) {
+      most = reach(mass);
+    } else {
+      // the bracket: running masses of the row's bins, in f32
+      clear_bins();
+      float* f = reinterpret_cast<float*>(s.count);
+      const float cf = (float)(weigh.c / 64.0);
+      each_piece([&](int c, const uint4& v) {
+        each_element(c, v, [&](int, uint32_t bits, uint32_t key) {
+          const float w = __builtin_amdgcn_exp2f((L::value(bits) - mx) * cf);
+          if (w > 0x1p-60f) atomicAdd(&f[key >> (B - 11)], w);
+        });
+      });
+      __syncthreads();
+      const int bin0 = kBins - 1 - 2 * t, bin1 = bin0 - 1;
+      // as whole numbers, for the scan
+      const uint64_t g0 = (uint64_t)(f[bin0] * 1048576.0f), g1 = (uint64_t)(f[bin1] * 1048576.0f);
+      uint64_t tot;
+      const uint64_t inc = block_scan_u64(g0 + g1, s.red, &tot), exc = inc - g0 - g1;
+      const double slack = fmin(0.002, (1.0 - (double)p) / 2);  // f32 sums of up to 2^18 terms
+      const double lo_goal = fmax((double)p - slack, 0.0) * (double)tot, hi_goal = ((double)p + slack) * (double)tot;
+      if (t == 0) {
+        s.found_bin = kBins - 1;
+        s.found_count = 0;
+      }
+      __syncthreads();
+      auto mark = [&](int bin, double before, double after) {
+        if (before <= lo_goal && after > lo_goal) s.found_bin = bin;    // the first of the bracket
+        if (before < hi_goal && after >= hi_goal) s.found_count = bin;  // its last
+      };
+      mark(bin0, (double)exc, (double)(exc + g0));
+      mark(bin1, (double)(exc + g0), (double)inc);
+      __syncthreads();
+      const uint32_t hi = s.found_bin << (B - 11) | ((1u << (B - 11)) - 1), lo = s.found_count << (B - 11);
+      const uint64_t top = exact_pass(std::true_type{}, lo, hi);
+      most = reach(s.total);
+      uint64_t in_list = 0, part = 0;
+      const bool fits = s.n_list <= kList;
+      if (fits)
+        for (int i = t; i < (int)s.n_list; i += kThreads) part += (uint64_t)weigh.whole(L::value_of_key(s.list[i].x));
+      block_scan_u64(part, s.red, &in_list);
+      if (fits && top < most && most <= top + in_list) {
+        start = top;
+        summed = from_list = true;
+      }
+    }
+
+    // descend the keys' bits, 11 at a time, to the key at which the running
+    // count (by_mass: the running mass) reaches `most`, over the list or the row
+    uint32_t prefix = 0, above = 0;
+    uint64_t above_mass = start, each = 0;
+#pragma unroll 1
+    for (int shift = B; shift > 0;) {
+      const int bits = min(11, shift), next = shift - bits;
+      clear_bins();
+      const bool first = shift == B;
+      auto see = [&](uint32_t key) {
+        if (!first && key >> (shift & 31) != prefix) return;
+        const uint32_t bin = (key >> next) & ((1u << bits) - 1);
+        atomicAdd(&s.count[bin], 1u);
+        const uint64_t w = (uint64_t)weigh.whole(L::value_of_key(key));
+        if (w) atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)w);
+      };
+      if (from_list) {
+        const int n = (int)s.n_list;
+        for (int i = t; i < n; i += kThreads) see(s.list[i].x);
+      } else {
+        each_piece([&](int c, const uint4& v) { each_element(c, v, [&](int, uint32_t, uint32_t key) { see(key); }); });
+      }
+      __syncthreads();
+      const Found f = find_bin(s, by_mass, most - (by_mass ? above_mass : above));
+      above += f.count;
+      above_mass += f.mass;
+      prefix = first ? f.bin : prefix << bits | f.bin;
+      shift = next;
+      if (shift == 0) each = s.mass[f.bin] / s.count[f.bin];  // of one of the ties
+    }
+    if (!by_mass) {
+      cut = {prefix, (uint32_t)k - above};
+      mass = above_mass + cut.ties * each;
+    } else {
       const uint32_t n = (uint32_t)((most - above_mass + each - 1) / each);
-      if (key > cut.key)
-        cut = {key, n};
-      else if (key == cut.key)
+      if (prefix > cut.key)
+        cut = {prefix, n};
+      else if (prefix == cut.key)
         cut.ties = min(cut.ties, n);
     }
   }
-  const double wmin = !greedy && mp > 0.0f ? fmin((double)mp, 1.0) : 0.0;
-  auto kept = [&](uint32_t key, float f, uint64_t* w) {  // keys above the cut
-    const double e = weight(f, mx, c);
-    *w = fixed(e);
-    return key > cut.key && e >= wmin;
-  };
-  const float xcut = cut.key ? logit_of_key<FMT>(cut.key) : -INFINITY;
-  const double ecut = cut.key ? (greedy ? 1.0 : weight(xcut, mx, c)) : 0.0;
-  const uint64_t wcut = ecut >= wmin ? fixed(ecut) : 0;
 
-  // masses above the cut and ties at it, tile by tile
-  const int tiles = (V + kTile - 1) >> kTileShift;
+  // ---- kept masses and ties by segment
+  const double ecut = cut.key ? weigh(L::value_of_key(cut.key)) : 0.0;
+  const uint64_t wcut = ecut >= wmin ? (uint64_t)rint(ecut * kOne) : 0;
   __syncthreads();
-  if (t < kMaxTiles) {
-    s.tile_mass[t] = 0;
-    s.tile_ties[t] = 0;
-  }
-  if (t == 0) s.token = 0;
-  __syncthreads();
-  for (int tile = 0; tile < tiles; tile++) {
-    uint64_t sum = 0;
-    uint32_t eq = 0;
-    const int hi = min(V, (tile + 1) << kTileShift);
-    for (int i = (tile << kTileShift) + t; i < hi; i += kThreads) {
-      const uint32_t key = key_of<FMT>(x[i]);
-      uint64_t w;
-      if (key > cut.key && kept(key, logit<FMT>(x[i]), &w)) sum += w;
-      eq += key == cut.key;
+  if (from_list) {
+    for (int i = t; i < (int)s.n_list; i += kThreads) {
+      const uint2 y = s.list[i];
+      const int seg = ((int)y.y + skip) / (E * 64);
+      if (y.x == cut.key) {
+        atomicAdd(&s.seg_ties[seg], 1u);
+      } else if (y.x > cut.key) {
+        const double w = weigh(L::value_of_key(y.x));
+        if (w >= wmin) atomicAdd((unsigned long long*)&s.seg_mass[seg], (unsigned long long)rint(w * kOne));
+      }
     }
-    sum = wave_scan_u64(sum);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) eq += __shfl_xor((int)eq, d, 64);
-    if ((t & 63) == 63) {
-      if (sum) atomicAdd((unsigned long long*)&s.tile_mass[tile], (unsigned long long)sum);
-      if (eq) atomicAdd(&s.tile_ties[tile], eq);
-    }
+  } else if (!summed) {
+    exact_pass(std::false_type{}, 0, cut.key);
   }
   __syncthreads();
-  uint64_t total = 0;
-  uint32_t eq = 0;
-  for (int i = 0; i < tiles; i++) {
-    total += s.tile_mass[i] + wcut * (uint64_t)min(s.tile_ties[i], cut.ties - min(eq, cut.ties));
-    eq += s.tile_ties[i];
-  }
-  const float uu = u[row];
-  uint64_t goal = uu > 0.0f ? (uint64_t)fmin((double)uu * (double)total, 9.2e18) : 0;
-  if (goal >= total) goal = total - 1;
-  // the tile, then the thread (8 tokens in order each), then the token
-  uint64_t before = 0;
-  uint32_t eq_before = 0;
-  int tile = 0;
-  for (; tile < tiles - 1; tile++) {
-    const uint64_t m = s.tile_mass[tile] +
-                       wcut * (uint64_t)min(s.tile_ties[tile], cut.ties - min(eq_before, cut.ties));
-    if (before + m > goal) break;
-    before += m;
-    eq_before += s.tile_ties[tile];
-  }
-  const int i0 = (tile << kTileShift) + t * (kTile / kThreads), i1 = min(V, i0 + kTile / kThreads);
-  uint32_t mine = 0;
-  for (int i = i0; i < i1; i++) mine += key_of<FMT>(x[i]) == cut.key;
-  uint64_t all;
-  uint32_t rank = eq_before + (uint32_t)block_scan_u64(mine, s.red, &all) - mine;
-  uint64_t sum = 0;
+
+  // ---- the segment: thread t has segment t (and the few past 1024 thread 1023)
+  const int ns = (np + 63) / 64;
+  uint64_t total;
+  uint32_t tie0;
+  uint64_t m0;
   {
-    uint32_t r = rank;
-    for (int i = i0; i < i1; i++) {
-      const uint32_t key = key_of<FMT>(x[i]);
-      uint64_t w;
-      if (key == cut.key)
-        sum += r++ < cut.ties ? wcut : 0;
-      else if (key > cut.key && kept(key, logit<FMT>(x[i]), &w))
-        sum += w;
+    uint32_t ties = 0;
+    const int s0 = t, s1 = t == kThreads - 1 ? ns : min(ns, t + 1);
+    for (int i = s0; i < s1; i++) ties += s.seg_ties[i];
+    uint64_t all;
+    tie0 = (uint32_t)block_scan_u64(ties, s.red, &all) - ties;
+    uint64_t sum = 0;
+    uint32_t r = tie0;
+    for (int i = s0; i < s1; i++) {
+      sum += s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(r, cut.ties));
+      r += s.seg_ties[i];
     }
-  }
-  uint64_t at = before + block_scan_u64(sum, s.red, &all) - sum;
-  if (at <= goal && goal < at + sum) {
-    for (int i = i0; i < i1; i++) {
-      const uint32_t key = key_of<FMT>(x[i]);
-      uint64_t w = 0;
-      if (key == cut.key)
-        w = rank++ < cut.ties ? wcut : 0;
-      else if (!(key > cut.key && kept(key, logit<FMT>(x[i]), &w)))
-        w = 0;
-      if (at <= goal && goal < at + w) s.token = i;
-      at += w;
+    m0 = block_scan_u64(sum, s.red, &total) - sum;
+    const float uu = u[row];
+    uint64_t goal = uu > 0.0f ? (uint64_t)fmin((double)uu * (double)total, 9.2e18) : 0;
+    if (goal >= total) goal = total - 1;
+    if (m0 <= goal && goal < m0 + sum) {
+      uint64_t at = m0;
+      r = tie0;
+      for (int i = s0; i < s1; i++) {
+        const uint64_t m = s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(r, cut.ties));
+        if (at <= goal && goal < at + m) {
+          s.segment = i;
+          s.seg_before = goal - at;  // what is left of the goal inside
+          s.seg_rank = r;
+        }
+        at += m;
+        r += s.seg_ties[i];
+      }
     }
   }
   __syncthreads();
-  if (t == 0) out[row] = s.token;
+  // ---- the token: one wave, a piece a lane
+  if (wave == 0) {
+    const int c = (int)s.segment * 64 + ln;
+    const uint4 v = piece(c);
+    uint32_t ties = 0;
+    each_element(c, v, [&](int i, uint32_t, uint32_t key) { ties += key == cut.key && (uint32_t)i < (uint32_t)V; });
+    const uint32_t rank = s.seg_rank + (uint32_t)wave_scan_u64(ties) - ties;
+    auto mass_of = [&](int i, uint32_t bits, uint32_t key, uint32_t& r) -> uint64_t {
+      if ((uint32_t)i >= (uint32_t)V || key < cut.key) return 0;
+      if (key == cut.key) return r++ < cut.ties ? wcut : 0;
+      const double d = weigh(L::value(bits));
+      return d >= wmin ? (uint64_t)rint(d * kOne) : 0;
+    };
+    uint64_t sum = 0;
+    uint32_t r = rank;
+    each_element(c, v, [&](int i, uint32_t bits, uint32_t key) { sum += mass_of(i, bits, key, r); });
+    uint64_t at = wave_scan_u64(sum) - sum;
+    const uint64_t goal = s.seg_before;
+    r = rank;
+    if (at <= goal && goal < at + sum)
+      each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
+        const uint64_t w = mass_of(i, bits, key, r);
+        if (at <= goal && goal < at + w) out[row] = i;
+        at += w;
+      });
+  }
 }
 
 }  // namespace
@@ -374,12 +621,12 @@ extern "C" int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, in
   const Settings set = {temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0};
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)B), block(kThreads);
-  if (dtype == AQ_F16)
-    hipLaunchKernelGGL(sample_kernel<AQ_F16>, grid, block, 0, s, (const uint16_t*)logits, (int)V, stride, u, set, tokens);
-  else if (dtype == AQ_BF16)
-    hipLaunchKernelGGL(sample_kernel<AQ_BF16>, grid, block, 0, s, (const uint16_t*)logits, (int)V, stride, u, set, tokens);
-  else
-    hipLaunchKernelGGL(sample_kernel<AQ_F32>, grid, block, 0, s, (const uint32_t*)logits, (int)V, stride, u, set, tokens);
+#define AQ_SAMPLE(F) \
+  hipLaunchKernelGGL(sample_kernel<F>, grid, block, 0, s, logits, (int)V, stride, u, set, tokens)
+  if (dtype == AQ_F16) AQ_SAMPLE(AQ_F16);
+  else if (dtype == AQ_BF16) AQ_SAMPLE(AQ_BF16);
+  else AQ_SAMPLE(AQ_F32);
+#undef AQ_SAMPLE
   AQ_LAUNCH_CHECK("aq_sample");
   return AQ_OK;
 }

@@ -65,7 +65,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     if (logits.stride(1) != 1 and V > 1) or (logits.stride(0) < V and B > 1):
         logits = logits.contiguous()
     stride = max(logits.stride(0), V)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(_lib.load().aq_sample(logits.data_ptr(), _DTYPES[logits.dtype], B, V, stride, u.data_ptr(), tp, kp,
                                          pp, mp, t0, min(max(int(k0), 0), V), p0, m0, out.data_ptr(),
                                          _lib.stream_of(dev)), "aq_sample")

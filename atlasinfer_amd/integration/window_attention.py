@@ -51,7 +51,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         return out
     q, k, v = (_lib.strided_rows(t) for t in (q, k, v))
     arr = [_lib.ptr_array(t.stride()[:3], ctypes.c_int64) for t in (q, k, v)]
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(_lib.load().aq_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), B, H, Hkv, M, N, D, *arr,
                                                    window, int(sinks), D ** -0.5 if scale is None else scale,
                                                    _lib.ptr(starts), out.data_ptr(), _lib.stream_of(dev)),

@@ -33,21 +33,17 @@ GROUP = 32  # elements that share a scale and a minimum
 BLOCK = 32  # slots whose values are interleaved
 
 
-def _on(t: torch.Tensor):
-    """The tensor's device as the current one (kernels are launched there)."""
-    return torch.cuda.device(t.device)
-
-
-def _need(cond: bool, what: str) -> None:
-    if not cond:
-        raise ValueError(what)
+def _refuse(what: str):
+    raise ValueError(what)
 
 
 def kv4_buffers(batch: int, kv_heads: int, slots: int, head_dim: int, device) -> Tuple[torch.Tensor, ...]:
     """Empty buffers of a 4-bit cache: key codes, key parameters, value codes,
     value parameters (layouts at aq_kv4_store in include/atlasinfer_amd.h)."""
-    _need(head_dim in (64, 128), f"kv4: head size {head_dim} (64 and 128 supported)")
-    _need(batch > 0 and kv_heads > 0 and 0 < slots <= 1 << 24, "kv4: batch, heads and slots must be positive")
+    if head_dim not in (64, 128):
+        _refuse(f"kv4: head size {head_dim} (64 and 128 supported)")
+    if batch <= 0 or kv_heads <= 0 or not 0 < slots <= 1 << 24:
+        _refuse("kv4: batch, heads and slots must be positive, slots at most 2^24")
     c = (slots + BLOCK - 1) // BLOCK * BLOCK
     return (torch.zeros(batch, kv_heads, c, head_dim // 2, dtype=torch.uint8, device=device),
             torch.zeros(batch, kv_heads, c, head_dim // GROUP, 2, dtype=torch.float16, device=device),
@@ -55,28 +51,41 @@ def kv4_buffers(batch: int, kv_heads: int, slots: int, head_dim: int, device) ->
             torch.zeros(batch, kv_heads, c // BLOCK, head_dim // GROUP, 4, 4, 4, dtype=torch.float16, device=device))
 
 
+# The checks below run on every step of a decoding loop: no message is put
+# together unless it is raised, and shapes are compared as they are.
+
+
 def _kv4_sizes(cache, slots: Optional[int]):
-    """(B, Hkv, D, slots) of a 4-bit cache's buffers, which are checked."""
-    _need(len(cache) == 4, "kv4: a cache is four buffers (kv4_buffers)")
+    """(B, Hkv, D, slots, device) of a 4-bit cache's buffers, which are checked."""
+    if len(cache) != 4:
+        _refuse("kv4: a cache is four buffers (kv4_buffers)")
     kc, kp, vc, vp = cache
-    _need(kc.dim() == 4 and kc.shape[3] in (32, 64) and kc.shape[2] % BLOCK == 0, f"kv4: key codes {tuple(kc.shape)}")
-    B, Hkv, c, D = kc.shape[0], kc.shape[1], kc.shape[2], kc.shape[3] * 2
-    want = [((B, Hkv, c, D // 2), torch.uint8), ((B, Hkv, c, D // GROUP, 2), torch.float16),
-            ((B, Hkv, c // BLOCK, D * 16), torch.uint8), ((B, Hkv, c // BLOCK, D // GROUP, 4, 4, 4), torch.float16)]
-    for t, (shape, dtype) in zip(cache, want):
-        _need(t.device.type == "cuda", "kv4: the cache must be on a HIP device")
-        _need(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous() and t.device == kc.device,
-              f"kv4: a buffer {tuple(t.shape)} {t.dtype}, expected contiguous {shape} {dtype}")
-    slots = c if slots is None else int(slots)
-    _need(c - BLOCK < slots <= c, f"kv4: {slots} slots in buffers of {c}")
-    return B, Hkv, D, slots
+    dev = kc.device
+    if kc.dim() != 4 or dev.type != "cuda":
+        _refuse(f"kv4: key codes {tuple(kc.shape)} on {dev}")
+    B, Hkv, c, half = kc.shape
+    if half not in (32, 64) or c % BLOCK or 0 in (B, Hkv, c):
+        _refuse(f"kv4: key codes {tuple(kc.shape)}")
+    n, g = c // BLOCK, half // 16
+    if not (kp.shape == (B, Hkv, c, g, 2) and vc.shape == (B, Hkv, n, 32 * half) and vp.shape == (B, Hkv, n, g, 4, 4, 4)
+            and kc.dtype == vc.dtype == torch.uint8 and kp.dtype == vp.dtype == torch.float16
+            and kc.is_contiguous() and kp.is_contiguous() and vc.is_contiguous() and vp.is_contiguous()
+            and kp.device == dev and vc.device == dev and vp.device == dev):
+        _refuse(f"kv4: buffers {[(tuple(t.shape), t.dtype, t.device) for t in cache]} are not those of kv4_buffers, "
+                "contiguous and on one device")
+    if slots is None:
+        slots = c
+    elif not c - BLOCK < slots <= c:
+        _refuse(f"kv4: {slots} slots in buffers of {c}")
+    return B, Hkv, 2 * half, slots, dev
 
 
 def _sinks(sinks: Optional[int], slots: int) -> int:
     if sinks is None:
         return -1
-    _need(0 <= sinks < slots, f"{sinks} sinks in {slots} slots")
-    return int(sinks)
+    if not 0 <= sinks < slots:
+        _refuse(f"{sinks} sinks in {slots} slots")
+    return sinks
 
 
 def _strides(t: torch.Tensor):
@@ -89,82 +98,83 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, cache, start: int = 0, lengths: 
     strides) into a 4-bit cache; of sequence b only the first ``lengths[b]``
     (int64 [B]).  ``sinks``: the cache is a window (None: it is not, and the
     positions must fit)."""
-    B, Hkv, D, slots = _kv4_sizes(cache, slots)
-    _need(k.dim() == 4 and k.shape == v.shape and k.shape[:2] == (B, Hkv) and k.shape[3] == D,
-          f"kv4_store: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
-    dev = cache[0].device
-    for t in (k, v):
-        _need(t.dtype == torch.float16 and t.device == dev, f"kv4_store: k and v must be fp16 on {dev}")
-    if lengths is not None:
-        _need(lengths.dtype == torch.int64 and lengths.shape == (B,) and lengths.is_contiguous() and lengths.device == dev,
-              f"kv4_store: lengths must be int64 [{B}] on {dev}")
-    S = k.shape[2]
-    _need(start >= 0 and (sinks is not None or start + S <= slots),
-          f"kv4_store: positions {start} .. {start + S - 1} in {slots} slots")
+    B, Hkv, D, slots, dev = _kv4_sizes(cache, slots)
+    S = k.shape[2] if k.dim() == 4 else -1
+    if k.shape != (B, Hkv, S, D) or v.shape != k.shape:
+        _refuse(f"kv4_store: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
+    if not (k.dtype == v.dtype == torch.float16 and k.device == dev and v.device == dev):
+        _refuse(f"kv4_store: k and v must be fp16 on {dev}")
+    if lengths is not None and not (lengths.dtype == torch.int64 and lengths.shape == (B,) and lengths.is_contiguous()
+                                    and lengths.device == dev):
+        _refuse(f"kv4_store: lengths must be int64 [{B}] on {dev}")
+    if start < 0 or (sinks is None and start + S > slots):
+        _refuse(f"kv4_store: positions {start} .. {start + S - 1} in {slots} slots")
     sk = _sinks(sinks, slots)
     if S == 0:
         return
     k, v = _lib.strided_rows(k), _lib.strided_rows(v)
-    with _on(k):
-        _lib.check(_lib.load().aq_kv4_store(k.data_ptr(), v.data_ptr(), B, Hkv, S, D, _strides(k), _strides(v),
-                                            int(start), _lib.ptr(lengths), *[t.data_ptr() for t in cache], slots, sk,
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().aq_kv4_store(k.data_ptr(), v.data_ptr(), B, Hkv, S, D, _strides(k), _strides(v), start,
+                                            _lib.ptr(lengths), *[t.data_ptr() for t in cache], slots, sk,
                                             _lib.stream_of(dev)), "aq_kv4_store")
 
 
 def kv4_load(cache, count: Optional[int] = None, slots: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first ``count`` slots (all of them) of a 4-bit cache in fp16: keys
     and values [B, Hkv, count, D]."""
-    B, Hkv, D, slots = _kv4_sizes(cache, slots)
-    count = slots if count is None else int(count)
-    _need(0 <= count <= slots, f"kv4_load: {count} of {slots} slots")
-    dev = cache[0].device
-    k, v = (torch.empty(B, Hkv, count, D, dtype=torch.float16, device=dev) for _ in range(2))
+    B, Hkv, D, slots, dev = _kv4_sizes(cache, slots)
+    if count is None:
+        count = slots
+    elif not 0 <= count <= slots:
+        _refuse(f"kv4_load: {count} of {slots} slots")
+    k = torch.empty(B, Hkv, count, D, dtype=torch.float16, device=dev)
+    v = torch.empty_like(k)
     if count:
-        with _on(k):
+        with _lib.on_device(dev):
             _lib.check(_lib.load().aq_kv4_load(*[t.data_ptr() for t in cache], B, Hkv, D, slots, count, k.data_ptr(),
                                                v.data_ptr(), _lib.stream_of(dev)), "aq_kv4_load")
     return k, v
 
 
-def _step_arguments(what, q, k_new, v_new, pos, rope, B, Hkv, D, dev):
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _step_arguments(what, q, k_new, v_new, pos, rope, out, workspace, B, Hkv, D, dev):
     """Checks of a step's tensors; (q, k_new, v_new contiguous, H, pos_stride,
-    cos, sin, rows of the rotary tables)."""
-    _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == D and q.shape[1] > 0 and q.shape[1] % Hkv == 0,
-          f"{what}: q {tuple(q.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
-    _need(tuple(k_new.shape) == (B, Hkv, D) and tuple(v_new.shape) == (B, Hkv, D),
-          f"{what}: k_new {tuple(k_new.shape)}, v_new {tuple(v_new.shape)}, expected {(B, Hkv, D)}")
-    for t in (q, k_new, v_new):
-        _need(t.dtype == torch.float16 and t.device == dev, f"{what}: q, k_new and v_new must be fp16 on {dev}")
-    _need(pos.dtype == torch.int64 and pos.device == dev and pos.dim() == 1 and pos.shape[0] in (1, B)
-          and pos.is_contiguous(), f"{what}: pos must be int64 [1] or [{B}] on {dev}")
+    addresses of the rotary tables, their rows, out)."""
+    H = q.shape[1] if q.dim() == 3 else 0
+    if H == 0 or q.shape != (B, H, D) or H % Hkv:
+        _refuse(f"{what}: q {tuple(q.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
+    if k_new.shape != (B, Hkv, D) or v_new.shape != (B, Hkv, D):
+        _refuse(f"{what}: k_new {tuple(k_new.shape)}, v_new {tuple(v_new.shape)}, expected {(B, Hkv, D)}")
+    if not (q.dtype == k_new.dtype == v_new.dtype == torch.float16 and q.device == dev and k_new.device == dev
+            and v_new.device == dev):
+        _refuse(f"{what}: q, k_new and v_new must be fp16 on {dev}")
+    n = pos.numel()
+    if not (pos.dtype == torch.int64 and pos.dim() == 1 and (n == B or n == 1) and pos.is_contiguous()
+            and pos.device == dev):
+        _refuse(f"{what}: pos must be int64 [1] or [{B}] on {dev}")
     cos = sin = None
     rows = 0
     if rope is not None:
         cos, sin = rope
         rows = cos.shape[0]
-        for t in (cos, sin):
-            _need(t.dtype == torch.float16 and t.device == dev and t.is_contiguous() and tuple(t.shape) == (rows, D)
-                  and rows > 0, f"{what}: rotary tables must be contiguous fp16 [positions, {D}] on {dev}")
-    q, k_new, v_new = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-                       for t in (q, k_new, v_new))
-    return q, k_new, v_new, q.shape[1], int(pos.shape[0] > 1), cos, sin, rows
-
-
-def _workspace(what, size: int, workspace: Optional[torch.Tensor], dev) -> torch.Tensor:
-    _need(size >= 0, f"{what}: sizes out of range")
-    if workspace is None:
-        return torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
-    _need(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev
-          and workspace.numel() >= size, f"{what}: the workspace must be uint8 of at least {size} bytes on {dev}")
-    return workspace
-
-
-def _result(what, out, q, dev):
+        if not (cos.shape == (rows, D) and sin.shape == (rows, D) and rows and cos.dtype == sin.dtype == torch.float16
+                and cos.is_contiguous() and sin.is_contiguous() and cos.device == dev and sin.device == dev):
+            _refuse(f"{what}: rotary tables must be contiguous fp16 [positions, {D}] on {dev}")
+        cos, sin = cos.data_ptr(), sin.data_ptr()
+    if workspace is not None and not (workspace.dtype == torch.uint8 and workspace.is_contiguous()
+                                      and workspace.device == dev):
+        _refuse(f"{what}: the workspace must be contiguous uint8 on {dev}")
+    if out is not None and not (out.shape == q.shape and out.dtype == torch.float16 and out.is_contiguous()
+                                and out.device == dev and out.data_ptr() % 16 == 0):
+        _refuse(f"{what}: out must be contiguous fp16 {tuple(q.shape)} on {dev}")
     if out is None:
-        return torch.empty_like(q)
-    _need(out.shape == q.shape and out.dtype == torch.float16 and out.is_contiguous() and out.device == dev
-          and out.data_ptr() % 16 == 0, f"{what}: out must be contiguous fp16 {tuple(q.shape)} on {dev}")
-    return out
+        out = torch.empty((B, H, D), dtype=torch.float16, device=dev)
+    return _aligned(q), _aligned(k_new), _aligned(v_new), H, int(n > 1), cos, sin, rows, out
 
 
 def kv4_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cache, pos: torch.Tensor, *,
@@ -178,20 +188,25 @@ def kv4_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, cac
     ``q_scale`` multiplies q before that.  ``sinks``: the cache is a window.
     ``workspace`` (uint8, aq_kv4_attention_workspace bytes) and ``out``: given, or
     allocated."""
-    B, Hkv, D, slots = _kv4_sizes(cache, slots)
-    dev = cache[0].device
-    q, k_new, v_new, H, pos_stride, cos, sin, rows = _step_arguments("kv4_attention", q, k_new, v_new, pos, rope, B,
-                                                                     Hkv, D, dev)
+    B, Hkv, D, slots, dev = _kv4_sizes(cache, slots)
+    q, k_new, v_new, H, pos_stride, cos, sin, rows, out = _step_arguments("kv4_attention", q, k_new, v_new, pos, rope,
+                                                                          out, workspace, B, Hkv, D, dev)
+    sk = _sinks(sinks, slots)
     L = _lib.load()
-    size = int(L.aq_kv4_attention_workspace(B, H, Hkv, D, slots))
-    ws = _workspace("kv4_attention", size, workspace, dev)
-    out = _result("kv4_attention", out, q, dev)
-    with _on(q):
-        _lib.check(L.aq_kv4_attention(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), *[t.data_ptr() for t in cache],
-                                      pos.data_ptr(), pos_stride, B, H, Hkv, D, slots, _sinks(sinks, slots),
-                                      scale, q_scale, _lib.ptr(cos), _lib.ptr(sin), rows, ws.data_ptr(), ws.numel(),
-                                      out.data_ptr(), _lib.stream_of(dev)), "aq_kv4_attention")
+    if workspace is None:
+        size = L.aq_kv4_attention_workspace(B, H, Hkv, D, slots)
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    kc, kp, vc, vp = cache
+    with _lib.on_device(dev):
+        _lib.check(L.aq_kv4_attention(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), kc.data_ptr(), kp.data_ptr(),
+                                      vc.data_ptr(), vp.data_ptr(), pos.data_ptr(), pos_stride, B, H, Hkv, D, slots, sk,
+                                      scale, q_scale, cos, sin, rows, *_space(workspace), out.data_ptr(),
+                                      _lib.stream_of(dev)), "aq_kv4_attention")
     return out
+
+
+def _space(workspace):
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
 
 
 def window_decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor,
@@ -201,24 +216,26 @@ def window_decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.T
     """kv4_attention over an fp16 cache k_cache, v_cache [B, Hkv, slots, D]; H is
     1, 2, 4 or 8 times Hkv."""
     what = "window_decode_attention"
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[3] in (64, 128),
-          f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     dev = k_cache.device
-    _need(dev.type == "cuda", f"{what}: the cache must be on a HIP device")
-    for t in (k_cache, v_cache):
-        _need(t.dtype == torch.float16 and t.is_contiguous() and t.device == dev,
-              f"{what}: the caches must be contiguous fp16 on {dev}")
+    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == torch.float16
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and dev.type == "cuda" and v_cache.device == dev):
+        _refuse(f"{what}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} must be contiguous fp16 of one shape on "
+                "one HIP device")
     B, Hkv, slots, D = k_cache.shape
-    q, k_new, v_new, H, pos_stride, cos, sin, rows = _step_arguments(what, q, k_new, v_new, pos, rope, B, Hkv, D, dev)
+    if D not in (64, 128) or 0 in (B, Hkv, slots):
+        _refuse(f"{what}: caches {tuple(k_cache.shape)} (head sizes 64 and 128 supported)")
+    q, k_new, v_new, H, pos_stride, cos, sin, rows, out = _step_arguments(what, q, k_new, v_new, pos, rope, out,
+                                                                          workspace, B, Hkv, D, dev)
+    sk = _sinks(sinks, slots)
     L = _lib.load()
-    ws = _workspace(what, int(L.aq_decode_attention_workspace(B, H, Hkv, D, slots)), workspace, dev)
-    out = _result(what, out, q, dev)
-    with _on(q):
+    if workspace is None:
+        workspace = torch.empty(max(16, L.aq_decode_attention_workspace(B, H, Hkv, D, slots)), dtype=torch.uint8,
+                                device=dev)
+    with _lib.on_device(dev):
         _lib.check(L.aq_window_decode_attention(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(),
-                                                v_cache.data_ptr(), pos.data_ptr(), pos_stride, B, H, Hkv, D, slots,
-                                                _sinks(sinks, slots), scale, q_scale, _lib.ptr(cos), _lib.ptr(sin),
-                                                rows, ws.data_ptr(), ws.numel(), out.data_ptr(), _lib.stream_of(dev)),
-                   "aq_window_decode_attention")
+                                                v_cache.data_ptr(), pos.data_ptr(), pos_stride, B, H, Hkv, D, slots, sk,
+                                                scale, q_scale, cos, sin, rows, *_space(workspace), out.data_ptr(),
+                                                _lib.stream_of(dev)), "aq_window_decode_attention")
     return out
 
 
@@ -229,8 +246,8 @@ class DecodeCache:
 
     def __init__(self, batch: int, kv_heads: int, slots: int, head_dim: int, *, bits: int = 16,
                  sinks: Optional[int] = None, device="cuda"):
-        _need(bits in (4, 16), f"DecodeCache: {bits} bits (4 and 16 supported)")
-        _need(head_dim in (64, 128), f"DecodeCache: head size {head_dim} (64 and 128 supported)")
+        if bits not in (4, 16) or head_dim not in (64, 128):
+            _refuse(f"DecodeCache: {bits} bits (4 and 16 supported), head size {head_dim} (64 and 128 supported)")
         _sinks(sinks, slots)
         self.batch, self.kv_heads, self.slots, self.head_dim = batch, kv_heads, slots, head_dim
         self.bits, self.sinks = bits, sinks
@@ -257,8 +274,8 @@ class DecodeCache:
             kv4_store(k, v, self.buffers, start, lengths, self.slots, self.sinks)
             return
         S = k.shape[2]
-        _need(start >= 0 and (self.sinks is not None or start + S <= self.slots),
-              f"DecodeCache: positions {start} .. {start + S - 1} in {self.slots} slots")
+        if start < 0 or (self.sinks is None and start + S > self.slots):
+            _refuse(f"DecodeCache: positions {start} .. {start + S - 1} in {self.slots} slots")
         if S == 0:
             return
         # the newest position of each slot, by sequence when their lengths differ
