@@ -21,12 +21,13 @@
 //   top-k    (k <= 512) of the 1024 threads' own maxima the k-th largest is a
 //            key that at least k tokens reach; the tokens that do (k and a few,
 //            for logits in any order) go to a list in LDS
-//   top-p    a histogram of masses in f32 brackets the key where the running mass
-//            reaches p; one exact pass sums what lies above the bracket and lists
-//            what lies inside
-//   the cut  by descending the keys' bits over the list (11 at a time, counts and
-//            masses in LDS); where list or bracket do not serve (more ties than
-//            the list has room for, large k) over the whole row
+//   top-p    a histogram of masses over the keys' first 11 bits has the bin in
+//            which the running mass reaches p; the next pass sums what lies above
+//            it and lists what lies inside
+//   the cut  of a list of up to 256 by comparing its members with each other (four
+//            threads each); else by descending the keys' bits, 11 at a time, with
+//            histograms of counts and masses in LDS, over the list or, where it
+//            overflows (ties, large k), the row
 //   token    kept masses by segments of 1 KiB, summed in the exact pass or from
 //            the list; one wave goes through the segment that the number falls in
 //
@@ -44,6 +45,8 @@ constexpr int kBins = 2048;  // 11 bits
 constexpr int64_t kMaxVocab = 1 << 18;
 constexpr double kOne = 4398046511104.0;  // 2^42
 constexpr int kList = 4096;
+constexpr int kSmallList = kThreads / 4;
+constexpr int kTable = 512;
 constexpr int kMaxListK = 512;
 constexpr int kMaxSegments = 1024 + 16;  // 2^18 f32 and a misaligned start
 
@@ -96,25 +99,25 @@ __device__ __forceinline__ uint32_t keys_of_word(uint32_t w) {
   }
 }
 
-// w = 2^(n / 64) 2^(r / 64), y = n + r, from a table of 2^(j / 64) and a
-// polynomial of degree 4 (|r| <= 1/2: relative error 4e-14).  y: 64 log2(e)
-// (x - max) / T; below -6400, and where it is not a number (x is not, or -inf at
-// T = inf), w is as good as 0.
-__device__ __forceinline__ double exp2_64th(double y, const double* table) {
-  y = fmin(fmax(y, -6400.0), 0.0);
-  const double n = rint(y), r = y - n;
-  constexpr double a = 0.010830424696249145;  // ln 2 / 64
-  constexpr double a2 = a * a / 2, a3 = a * a * a / 6, a4 = a * a * a * a / 24;
-  const double q = fma(r, fma(r, fma(r, fma(r, a4, a3), a2), a), 1.0);
-  const int i = (int)n;
-  return ldexp(table[i & 63] * q, i >> 6);
-}
-
+// exp((x - mx) / T) in units of 2^-42, rounded to a whole number: 2^(n / 512)
+// 2^(r / 512) with y = n + r, y = (x - mx) c, c = 512 log2(e) / T, from a table of
+// 2^(j / 512 + 42) and a polynomial of degree 3 (|r| <= 1/2: relative error 1e-14).
+// Adding 1.5 2^52 rounds y to n and leaves n in the low bits; its upper part goes to
+// the exponent; adding 2^52 rounds the result.  (rndne, cvt and ldexp in 64 bits
+// take four times as long as an addition.)  Where y is not a number (x is not, or
+// -inf at T = inf) or below -512 x 60, the result is 0.
 struct Weigh {
   double mx, c;
   const double* table;
-  __device__ __forceinline__ double operator()(float x) const { return exp2_64th(((double)x - mx) * c, table); }
-  __device__ __forceinline__ double whole(float x) const { return rint((*this)(x) * kOne); }
+  __device__ __forceinline__ double operator()(float x) const {
+    constexpr double a = 0.0013538030870311431, a2 = a * a / 2, a3 = a * a * a / 6;  // ln 2 / 512
+    const double y = fmin(fmax(((double)x - mx) * c, -30720.0), 0.0);
+    const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
+    const int n = (int)__builtin_bit_cast(uint64_t, t);
+    const double v = table[n & (kTable - 1)] * fma(r, fma(r, fma(r, a3, a2), a), 1.0);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v) + ((uint64_t)(uint32_t)((n >> 9) << 20) << 32);
+    return (__builtin_bit_cast(double, b) + 4503599627370496.0) - 4503599627370496.0;
+  }
 };
 
 template <int CTRL, int ROWS>
@@ -159,9 +162,11 @@ struct Shared {
   uint64_t seg_mass[kMaxSegments];
   uint32_t seg_ties[kMaxSegments];
   uint2 list[kList];  // (key, index)
-  double table[64];
+  double table[kTable];
+  uint64_t sorted_mass[kSmallList];
+  uint32_t sorted_index[kSmallList];
   uint64_t red[kWaves];
-  uint64_t found_mass, total;
+  uint64_t found_mass;
   uint32_t found_bin, found_count, n_list, segment, seg_rank, token;
   uint64_t seg_before;
 };
@@ -171,15 +176,22 @@ struct Found {
   uint64_t mass;
 };
 
+// A token stays while less than this of the mass m lies before it; the first one
+// always.
+__device__ __forceinline__ uint64_t reach(float p, uint64_t m) {
+  return min(m, (uint64_t)fmax(ceil((double)p * (double)m), 1.0));
+}
+
 // The bin, from the highest down, in which the running count (by_mass: the
-// running mass) reaches `most`, and what lies above it.  The caller knows that
-// one does.
-__device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t most) {
+// running mass) reaches `most` (0: that of the bins' whole mass and p), and what
+// lies above it.  The caller knows that one does.
+__device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& most, float p) {
   const int t = threadIdx.x;
   const int b0 = kBins - 1 - 2 * t, b1 = b0 - 1;  // this thread's
   const uint64_t m0 = s.mass[b0], m1 = s.mass[b1], c0 = s.count[b0], c1 = s.count[b1];
   uint64_t all;
   const uint64_t im = block_scan_u64(m0 + m1, s.red, &all), bm = im - m0 - m1;
+  if (most == 0) most = reach(p, all);
   const uint64_t ic = block_scan_u64(c0 + c1, s.red, &all), bc = ic - c0 - c1;
   // a bin is the one if what lies above it does not reach `most` and with it does
   auto take = [&](int bin, uint64_t mb, uint64_t cb, uint64_t m, uint64_t c) {
@@ -258,15 +270,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       f(c, v);
     }
   };
-  // the same in fours, for little work
-  auto each_four = [&](auto f) {
+  // the same eight at a time, for little work: f(n, piece, its 16 bytes)
+  auto each_eight = [&](auto f, auto after) {
 #pragma unroll 1
-    for (int c = t; c - t < np; c += 4 * kThreads) {
-      uint4 v[4];
+    for (int c = t; c - t < np; c += 8 * kThreads) {
+      uint4 v[8];
 #pragma unroll
-      for (int n = 0; n < 4; n++) v[n] = load(c + n * kThreads);
+      for (int n = 0; n < 8; n++) v[n] = load(c + n * kThreads);
 #pragma unroll
-      for (int n = 0; n < 4; n++) f(c + n * kThreads, v[n]);
+      for (int n = 0; n < 8; n++) f(n, v[n]);
+      after(c);
     }
   };
   // f(index, bits, key) for the piece's elements
@@ -285,7 +298,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   };
 
   // ---- the largest key, each thread's own on the way
-  if (t < 64) s.table[t] = exp2((double)t / 64.0);
   if (t == 0) {
     s.n_list = 0;
     s.token = 0;
@@ -297,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   uint32_t own;
   {
     uint32_t acc = 0;
-    each_four([&](int, const uint4& v) {
+    each_eight([&](int, const uint4& v) {
       const uint4 q = keys_of(v);
       if constexpr (FMT == AQ_F32) {
         acc = max(max(max(acc, q.x), q.y), max(q.z, q.w));
@@ -307,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         a = __builtin_elementwise_max(a, __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
         acc = __builtin_bit_cast(uint32_t, a);
       }
-    });
+    }, [](int) {});
     own = FMT == AQ_F32 ? acc : max(acc & 0xFFFF, acc >> 16);
   }
   uint32_t best = own;
@@ -318,12 +330,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 #pragma unroll
   for (int i = 0; i < kWaves; i++) best = max(best, (uint32_t)s.red[i]);
   const float mx = L::value_of_key(best);
-  // 64 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
+  // 512 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
   // the maximum would) and every number nothing
   const bool endless = mx == INFINITY;
-  const Weigh weigh = {endless ? 1e39 : (double)mx, endless ? 1.0 : 92.33248261893425 / (double)T, s.table};
+  const Weigh weigh = {endless ? 1e39 : (double)mx, endless ? 1.0 : 738.6598609514740 / (double)T, s.table};
   const bool greedy = !(T > 0.0f) || mx == -INFINITY;  // also a row without a token to choose: its first
-  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) : 0.0;
+  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) * kOne : 0.0;
   if (greedy) {
     if (t == 0) s.token = 0xFFFFFFFFu;
     __syncthreads();
@@ -340,6 +352,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     if (t == 0) out[row] = s.token;
     return;
   }
+  if (t < kTable) s.table[t] = exp2((double)t / kTable) * kOne;
 
   auto clear_bins = [&] {
     __syncthreads();
@@ -355,22 +368,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     if (at < kList) s.list[at] = make_uint2(key, (uint32_t)i);
   };
 
-  // One exact pass: masses of keys above `hi` by segment (of w >= wmin).  LISTING:
-  // keys from `lo` to `hi` go to the list, and the whole row's mass to s.total; else
-  // the keys equal to hi are counted by segment.  Returns the mass above hi,
-  // whatever its w.
-  auto exact_pass = [&](auto listing, uint32_t lo, uint32_t hi) -> uint64_t {
+  // Masses of keys above `hi` by segment (of w >= wmin).  LISTING: keys from `lo` to
+  // `hi` go to the list; else the keys equal to hi are counted by segment.
+  auto sum_segments = [&](auto listing, uint32_t lo, uint32_t hi) {
     constexpr bool LISTING = decltype(listing)::value;
-    double all = 0.0, top = 0.0;
     each_piece([&](int c, const uint4& v) {
       double sum = 0.0;
       uint32_t ties = 0;
       each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-        if (LISTING || __ballot(key > hi)) {  // the exponential only where a lane asks for it
-          const double w = weigh(L::value(bits)), n = rint(w * kOne), j = key > hi ? n : 0.0;
-          all += n;
-          top += j;
-          sum += w >= wmin ? j : 0.0;
+        if (__ballot(key > hi)) {  // the exponential only where a lane asks for it
+          const double w = weigh(L::value(bits));
+          sum += key > hi && w >= wmin ? w : 0.0;
         }
         if (LISTING) {
           if (key >= lo && key <= hi) append(i, key);
@@ -378,107 +386,121 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
           ties += (uint32_t)__popcll(__ballot(key == hi && (uint32_t)i < (uint32_t)V));
         }
       });
-      sum = wave_group_sum_f64<64>(sum);
+      sum = wave_group_sum_f64<64>(sum);  // 2^9 whole numbers of up to 2^42: exact
       if (ln == 0) {  // 64 pieces are a segment
         s.seg_mass[c >> 6] = (uint64_t)sum;
         s.seg_ties[c >> 6] = ties;
       }
     });
-    // 2^8 tokens of up to 2^42: each thread's sum is exact in 64-bit floating point
-    uint64_t a = 0, b;
-    if (LISTING) block_scan_u64((uint64_t)all, s.red, &a);
-    block_scan_u64((uint64_t)top, s.red, &b);
-    if (LISTING && t == 0) s.total = a;
     __syncthreads();
-    return b;
+  };
+
+  const bool by_k = k > 0 && k < V, by_p = p < 1.0f;
+  const float uu = u[row];
+  auto goal_of = [&](uint64_t total) {
+    const uint64_t g = uu > 0.0f ? (uint64_t)fmin((double)uu * (double)total, 9.2e18) : 0;
+    return min(g, total - 1);
+  };
+  // The whole rest for a list of at most 256 that holds the first k: four
+  // threads a member count what comes before it.
+  auto small_list = [&] {
+    const int n = (int)s.n_list, i = t >> 2;
+    const uint2 me = i < n ? s.list[i] : make_uint2(0, 0);
+    uint32_t r = 0;
+#pragma unroll 1
+    for (int j = t & 3; j < n; j += 4) {
+      const uint2 o = s.list[j];
+      r += o.x > me.x || (o.x == me.x && o.y < me.y);
+    }
+    r += xlane_partner_u32<1>(r);
+    r += xlane_partner_u32<2>(r);
+    const uint64_t w = i < n ? (uint64_t)weigh(L::value_of_key(me.x)) : 0;
+    if (i < n && (t & 3) == 0) {
+      s.sorted_mass[r] = w;
+      s.sorted_index[r] = me.y;
+    }
+    __syncthreads();
+    // every wave by itself: four of the sorted members a lane
+    uint64_t m[4], sum = 0;
+    int last = min(n, k);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      m[e] = 4 * ln + e < last ? s.sorted_mass[4 * ln + e] : 0;
+      sum += m[e];
+    }
+    uint64_t inc = wave_scan_u64(sum);
+    const uint64_t most = by_p ? reach(p, __shfl(inc, 63, 64)) : ~0ull;
+    uint64_t at = inc - sum;
+    int stay = 0;
+    sum = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const bool in = 4 * ln + e < last && at < most && (double)m[e] >= wmin;
+      at += m[e];
+      stay += in;
+      sum += in ? m[e] : 0;
+    }
+    last = __builtin_amdgcn_readlane(wave_incl_scan_i32<64>(stay), 63);
+    const uint64_t goal = goal_of(__shfl(wave_scan_u64(sum), 63, 64));
+    // the kept ones by index
+    uint64_t before = 0;
+#pragma unroll 1
+    for (int j = t & 3; j < last; j += 4)
+      if (s.sorted_index[j] < me.y) before += s.sorted_mass[j];
+    before += (uint64_t)__shfl_xor((long long)before, 1, 64);
+    before += (uint64_t)__shfl_xor((long long)before, 2, 64);
+    if ((t & 3) == 0 && i < n && (int)r < last && before <= goal && goal < before + w) out[row] = me.y;
   };
 
   Cut cut = {0, 0};  // everything
   bool from_list = false, summed = false;
-  const bool by_k = k > 0 && k < V, by_p = p < 1.0f;
   uint64_t mass = 0;
   // the cut of the first k, then that of the mass p of these
 #pragma unroll 1
   for (int stage = 0; stage < 2; stage++) {
     const bool by_mass = stage == 1;
     if (by_mass ? !by_p : !by_k) continue;
-    uint64_t most = (uint64_t)k, start = 0;
-    // a token stays while less than this lies before it; the first one always
-    auto reach = [&](uint64_t m) { return min(m, (uint64_t)fmax(ceil((double)p * (double)m), 1.0)); };
-    if (!by_mass) {
-      if (k <= kMaxListK) {
-        clear_bins();
-        atomicAdd(&s.count[own >> (B - 11)], 1u);
-        __syncthreads();
-        const uint32_t least = find_bin(s, false, (uint64_t)k).bin << (B - 11);
-        if (own >= least) {  // a thread whose largest is less has none
-#pragma unroll 1
-          for (int c = t; c < np; c += kThreads) {
-            const uint4 v = load(c), q = keys_of(v);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-            bool any = false;
-#pragma unroll
-            for (int n = 0; n < 4; n++) any = any || (FMT == AQ_F32 ? w[n] : max(w[n] & 0xFFFF, w[n] >> 16)) >= least;
-            if (any)
-              each_element(c, v, [&](int i, uint32_t, uint32_t key) {
-                if (key >= least) append(i, key);
-              });
-          }
-        }
-        __syncthreads();
-        from_list = s.n_list <= kList;
-      }
-    } else if (by_k) {
-      most = reach(mass);
-    } else {
-      // the bracket: running masses of the row's bins, in f32
+    uint64_t most = by_mass ? (by_k ? reach(p, mass) : 0) : (uint64_t)k;
+    if (!by_mass && k <= kMaxListK) {
       clear_bins();
-      float* f = reinterpret_cast<float*>(s.count);
-      const float cf = (float)(weigh.c / 64.0);
-      each_piece([&](int c, const uint4& v) {
-        each_element(c, v, [&](int, uint32_t bits, uint32_t key) {
-          const float w = __builtin_amdgcn_exp2f((L::value(bits) - mx) * cf);
-          if (w > 0x1p-60f) atomicAdd(&f[key >> (B - 11)], w);
-        });
-      });
+      atomicAdd(&s.count[own >> (B - 11)], 1u);
       __syncthreads();
-      const int bin0 = kBins - 1 - 2 * t, bin1 = bin0 - 1;
-      // as whole numbers, for the scan
-      const uint64_t g0 = (uint64_t)(f[bin0] * 1048576.0f), g1 = (uint64_t)(f[bin1] * 1048576.0f);
-      uint64_t tot;
-      const uint64_t inc = block_scan_u64(g0 + g1, s.red, &tot), exc = inc - g0 - g1;
-      const double slack = fmin(0.002, (1.0 - (double)p) / 2);  // f32 sums of up to 2^18 terms
-      const double lo_goal = fmax((double)p - slack, 0.0) * (double)tot, hi_goal = ((double)p + slack) * (double)tot;
-      if (t == 0) {
-        s.found_bin = kBins - 1;
-        s.found_count = 0;
+      const uint32_t least = find_bin(s, false, most, p).bin << (B - 11);
+      if (own >= least) {  // a thread whose largest is less has none
+        uint32_t which = 0;
+        each_eight([&](int n, const uint4& v) {
+          const uint4 q = keys_of(v);
+          uint32_t a;
+          if constexpr (FMT == AQ_F32) {
+            a = max(max(q.x, q.y), max(q.z, q.w));
+          } else {
+            const u16x2 m = __builtin_elementwise_max(
+                __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.x), __builtin_bit_cast(u16x2, q.y)),
+                __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
+            a = max(m.x, m.y);
+          }
+          which |= (a >= least ? 1u : 0u) << n;
+        }, [&](int c) {
+          for (; which; which &= which - 1) {
+            const int d = c + __builtin_ctz(which) * kThreads;
+            each_element(d, load(d), [&](int i, uint32_t, uint32_t key) {
+              if (key >= least) append(i, key);
+            });
+          }
+        });
       }
       __syncthreads();
-      auto mark = [&](int bin, double before, double after) {
-        if (before <= lo_goal && after > lo_goal) s.found_bin = bin;    // the first of the bracket
-        if (before < hi_goal && after >= hi_goal) s.found_count = bin;  // its last
-      };
-      mark(bin0, (double)exc, (double)(exc + g0));
-      mark(bin1, (double)(exc + g0), (double)inc);
-      __syncthreads();
-      const uint32_t hi = s.found_bin << (B - 11) | ((1u << (B - 11)) - 1), lo = s.found_count << (B - 11);
-      const uint64_t top = exact_pass(std::true_type{}, lo, hi);
-      most = reach(s.total);
-      uint64_t in_list = 0, part = 0;
-      const bool fits = s.n_list <= kList;
-      if (fits)
-        for (int i = t; i < (int)s.n_list; i += kThreads) part += (uint64_t)weigh.whole(L::value_of_key(s.list[i].x));
-      block_scan_u64(part, s.red, &in_list);
-      if (fits && top < most && most <= top + in_list) {
-        start = top;
-        summed = from_list = true;
+      from_list = s.n_list <= kList;
+      if (s.n_list <= kSmallList) {
+        small_list();
+        return;
       }
     }
 
     // descend the keys' bits, 11 at a time, to the key at which the running
     // count (by_mass: the running mass) reaches `most`, over the list or the row
     uint32_t prefix = 0, above = 0;
-    uint64_t above_mass = start, each = 0;
+    uint64_t above_mass = 0, each = 0;
 #pragma unroll 1
     for (int shift = B; shift > 0;) {
       const int bits = min(11, shift), next = shift - bits;
@@ -488,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         if (!first && key >> (shift & 31) != prefix) return;
         const uint32_t bin = (key >> next) & ((1u << bits) - 1);
         atomicAdd(&s.count[bin], 1u);
-        const uint64_t w = (uint64_t)weigh.whole(L::value_of_key(key));
+        const uint64_t w = (uint64_t)weigh(L::value_of_key(key));
         if (w) atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)w);
       };
       if (from_list) {
@@ -498,12 +520,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         each_piece([&](int c, const uint4& v) { each_element(c, v, [&](int, uint32_t, uint32_t key) { see(key); }); });
       }
       __syncthreads();
-      const Found f = find_bin(s, by_mass, most - (by_mass ? above_mass : above));
+      uint64_t left = most - (by_mass ? above_mass : above);
+      const Found f = find_bin(s, by_mass, left, p);
+      if (first) most = left;
       above += f.count;
       above_mass += f.mass;
       prefix = first ? f.bin : prefix << bits | f.bin;
       shift = next;
       if (shift == 0) each = s.mass[f.bin] / s.count[f.bin];  // of one of the ties
+      if (first && by_mass && !by_k) {
+        sum_segments(std::true_type{}, prefix << next, prefix << next | ((1u << next) - 1));
+        summed = from_list = s.n_list <= kList;
+      }
     }
     if (!by_mass) {
       cut = {prefix, (uint32_t)k - above};
@@ -519,7 +547,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 
   // ---- kept masses and ties by segment
   const double ecut = cut.key ? weigh(L::value_of_key(cut.key)) : 0.0;
-  const uint64_t wcut = ecut >= wmin ? (uint64_t)rint(ecut * kOne) : 0;
+  const uint64_t wcut = ecut >= wmin ? (uint64_t)ecut : 0;
   __syncthreads();
   if (from_list) {
     for (int i = t; i < (int)s.n_list; i += kThreads) {
@@ -529,11 +557,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         atomicAdd(&s.seg_ties[seg], 1u);
       } else if (y.x > cut.key) {
         const double w = weigh(L::value_of_key(y.x));
-        if (w >= wmin) atomicAdd((unsigned long long*)&s.seg_mass[seg], (unsigned long long)rint(w * kOne));
+        if (w >= wmin) atomicAdd((unsigned long long*)&s.seg_mass[seg], (unsigned long long)w);
       }
     }
   } else if (!summed) {
-    exact_pass(std::false_type{}, 0, cut.key);
+    sum_segments(std::false_type{}, 0, cut.key);
   }
   __syncthreads();
 
@@ -555,9 +583,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       r += s.seg_ties[i];
     }
     m0 = block_scan_u64(sum, s.red, &total) - sum;
-    const float uu = u[row];
-    uint64_t goal = uu > 0.0f ? (uint64_t)fmin((double)uu * (double)total, 9.2e18) : 0;
-    if (goal >= total) goal = total - 1;
+    const uint64_t goal = goal_of(total);
     if (m0 <= goal && goal < m0 + sum) {
       uint64_t at = m0;
       r = tie0;
@@ -585,7 +611,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       if ((uint32_t)i >= (uint32_t)V || key < cut.key) return 0;
       if (key == cut.key) return r++ < cut.ties ? wcut : 0;
       const double d = weigh(L::value(bits));
-      return d >= wmin ? (uint64_t)rint(d * kOne) : 0;
+      return d >= wmin ? (uint64_t)d : 0;
     };
     uint64_t sum = 0;
     uint32_t r = rank;

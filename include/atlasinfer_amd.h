@@ -513,7 +513,7 @@ int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* 
  * the running mass of the kept ones exceeds u[b] times their whole mass (u >= 1:
  * the last).  temperature <= 0, or a row without a logit above -inf: the largest
  * logit, the lowest index of equal ones.  NaN counts as -inf; logits of +inf
- * share the whole mass.  Masses are sums of w rounded to 2^-45.
+ * share the whole mass.  Masses are sums of w rounded to 2^-42.
  *   logits  dtype AQ_F16, AQ_BF16 or AQ_F32 [B, V], rows `stride` elements apart,
  *           V <= 262144
  *   u       f32 [B], in [0, 1)      tokens  int64 [B] (out)
