@@ -10,57 +10,97 @@ namespace {
 
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_s4;
 
 constexpr int kQ = 128;  // queries a workgroup, 32 a wave
 constexpr int kK = 64;   // keys a tile
+constexpr float kGrow = 8.0f;
 
 struct WindowArgs {
   const uint16_t *q, *k, *v;
   int64_t qs[3], ks[3], vs[3];
   const int* starts;
   uint16_t* out;
-  int H, G, M, N, window, sinks;
-  float scale2;
+  int H, G, M, N, window, sinks, blocks, items, per;
+  float c;  // |scale| log2(e)
+  uint32_t flip;  // sign bits of a negative scale, for the queries
 };
+
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// 16 bytes a lane from a buffer's byte `off` straight to LDS, at dst + 16 lane;
+// zeros past the buffer's end.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (void*)dst, 16, off, 0, 0, 0);
+}
+
+// Four rows of 16 fp16 numbers in LDS, 8 bytes given by each of 16 lanes in
+// order: lane i gets column i.
+__device__ __forceinline__ half4v read_turned(const uint8_t* p) {
+  return __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_u8*)p));
+}
 
 __device__ __forceinline__ bool not_finite8(uint4 x) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) bad = bad || (w[i] & 0x7C00u) == 0x7C00u || (w[i] & 0x7C000000u) == 0x7C000000u;
+  for (int i = 0; i < 4; i++) bad = bad | ((w[i] & 0x7C00u) == 0x7C00u) | ((w[i] & 0x7C000000u) == 0x7C000000u);
   return bad;
 }
 
-// Scores are taken transposed (keys as rows of mfma 32 x 32 x 16), so that a
-// lane has 16 scores of one query and its numerators are the second product's
-// operand as they are; the values lie transposed in LDS, the keys of each 16 in
-// the order in which a lane has them.
+// A tile's rows lie in LDS one after the other, 16-byte pieces permuted within
+// each so that the reads below meet every bank equally: piece c of key r at place
+// c ^ (r & 7) of a key row, pairs of pieces c / 2 at (c / 2) ^ (r & 3) of a value row.
 template <int D>
-__global__ __launch_bounds__(256) void window_attention_kernel(WindowArgs a) {
-  constexpr int KS = D + 8;       // LDS row of keys, in fp16
-  constexpr int VS = kK + 8;      // LDS row of one element of the values
-  constexpr int NC = D / 8;       // 16-byte pieces of a row
-  constexpr int KP = kK * NC / 256;  // pieces of keys a thread
-  __shared__ uint16_t kl[kK * KS];
-  __shared__ uint16_t vl[D * VS];
-  __shared__ int bad;
+__device__ __forceinline__ int k_place(int r, int c) { return r * (D * 2) + (c ^ (r & 7)) * 16; }
+template <int D>
+__device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) * 16; }
+
+// One workgroup: 128 queries of a head, 32 a wave; tiles of 64 keys and values
+// go straight from memory to LDS (direct loads, the next tile's on their way
+// during a tile; one barrier a tile).
+//   scores   transposed, s^T = k q^T (mfma 32 x 32 x 16): a lane has 32 scores of
+//            one query, another lane the other 32, so maxima and sums need one
+//            exchange
+//   softmax  p = e^(s - m) with m the maximum when it last moved: it moves only
+//            when a score passes it by 2^8 (p stays below 2^8, exact in range for
+//            fp16 and f32 alike), which spares scaling the sums nearly always
+//   values   o^T = v^T p^T: the numerators, rounded to fp16, are the operand as
+//            they are; the values come out of their rows transposed
+//            (ds_read_tr16_b64: four keys of 16 elements for 16 lanes)
+//   sums     of the rounded numerators (v_dot2), so that rounding them does not
+//            shift the mean
+// Bound by the matrix unit and the softmax's exponentials together.
+template <int D>
+__global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) {
+  constexpr int NC = D / 8;                    // 16-byte pieces of a row
+  constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
+  constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // two stages of keys, values
+  __shared__ int bad[2];
   const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int head = blockIdx.y, b = blockIdx.z, q0 = blockIdx.x * kQ;
+  // runs of neighbouring items to an XCD (they share keys and values in its L2)
+  const int item = (int)(blockIdx.x & 7) * a.per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= a.per || item >= a.items) return;
+  // heads of a group next to each other, late blocks (more keys) first
+  const int g = item % a.G, qb = a.blocks - 1 - item / a.G % a.blocks, u = item / a.G / a.blocks;
+  const int hkv = a.H / a.G, b = u / hkv, j = u % hkv, head = j * a.G + g, q0 = qb * kQ;
   const int off = a.N - a.M;
   const int start = a.starts ? max(0, a.starts[b]) : 0;
-  const uint16_t* kb = a.k + b * a.ks[0] + (head / a.G) * a.ks[1];
-  const uint16_t* vb = a.v + b * a.vs[0] + (head / a.G) * a.vs[1];
+  const uint16_t* kb = a.k + b * a.ks[0] + j * a.ks[1];
+  const uint16_t* vb = a.v + b * a.vs[0] + j * a.vs[1];
 
   // positions of the workgroup's queries, and the tiles with keys they see
   const int lo = off + q0, hi = off + min(q0 + kQ, a.M) - 1;
-  int64_t near64 = (int64_t)lo - a.window + 1;
-  const int near = (int)max(near64, (int64_t)start);
+  const int near = max(lo - a.window + 1, start);
   const int b0 = near / kK, b1 = hi >= start ? hi / kK : b0 - 1;
-  const int64_t sink_end = min((int64_t)start + a.sinks, (int64_t)hi + 1);  // sinks are start .. sink_end - 1
+  const int sink_end = (int)min((int64_t)start + a.sinks, (int64_t)hi + 1);  // sinks are start .. sink_end - 1
   const int a0 = start / kK;
-  const int na = sink_end > start ? max(0, min((int)((sink_end - 1) / kK) + 1, b0) - a0) : 0;
+  const int na = sink_end > start ? max(0, min((sink_end - 1) / kK + 1, b0) - a0) : 0;
   const int tiles = na + max(0, b1 - b0 + 1);
   auto tile_at = [&](int i) { return i < na ? a0 + i : b0 + i - na; };
 
@@ -69,7 +109,11 @@ __global__ __launch_bounds__(256) void window_attention_kernel(WindowArgs a) {
   {
     const uint16_t* qp = a.q + b * a.qs[0] + head * a.qs[1] + (int64_t)min(qi, a.M - 1) * a.qs[2] + 8 * h;
 #pragma unroll
-    for (int s = 0; s < D / 16; s++) qv[s] = *reinterpret_cast<const half8v*>(qp + 16 * s);
+    for (int s = 0; s < D / 16; s++) {
+      uint4 x = *reinterpret_cast<const uint4*>(qp + 16 * s);
+      x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
+      qv[s] = __builtin_bit_cast(half8v, x);
+    }
   }
   float16v o[D / 32];
 #pragma unroll
@@ -78,99 +122,115 @@ __global__ __launch_bounds__(256) void window_attention_kernel(WindowArgs a) {
     for (int i = 0; i < 16; i++) o[e][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
   const int wlo = off + q0 + wave * 32, whi = min(wlo + 31, a.N - 1);  // the wave's positions
+  const float grow = kGrow / a.c;
 
-  uint4 kr[KP], vr[4];
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  // values: a thread has four keys of one 16-byte piece (D = 64: half of them)
-  const int vq = t & 15, vd = t >> 4;
-  auto load = [&](int tile) {
-    const int k0 = tile * kK;
+  // this lane's part of the loads: piece n of the wave covers rows of the tile
+  int row[PN], ko[PN], vo[PN];
 #pragma unroll
-    for (int n = 0; n < KP; n++) {
-      const int i = n * 256 + t, r = k0 + i / NC;
-      kr[n] = r < a.N ? *reinterpret_cast<const uint4*>(kb + (int64_t)r * a.ks[2] + i % NC * 8) : zero;
-    }
+  for (int n = 0; n < PN; n++) {
+    row[n] = (wave * PN + n) * (64 / NC) + ln / NC;
+    const int pc = ln % NC;
+    ko[n] = row[n] * (int)a.ks[2] * 2 + (pc ^ (row[n] & 7)) * 16;
+    vo[n] = row[n] * (int)a.vs[2] * 2 + ((((pc >> 1) ^ (row[n] & 3)) << 1) | (pc & 1)) * 16;
+  }
+  auto load = [&](int i) {
+    const int k0 = tile_at(i) * kK;
+    uint8_t* st = lds + (i & 1) * (2 * TB) + wave * PN * 1024;
+    // rows past the last read as zeros, values before the start too, whatever is there
+    const int rows = min(a.N - k0, kK);
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(kb + (int64_t)k0 * a.ks[2]), (short)0, ((rows - 1) * (int)a.ks[2] + D) * 2, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(vb + (int64_t)k0 * a.vs[2]), (short)0, ((rows - 1) * (int)a.vs[2] + D) * 2, 0x00020000);
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
-      const int r = k0 + 4 * vq + n;  // keys before start or past the end count as zeros whatever is there
-      vr[n] = vd < NC && r < a.N && r >= start ? *reinterpret_cast<const uint4*>(vb + (int64_t)r * a.vs[2] + vd * 8) : zero;
+    for (int n = 0; n < PN; n++) load_to_lds(kr, st + n * 1024, ko[n]);
+    const int first = start - k0;
+    if (first > 0) {
+#pragma unroll
+      for (int n = 0; n < PN; n++)
+        load_to_lds(vr, st + TB + n * 1024, row[n] < first ? (int)0x80000000 : vo[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < PN; n++) load_to_lds(vr, st + TB + n * 1024, vo[n]);
     }
   };
-  if (t == 0) bad = 0;
-  if (tiles > 0) load(tile_at(0));
+  // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h (e & 3;
+  // e + 4 lies 128 bytes on); values of keys 4 h + r, 16 elements of 32 e (e & 1)
+  int kf[4], vf[2];
+#pragma unroll
+  for (int e = 0; e < 4; e++) kf[e] = k_place<D>(c, 2 * e + h);
+  const int r4 = (ln >> 2) & 3;
+#pragma unroll
+  for (int e = 0; e < 2; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
+
+  if (t < 2) bad[t] = 0;
+  if (tiles > 0) load(0);
   for (int i = 0; i < tiles; i++) {
     const int k0 = tile_at(i) * kK;
-    __syncthreads();  // the tile before has been read
-    if (t == 0) bad = 0;
-    __syncthreads();
+    const uint8_t* st = lds + (i & 1) * (2 * TB);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile is there
+    if (!(k0 + kK - 1 <= lo && k0 > hi - a.window && k0 >= start)) {
+      // a tile that the mask cuts for some query: whether its values are finite
+      bool x = false;
 #pragma unroll
-    for (int n = 0; n < KP; n++) {
-      const int x = n * 256 + t;
-      *reinterpret_cast<uint4*>(kl + x / NC * KS + x % NC * 8) = kr[n];
+      for (int n = 0; n < PN; n++) x = x | not_finite8(*reinterpret_cast<const uint4*>(st + TB + (wave * PN + n) * 1024 + ln * 16));
+      if (__ballot(x) && ln == 0) bad[i & 1] = i + 1;
     }
-    if (vd < NC) {
-      // key 16 s + 8 x + 4 y + z at place 16 s + 8 y + 4 x + z
-      const int place = (vq >> 2) * 16 + (vq & 1) * 8 + ((vq >> 1) & 1) * 4;
-      const uint16_t* r0 = reinterpret_cast<const uint16_t*>(vr);
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        uint2 w;
-        w.x = (uint32_t)r0[e] | (uint32_t)r0[8 + e] << 16;
-        w.y = (uint32_t)r0[16 + e] | (uint32_t)r0[24 + e] << 16;
-        *reinterpret_cast<uint2*>(vl + (vd * 8 + e) * VS + place) = w;
-      }
-      if (not_finite8(vr[0]) || not_finite8(vr[1]) || not_finite8(vr[2]) || not_finite8(vr[3])) bad = 1;
-    }
-    if (i + 1 < tiles) load(tile_at(i + 1));
-    __syncthreads();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's part; the tile before is done with
+    if (i + 1 < tiles) load(i + 1);
     // whether this wave's queries see none, all or some of the tile
-    const bool none = k0 > whi || (k0 + kK - 1 <= wlo - a.window && k0 >= sink_end) || k0 + kK <= start;
-    if (none) continue;
+    if (k0 > whi || (k0 + kK - 1 <= wlo - a.window && k0 >= sink_end) || k0 + kK <= start) continue;
     const bool all = k0 + kK - 1 <= wlo && k0 > whi - a.window && k0 >= start;
-    float x[32];
+    float16v x[2];
 #pragma unroll
     for (int s = 0; s < 2; s++) {
-      float16v acc;
 #pragma unroll
-      for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+      for (int e = 0; e < 16; e++) x[s][e] = 0.0f;
 #pragma unroll
       for (int e = 0; e < D / 16; e++) {
-        const half8v kf = *reinterpret_cast<const half8v*>(kl + (s * 32 + c) * KS + e * 16 + 8 * h);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qv[e], acc, 0, 0, 0);
+        const half8v f = *reinterpret_cast<const half8v*>(st + kf[e & 3] + (e >> 2) * 128 + s * 32 * (D * 2));
+        x[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qv[e], x[s], 0, 0, 0);
       }
-#pragma unroll
-      for (int e = 0; e < 16; e++) x[16 * s + e] = acc[e] * a.scale2;
     }
     if (!all) {
+      const int last = qpos - k0 - 4 * h, from = max(last - a.window + 1, start - k0 - 4 * h);
+      const int sink0 = start - k0 - 4 * h, sink1 = sink0 + a.sinks;
 #pragma unroll
-      for (int e = 0; e < 32; e++) {
-        const int key = k0 + 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * h + (e & 3);
-        const bool sees = key <= qpos && key >= start && (qpos - key < a.window || key - start < a.sinks);
-        x[e] = sees ? x[e] : -INFINITY;
-      }
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int key = 32 * s + 8 * (e >> 2) + (e & 3);
+          const bool sees = (key <= last) & ((key >= from) | ((key >= sink0) & (key < sink1)));
+          x[s][e] = sees ? x[s][e] : -INFINITY;
+        }
     }
-    float mx = x[0];
+    float mx = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
-    for (int e = 1; e < 32; e++) mx = fmaxf(mx, x[e]);
-    mx = fmaxf(m, xlane_level_max_f32<6>(mx));
-    if (__ballot(mx != m)) {
-      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+    for (int e = 1; e < 16; e++) mx = fmaxf(mx, fmaxf(x[0][e], x[1][e]));
+    mx = xlane_level_max_f32<6>(mx);
+    if (__ballot(mx > m + grow || (m == -INFINITY && mx > m))) {
+      const float n = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - n) * a.c);
       l *= f;
 #pragma unroll
       for (int e = 0; e < D / 32; e++) o[e] *= f;
-      m = mx;
+      m = n;
     }
-    const float base = m == -INFINITY ? 0.0f : m;
+    const float base = m == -INFINITY ? 0.0f : -m * a.c;
     half8v p[4];
+    const half2v one = {(f16)1.0f, (f16)1.0f};
 #pragma unroll
-    for (int e = 0; e < 32; e++) {
-      const float w = __builtin_amdgcn_exp2f(x[e] - base);
-      l += w;
-      p[e >> 3][e & 7] = rn_h(w);
+    for (int e = 0; e < 32; e += 2) {
+      half2v w;
+      w.x = rn_h(__builtin_amdgcn_exp2f(fmaf(x[e >> 4][e & 15], a.c, base)));
+      w.y = rn_h(__builtin_amdgcn_exp2f(fmaf(x[e >> 4][(e & 15) + 1], a.c, base)));
+      l = __builtin_amdgcn_fdot2(w, one, l, false);
+      p[e >> 3][e & 7] = w.x;
+      p[e >> 3][(e & 7) + 1] = w.y;
     }
-    if (!all && bad) {
+    if (!all && bad[i & 1] == i + 1) {
       // an infinity or NaN among the values of a tile that the mask cuts: the
       // terms one by one, leaving out those of weight zero
+#pragma unroll 1
       for (int key = 0; key < kK; key++) {
         const int s = key >> 4, y = (key >> 2) & 1, e8 = ((key >> 3) & 1) * 4 + (key & 3);
         f16 w = (f16)0.0f;
@@ -180,13 +240,13 @@ __global__ __launch_bounds__(256) void window_attention_kernel(WindowArgs a) {
           for (int e = 0; e < 8; e++)
             if (n == s && e == e8) w = p[n][e];
         const float wf = __shfl((float)w, c + 32 * y, 64);
-        const uint16_t* vp = vl + s * 16 + y * 8 + e8;
 #pragma unroll
         for (int e = 0; e < D / 32; e++)
 #pragma unroll
           for (int n = 0; n < 16; n++) {
             const int d = 32 * e + 8 * (n >> 2) + 4 * h + (n & 3);
-            if (wf != 0.0f) o[e][n] = fmaf(wf, (float)bits_to_h(vp[d * VS]), o[e][n]);
+            const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + TB + v_place<D>(key, d >> 3) + (d & 7) * 2);
+            if (wf != 0.0f) o[e][n] = fmaf(wf, (float)bits_to_h(vd), o[e][n]);
           }
       }
       continue;
@@ -195,8 +255,10 @@ __global__ __launch_bounds__(256) void window_attention_kernel(WindowArgs a) {
     for (int s = 0; s < 4; s++)
 #pragma unroll
       for (int e = 0; e < D / 32; e++) {
-        const half8v vf = *reinterpret_cast<const half8v*>(vl + (e * 32 + c) * VS + s * 16 + 8 * h);
-        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[s], o[e], 0, 0, 0);
+        // keys 16 s + 4 h + 0 .. 3, then 8 on: the order in which a lane has the numerators
+        const uint8_t* f = st + TB + vf[e & 1] + (e >> 1) * 128 + s * 16 * (D * 2);
+        const half8v w = __builtin_shufflevector(read_turned(f), read_turned(f + 8 * (D * 2)), 0, 1, 2, 3, 4, 5, 6, 7);
+        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p[s], o[e], 0, 0, 0);
       }
   }
   l = xlane_level_sum_f32<6>(l);
@@ -234,6 +296,8 @@ extern "C" int aq_window_attention(const void* q, const void* k, const void* v, 
   for (int i = 0; i < 3; i++)
     AQ_CHECK_ARG(q_strides[i] % 8 == 0 && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0,
                  "aq_window_attention: strides must be multiples of 8");
+  AQ_CHECK_ARG(k_strides[2] >= 0 && v_strides[2] >= 0 && k_strides[2] <= (1 << 23) && v_strides[2] <= (1 << 23),
+               "aq_window_attention: positions of k and v more than 2^23 elements apart");
   AQ_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)out % 16 == 0 &&
                    (uintptr_t)starts % 4 == 0,
                "aq_window_attention: q, k, v and out must be 16-byte aligned");
@@ -254,8 +318,14 @@ extern "C" int aq_window_attention(const void* q, const void* k, const void* v, 
   a.N = (int)N;
   a.window = (int)std::min<int64_t>(window, N);
   a.sinks = (int)std::min<int64_t>(sinks, N);
-  a.scale2 = scale * 1.44269504f;
-  const dim3 grid((unsigned)aq::ceil_div(M, kQ), (unsigned)H, (unsigned)B);
+  a.c = fabsf(scale) * 1.44269504f;
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.blocks = (int)aq::ceil_div(M, kQ);
+  const int64_t items = B * H * a.blocks;
+  AQ_CHECK_ARG(items <= (1 << 30), "aq_window_attention: %lld blocks of queries", (long long)items);
+  a.items = (int)items;
+  a.per = (int)aq::ceil_div(items, 8);
+  const dim3 grid((unsigned)(8 * a.per));
   if (D == 64)
     hipLaunchKernelGGL((window_attention_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, a);
   else
