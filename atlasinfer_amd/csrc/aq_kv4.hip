@@ -216,8 +216,16 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Cache4 c, int slots, int 
 
 // ---------------------------------------------------------------- a decode step
 
-constexpr int kMaxWaves4 = 4;
-constexpr int64_t kMaxSpans4 = 64;
+// Splitting of the slots among workgroups: up to 16 blocks are one span of up to
+// 8 waves, one block each in turn (16 sequences x 8 heads at 300 of 512: 7.3 us,
+// in 4 spans 10.7; one sequence of 24 blocks 10.5 against 8.8, so split).  Else
+// spans of nt blocks and 4 waves, nt the smallest power of two from 4 that leaves
+// at most 64 spans a head and at most 1024 workgroups, or reaches 32 (8 sequences
+// x 8 heads at 4000: 9 spans of 16 17.4 us, 17 of 8 19.7; 32 sequences of up to
+// 16384: 16 spans of 32 94 us, 8 of 64 96, 4 of 128 107, 32 of 16 103).
+constexpr int kMaxWaves4 = 8;
+constexpr int64_t kOneSpan4 = 16, kFirstSpan4 = 4, kLongSpan4 = 32;
+constexpr int64_t kMaxSpans4 = 64, kMaxGroups4 = 1024;
 constexpr int kHeads = 16;  // query heads a workgroup takes: a tile's columns
 
 struct Split4 {
@@ -228,11 +236,13 @@ inline Split4 split4_of(int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t sl
   Split4 sp;
   const int64_t blocks = (slots + kSlotBlock - 1) / kSlotBlock;
   sp.hb = (G + kHeads - 1) / kHeads;
-  sp.nt = 4;
   auto spans = [&](int64_t nt) { return (blocks + nt - 1) / nt; };
-  while (sp.nt < blocks && (spans(sp.nt) > kMaxSpans4 || B * Hkv * sp.hb * spans(sp.nt) > 1024)) sp.nt *= 2;
+  sp.nt = kFirstSpan4;
+  while (sp.nt < blocks && (spans(sp.nt) > kMaxSpans4 || (B * Hkv * sp.hb * spans(sp.nt) > kMaxGroups4 && sp.nt < kLongSpan4)))
+    sp.nt *= 2;
+  if (blocks <= kOneSpan4) sp.nt = blocks;
   sp.ns = spans(sp.nt);
-  sp.nw = std::min<int64_t>(kMaxWaves4, blocks);
+  sp.nw = std::min<int64_t>(sp.ns == 1 ? kMaxWaves4 : 4, std::min(blocks, sp.nt));
   sp.part_floats = kHeads * D + 2 * kHeads;
   sp.bytes = sp.ns > 1 ? B * Hkv * sp.hb * sp.ns * sp.part_floats * 4 : 0;
   return sp;
@@ -247,12 +257,14 @@ __device__ __forceinline__ f16 turned(f16 x, f16 partner, bool lo, uint16_t c, u
 
 // Nibbles n and n + 4 of a word, n = 0 .. 3, as a pair of fp16 numbers 0 .. 15:
 // under the exponent of 1024 a nibble in the lowest bits counts 1 each, one
-// four bits up 16 each; taking the 1024 away again is exact.
-__device__ __forceinline__ half2v pair_of(uint32_t w, int n) {
+// four bits up 16 each; taking the 1024 away again is exact.  `magic` is 1024
+// twice in a vector register (a vector instruction takes one scalar operand, and
+// the mask is that), so that mask and exponent are one instruction.
+__device__ __forceinline__ half2v pair_of(uint32_t w, int n, uint32_t magic) {
   const half2v big = {(f16)1024.0f, (f16)1024.0f}, sixteenth = {(f16)0.0625f, (f16)0.0625f}, off = {(f16)-64.0f, (f16)-64.0f};
   if (n & 2) w >>= 8;
-  if (n & 1) return __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x64006400u), sixteenth, off);
-  return __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) - big;
+  if (n & 1) return __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00F000F0u) | magic), sixteenth, off);
+  return __builtin_bit_cast(half2v, (w & 0x000F000Fu) | magic) - big;
 }
 
 __device__ __forceinline__ uint32_t splat_lo(uint32_t x) { return (x & 0xFFFF) | x << 16; }
@@ -274,9 +286,16 @@ __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_
 // numerators rounded to fp16 as the second product's operand, which they are
 // without an exchange, and the values' rows.  The denominator is the product of
 // the same numerators with ones, so rounding them does not shift the mean.
-// Dequantized keys and values are rounded to fp16 once each (fma).
+// Dequantized keys and values are rounded to fp16 once each (fma): four packed
+// instructions for eight elements; scales applied to exact sums in f32 instead
+// would take twice as many and gain a factor of two in error (4e-4 of the result,
+// 2e-4 of which is the output's own rounding).
+// Bound by HBM and by unpacking together: a step of 32 slots of D = 128 is about
+// 400 vector instructions a wave for 5 KiB (32 sequences x 8 heads of up to 16384
+// slots, half of them in use: 336 MB in 88 us, 3.8 TB/s, of which instruction
+// issue alone is 45).
 template <int D>
-__global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
+__global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, Cache4 c,
     const int64_t* __restrict__ pos_p, int pos_stride, int H, int Hkv, int hb, int slots, int sinks, float scale2,
     float q_scale, const uint16_t* __restrict__ rcos, const uint16_t* __restrict__ rsin, int64_t max_pos, int nt,
@@ -301,42 +320,78 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
   uint16_t* kp = c.kp + head * nblk * (kSlotBlock * NK * 2);
   uint8_t* vc = c.vc + head * nblk * (16 * D);
   uint16_t* vp = c.vp + head * nblk * (NK * 64);
+  const int l = ln & 15, r = ln >> 4;
   const bool owner = slot / (kSlotBlock * nt) == z && h0 == 0;  // writes the new row
   const bool holds = slot / (kSlotBlock * nt) == z;
 
-  __shared__ uint16_t qs[kHeads][D];
+  // a step's loads: whole rows and blocks, in the buffers whatever the step
+  struct Step {
+    u32x4 k[2], v[ND / 4];
+    uint32_t kpar[2];
+    uint2 vpar;
+  };
+  const int kr = r * (D / 8);
+  auto load = [&](Step& x, int blk) {
+    blk = min(blk, nblk - 1);
+    const uint8_t* kb = kc + (int64_t)blk * (kSlotBlock * D / 2) + l * (D / 2) + kr;
+    const uint16_t* pb = kp + (int64_t)blk * (kSlotBlock * NK * 2) + (l * NK + (D == 128 ? r : r >> 1)) * 2;
+    const uint8_t* vb = vc + (int64_t)blk * (16 * D) + ln * 16;
+#pragma unroll
+    for (int tt = 0; tt < 2; tt++) {
+      if constexpr (D == 128) {
+        x.k[tt] = *reinterpret_cast<const u32x4*>(kb + tt * 16 * (D / 2));
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(kb + tt * 16 * (D / 2));
+        x.k[tt] = u32x4{y.x, y.y, 0, 0};
+      }
+      x.kpar[tt] = *reinterpret_cast<const uint32_t*>(pb + tt * 16 * NK * 2);
+    }
+#pragma unroll
+    for (int e = 0; e < ND / 4; e++) x.v[e] = *reinterpret_cast<const u32x4*>(vb + e * 1024);
+    x.vpar = *reinterpret_cast<const uint2*>(vp + (int64_t)blk * (NK * 64) + v_param((l >> 2) % NK, r, l & 3));
+  };
+  // the first rows are on their way while the queries are staged
+  Step sa, sb;
+  load(sa, blk0 + wave);
+  __shared__ __attribute__((aligned(16))) uint16_t qs[kHeads][D];
   __shared__ uint32_t new_k[D / 8], new_v[D / 8], new_kp[NK], new_vp[NK];
   extern __shared__ float res[];  // [nw][kHeads][D + 2]
 
   const uint16_t* cs = rcos ? rcos + pos * D : nullptr;
   const uint16_t* sn = rsin ? rsin + pos * D : nullptr;
-  const uint16_t* qb = q + ((int64_t)b * H + (int64_t)j * G + h0) * D;
-  for (int i = t; i < kHeads * D; i += 64 * nw) {
-    const int g = i / D, d = i % D;
-    f16 x = (f16)0.0f;
-    if (g < heads) {
-      x = bits_to_h(qb[i]);
-      if (q_scale != 1.0f) x = rn_h((float)x * q_scale);
-      if (cs) {
-        f16 y = bits_to_h(qb[i - d + (d + D / 2) % D]);
-        if (q_scale != 1.0f) y = rn_h((float)y * q_scale);
-        x = turned(x, y, d < D / 2, cs[d], sn[d]);
-      }
+  // eight elements of a row, scaled and rotated; all loads first
+  auto prepared = [&](const uint16_t* row, int d, float f, bool rot, uint16_t(&x)[8]) {
+    auto half = [](const uint4& w, int i) { return bits_to_h((uint16_t)((&w.x)[i >> 1] >> (16 * (i & 1)))); };
+    const uint4 own = *reinterpret_cast<const uint4*>(row + d);
+    if (rot) {
+      const uint4 other = *reinterpret_cast<const uint4*>(row + (d + D / 2) % D);
+      const uint4 cv = *reinterpret_cast<const uint4*>(cs + d), sv = *reinterpret_cast<const uint4*>(sn + d);
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        x[i] = h_to_bits(turned(rn_h((float)half(own, i) * f), rn_h((float)half(other, i) * f), d < D / 2,
+                                h_to_bits(half(cv, i)), h_to_bits(half(sv, i))));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = h_to_bits(rn_h((float)half(own, i) * f));  // f = 1 is exact
     }
-    qs[g][d] = h_to_bits(x);
+  };
+  const uint16_t* qb = q + ((int64_t)b * H + (int64_t)j * G + h0) * D;
+  for (int i = t; i < kHeads * (D / 8); i += 64 * nw) {
+    const int g = i / (D / 8), d = i % (D / 8) * 8;
+    uint16_t x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (g < heads) prepared(qb + g * D, d, q_scale, rcos != nullptr, x);
+    uint4 w;
+#pragma unroll
+    for (int n = 0; n < 4; n++) (&w.x)[n] = (uint32_t)x[2 * n] | (uint32_t)x[2 * n + 1] << 16;
+    *reinterpret_cast<uint4*>(&qs[g][d]) = w;
   }
   if (holds && t < 64) {
     // the step's own row, keys in the wave's lower half, values in its upper
     const bool val = t >= 32;
     const int d = (t & 31) * 8;
     if (d < D) {
-      const uint16_t* src = (val ? v_new : k_new) + head * D;
       uint16_t x[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[i] = src[d + i];
-        if (!val && cs) x[i] = h_to_bits(turned(bits_to_h(x[i]), bits_to_h(src[(d + i + D / 2) % D]), d + i < D / 2, cs[d + i], sn[d + i]));
-      }
+      prepared((val ? v_new : k_new) + head * D, d, 1.0f, !val && rcos, x);
       uint16_t sb, mb;
       const uint32_t w = quantize8(x, &sb, &mb);
       (val ? new_v : new_k)[d / 8] = w;
@@ -345,7 +400,6 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
   }
   __syncthreads();
 
-  const int l = ln & 15, r = ln >> 4;
   // the queries as the scores' second operand: head l, elements
   // (D / 4) r + 8 kk + the order in which pair_of gives a word's nibbles
   half8v qv[NK];
@@ -359,25 +413,15 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
   for (int e = 0; e < ND; e++) o[e] = float4v{0, 0, 0, 0};
   den = float4v{0, 0, 0, 0};
   float m = -INFINITY;
+  uint32_t magic = 0x64006400u;
+  asm volatile("" : "+v"(magic));
   half8v ones;
 #pragma unroll
   for (int n = 0; n < 8; n++) ones[n] = (f16)1.0f;
 
-  for (int blk = blk0 + wave; blk < blk1; blk += nw) {
+  auto step = [&](Step& y, int blk) {
+    uint2& vpar = y.vpar;
     const int s0 = blk * kSlotBlock;
-    uint32_t kw[2][NK], kpar[2], vw[ND];
-    uint2 vpar;
-#pragma unroll
-    for (int tt = 0; tt < 2; tt++) {
-      const int row = s0 + 16 * tt + l;
-#pragma unroll
-      for (int kk = 0; kk < NK; kk++) kw[tt][kk] = *reinterpret_cast<const uint32_t*>(kc + (int64_t)row * (D / 2) + r * (D / 8) + kk * 4);
-      kpar[tt] = *reinterpret_cast<const uint32_t*>(kp + ((int64_t)row * NK + (D == 128 ? r : r >> 1)) * 2);
-    }
-#pragma unroll
-    for (int e = 0; e < ND; e++)
-      vw[e] = *reinterpret_cast<const uint32_t*>(vc + (int64_t)blk * (16 * D) + (e >> 2) * 1024 + ln * 16 + (e & 3) * 4);
-    vpar = *reinterpret_cast<const uint2*>(vp + (int64_t)blk * (NK * 64) + v_param((l >> 2) % NK, r, l & 3));
     if (slot / kSlotBlock == blk) {
       // the step's own row replaces what the slot held, here and in memory
       const int at = slot % kSlotBlock, n = (at >> 4) * 4 + (at & 3);
@@ -386,20 +430,21 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
         if (16 * tt + l == at) {
 #pragma unroll
           for (int kk = 0; kk < NK; kk++) {
-            kw[tt][kk] = new_k[r * (D / 32) + kk];
-            if (owner) *reinterpret_cast<uint32_t*>(kc + (int64_t)slot * (D / 2) + r * (D / 8) + kk * 4) = kw[tt][kk];
+            y.k[tt][kk] = new_k[r * (D / 32) + kk];
+            if (owner) *reinterpret_cast<uint32_t*>(kc + (int64_t)slot * (D / 2) + kr + kk * 4) = y.k[tt][kk];
           }
-          kpar[tt] = new_kp[D == 128 ? r : r >> 1];
+          y.kpar[tt] = new_kp[D == 128 ? r : r >> 1];
           if (owner && (D == 128 || (r & 1) == 0))
-            *reinterpret_cast<uint32_t*>(kp + ((int64_t)slot * NK + (D == 128 ? r : r >> 1)) * 2) = kpar[tt];
+            *reinterpret_cast<uint32_t*>(kp + ((int64_t)slot * NK + (D == 128 ? r : r >> 1)) * 2) = y.kpar[tt];
         }
       if (r == ((at & 15) >> 2)) {
 #pragma unroll
         for (int e = 0; e < ND; e++) {
           const int d = e * 16 + l;
           const uint32_t code = (new_v[d / 8] >> (4 * (d & 7))) & 15;
-          vw[e] = (vw[e] & ~(15u << (4 * n))) | code << (4 * n);
-          if (owner) *reinterpret_cast<uint32_t*>(vc + (int64_t)blk * (16 * D) + (e >> 2) * 1024 + ln * 16 + (e & 3) * 4) = vw[e];
+          const uint32_t w = (y.v[e >> 2][e & 3] & ~(15u << (4 * n))) | code << (4 * n);
+          y.v[e >> 2][e & 3] = w;
+          if (owner) *reinterpret_cast<uint32_t*>(vc + (int64_t)blk * (16 * D) + (e >> 2) * 1024 + ln * 16 + (e & 3) * 4) = w;
         }
         if ((l & 3) == (at & 3)) {
           const uint32_t p = new_vp[(l >> 2) % NK];
@@ -421,14 +466,14 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
     float x[8];
 #pragma unroll
     for (int tt = 0; tt < 2; tt++) {
-      const half2v s2 = __builtin_bit_cast(half2v, splat_lo(kpar[tt])), m2 = __builtin_bit_cast(half2v, splat_hi(kpar[tt]));
+      const half2v s2 = __builtin_bit_cast(half2v, splat_lo(y.kpar[tt])), m2 = __builtin_bit_cast(half2v, splat_hi(y.kpar[tt]));
       float4v acc = {0, 0, 0, 0};
 #pragma unroll
       for (int kk = 0; kk < NK; kk++) {
         half8v a;
 #pragma unroll
         for (int n = 0; n < 4; n++) {
-          const half2v v2 = __builtin_elementwise_fma(pair_of(kw[tt][kk], n), s2, m2);
+          const half2v v2 = __builtin_elementwise_fma(pair_of(y.k[tt][kk], n, magic), s2, m2);
           a[2 * n] = v2.x;
           a[2 * n + 1] = v2.y;
         }
@@ -477,7 +522,7 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
         half8v a;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const half2v v2 = __builtin_elementwise_fma(pair_of(vw[e], i), s2[i], m2[i]);
+          const half2v v2 = __builtin_elementwise_fma(pair_of(y.v[e >> 2][e & 3], i, magic), s2[i], m2[i]);
           a[2 * i] = v2.x;
           a[2 * i + 1] = v2.y;
         }
@@ -490,6 +535,14 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
       values(std::integral_constant<int, 2>{});
       values(std::integral_constant<int, 3>{});
     }
+  };
+  for (int blk = blk0 + wave; blk < blk1; blk += 2 * nw) {
+    load(sb, blk + nw);
+    __builtin_amdgcn_sched_barrier(0);
+    step(sa, blk);
+    load(sa, blk + 2 * nw);
+    __builtin_amdgcn_sched_barrier(0);
+    if (blk + nw < blk1) step(sb, blk + nw);
   }
 
   // the waves' sums meet: maximum over the waves, each scaled to it, in order
@@ -532,29 +585,46 @@ __global__ __launch_bounds__(64 * kMaxWaves4) void kv4_attention_kernel(
   }
 }
 
-// Merges the spans' (maximum, denominator, sum) of one query head, in order.
+// Merges the spans' (maximum, denominator, sum) of one query head: every wave
+// has all spans' (m, l), one a lane; 256 / D groups of threads take every
+// (256 / D)-th span in order, eight loads in flight, and are added in order.
 template <int D>
-__global__ __launch_bounds__(D) void kv4_combine_kernel(const int64_t* __restrict__ pos_p, int pos_stride, int H,
-                                                        int Hkv, int hb, int slots, int64_t max_pos, int nt, int ns,
-                                                        const float* __restrict__ part, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(256) void kv4_combine_kernel(const int64_t* __restrict__ pos_p, int pos_stride, int H,
+                                                          int Hkv, int hb, int slots, int64_t max_pos, int nt, int ns,
+                                                          const float* __restrict__ part, uint16_t* __restrict__ out) {
   constexpr int PF = kHeads * D + 2 * kHeads;
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+  constexpr int NG = 256 / D;
+  const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x, grp = t / D, d = t % D, z = t & 63;
   const int G = H / Hkv, j = h / G, tile = h % G / kHeads, g = h % G % kHeads;
   const int64_t pos = pos_p[(int64_t)b * pos_stride];
   if (pos < 0 || pos >= max_pos) return;
   const int nact = (int)min(pos, (int64_t)slots - 1) / (kSlotBlock * nt) + 1;
-  if (nact == 1) return;
+  if (nact == 1) return;  // that span wrote out
   const float* pk = part + (((int64_t)b * Hkv + j) * hb + tile) * ns * PF;
-  float mx = -INFINITY;
-  for (int z = 0; z < nact; z++) mx = fmaxf(mx, pk[(int64_t)z * PF + kHeads * D + g]);
-  float num = 0.0f, sum = 0.0f;
-  for (int z = 0; z < nact; z++) {
-    const float* y = pk + (int64_t)z * PF;
-    const float mz = y[kHeads * D + g], f = mz == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mz - mx);
-    num = fmaf(y[g * D + d], f, num);
-    sum = fmaf(y[kHeads * D + kHeads + g], f, sum);
+  __shared__ float f[kMaxSpans4], sum[NG][D];
+  const float m = z < nact ? pk[(int64_t)z * PF + kHeads * D + g] : -INFINITY;
+  const float l = z < nact ? pk[(int64_t)z * PF + kHeads * D + kHeads + g] : 0.0f;
+  const float mx = wave_group_max_f32<64>(m);
+  const float e = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+  const float den = wave_group_sum_f32<64>(l * e);
+  if (t < 64) f[z] = e;
+  __syncthreads();
+  float num = 0.0f;
+  for (int z0 = grp; z0 < nact; z0 += 8 * NG) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = z0 + NG * k < nact ? pk[(int64_t)(z0 + NG * k) * PF + g * D + d] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (z0 + NG * k < nact) num = fmaf(v[k], f[z0 + NG * k], num);
   }
-  out[((int64_t)b * H + h) * D + d] = h_to_bits(rn_h(num / sum));
+  sum[grp][d] = num;
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int k = 1; k < NG; k++) num += sum[k][d];
+    out[((int64_t)b * H + h) * D + d] = h_to_bits(rn_h(num / den));
+  }
 }
 
 int check_cache4(const char* what, const void* kc, const void* kp, const void* vc, const void* vp, int64_t B, int64_t Hkv,
@@ -639,9 +709,10 @@ extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_
   AQ_CHECK_ARG(sinks >= -1 && sinks < slots, "aq_kv4_attention: %lld sinks in %lld slots", (long long)sinks,
                (long long)slots);
   AQ_CHECK_ARG(!rope_cos || rope_rows > 0, "aq_kv4_attention: %lld rows of rope_cos", (long long)rope_rows);
-  AQ_CHECK_ARG((uintptr_t)q % 2 == 0 && (uintptr_t)k_new % 2 == 0 && (uintptr_t)v_new % 2 == 0 && (uintptr_t)out % 2 == 0 &&
+  AQ_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)k_new % 16 == 0 && (uintptr_t)v_new % 16 == 0 &&
+                   (uintptr_t)out % 16 == 0 && (uintptr_t)rope_cos % 16 == 0 && (uintptr_t)rope_sin % 16 == 0 &&
                    (uintptr_t)pos % 8 == 0,
-               "aq_kv4_attention: misaligned buffer");
+               "aq_kv4_attention: q, k_new, v_new, out and the rotary tables must be 16-byte aligned");
   const Split4 sp = split4_of(B, Hkv, H / Hkv, D, slots);
   AQ_CHECK_ARG(Hkv * sp.hb <= 65535 && H <= 65535, "aq_kv4_attention: sizes out of range");
   AQ_CHECK_ARG(sp.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= sp.bytes),
@@ -663,7 +734,7 @@ extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_
                        (const uint16_t*)rope_sin, max_pos, (int)sp.nt, (int)sp.ns, (float*)workspace,                 \
                        (uint16_t*)out);                                                                               \
     if (sp.ns > 1)                                                                                                    \
-      hipLaunchKernelGGL((kv4_combine_kernel<DD>), dim3((unsigned)H, (unsigned)B), dim3(DD), 0, s, pos,               \
+      hipLaunchKernelGGL((kv4_combine_kernel<DD>), dim3((unsigned)H, (unsigned)B), dim3(256), 0, s, pos,               \
                          (int)pos_stride, (int)H, (int)Hkv, (int)sp.hb, (int)slots, max_pos, (int)sp.nt, (int)sp.ns,  \
                          (const float*)workspace, (uint16_t*)out);                                                    \
   } while (0)

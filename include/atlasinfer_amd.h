@@ -489,7 +489,7 @@ int aq_kv4_load(const void* k_codes, const void* k_params, const void* v_codes, 
  * over the slots in use, as the values they stand for (each rounded to fp16;
  * scores and sums in f32, the softmax's numerators rounded to fp16).  H any
  * multiple of Hkv.  q, k_new, v_new, pos, q_scale, rope_* and which sequences
- * are run: as there; workspace: aq_kv4_attention_workspace bytes (may be 0,
+ * are run: as there, q, k_new, v_new, out and the tables 16-byte aligned; workspace: aq_kv4_attention_workspace bytes (may be 0,
  * then NULL will do; -1 for sizes it cannot take), 16-byte aligned, no initial
  * contents; calls that overlap in time must not share one.
  */
