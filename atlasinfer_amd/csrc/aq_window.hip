@@ -43,12 +43,15 @@ __device__ __forceinline__ half4v read_turned(const uint8_t* p) {
   return __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_u8*)p));
 }
 
-__device__ __forceinline__ bool not_finite8(uint4 x) {
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The larger of m and the magnitudes of eight fp16 numbers, as pairs of bits:
+// from 0x7C00 on one is not finite.
+__device__ __forceinline__ u16x2 magnitudes8(u16x2 m, uint4 x) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) bad = bad | ((w[i] & 0x7C00u) == 0x7C00u) | ((w[i] & 0x7C000000u) == 0x7C000000u);
-  return bad;
+  for (int i = 0; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+  return m;
 }
 
 // A tile's rows lie in LDS one after the other, 16-byte pieces permuted within
@@ -60,8 +63,8 @@ template <int D>
 __device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) * 16; }
 
 // One workgroup: 128 queries of a head, 32 a wave; tiles of 64 keys and values
-// go straight from memory to LDS (direct loads, the next tile's on their way
-// during a tile; one barrier a tile).
+// go straight from memory to LDS (direct loads, one tile ahead for D = 128, three
+// for 64, whose tiles take half as long as a load; one barrier a tile).
 //   scores   transposed, s^T = k q^T (mfma 32 x 32 x 16): a lane has 32 scores of
 //            one query, another lane the other 32, so maxima and sums need one
 //            exchange
@@ -79,8 +82,9 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
   constexpr int NC = D / 8;                    // 16-byte pieces of a row
   constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
   constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // two stages of keys, values
-  __shared__ int bad[2];
+  constexpr int NS = D == 64 ? 4 : 2;          // stages: 64 KiB
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * 2 * TB];  // keys and values of each stage
+  __shared__ int bad[NS];
   const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // runs of neighbouring items to an XCD (they share keys and values in its L2)
@@ -135,7 +139,7 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
   }
   auto load = [&](int i) {
     const int k0 = tile_at(i) * kK;
-    uint8_t* st = lds + (i & 1) * (2 * TB) + wave * PN * 1024;
+    uint8_t* st = lds + (i & (NS - 1)) * (2 * TB) + wave * PN * 1024;
     // rows past the last read as zeros, values before the start too, whatever is there
     const int rows = min(a.N - k0, kK);
     const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
@@ -163,21 +167,25 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
 #pragma unroll
   for (int e = 0; e < 2; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
 
-  if (t < 2) bad[t] = 0;
-  if (tiles > 0) load(0);
+  if (t < NS) bad[t] = 0;
+  for (int i = 0; i < min(NS - 1, tiles); i++) load(i);
   for (int i = 0; i < tiles; i++) {
     const int k0 = tile_at(i) * kK;
-    const uint8_t* st = lds + (i & 1) * (2 * TB);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the tile is there
+    const uint8_t* st = lds + (i & (NS - 1)) * (2 * TB);
+    // this wave's part of the tile is there; the NS - 2 tiles after it may be on their way
+    if (i + NS - 2 < tiles)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * PN) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (!(k0 + kK - 1 <= lo && k0 > hi - a.window && k0 >= start)) {
       // a tile that the mask cuts for some query: whether its values are finite
-      bool x = false;
+      u16x2 m = 0;
 #pragma unroll
-      for (int n = 0; n < PN; n++) x = x | not_finite8(*reinterpret_cast<const uint4*>(st + TB + (wave * PN + n) * 1024 + ln * 16));
-      if (__ballot(x) && ln == 0) bad[i & 1] = i + 1;
+      for (int n = 0; n < PN; n++) m = magnitudes8(m, *reinterpret_cast<const uint4*>(st + TB + (wave * PN + n) * 1024 + ln * 16));
+      if (__ballot(max(m.x, m.y) >= 0x7C00) && ln == 0) bad[i & (NS - 1)] = i + 1;
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's part; the tile before is done with
-    if (i + 1 < tiles) load(i + 1);
+    if (i + NS - 1 < tiles) load(i + NS - 1);
     // whether this wave's queries see none, all or some of the tile
     if (k0 > whi || (k0 + kK - 1 <= wlo - a.window && k0 >= sink_end) || k0 + kK <= start) continue;
     const bool all = k0 + kK - 1 <= wlo && k0 > whi - a.window && k0 >= start;
@@ -193,16 +201,32 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
       }
     }
     if (!all) {
+      // a key is seen when it lies in one of two ranges: near the query, or among
+      // the sinks, both up to the query (each a subtraction, an unsigned comparison
+      // and a selection: conditions joined as masks would go through the scalar unit
+      // and take five times as long)
       const int last = qpos - k0 - 4 * h, from = max(last - a.window + 1, start - k0 - 4 * h);
-      const int sink0 = start - k0 - 4 * h, sink1 = sink0 + a.sinks;
+      const int sink0 = start - k0 - 4 * h;
+      const uint32_t near_n = (uint32_t)max(last - from + 1, 0);
+      const uint32_t sink_n = (uint32_t)max(min(a.sinks, last - sink0 + 1), 0);
+      if (k0 < sink_end) {
 #pragma unroll
-      for (int s = 0; s < 2; s++)
+        for (int s = 0; s < 2; s++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const int key = 32 * s + 8 * (e >> 2) + (e & 3);
-          const bool sees = (key <= last) & ((key >= from) | ((key >= sink0) & (key < sink1)));
-          x[s][e] = sees ? x[s][e] : -INFINITY;
-        }
+          for (int e = 0; e < 16; e++) {
+            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
+            const float y = (uint32_t)(key - sink0) < sink_n ? x[s][e] : -INFINITY;
+            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : y;
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
+            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : -INFINITY;
+          }
+      }
     }
     float mx = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
@@ -227,7 +251,7 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
       p[e >> 3][e & 7] = w.x;
       p[e >> 3][(e & 7) + 1] = w.y;
     }
-    if (!all && bad[i & 1] == i + 1) {
+    if (!all && bad[i & (NS - 1)] == i + 1) {
       // an infinity or NaN among the values of a tile that the mask cuts: the
       // terms one by one, leaving out those of weight zero
 #pragma unroll 1
