@@ -11,6 +11,7 @@ namespace {
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4v lds_s4;
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
     }
     float mx = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
-    for (int e = 1; e < 16; e++) mx = fmaxf(mx, fmaxf(x[0][e], x[1][e]));
+    for (int e = 1; e < 16; e++) mx = fmaxf(fmaxf(mx, x[0][e]), x[1][e]);  // v_max3
     mx = xlane_level_max_f32<6>(mx);
     if (__ballot(mx > m + grow || (m == -INFINITY && mx > m))) {
       const float n = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - n) * a.c);
@@ -240,37 +241,38 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
       m = n;
     }
     const float base = m == -INFINITY ? 0.0f : -m * a.c;
-    half8v p[4];
+    uint32_t p[16];  // the numerators in pairs: p[4 n .. 4 n + 3] are the operand of 16 keys
     const half2v one = {(f16)1.0f, (f16)1.0f};
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      half2v w;
-      w.x = rn_h(__builtin_amdgcn_exp2f(fmaf(x[e >> 4][e & 15], a.c, base)));
-      w.y = rn_h(__builtin_amdgcn_exp2f(fmaf(x[e >> 4][(e & 15) + 1], a.c, base)));
-      l = __builtin_amdgcn_fdot2(w, one, l, false);
-      p[e >> 3][e & 7] = w.x;
-      p[e >> 3][(e & 7) + 1] = w.y;
+    for (int e = 0; e < 16; e++) {
+      const int y = 2 * e & 15;
+      const float2v w = {__builtin_amdgcn_exp2f(fmaf(x[e >> 3][y], a.c, base)),
+                         __builtin_amdgcn_exp2f(fmaf(x[e >> 3][y + 1], a.c, base))};
+      const half2v r = __builtin_convertvector(w, half2v);  // one conversion for both, to nearest
+      l = __builtin_amdgcn_fdot2(r, one, l, false);
+      p[e] = __builtin_bit_cast(uint32_t, r);
     }
     if (!all && bad[i & (NS - 1)] == i + 1) {
       // an infinity or NaN among the values of a tile that the mask cuts: the
       // terms one by one, leaving out those of weight zero
+      // (the sums pass an empty asm here, so that what the compiler does for this
+      // loop's sake, copying them, it does here and not on the common path)
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
 #pragma unroll 1
       for (int key = 0; key < kK; key++) {
-        const int s = key >> 4, y = (key >> 2) & 1, e8 = ((key >> 3) & 1) * 4 + (key & 3);
-        f16 w = (f16)0.0f;
+        const int y = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
+        uint32_t w = p[0];
 #pragma unroll
-        for (int n = 0; n < 4; n++)
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (n == s && e == e8) w = p[n][e];
-        const float wf = __shfl((float)w, c + 32 * y, 64);
+        for (int e = 1; e < 16; e++) w = e == n ? p[e] : w;
+        const float wf = __shfl((float)bits_to_h((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * y, 64);
 #pragma unroll
         for (int e = 0; e < D / 32; e++)
 #pragma unroll
-          for (int n = 0; n < 16; n++) {
-            const int d = 32 * e + 8 * (n >> 2) + 4 * h + (n & 3);
+          for (int z = 0; z < 16; z++) {
+            const int d = 32 * e + 8 * (z >> 2) + 4 * h + (z & 3);
             const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + TB + v_place<D>(key, d >> 3) + (d & 7) * 2);
-            if (wf != 0.0f) o[e][n] = fmaf(wf, (float)bits_to_h(vd), o[e][n]);
+            if (wf != 0.0f) o[e][z] = fmaf(wf, (float)bits_to_h(vd), o[e][z]);
           }
       }
       continue;
@@ -282,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
         // keys 16 s + 4 h + 0 .. 3, then 8 on: the order in which a lane has the numerators
         const uint8_t* f = st + TB + vf[e & 1] + (e >> 1) * 128 + s * 16 * (D * 2);
         const half8v w = __builtin_shufflevector(read_turned(f), read_turned(f + 8 * (D * 2)), 0, 1, 2, 3, 4, 5, 6, 7);
-        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, p[s], o[e], 0, 0, 0);
+        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w, __builtin_bit_cast(half8v, u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}), o[e], 0, 0, 0);
       }
   }
   l = xlane_level_sum_f32<6>(l);
