@@ -1,4 +1,4 @@
-"""Greedy decoding with each step captured in one HIP graph.
+"""Decoding, greedy or sampled, with each step captured in one HIP graph.
 
 The reference decodes with HF ``generate`` (examples/run_atlas_inference.py
 :244-264), one eager forward per token; on a GPU as fast as this one that
@@ -8,8 +8,8 @@ token moves.  ``GraphDecoder`` takes a model whose Linears were swapped by
 model), runs the prompt through the model's own forward, then records one
 decode step -- embeddings, every layer (the QuantizedLinear launches, the
 attention over a static key/value cache, the norms and activations), the
-final norm, the lm_head and the greedy choice -- in a HIP graph and replays
-it once per token.
+final norm, the lm_head and the choice of the token -- in a HIP graph and
+replays it once per token.
 
 Everything a replay reads that changes from token to token is device
 memory updated in place by the graph itself: the current token ``tok``
@@ -37,19 +37,37 @@ cache spans' partial results), the output projection, the SiLU product
 (``aq_silu_mul``) and the down projection.  Elsewhere (CPU, other dtypes,
 head sizes other than 64 and 128) the same step runs as torch operations.
 
-Limits: greedy decoding, equal-length prompts without padding (batch rows
-share ``pos``), no beam search, no sliding-window attention.
+Options (on the GPU path with an fp16 model):
+
+* ``sampling=True``: the token is sampled (``sample_tokens``: temperature, top-k,
+  top-p, min-p) instead of the largest logit's.  The settings are device memory,
+  one per sequence, and so are the random numbers, one per sequence and step
+  drawn ahead, so a captured graph takes new ones.
+* ``kv_bits=4``: keys and values are kept in 4 bits (``DecodeCache``): 5/16 of
+  the memory and of the bytes a step reads.  The prompt itself attends to its own
+  keys and values as they are.
+* ``window``, ``sinks``: attention through a sliding window, the first ``sinks``
+  positions staying visible; the cache holds just these, so ``max_len`` bounds
+  positions but not memory.  A model whose configuration has a sliding window
+  shorter than ``max_len`` gets that window by itself.
+
+Limits: equal-length prompts without padding (batch rows share ``pos``), no
+beam search.
 """
 from __future__ import annotations
 
 from typing import Optional
 
+import contextlib
 import ctypes
 
 import torch
 import torch.nn.functional as F
 
 from .. import _lib
+from ..memory.decode_cache import DecodeCache
+from .sampling import sample_tokens
+from .window_attention import window_prompts
 
 
 def _kind(model) -> str:
@@ -62,12 +80,14 @@ def _kind(model) -> str:
 
 
 class GraphDecoder:
-    """Greedy decode of ``model`` for ``batch`` sequences of up to
-    ``max_len`` positions (prompt + new tokens), one HIP graph replay per
-    token.  ``graph=False`` runs the same step eagerly (no capture), which is
+    """Decode of ``model`` for ``batch`` sequences of up to ``max_len``
+    positions (prompt + new tokens), one HIP graph replay per token: greedy, or
+    sampled with ``sampling=True``; ``kv_bits`` 16 or 4, ``window`` and ``sinks``:
+    the cache.  ``graph=False`` runs the same step eagerly (no capture), which is
     also how it runs on a CPU."""
 
-    def __init__(self, model, batch: int, max_len: int, graph: bool = True):
+    def __init__(self, model, batch: int, max_len: int, graph: bool = True, *, kv_bits: int = 16,
+                 window: Optional[int] = None, sinks: int = 0, sampling: bool = False):
         self.model = model
         self.kind = _kind(model)
         cfg = model.config
@@ -85,8 +105,8 @@ class GraphDecoder:
             self.D = cfg.hidden_size // self.H
         else:
             self.layers = list(model.model.layers)
-            if getattr(cfg, "sliding_window", None) not in (None, 0) and cfg.sliding_window < self.L:
-                raise NotImplementedError("GraphDecoder: sliding-window attention shorter than max_len")
+            if window is None and getattr(cfg, "sliding_window", None) not in (None, 0):
+                window = cfg.sliding_window
             self.H = cfg.num_attention_heads
             self.Hkv = getattr(cfg, "num_key_value_heads", None) or self.H
             self.D = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.H
@@ -98,9 +118,36 @@ class GraphDecoder:
         self.out = torch.zeros(B, L, dtype=torch.long, device=dev)
         self.logits = None  # the last step's logits (a static buffer once captured)
         self.ar = torch.arange(L, device=dev)
-        # keys and values [B, Hkv, L, D]: a position's key is one row
-        self.k = [torch.zeros(B, self.Hkv, L, self.D, dtype=self.dtype, device=dev) for _ in self.layers]
-        self.v = [torch.zeros(B, self.Hkv, L, self.D, dtype=self.dtype, device=dev) for _ in self.layers]
+        # on the GPU: the attention of a step in one HIP kernel
+        # (aq_decode_attention), q/k/v and gate/up in one grouped launch each
+        self.fused = (self.dev.type == "cuda" and self.dtype == torch.float16 and self.D in (64, 128)
+                      and self.H % self.Hkv == 0 and self.H // self.Hkv in (1, 2, 4, 8))
+        if window is not None and (window < 1 or sinks < 0):
+            raise ValueError(f"GraphDecoder: window {window}, {sinks} sinks")
+        if window is None and sinks:
+            raise ValueError("GraphDecoder: sinks without a window")
+        # the window, None where it reaches back to the first position anyway
+        self.window = window if window is not None and sinks + window < L else None
+        self.sinks, self.kv_bits, self.sampling = sinks, kv_bits, sampling
+        if kv_bits not in (4, 16):
+            raise ValueError(f"GraphDecoder: kv_bits {kv_bits} (4 or 16)")
+        if not self.fused and (self.window is not None or kv_bits != 16 or sampling):
+            raise NotImplementedError("GraphDecoder: a sliding window shorter than max_len, kv_bits=4 and sampling need "
+                                      "an fp16 model on a HIP device, head size 64 or 128")
+        self.caches = None
+        if self.window is not None or kv_bits != 16:
+            slots, keep = (L, None) if self.window is None else (sinks + self.window, sinks)
+            self.caches = [DecodeCache(B, self.Hkv, slots, self.D, bits=kv_bits, sinks=keep, device=dev)
+                           for _ in self.layers]
+            self.k = self.v = None
+        else:
+            # keys and values [B, Hkv, L, D]: a position's key is one row
+            self.k = [torch.zeros(B, self.Hkv, L, self.D, dtype=self.dtype, device=dev) for _ in self.layers]
+            self.v = [torch.zeros(B, self.Hkv, L, self.D, dtype=self.dtype, device=dev) for _ in self.layers]
+        if sampling:
+            self.u = torch.zeros(L, B, dtype=torch.float32, device=dev)  # a number per token and sequence
+            self.settings = dict(temperature=torch.ones(B, device=dev), top_k=torch.zeros(B, dtype=torch.int32, device=dev),
+                                 top_p=torch.ones(B, device=dev), min_p=torch.zeros(B, device=dev))
         if self.kind == "llama":
             rot = model.model.rotary_emb
             pos_ids = torch.arange(L, device=dev)[None]
@@ -110,17 +157,14 @@ class GraphDecoder:
         self.graph = None
         self.captured = False
         self.S, self._n = 0, 0
-        # on the GPU: the attention of a step in one HIP kernel
-        # (aq_decode_attention), q/k/v and gate/up in one grouped launch each
-        self.fused = (self.dev.type == "cuda" and self.dtype == torch.float16 and self.D in (64, 128)
-                      and self.H % self.Hkv == 0 and self.H // self.Hkv in (1, 2, 4, 8))
         if self.dev.type == "cuda":
             self._lib = _lib.load()
         if self.fused:
             # the attention kernel's per-span partial results: one workspace
             # for every layer (the layers' calls follow each other on one
             # stream)
-            nb = self._lib.aq_decode_attention_workspace(B, self.H, self.Hkv, self.D, L)
+            nb = (self._lib.aq_decode_attention_workspace(B, self.H, self.Hkv, self.D, L) if self.caches is None
+                  else self.caches[0].workspace_bytes(self.H))
             if nb < 0:
                 raise ValueError("aq_decode_attention_workspace refused these sizes")
             self.ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
@@ -139,6 +183,9 @@ class GraphDecoder:
         pos; k, v written at pos; attention over positions 0..pos."""
         B, H, Hkv, D = self.B, self.H, self.Hkv, self.D
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        if self.caches is not None:
+            return self.caches[li].attend(q, k, v, self.pos, scale=scale, q_scale=q_scale,
+                                          rope=(self.cos, self.sin) if rope else None, workspace=self.ws).view(B, H * D)
         o = torch.empty(B, H * D, dtype=self.dtype, device=self.dev)
         cs, sn = (self.cos.data_ptr(), self.sin.data_ptr()) if rope else (None, None)
         _lib.check(self._lib.aq_decode_attention(
@@ -399,12 +446,32 @@ class GraphDecoder:
                 x = layer_fn(li, layer, x)
             x = final(x)
         logits = m.lm_head(x)  # [B, V]
-        nxt = self._argmax(logits)
+        nxt = self._choose(logits, self.slot)
         self.tok.copy_(nxt)
         self.out.index_copy_(1, self.slot, nxt.view(self.B, 1))
         self.pos.add_(1)
         self.slot.add_(1)
         return logits
+
+    def _choose(self, logits, slot):
+        """The next tokens: the largest logits', or sampled with the random
+        numbers of output slot ``slot`` (device int64 [1])."""
+        if not self.sampling:
+            return self._argmax(logits)
+        return sample_tokens(logits, self.u.index_select(0, slot).view(self.B), **self.settings)
+
+    def set_sampling(self, temperature=None, top_k=None, top_p=None, min_p=None, generator=None) -> None:
+        """New settings (a number, or one per sequence; None: as they are; at first
+        the whole distribution at temperature 1) and fresh random numbers for the
+        tokens to come, from ``generator`` (torch's default one of the device)."""
+        if not self.sampling:
+            raise ValueError("GraphDecoder: built without sampling=True")
+        for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            if value is not None:
+                t = self.settings[name]
+                t.copy_(torch.as_tensor(value, device=self.dev).to(t.dtype).expand(self.B))
+        dev = self.dev if generator is None else generator.device
+        self.u.copy_(torch.rand(self.u.shape, generator=generator, device=dev))
 
     @staticmethod
     def _argmax(logits):
@@ -448,12 +515,17 @@ class GraphDecoder:
             self._capture()
         from transformers import DynamicCache
         cache = DynamicCache()
-        out = self.model(input_ids=input_ids.to(self.dev), past_key_values=cache, use_cache=True)
+        with contextlib.nullcontext() if self.window is None else window_prompts(self.model, self.window, self.sinks):
+            out = self.model(input_ids=input_ids.to(self.dev), past_key_values=cache, use_cache=True)
         for li in range(len(self.layers)):
             kl, vl = cache.layers[li].keys, cache.layers[li].values  # [B, Hkv, S, D]
+            if self.caches is not None:
+                self.caches[li].store(kl, vl)
+                continue
             self.k[li][:, :, :S].copy_(kl)
             self.v[li][:, :, :S].copy_(vl)
-        first = self._argmax(out.logits[:, -1])
+        self.slot.zero_()
+        first = self._choose(out.logits[:, -1], self.slot)
         self.tok.copy_(first)
         self.out.zero_()
         self.out[:, 0].copy_(first)
@@ -479,11 +551,15 @@ class GraphDecoder:
         return self.logits
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
-        """Prompt + ``max_new_tokens`` greedy tokens, [B, S + max_new_tokens]."""
+    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, **sampling) -> torch.Tensor:
+        """Prompt + ``max_new_tokens`` tokens, [B, S + max_new_tokens]: greedy, or
+        of a decoder built with ``sampling=True`` sampled with fresh random numbers,
+        ``sampling`` being set_sampling's arguments."""
         S = input_ids.shape[1]
         if S + max_new_tokens > self.L:
             raise ValueError(f"generate: {S} + {max_new_tokens} positions exceed the cache ({self.L})")
+        if self.sampling or sampling:
+            self.set_sampling(**sampling)
         self.prefill(input_ids)
         for _ in range(max_new_tokens - 1):
             self.step()

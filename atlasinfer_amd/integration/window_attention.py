@@ -1,14 +1,16 @@
 """Attention of a prompt through a sliding window with sinks.
 
 ``window_attention`` is the kernel's call (``aq_window_attention``);
-``use_window_attention`` makes an HF OPT / Llama / Mistral model's own forward
-use it, which ``GraphDecoder(window=...)`` does for its prompts.  No counterpart
+``window_prompts`` makes an HF OPT / Llama / Mistral model's own forward use it
+for a while, which ``GraphDecoder(window=...)`` does for its prompts.  No counterpart
 in the reference, whose attention (integration/atlas_wrappers.py:161-262) sees
 every position through torch's SDPA and a dense mask.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import threading
 from typing import Optional
 
 import torch
@@ -57,3 +59,33 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
                                                    _lib.ptr(starts), out.data_ptr(), _lib.stream_of(dev)),
                    "aq_window_attention")
     return out
+
+
+_NAME = "atlas_window"  # this attention's name among HF's
+_current = threading.local()  # (window, sinks) of the innermost window_prompts
+
+
+def _attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
+    """HF's attention interface: [B, H, M, D] and [B, Hkv, N, D] to [B, M, H, D]."""
+    window, sinks = _current.value
+    return window_attention(query, key, value, window=window, sinks=sinks, scale=scaling), None
+
+
+@contextlib.contextmanager
+def window_prompts(model, window: Optional[int], sinks: int = 0):
+    """Within the context ``model``'s forward (HF OPT, Llama or Mistral, fp16 on a
+    HIP device) attends through a sliding window with sinks, whatever its
+    configuration says; prompts without padding (the attention mask is not
+    looked at)."""
+    from transformers import AttentionInterface
+    from transformers.masking_utils import AttentionMaskInterface
+    AttentionInterface.register(_NAME, _attention)
+    AttentionMaskInterface.register(_NAME, lambda *args, **kwargs: None)  # no dense mask is made
+    before, outer = model.config._attn_implementation, getattr(_current, "value", None)
+    _current.value = (window, sinks)
+    model.set_attn_implementation(_NAME)
+    try:
+        yield model
+    finally:
+        model.set_attn_implementation(before)
+        _current.value = outer

@@ -81,3 +81,47 @@ def test_norm_folds_only_fp16_norms():
             assert not gd._norm_folds(norm)
             norm.bias = None
             assert not gd._norm_folds(norm)
+
+
+def test_options_need_the_gpu_path():
+    """A window shorter than max_len (asked for, or the model's own), the 4-bit
+    cache and sampling run on the GPU path only; a longer window changes nothing."""
+    m = _model("mistral")
+    for kw in (dict(window=8), dict(kv_bits=4), dict(sampling=True)):
+        with pytest.raises(NotImplementedError):
+            GraphDecoder(m, batch=1, max_len=16, graph=False, **kw)
+    m.config.sliding_window = 8
+    with pytest.raises(NotImplementedError):
+        GraphDecoder(m, batch=1, max_len=16, graph=False)
+    assert GraphDecoder(m, batch=1, max_len=8, graph=False).window is None
+
+
+def test_window_prompts_reach_the_attention(monkeypatch):
+    """The context hands every layer's queries, keys and values, the window and
+    the model's scale to window_attention, and leaves the model as it was."""
+    from atlasinfer_amd.integration import window_attention as W
+    seen = []
+
+    def plain(q, k, v, window, sinks, scale):
+        seen.append((tuple(q.shape), tuple(k.shape), window, sinks, scale))
+        G, N = q.shape[1] // k.shape[1], k.shape[2]
+        s = q @ k.repeat_interleave(G, 1).transpose(2, 3) * scale
+        i, j = torch.arange(N)[:, None], torch.arange(N)[None]
+        s = s.masked_fill(~((j <= i) & ((i - j < window) | (j < sinks))), -float("inf"))
+        return (s.softmax(-1) @ v.repeat_interleave(G, 1)).transpose(1, 2).contiguous()
+
+    monkeypatch.setattr(W, "window_attention", plain)
+    ids = torch.randint(0, 256, (2, 11))
+    for kind, heads, scale in (("opt", 4, 1.0), ("llama", 2, 32 ** -0.5), ("mistral", 2, 32 ** -0.5)):
+        m = _model(kind)
+        with torch.no_grad():
+            whole = m(input_ids=ids).logits
+            seen.clear()
+            with W.window_prompts(m, 100):
+                same = m(input_ids=ids).logits
+            with W.window_prompts(m, 3, 1):
+                short = m(input_ids=ids).logits
+            assert torch.equal(m(input_ids=ids).logits, whole)
+        assert seen == [((2, 4, 11, 32), (2, heads, 11, 32), w, s, scale) for w, s in [(100, 0)] * 2 + [(3, 1)] * 2]
+        assert (same - whole).abs().max() < 1e-5 and (short - whole).abs().max() > 1e-4
+        assert torch.allclose(short[:, :4], whole[:, :4], atol=1e-5)  # these see everything through window and sink
