@@ -47,6 +47,7 @@ constexpr double kOne = 4398046511104.0;  // 2^42
 constexpr int kList = 4096;
 constexpr int kSmallList = kThreads / 4;
 constexpr int kTable = 512;
+constexpr int kMaxParts = 32;
 constexpr int kMaxListK = 512;
 constexpr int kMaxSegments = 1024 + 16;  // 2^18 f32 and a misaligned start
 
@@ -189,10 +190,19 @@ __device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& mos
   const int t = threadIdx.x;
   const int b0 = kBins - 1 - 2 * t, b1 = b0 - 1;  // this thread's
   const uint64_t m0 = s.mass[b0], m1 = s.mass[b1], c0 = s.count[b0], c1 = s.count[b1];
-  uint64_t all;
-  const uint64_t im = block_scan_u64(m0 + m1, s.red, &all), bm = im - m0 - m1;
-  if (most == 0) most = reach(p, all);
-  const uint64_t ic = block_scan_u64(c0 + c1, s.red, &all), bc = ic - c0 - c1;
+  uint64_t bm = 0, bc = 0;
+#pragma unroll 1
+  for (int i = 0; i < 2; i++) {  // both scans by the same instructions: they run once, most time goes to fetching them
+    const uint64_t v = i ? c0 + c1 : m0 + m1;
+    uint64_t all;
+    const uint64_t before = block_scan_u64(v, s.red, &all) - v;
+    if (i) {
+      bc = before;
+    } else {
+      bm = before;
+      if (most == 0) most = reach(p, all);
+    }
+  }
   // a bin is the one if what lies above it does not reach `most` and with it does
   auto take = [&](int bin, uint64_t mb, uint64_t cb, uint64_t m, uint64_t c) {
     const uint64_t lo = by_mass ? mb : cb, hi = by_mass ? mb + m : cb + c;
@@ -209,33 +219,70 @@ __device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& mos
   return f;
 }
 
+// The highest key edge (of the first 11 bits) that at least k of the threads'
+// keys reach; s.count is the scratch.
+__device__ __forceinline__ uint32_t edge_of_kth(Shared& s, uint32_t key, int bits, uint32_t k) {
+  const int t = threadIdx.x, w = t >> 6;
+  uint32_t* red = reinterpret_cast<uint32_t*>(s.red);
+  s.count[t] = 0;
+  s.count[t + kThreads] = 0;
+  __syncthreads();
+  atomicAdd(&s.count[key >> (bits - 11)], 1u);
+  __syncthreads();
+  const int b0 = kBins - 1 - 2 * t;
+  const uint32_t c0 = s.count[b0], c1 = s.count[b0 - 1];
+  uint32_t inc = (uint32_t)wave_incl_scan_i32<64>((int)(c0 + c1));
+  if ((t & 63) == 63) red[w] = inc;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; i++) inc += i < w ? red[i] : 0;
+  const uint32_t before = inc - c0 - c1;
+  if (before < k && inc >= k) s.found_bin = before + c0 >= k ? b0 : b0 - 1;
+  __syncthreads();
+  return s.found_bin << (bits - 11);
+}
+
 // A cut: keys above `key`, and the first `ties` of those equal to it.
 struct Cut {
   uint32_t key, ties;
 };
 
+// A row, or the part of it from piece c0 to c1, as 16-byte pieces dealt to the
+// workgroup's threads in turn; `skip` elements of the first piece lie before the
+// row.
 template <int FMT>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict__ logits, int V, int64_t stride,
-                                                          const float* __restrict__ u, Settings set,
-                                                          int64_t* __restrict__ out) {
+struct Row {
   typedef Logit<FMT> L;
-  constexpr int B = L::kBits, E = L::kPer;
-  __shared__ Shared s;
-  const int t = threadIdx.x, row = blockIdx.x, ln = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const uint8_t* x = (const uint8_t*)logits + (int64_t)row * stride * (B / 8);
-  const float T = set.t ? set.t[row] : set.t0, p = set.p ? set.p[row] : set.p0, mp = set.m ? set.m[row] : set.m0;
-  const int k = set.k ? set.k[row] : set.k0;
+  static constexpr int E = L::kPer;
+  const uint8_t* x;
+  const uint4* pieces;
+  int V, skip, np, inside, outside, c0, c1;
+  uint4 head, tail;
 
-  // the row as 16-byte pieces; `skip` elements of the first lie before it
-  const int skip = (int)((uintptr_t)x % 16) / (B / 8);
-  const uint4* pieces = reinterpret_cast<const uint4*>(x - skip * (B / 8));
-  const int np = (V + skip + E - 1) / E;
-  // pieces inside..outside - 1 lie in the row as a whole
-  const int inside = skip ? 1 : 0, outside = (V + skip) / E;
-  const uint4 none = make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu);  // NaNs, which count as -inf
-  auto load_edge = [&](int c) {  // the elements that there are
-    uint4 r = none;
+  // NaNs, which count as -inf
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu); }
+
+  __device__ __forceinline__ Row(const void* logits, int64_t row, int64_t stride, int V_) : V(V_) {
+    x = (const uint8_t*)logits + row * stride * (L::kBits / 8);
+    skip = (int)((uintptr_t)x % 16) / (L::kBits / 8);
+    pieces = reinterpret_cast<const uint4*>(x - skip * (L::kBits / 8));
+    np = (V + skip + E - 1) / E;
+    // pieces inside .. outside - 1 lie in the row as a whole
+    inside = skip ? 1 : 0;
+    outside = (V + skip) / E;
+    take(0, np);
+  }
+  __device__ __forceinline__ void take(int from, int to) {
+    c0 = from;
+    c1 = to;
+    // the pieces that reach over the row's ends, in the threads that have them
+    head = tail = none();
+    const int t = threadIdx.x;
+    if (skip && c0 == 0 && t == 0) head = edge(0);
+    if (outside < np && np - 1 >= c0 && np - 1 < c1 && t == (np - 1 - c0) % kThreads) tail = edge(np - 1);
+  }
+  __device__ __forceinline__ uint4 edge(int c) const {  // the elements that there are
+    uint4 r = none();
     const int i = c * E - skip;
 #pragma unroll
     for (int e = 0; e < E; e++)
@@ -246,44 +293,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
           reinterpret_cast<uint16_t*>(&r)[e] = reinterpret_cast<const uint16_t*>(x)[i + e];
       }
     return r;
-  };
-  auto piece = [&](int c) { return c >= inside && c < outside ? pieces[c] : c < np ? load_edge(c) : none; };
-  // the pieces that reach over the row's ends, in the threads that have them
-  uint4 head = none, tail = none;
-  if (skip && t == 0) head = load_edge(0);
-  if (outside < np && t == (np - 1) % kThreads) tail = load_edge(np - 1);
-  auto load = [&](int c) {
-    uint4 v = inside < outside ? pieces[min(max(c, inside), outside - 1)] : none;
-    if (c >= outside) v = c == np - 1 ? tail : none;
+  }
+  // any piece, in any thread
+  __device__ __forceinline__ uint4 piece(int c) const { return c >= inside && c < outside ? pieces[c] : c < np ? edge(c) : none(); }
+  // one of the thread's own
+  __device__ __forceinline__ uint4 load(int c) const {
+    uint4 v = inside < outside ? pieces[min(max(c, inside), outside - 1)] : none();
+    if (c >= outside) v = c == np - 1 ? tail : none();
     if (c < inside) v = head;
     return v;
-  };
-  // f(piece, its 16 bytes) for every piece of the row, in order within a thread;
-  // the next one's load is on its way meanwhile.  The whole workgroup calls f
-  // together, for pieces past the end too.
-  auto each_piece = [&](auto f) {
-    uint4 next = load(t);
+  }
+  // f(piece, its 16 bytes) for every piece, in order within a thread; the next
+  // one's load is on its way meanwhile.  The whole workgroup calls f together, for
+  // pieces past the end too (of a part: pieces of the next one, which are not this
+  // part's, as nothing).
+  template <class F>
+  __device__ __forceinline__ void each_piece(F f) const {
+    uint4 next = load(c0 + threadIdx.x);
 #pragma unroll 1
-    for (int c = t; c - t < np; c += kThreads) {
-      const uint4 v = next;
+    for (int c = c0 + threadIdx.x; c - (int)threadIdx.x < c1; c += kThreads) {
+      const uint4 v = c < c1 ? next : none();
       next = load(c + kThreads);
       f(c, v);
     }
-  };
-  // the same eight at a time, for little work: f(n, piece, its 16 bytes)
-  auto each_eight = [&](auto f, auto after) {
-#pragma unroll 1
-    for (int c = t; c - t < np; c += 8 * kThreads) {
-      uint4 v[8];
-#pragma unroll
-      for (int n = 0; n < 8; n++) v[n] = load(c + n * kThreads);
-#pragma unroll
-      for (int n = 0; n < 8; n++) f(n, v[n]);
-      after(c);
-    }
-  };
-  // f(index, bits, key) for the piece's elements
-  auto each_element = [&](int c, uint4 v, auto f) {
+  }
+  // f(index, bits, key) for a piece's elements
+  template <class F>
+  __device__ __forceinline__ void each_element(int c, uint4 v, F f) const {
     const int i0 = c * E - skip;
 #pragma unroll 1
     for (int i = i0; i < i0 + E; i += E / 4) {
@@ -292,10 +328,231 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       if (FMT != AQ_F32) f(i + 1, v.x >> 16, q >> 16);
       v.x = v.y, v.y = v.z, v.z = v.w;
     }
-  };
-  auto keys_of = [&](const uint4& v) {
-    return make_uint4(keys_of_word<FMT>(v.x), keys_of_word<FMT>(v.y), keys_of_word<FMT>(v.z), keys_of_word<FMT>(v.w));
-  };
+  }
+  static __device__ __forceinline__ uint32_t largest_key(const uint4& v) {
+    const uint4 q = make_uint4(keys_of_word<FMT>(v.x), keys_of_word<FMT>(v.y), keys_of_word<FMT>(v.z), keys_of_word<FMT>(v.w));
+    if constexpr (FMT == AQ_F32) {
+      return max(max(q.x, q.y), max(q.z, q.w));
+    } else {
+      const u16x2 m = __builtin_elementwise_max(
+          __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.x), __builtin_bit_cast(u16x2, q.y)),
+          __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
+      return max(m.x, m.y);
+    }
+  }
+  // the largest keys of the thread's pieces c, c + 1024, .. (eight), and of all eight
+  __device__ __forceinline__ uint32_t largest_of_eight(int c, uint32_t (&keys)[8]) const {
+    uint4 v[8];
+#pragma unroll
+    for (int n = 0; n < 8; n++) v[n] = load(c + n * kThreads);
+    uint32_t own = 0;
+#pragma unroll
+    for (int n = 0; n < 8; n++) {
+      keys[n] = c + n * kThreads < c1 ? largest_key(v[n]) : 0;
+      own = max(own, keys[n]);
+    }
+    return own;
+  }
+  // the thread's own largest key (and those of its last eight pieces), and the
+  // workgroup's in *best
+  __device__ __forceinline__ uint32_t largest(uint64_t* lds, uint32_t (&keys)[8], uint32_t* best) const {
+    uint32_t own = 0;
+#pragma unroll 1
+    for (int c = c0 + threadIdx.x; c - (int)threadIdx.x < c1; c += 8 * kThreads) own = max(own, largest_of_eight(c, keys));
+    uint32_t b = own;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, d, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = b;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) b = max(b, (uint32_t)lds[i]);
+    *best = b;
+    return own;
+  }
+};
+
+// What the parts of a row leave for each other and for the last kernel.
+struct PartsOfRow {
+  uint64_t mass[kBins];
+  uint64_t seg_mass[kMaxSegments];
+  uint2 list[kList];
+  uint32_t best[kMaxParts];
+  uint32_t n_list, pad[3];
+};
+
+__device__ __forceinline__ Weigh weigh_from(float mx, float T, const double* table) {
+  // 512 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
+  // the maximum would) and every number nothing
+  const bool endless = mx == INFINITY;
+  return Weigh{endless ? 1e39 : (double)mx, endless ? 1.0 : 738.6598609514740 / (double)T, table};
+}
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable) * kOne;
+}
+
+__device__ __forceinline__ void append(Shared& s, int V, int i, uint32_t key) {
+  if ((uint32_t)i >= (uint32_t)V) return;
+  const uint32_t at = atomicAdd(&s.n_list, 1u);
+  if (at < kList) s.list[at] = make_uint2(key, (uint32_t)i);
+}
+
+// Masses of keys above `hi` by segment (of w >= wmin), to seg_mass.  LISTING: keys
+// from `lo` to `hi` go to the list; else the keys equal to hi are counted by
+// segment.
+template <int FMT, bool LISTING>
+__device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, const Weigh& weigh, double wmin, uint32_t lo,
+                                             uint32_t hi, uint64_t* seg_mass) {
+  row.each_piece([&](int c, const uint4& v) {
+    double sum = 0.0;
+    uint32_t ties = 0;
+    row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
+      if (__ballot(key > hi)) {  // the exponential only where a lane asks for it
+        const double w = weigh(Logit<FMT>::value(bits));
+        sum += key > hi && w >= wmin ? w : 0.0;
+      }
+      if (LISTING) {
+        if (key >= lo && key <= hi && c < row.c1) append(s, row.V, i, key);
+      } else {
+        ties += (uint32_t)__popcll(__ballot(key == hi && (uint32_t)i < (uint32_t)row.V));
+      }
+    });
+    sum = wave_group_sum_f64<64>(sum);  // 2^9 whole numbers of up to 2^42: exact
+    if ((threadIdx.x & 63) == 0 && c < row.c1) {  // 64 pieces are a segment
+      seg_mass[c >> 6] = (uint64_t)sum;
+      if (!LISTING) s.seg_ties[c >> 6] = ties;
+    }
+  });
+  __syncthreads();
+}
+
+__device__ __forceinline__ void clear_bins(Shared& s) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+    s.mass[i] = 0;
+    s.count[i] = 0;
+  }
+  __syncthreads();
+}
+
+// ---- long rows that one workgroup each would leave most of the GPU idle for:
+// parts of a row in a workgroup each, three passes, and then sample_kernel for what
+// is left (a list and the segments' masses).  For rows without top-k, whose every
+// exponential is needed; the others are left to sample_kernel whole.
+
+template <int FMT>
+__device__ __forceinline__ Row<FMT> part_of(const void* logits, int V, int64_t stride, int per) {
+  Row<FMT> row(logits, blockIdx.y, stride, V);
+  row.take((int)blockIdx.x * per, min((int)(blockIdx.x + 1) * per, row.np));
+  return row;
+}
+
+__device__ __forceinline__ bool in_parts(const Settings& set, int row, int V) {
+  const int k = set.k ? set.k[row] : set.k0;
+  const float T = set.t ? set.t[row] : set.t0;
+  return !(k > 0 && k < V) && T > 0.0f;
+}
+
+// The part's largest key; the row's bins and list emptied.
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(const void* __restrict__ logits, int V, int64_t stride,
+                                                              int per, Settings set, PartsOfRow* __restrict__ ws) {
+  __shared__ uint64_t red[kWaves];
+  if (!in_parts(set, blockIdx.y, V)) return;
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  PartsOfRow& w = ws[blockIdx.y];
+  uint32_t best, keys8[8];
+  row.largest(red, keys8, &best);
+  if (threadIdx.x == 0) w.best[blockIdx.x] = best;
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < kBins; i += gridDim.x * kThreads) w.mass[i] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) w.n_list = 0;
+}
+
+__device__ __forceinline__ uint32_t best_of(const PartsOfRow& w, int parts) {
+  uint32_t b = 0;
+  for (int i = 0; i < parts; i++) b = max(b, w.best[i]);
+  return b;
+}
+
+// The part's masses by the keys' first 11 bits, added to the row's.
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const void* __restrict__ logits, int V, int64_t stride,
+                                                               int per, Settings set, PartsOfRow* __restrict__ ws) {
+  __shared__ uint64_t mass[kBins];
+  __shared__ double table[kTable];
+  const int b = blockIdx.y;
+  const float p = set.p ? set.p[b] : set.p0, T = set.t ? set.t[b] : set.t0;
+  if (!in_parts(set, b, V) || !(p < 1.0f)) return;
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  PartsOfRow& w = ws[b];
+  const float mx = Logit<FMT>::value_of_key(best_of(w, gridDim.x));
+  if (mx == -INFINITY) return;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = 0;
+  fill_table(table);
+  __syncthreads();
+  const Weigh weigh = weigh_from(mx, T, table);
+  row.each_piece([&](int c, const uint4& v) {
+    row.each_element(c, v, [&](int, uint32_t bits, uint32_t key) {
+      const uint64_t m = (uint64_t)weigh(Logit<FMT>::value(bits));
+      if (m) atomicAdd((unsigned long long*)&mass[key >> (Logit<FMT>::kBits - 11)], (unsigned long long)m);
+    });
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kThreads)
+    if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
+}
+
+// The part's segments above the bin in which the running mass reaches p, and its
+// members of that bin (without top-p: all segments).
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* __restrict__ logits, int V,
+                                                                   int64_t stride, int per, Settings set,
+                                                                   PartsOfRow* __restrict__ ws) {
+  __shared__ Shared s;
+  __shared__ uint32_t at;
+  const int b = blockIdx.y, t = threadIdx.x;
+  const float p = set.p ? set.p[b] : set.p0, T = set.t ? set.t[b] : set.t0, mp = set.m ? set.m[b] : set.m0;
+  if (!in_parts(set, b, V)) return;
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  PartsOfRow& w = ws[b];
+  const float mx = Logit<FMT>::value_of_key(best_of(w, gridDim.x));
+  if (mx == -INFINITY) return;
+  fill_table(s.table);
+  if (t == 0) s.n_list = 0;
+  uint32_t lo = 1, hi = 0;  // no list, everything above
+  if (p < 1.0f) {
+    for (int i = t; i < kBins; i += kThreads) {
+      s.mass[i] = w.mass[i];
+      s.count[i] = 0;
+    }
+    __syncthreads();
+    uint64_t most = 0;
+    lo = find_bin(s, true, most, p).bin << (Logit<FMT>::kBits - 11);
+    hi = lo | ((1u << (Logit<FMT>::kBits - 11)) - 1);
+  }
+  __syncthreads();
+  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) * kOne : 0.0;
+  sum_segments<FMT, true>(s, row, weigh_from(mx, T, s.table), wmin, lo, hi, w.seg_mass);
+  const uint32_t n = s.n_list;  // more than there is room for is counted all the same
+  if (t == 0) at = atomicAdd(&w.n_list, n);
+  __syncthreads();
+  for (uint32_t i = t; i < min(n, (uint32_t)kList) && at + i < kList; i += kThreads) w.list[at + i] = s.list[i];
+}
+
+template <int FMT>
+__global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict__ logits, int V, int64_t stride,
+                                                          const float* __restrict__ u, Settings set,
+                                                          const PartsOfRow* __restrict__ ws, int parts,
+                                                          int64_t* __restrict__ out) {
+  typedef Logit<FMT> L;
+  constexpr int B = L::kBits, E = L::kPer;
+  __shared__ Shared s;
+  const int t = threadIdx.x, row = blockIdx.x, ln = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const float T = set.t ? set.t[row] : set.t0, p = set.p ? set.p[row] : set.p0, mp = set.m ? set.m[row] : set.m0;
+  const int k = set.k ? set.k[row] : set.k0;
+  const Row<FMT> r(logits, row, stride, V);
+  const int skip = r.skip, np = r.np;
 
   // ---- the largest key, each thread's own on the way
   if (t == 0) {
@@ -306,34 +563,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     s.seg_mass[i] = 0;
     s.seg_ties[i] = 0;
   }
-  uint32_t own;
-  {
-    uint32_t acc = 0;
-    each_eight([&](int, const uint4& v) {
-      const uint4 q = keys_of(v);
-      if constexpr (FMT == AQ_F32) {
-        acc = max(max(max(acc, q.x), q.y), max(q.z, q.w));
-      } else {
-        u16x2 a = __builtin_bit_cast(u16x2, acc);
-        a = __builtin_elementwise_max(a, __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.x), __builtin_bit_cast(u16x2, q.y)));
-        a = __builtin_elementwise_max(a, __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
-        acc = __builtin_bit_cast(uint32_t, a);
-      }
-    }, [](int) {});
-    own = FMT == AQ_F32 ? acc : max(acc & 0xFFFF, acc >> 16);
-  }
-  uint32_t best = own;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, d, 64));
-  if (ln == 0) s.red[wave] = best;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWaves; i++) best = max(best, (uint32_t)s.red[i]);
+  // of a row whose parts have been summed: their largest
+  const PartsOfRow* done = parts > 1 && in_parts(set, row, V) && best_of(ws[row], parts) > L::kLowest ? ws + row : nullptr;
+  uint32_t own = 0, best, keys8[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (done)
+    best = best_of(*done, parts);
+  else
+    own = r.largest(s.red, keys8, &best);
   const float mx = L::value_of_key(best);
-  // 512 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
-  // the maximum would) and every number nothing
-  const bool endless = mx == INFINITY;
-  const Weigh weigh = {endless ? 1e39 : (double)mx, endless ? 1.0 : 738.6598609514740 / (double)T, s.table};
+  const Weigh weigh = weigh_from(mx, T, s.table);
   const bool greedy = !(T > 0.0f) || mx == -INFINITY;  // also a row without a token to choose: its first
   const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) * kOne : 0.0;
   if (greedy) {
@@ -343,7 +581,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       uint32_t i0 = 0xFFFFFFFFu;
 #pragma unroll 1
       for (int c = t; c < np && i0 == 0xFFFFFFFFu; c += kThreads)
-        each_element(c, load(c), [&](int i, uint32_t, uint32_t key) {
+        r.each_element(c, r.load(c), [&](int i, uint32_t, uint32_t key) {
           if (key == best && (uint32_t)i < (uint32_t)V) i0 = min(i0, (uint32_t)i);
         });
       atomicMin(&s.token, i0);
@@ -352,48 +590,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     if (t == 0) out[row] = s.token;
     return;
   }
-  if (t < kTable) s.table[t] = exp2((double)t / kTable) * kOne;
-
-  auto clear_bins = [&] {
-    __syncthreads();
-    for (int i = t; i < kBins; i += kThreads) {
-      s.mass[i] = 0;
-      s.count[i] = 0;
-    }
-    __syncthreads();
-  };
-  auto append = [&](int i, uint32_t key) {
-    if ((uint32_t)i >= (uint32_t)V) return;
-    const uint32_t at = atomicAdd(&s.n_list, 1u);
-    if (at < kList) s.list[at] = make_uint2(key, (uint32_t)i);
-  };
-
-  // Masses of keys above `hi` by segment (of w >= wmin).  LISTING: keys from `lo` to
-  // `hi` go to the list; else the keys equal to hi are counted by segment.
-  auto sum_segments = [&](auto listing, uint32_t lo, uint32_t hi) {
-    constexpr bool LISTING = decltype(listing)::value;
-    each_piece([&](int c, const uint4& v) {
-      double sum = 0.0;
-      uint32_t ties = 0;
-      each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-        if (__ballot(key > hi)) {  // the exponential only where a lane asks for it
-          const double w = weigh(L::value(bits));
-          sum += key > hi && w >= wmin ? w : 0.0;
-        }
-        if (LISTING) {
-          if (key >= lo && key <= hi) append(i, key);
-        } else {
-          ties += (uint32_t)__popcll(__ballot(key == hi && (uint32_t)i < (uint32_t)V));
-        }
-      });
-      sum = wave_group_sum_f64<64>(sum);  // 2^9 whole numbers of up to 2^42: exact
-      if (ln == 0) {  // 64 pieces are a segment
-        s.seg_mass[c >> 6] = (uint64_t)sum;
-        s.seg_ties[c >> 6] = ties;
-      }
-    });
-    __syncthreads();
-  };
+  fill_table(s.table);
+  __syncthreads();
 
   const bool by_k = k > 0 && k < V, by_p = p < 1.0f;
   const float uu = u[row];
@@ -407,10 +605,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     const int n = (int)s.n_list, i = t >> 2;
     const uint2 me = i < n ? s.list[i] : make_uint2(0, 0);
     uint32_t r = 0;
-#pragma unroll 1
+#pragma unroll 4
     for (int j = t & 3; j < n; j += 4) {
       const uint2 o = s.list[j];
-      r += o.x > me.x || (o.x == me.x && o.y < me.y);
+      r += (o.x > me.x) | ((o.x == me.x) & (o.y < me.y));
     }
     r += xlane_partner_u32<1>(r);
     r += xlane_partner_u32<2>(r);
@@ -444,9 +642,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     const uint64_t goal = goal_of(__shfl(wave_scan_u64(sum), 63, 64));
     // the kept ones by index
     uint64_t before = 0;
-#pragma unroll 1
-    for (int j = t & 3; j < last; j += 4)
-      if (s.sorted_index[j] < me.y) before += s.sorted_mass[j];
+#pragma unroll 4
+    for (int j = t & 3; j < last; j += 4) before += s.sorted_index[j] < me.y ? s.sorted_mass[j] : 0;
     before += (uint64_t)__shfl_xor((long long)before, 1, 64);
     before += (uint64_t)__shfl_xor((long long)before, 2, 64);
     if ((t & 3) == 0 && i < n && (int)r < last && before <= goal && goal < before + w) out[row] = me.y;
@@ -462,32 +659,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     if (by_mass ? !by_p : !by_k) continue;
     uint64_t most = by_mass ? (by_k ? reach(p, mass) : 0) : (uint64_t)k;
     if (!by_mass && k <= kMaxListK) {
-      clear_bins();
-      atomicAdd(&s.count[own >> (B - 11)], 1u);
-      __syncthreads();
-      const uint32_t least = find_bin(s, false, most, p).bin << (B - 11);
+      const uint32_t least = edge_of_kth(s, own, B, (uint32_t)k);
       if (own >= least) {  // a thread whose largest is less has none
-        uint32_t which = 0;
-        each_eight([&](int n, const uint4& v) {
-          const uint4 q = keys_of(v);
-          uint32_t a;
-          if constexpr (FMT == AQ_F32) {
-            a = max(max(q.x, q.y), max(q.z, q.w));
-          } else {
-            const u16x2 m = __builtin_elementwise_max(
-                __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.x), __builtin_bit_cast(u16x2, q.y)),
-                __builtin_elementwise_max(__builtin_bit_cast(u16x2, q.z), __builtin_bit_cast(u16x2, q.w)));
-            a = max(m.x, m.y);
-          }
-          which |= (a >= least ? 1u : 0u) << n;
-        }, [&](int c) {
+#pragma unroll 1
+        for (int c = t; c < np; c += 8 * kThreads) {
+          if (np > 8 * kThreads) r.largest_of_eight(c, keys8);
+          uint32_t which = 0;  // of eight pieces those that have one
+#pragma unroll
+          for (int n = 0; n < 8; n++) which |= (keys8[n] >= least ? 1u : 0u) << n;
           for (; which; which &= which - 1) {
             const int d = c + __builtin_ctz(which) * kThreads;
-            each_element(d, load(d), [&](int i, uint32_t, uint32_t key) {
-              if (key >= least) append(i, key);
+            r.each_element(d, r.load(d), [&](int i, uint32_t, uint32_t key) {
+              if (key >= least) append(s, V, i, key);
             });
           }
-        });
+        }
       }
       __syncthreads();
       from_list = s.n_list <= kList;
@@ -504,7 +690,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 #pragma unroll 1
     for (int shift = B; shift > 0;) {
       const int bits = min(11, shift), next = shift - bits;
-      clear_bins();
+      clear_bins(s);
       const bool first = shift == B;
       auto see = [&](uint32_t key) {
         if (!first && key >> (shift & 31) != prefix) return;
@@ -513,11 +699,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         const uint64_t w = (uint64_t)weigh(L::value_of_key(key));
         if (w) atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)w);
       };
-      if (from_list) {
+      if (first && done) {
+        for (int i = t; i < kBins; i += kThreads) s.mass[i] = done->mass[i];
+      } else if (from_list) {
         const int n = (int)s.n_list;
         for (int i = t; i < n; i += kThreads) see(s.list[i].x);
       } else {
-        each_piece([&](int c, const uint4& v) { each_element(c, v, [&](int, uint32_t, uint32_t key) { see(key); }); });
+        r.each_piece([&](int c, const uint4& v) { r.each_element(c, v, [&](int, uint32_t, uint32_t key) { see(key); }); });
       }
       __syncthreads();
       uint64_t left = most - (by_mass ? above_mass : above);
@@ -529,7 +717,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       shift = next;
       if (shift == 0) each = s.mass[f.bin] / s.count[f.bin];  // of one of the ties
       if (first && by_mass && !by_k) {
-        sum_segments(std::true_type{}, prefix << next, prefix << next | ((1u << next) - 1));
+        if (done) {
+          if (t == 0) s.n_list = done->n_list;
+          for (int i = t; i < (int)min(done->n_list, (uint32_t)kList); i += kThreads) s.list[i] = done->list[i];
+          __syncthreads();
+        } else {
+          sum_segments<FMT, true>(s, r, weigh, wmin, prefix << next, prefix << next | ((1u << next) - 1), s.seg_mass);
+        }
         summed = from_list = s.n_list <= kList;
       }
     }
@@ -549,6 +743,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   const double ecut = cut.key ? weigh(L::value_of_key(cut.key)) : 0.0;
   const uint64_t wcut = ecut >= wmin ? (uint64_t)ecut : 0;
   __syncthreads();
+  if (done && (!by_p || summed)) {
+    summed = true;
+    for (int i = t; i < (np + 63) / 64; i += kThreads) s.seg_mass[i] = done->seg_mass[i];
+    __syncthreads();
+  }
   if (from_list) {
     for (int i = t; i < (int)s.n_list; i += kThreads) {
       const uint2 y = s.list[i];
@@ -561,7 +760,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       }
     }
   } else if (!summed) {
-    sum_segments(std::false_type{}, 0, cut.key);
+    sum_segments<FMT, false>(s, r, weigh, wmin, 0, cut.key, s.seg_mass);
   }
   __syncthreads();
 
@@ -577,25 +776,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     uint64_t all;
     tie0 = (uint32_t)block_scan_u64(ties, s.red, &all) - ties;
     uint64_t sum = 0;
-    uint32_t r = tie0;
+    uint32_t rank = tie0;
     for (int i = s0; i < s1; i++) {
-      sum += s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(r, cut.ties));
-      r += s.seg_ties[i];
+      sum += s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(rank, cut.ties));
+      rank += s.seg_ties[i];
     }
     m0 = block_scan_u64(sum, s.red, &total) - sum;
     const uint64_t goal = goal_of(total);
     if (m0 <= goal && goal < m0 + sum) {
       uint64_t at = m0;
-      r = tie0;
+      rank = tie0;
       for (int i = s0; i < s1; i++) {
-        const uint64_t m = s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(r, cut.ties));
+        const uint64_t m = s.seg_mass[i] + wcut * (uint64_t)min(s.seg_ties[i], cut.ties - min(rank, cut.ties));
         if (at <= goal && goal < at + m) {
           s.segment = i;
           s.seg_before = goal - at;  // what is left of the goal inside
-          s.seg_rank = r;
+          s.seg_rank = rank;
         }
         at += m;
-        r += s.seg_ties[i];
+        rank += s.seg_ties[i];
       }
     }
   }
@@ -603,25 +802,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   // ---- the token: one wave, a piece a lane
   if (wave == 0) {
     const int c = (int)s.segment * 64 + ln;
-    const uint4 v = piece(c);
+    const uint4 v = r.piece(c);
     uint32_t ties = 0;
-    each_element(c, v, [&](int i, uint32_t, uint32_t key) { ties += key == cut.key && (uint32_t)i < (uint32_t)V; });
+    r.each_element(c, v, [&](int i, uint32_t, uint32_t key) { ties += key == cut.key && (uint32_t)i < (uint32_t)V; });
     const uint32_t rank = s.seg_rank + (uint32_t)wave_scan_u64(ties) - ties;
-    auto mass_of = [&](int i, uint32_t bits, uint32_t key, uint32_t& r) -> uint64_t {
+    auto mass_of = [&](int i, uint32_t bits, uint32_t key, uint32_t& n) -> uint64_t {
       if ((uint32_t)i >= (uint32_t)V || key < cut.key) return 0;
-      if (key == cut.key) return r++ < cut.ties ? wcut : 0;
+      if (key == cut.key) return n++ < cut.ties ? wcut : 0;
       const double d = weigh(L::value(bits));
       return d >= wmin ? (uint64_t)d : 0;
     };
     uint64_t sum = 0;
-    uint32_t r = rank;
-    each_element(c, v, [&](int i, uint32_t bits, uint32_t key) { sum += mass_of(i, bits, key, r); });
+    uint32_t n = rank;
+    r.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) { sum += mass_of(i, bits, key, n); });
     uint64_t at = wave_scan_u64(sum) - sum;
     const uint64_t goal = s.seg_before;
-    r = rank;
+    n = rank;
     if (at <= goal && goal < at + sum)
-      each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-        const uint64_t w = mass_of(i, bits, key, r);
+      r.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
+        const uint64_t w = mass_of(i, bits, key, n);
         if (at <= goal && goal < at + w) out[row] = i;
         at += w;
       });
@@ -630,10 +829,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 
 }  // namespace
 
+// Workgroups a row is split into: enough to fill the GPU, 1024 pieces each at
+// least, for rows that have 2048 (top-p of 64 rows of 128256: one workgroup each
+// 106 us, four 58; of one row in fp32 118 us and, in 31, 46).  One setting of top-k for all rows rules the split out.
+static int parts_of(int64_t B, int64_t V, int dtype, bool top_k) {
+  const int64_t per = dtype == AQ_F32 ? 4 : 8, pieces = V / per;
+  if (top_k || pieces < 2048) return 1;
+  return (int)std::min<int64_t>(std::min<int64_t>(kMaxParts, 256 / B), pieces / 1024);
+}
+
+extern "C" int64_t aq_sample_workspace(int64_t B, int64_t V, int dtype, int32_t top_k0) {
+  if (B <= 0 || B > 65535 || V <= 0 || V > kMaxVocab || dtype < AQ_F16 || dtype > AQ_F32) return -1;
+  return parts_of(B, V, dtype, top_k0 > 0 && top_k0 < V) > 1 ? B * (int64_t)sizeof(PartsOfRow) : 0;
+}
+
 extern "C" int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t stride, const float* u,
                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                          float temperature0, int32_t top_k0, float top_p0, float min_p0, int64_t* tokens,
-                         void* stream) {
+                         void* workspace, int64_t ws_bytes, void* stream) {
   AQ_CHECK_ARG(logits && u && tokens, "aq_sample: null pointer");
   AQ_CHECK_ARG(dtype == AQ_F16 || dtype == AQ_BF16 || dtype == AQ_F32, "aq_sample: dtype %d (fp16, bf16, fp32)", dtype);
   AQ_CHECK_ARG(V > 0 && V <= kMaxVocab, "aq_sample: %lld logits a row (1 .. %lld)", (long long)V, (long long)kMaxVocab);
@@ -646,9 +859,27 @@ extern "C" int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, in
                "aq_sample: misaligned buffer");
   const Settings set = {temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0};
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)B), block(kThreads);
-#define AQ_SAMPLE(F) \
-  hipLaunchKernelGGL(sample_kernel<F>, grid, block, 0, s, logits, (int)V, stride, u, set, tokens)
+  // (greedy rows need one pass and no exponential)
+  int parts = parts_of(B, V, dtype, !top_k && ((top_k0 > 0 && top_k0 < V) || (!temperature && !(temperature0 > 0.0f))));
+  AQ_CHECK_ARG(!workspace || (uintptr_t)workspace % 16 == 0, "aq_sample: the workspace must be 16-byte aligned");
+  if (parts > 1 && (!workspace || ws_bytes < B * (int64_t)sizeof(PartsOfRow))) parts = 1;
+  PartsOfRow* ws = (PartsOfRow*)workspace;
+  // parts of whole segments; a misaligned row has one piece more
+  const int64_t pieces = V / (16 / size) + 2;
+  const int per = (int)(aq::ceil_div(aq::ceil_div(pieces, parts), 64) * 64);
+  parts = (int)aq::ceil_div(pieces, per);
+  const dim3 grid((unsigned)B), cut((unsigned)parts, (unsigned)B), block(kThreads);
+#define AQ_SAMPLE(F)                                                                                                  \
+  do {                                                                                                                \
+    if (parts > 1) {                                                                                                  \
+      hipLaunchKernelGGL(sample_max_kernel<F>, cut, block, 0, s, logits, (int)V, stride, per, set, ws);               \
+      if (top_p || top_p0 < 1.0f)                                                                                     \
+        hipLaunchKernelGGL(sample_bins_kernel<F>, cut, block, 0, s, logits, (int)V, stride, per, set, ws);            \
+      hipLaunchKernelGGL(sample_segments_kernel<F>, cut, block, 0, s, logits, (int)V, stride, per, set, ws);          \
+    }                                                                                                                 \
+    hipLaunchKernelGGL(sample_kernel<F>, grid, block, 0, s, logits, (int)V, stride, u, set, (const PartsOfRow*)ws,    \
+                       parts, tokens);                                                                                \
+  } while (0)
   if (dtype == AQ_F16) AQ_SAMPLE(AQ_F16);
   else if (dtype == AQ_BF16) AQ_SAMPLE(AQ_BF16);
   else AQ_SAMPLE(AQ_F32);

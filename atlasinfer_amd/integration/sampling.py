@@ -65,8 +65,11 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 
     if (logits.stride(1) != 1 and V > 1) or (logits.stride(0) < V and B > 1):
         logits = logits.contiguous()
     stride = max(logits.stride(0), V)
+    L, dtype = _lib.load(), _DTYPES[logits.dtype]
+    k0 = min(max(int(k0), 0), V)
+    size = L.aq_sample_workspace(B, V, dtype, k0)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     with _lib.on_device(dev):
-        _lib.check(_lib.load().aq_sample(logits.data_ptr(), _DTYPES[logits.dtype], B, V, stride, u.data_ptr(), tp, kp,
-                                         pp, mp, t0, min(max(int(k0), 0), V), p0, m0, out.data_ptr(),
-                                         _lib.stream_of(dev)), "aq_sample")
+        _lib.check(L.aq_sample(logits.data_ptr(), dtype, B, V, stride, u.data_ptr(), tp, kp, pp, mp, t0, k0, p0, m0,
+                               out.data_ptr(), _lib.ptr(ws), size, _lib.stream_of(dev)), "aq_sample")
     return out

@@ -519,10 +519,16 @@ int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* 
  *   u       f32 [B], in [0, 1)      tokens  int64 [B] (out)
  *   temperature, top_p, min_p  f32 [B], top_k int32 [B]: one setting a row, or
  *           NULL: temperature0, top_p0, min_p0, top_k0 for all rows
+ *   workspace  aq_sample_workspace(B, V, dtype, top_k0) bytes (top_k0 = 0 with
+ *           top_k), 16-byte aligned, no initial contents; calls that overlap in time
+ *           must not share one.  It lets several workgroups share a long row; with
+ *           less, or NULL, one workgroup takes each.  The tokens are the same.
  */
+int64_t aq_sample_workspace(int64_t B, int64_t V, int dtype, int32_t top_k0);
 int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t stride, const float* u,
               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
-              float temperature0, int32_t top_k0, float top_p0, float min_p0, int64_t* tokens, void* stream);
+              float temperature0, int32_t top_k0, float top_p0, float min_p0, int64_t* tokens, void* workspace,
+              int64_t ws_bytes, void* stream);
 
 /*
  * Residual add and normalisation of `rows` rows of n fp16 (n a multiple of

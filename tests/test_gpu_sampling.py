@@ -130,6 +130,45 @@ def test_strides_largest_vocabulary_and_distribution():
     assert ((share - torch.softmax(row[0].cpu(), 0)).abs() <= 1.0 / n).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,V", [(1, 16384), (1, 50272), (3, 50273), (2, 128256), (100, 20011), (1, 1 << 18)])
+def test_rows_in_parts(dtype, B, V):
+    """Long rows of small batches are shared by workgroups: the same tokens as
+    the plain form's and as one workgroup's, misaligned rows, ties past the
+    list's room, greedy and top-k rows among others, a row without a token."""
+    from atlasinfer_amd import _lib
+    g = torch.Generator(device=DEV).manual_seed(V + B)
+    n = min(B, 4)
+    wide = torch.empty(B, V + 3, dtype=dtype, device=DEV)
+    wide[:, 1:V + 1] = _logits(g, B, V, dtype, 1.5)
+    x, u = wide[:, 1:V + 1], torch.rand(B, generator=g, device=DEV)
+    for t, k, p, m in [(0.8, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (1.2, 0, 1.0, 0.03), (3.0, 0, 0.6, 0.01)]:
+        assert _lib.load().aq_sample_workspace(B, V, 0, k) > 0 or dtype == torch.float32 or B > 64
+        got = sample_tokens(x, u, t, k, p, m)
+        want = reference(x[:n], u[:n], [f32(t)] * n, [k] * n, [f32(p)] * n, [f32(m)] * n)
+        assert torch.equal(got[:n].cpu(), want), (t, k, p, m)
+        # one workgroup a row: the same call with settings that rule the parts out
+        one = torch.empty_like(got)
+        _lib.check(_lib.load().aq_sample(x.data_ptr(), [torch.float16, torch.bfloat16, torch.float32].index(dtype), B, V,
+                                         x.stride(0), u.data_ptr(), None, None, None, None, t, k, p, m, one.data_ptr(),
+                                         None, 0, _lib.stream_of(DEV)), "aq_sample")
+        assert torch.equal(one, got)
+    flat = torch.zeros(4, V, dtype=dtype, device=DEV)  # one value; two; none; one number among -inf
+    flat[1, ::3] = 1.0
+    flat[2] = -float("inf")
+    flat[3] = -float("inf")
+    flat[3, V // 2] = -3.0
+    v = torch.tensor([0.999, 0.3, 0.5, 0.7], device=DEV)
+    for p in (1.0, 0.7):
+        assert torch.equal(sample_tokens(flat, v, 1.0, 0, p).cpu(), reference(flat, v, [1.0] * 4, [0] * 4, [f32(p)] * 4, [0.0] * 4))
+    # rows of every kind in one call
+    y, w = x[:n].contiguous(), u[:n].contiguous()
+    t = torch.tensor([0.0, 0.7, 1.0, 1.5][:n], device=DEV)
+    k = torch.tensor([0, 40, 0, 0][:n], dtype=torch.int32, device=DEV)
+    p = torch.tensor([0.9, 0.9, 1.0, 0.95][:n], device=DEV)
+    assert torch.equal(sample_tokens(y, w, t, k, p).cpu(), reference(y, w, t.tolist(), k.tolist(), p.tolist(), [0.0] * n))
+
+
 def test_in_a_graph():
     g = torch.Generator(device=DEV).manual_seed(6)
     x, u = _logits(g, 3, 20000, torch.float16), torch.rand(3, generator=g, device=DEV)
@@ -142,7 +181,15 @@ def test_in_a_graph():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = sample_tokens(x, u, t, 50, 0.9)
+    whole, u2 = _logits(g, 2, 128256, torch.float16), torch.rand(2, generator=g, device=DEV)
+    parts = torch.cuda.CUDAGraph()
+    sample_tokens(whole, u2, 0.9, 0, 0.95)
+    with torch.cuda.graph(parts):
+        out2 = sample_tokens(whole, u2, 0.9, 0, 0.95)
     for i in range(8):
+        whole.copy_(_logits(g, 2, 128256, torch.float16))
+        parts.replay()
+        assert torch.equal(out2, sample_tokens(whole, u2, 0.9, 0, 0.95))
         x.copy_(_logits(g, 3, 20000, torch.float16))
         u.copy_(torch.rand(3, generator=g, device=DEV))
         t.fill_(0.2 * i)
