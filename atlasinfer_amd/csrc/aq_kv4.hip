@@ -267,13 +267,42 @@ __device__ __forceinline__ half2v pair_of(uint32_t w, int n, uint32_t magic) {
   return __builtin_bit_cast(half2v, (w & 0x000F000Fu) | magic) - big;
 }
 
-__device__ __forceinline__ uint32_t splat_lo(uint32_t x) { return (x & 0xFFFF) | x << 16; }
-__device__ __forceinline__ uint32_t splat_hi(uint32_t x) { return (x >> 16) | (x & 0xFFFF0000u); }
+// The same pair with 1024 (n even) or 64 (n odd: a nibble four bits up counts 1 each
+// under that exponent) left in, one instruction a pair.
+__device__ __forceinline__ uint32_t raised_pair_of(uint32_t w, int n, uint32_t magic, uint32_t magic64) {
+  if (n & 2) w >>= 8;
+  return n & 1 ? (w & 0x00F000F0u) | magic64 : (w & 0x000F000Fu) | magic;
+}
 
-// The value of lane n of each row of 16 lanes, in the whole row.
+// Words n of the lanes (l, r), r = lane / 16, a group of keys each (D = 128: group r
+// in words 0 .. 3; D = 64: group r / 2 in words 0, 1), exchanged among the r so that
+// word n is of group n in every lane: word_of says which word of the group.
+template <int D>
+__device__ __forceinline__ void groups_apart(u32x4& w) {
+  if constexpr (D == 128) {
+    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    w = u32x4{c[0], c[1], d[0], d[1]};
+  } else {
+    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[1], false, false);
+    w = u32x4{a[0], a[1], 0, 0};
+  }
+}
+template <int D>
+__device__ __forceinline__ int word_of(int r) {
+  return D == 128 ? r : 2 * (r & 1) + (r >> 1);
+}
+
+// The pair of lane n of each row of 16 lanes, in the whole row: one instruction for
+// both words (the builtin has one word only, the intrinsic behind it two).
+extern "C" __device__ uint64_t update_dpp_u64(uint64_t old, uint64_t x, int ctrl, int rows, int banks,
+                                              bool bound) __asm("llvm.amdgcn.update.dpp.i64");
 template <int N>
-__device__ __forceinline__ uint32_t row16_bcast(uint32_t x) {
-  return __builtin_amdgcn_mov_dpp(x, 0x150 + N, 0xF, 0xF, false);  // row_newbcast
+__device__ __forceinline__ uint2 row16_bcast(uint2 x) {
+  const uint64_t v = update_dpp_u64(0, (uint64_t)x.y << 32 | x.x, 0x150 + N, 0xF, 0xF, true);  // row_newbcast
+  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
 }
 
 __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_f32<6>(xlane_level_max_f32<5>(x)); }
@@ -283,19 +312,22 @@ __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_
 // of 32 slots: scores of 2 x 16 slots against up to 16 query heads
 // (mfma 16 x 16 x 32, keys as rows, so that a lane's results are 2 x 4 slots of
 // one head), the running softmax of a head in the four lanes that hold it, the
-// numerators rounded to fp16 as the second product's operand, which they are
-// without an exchange, and the values' rows.  The denominator is the product of
-// the same numerators with ones, so rounding them does not shift the mean.
-// Dequantized keys and values are rounded to fp16 once each (fma): four packed
-// instructions for eight elements; scales applied to exact sums in f32 instead
-// would take twice as many and gain a factor of two in error (4e-4 of the result,
-// 2e-4 of which is the output's own rounding).
-// Bound by HBM and by unpacking together: a step of 32 slots of D = 128 is about
-// 400 vector instructions a wave for 5 KiB (32 sequences x 8 heads of up to 16384
-// slots, half of them in use: 336 MB in 88 us, 3.8 TB/s, of which instruction
-// issue alone is 45).
+// numerators as the second product's operand, which they are without an exchange,
+// and the values' rows.
+//   Scores: the products of one group's codes, whole numbers as fp16, with the
+// query are exact to f32 and scaled there; the minima meet the sums of the query
+// in a product of f32 (16 x 16 x 4).  Keys rounded to fp16 (a fused multiply-add a
+// pair, the scales then inside the product) gave 4.2e-4 of the result against 2.1e-4
+// of the output's own rounding, at 89 us for the long case below instead of 95.
+//   Numerators are two fp16 numbers each, the second what the first leaves over: with
+// one alone the error is 3.0e-4 and 91 us.  With both 2.6e-4: what is left beside
+// the output's rounding is that of the values s c + m to fp16, once each (fma).  The
+// denominator is the product of the same numerators with ones.
+// Bound by HBM and by the instructions together: a step of 32 slots of D = 128 is 290
+// vector and 29 matrix instructions a wave for 5 KiB (32 sequences x 8 heads of up to
+// 16384 slots, half of them in use: 336 MB in 95 us, 3.5 TB/s).
 template <int D>
-__global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
+__global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, Cache4 c,
     const int64_t* __restrict__ pos_p, int pos_stride, int H, int Hkv, int hb, int slots, int sinks, float scale2,
     float q_scale, const uint16_t* __restrict__ rcos, const uint16_t* __restrict__ rsin, int64_t max_pos, int nt,
@@ -327,14 +359,15 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
   // a step's loads: whole rows and blocks, in the buffers whatever the step
   struct Step {
     u32x4 k[2], v[ND / 4];
-    uint32_t kpar[2];
+    uint32_t kpar[2], kscale[2];  // (s, m) of (row l, group r % NK) and of (row 4 r + l % 4, group l / 4)
     uint2 vpar;
   };
   const int kr = r * (D / 8);
   auto load = [&](Step& x, int blk) {
     blk = min(blk, nblk - 1);
     const uint8_t* kb = kc + (int64_t)blk * (kSlotBlock * D / 2) + l * (D / 2) + kr;
-    const uint16_t* pb = kp + (int64_t)blk * (kSlotBlock * NK * 2) + (l * NK + (D == 128 ? r : r >> 1)) * 2;
+    const uint16_t* pb = kp + (int64_t)blk * (kSlotBlock * NK * 2) + (l * NK + r % NK) * 2;
+    const uint16_t* sb = kp + (int64_t)blk * (kSlotBlock * NK * 2) + ((4 * r + (l & 3)) * NK + (l >> 2) % NK) * 2;
     const uint8_t* vb = vc + (int64_t)blk * (16 * D) + ln * 16;
 #pragma unroll
     for (int tt = 0; tt < 2; tt++) {
@@ -345,6 +378,7 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
         x.k[tt] = u32x4{y.x, y.y, 0, 0};
       }
       x.kpar[tt] = *reinterpret_cast<const uint32_t*>(pb + tt * 16 * NK * 2);
+      x.kscale[tt] = *reinterpret_cast<const uint32_t*>(sb + tt * 16 * NK * 2);
     }
 #pragma unroll
     for (int e = 0; e < ND / 4; e++) x.v[e] = *reinterpret_cast<const u32x4*>(vb + e * 1024);
@@ -400,21 +434,33 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
   }
   __syncthreads();
 
-  // the queries as the scores' second operand: head l, elements
-  // (D / 4) r + 8 kk + the order in which pair_of gives a word's nibbles
+  // the queries as the scores' second operand: head l, elements 32 kk +
+  // 8 word_of(r) + the order in which pair_of gives a word's nibbles; what the
+  // nibbles' 1024 and 64 add to the products of group r, and the sum of the queries
+  // over it, which the keys' minima multiply
   half8v qv[NK];
+  float lift = 0.0f, qsum = 0.0f;
 #pragma unroll
-  for (int kk = 0; kk < NK; kk++)
+  for (int kk = 0; kk < NK; kk++) {
+    half8v offs, ones;
 #pragma unroll
-    for (int n = 0; n < 8; n++) qv[kk][n] = bits_to_h(qs[l][(D / 4) * r + 8 * kk + (n >> 1) + 4 * (n & 1)]);
+    for (int n = 0; n < 8; n++) {
+      qv[kk][n] = bits_to_h(qs[l][32 * kk + 8 * word_of<D>(r) + (n >> 1) + 4 * (n & 1)]);
+      offs[n] = (f16)(n & 2 ? -64.0f : -1024.0f);
+      ones[n] = (f16)1.0f;
+    }
+    const float a = __builtin_amdgcn_mfma_f32_16x16x32_f16(offs, qv[kk], float4v{0, 0, 0, 0}, 0, 0, 0)[0];
+    const float b = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qv[kk], float4v{0, 0, 0, 0}, 0, 0, 0)[0];
+    if (r == kk) lift = a, qsum = b;
+  }
 
   float4v o[ND], den;
 #pragma unroll
   for (int e = 0; e < ND; e++) o[e] = float4v{0, 0, 0, 0};
   den = float4v{0, 0, 0, 0};
   float m = -INFINITY;
-  uint32_t magic = 0x64006400u;
-  asm volatile("" : "+v"(magic));
+  uint32_t magic = 0x64006400u, magic64 = 0x54005400u;
+  asm volatile("" : "+v"(magic), "+v"(magic64));
   half8v ones;
 #pragma unroll
   for (int n = 0; n < 8; n++) ones[n] = (f16)1.0f;
@@ -433,10 +479,12 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
             y.k[tt][kk] = new_k[r * (D / 32) + kk];
             if (owner) *reinterpret_cast<uint32_t*>(kc + (int64_t)slot * (D / 2) + kr + kk * 4) = y.k[tt][kk];
           }
-          y.kpar[tt] = new_kp[D == 128 ? r : r >> 1];
-          if (owner && (D == 128 || (r & 1) == 0))
-            *reinterpret_cast<uint32_t*>(kp + ((int64_t)slot * NK + (D == 128 ? r : r >> 1)) * 2) = y.kpar[tt];
+          y.kpar[tt] = new_kp[r % NK];
+          if (owner && r < NK) *reinterpret_cast<uint32_t*>(kp + ((int64_t)slot * NK + r) * 2) = y.kpar[tt];
         }
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++)
+        if (16 * tt + 4 * r + (l & 3) == at) y.kscale[tt] = new_kp[(l >> 2) % NK];
       if (r == ((at & 15) >> 2)) {
 #pragma unroll
         for (int e = 0; e < ND; e++) {
@@ -463,26 +511,49 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
       if (s0 + 4 * r + i > last) vpar.x &= 0xFFFF0000u, vpar.y &= 0xFFFF0000u;
       if (s0 + 16 + 4 * r + i > last) vpar.x &= 0xFFFFu, vpar.y &= 0xFFFFu;
     }
-    float x[8];
+    // q . (s c + m) = sum over groups of s (q . (c + lift)) - s (q . lift) + m sum(q):
+    // products of whole numbers with q, scaled in f32
+    float4v acc[2];
+    float s_of[2];
 #pragma unroll
     for (int tt = 0; tt < 2; tt++) {
-      const half2v s2 = __builtin_bit_cast(half2v, splat_lo(y.kpar[tt])), m2 = __builtin_bit_cast(half2v, splat_hi(y.kpar[tt]));
-      float4v acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int kk = 0; kk < NK; kk++) {
-        half8v a;
-#pragma unroll
-        for (int n = 0; n < 4; n++) {
-          const half2v v2 = __builtin_elementwise_fma(pair_of(y.k[tt][kk], n, magic), s2, m2);
-          a[2 * n] = v2.x;
-          a[2 * n + 1] = v2.y;
-        }
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qv[kk], acc, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) x[4 * tt + i] = acc[i] * scale2;
+      groups_apart<D>(y.k[tt]);
+      s_of[tt] = (float)bits_to_h((uint16_t)y.kscale[tt]);
+      acc[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)bits_to_h((uint16_t)(y.kpar[tt] >> 16)), qsum, float4v{0, 0, 0, 0}, 0, 0, 0);
+      acc[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)bits_to_h((uint16_t)y.kpar[tt]), lift, acc[tt], 0, 0, 0);
     }
+    auto group = [&](auto gc) {
+      constexpr int g = decltype(gc)::value;
+      float4v d[2];
+#pragma unroll
+      for (int tt = 0; tt < 2; tt++) {
+        u32x4 a;
+#pragma unroll
+        for (int n = 0; n < 4; n++) a[n] = raised_pair_of(y.k[tt][g], n, magic, magic64);
+        d[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, a), qv[g], float4v{0, 0, 0, 0}, 0, 0, 0);
+      }
+      auto of_slot = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const uint2 p = row16_bcast<4 * g + i>(make_uint2(__builtin_bit_cast(uint32_t, s_of[0]), __builtin_bit_cast(uint32_t, s_of[1])));
+        acc[0][i] = fmaf(__builtin_bit_cast(float, p.x), d[0][i], acc[0][i]);
+        acc[1][i] = fmaf(__builtin_bit_cast(float, p.y), d[1][i], acc[1][i]);
+      };
+      of_slot(std::integral_constant<int, 0>{});
+      of_slot(std::integral_constant<int, 1>{});
+      of_slot(std::integral_constant<int, 2>{});
+      of_slot(std::integral_constant<int, 3>{});
+    };
+    group(std::integral_constant<int, 0>{});
+    group(std::integral_constant<int, 1>{});
+    if constexpr (NK == 4) {
+      group(std::integral_constant<int, 2>{});
+      group(std::integral_constant<int, 3>{});
+    }
+    float x[8];
+#pragma unroll
+    for (int n = 0; n < 8; n++) x[n] = acc[n >> 2][n & 3];
     if (edge) {
+      asm volatile("");  // a branch: few blocks are at the edge
 #pragma unroll
       for (int n = 0; n < 8; n++)
         if (s0 + 16 * (n >> 2) + 4 * r + (n & 3) > last) x[n] = -INFINITY;
@@ -490,33 +561,37 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
     float mx = x[0];
 #pragma unroll
     for (int n = 1; n < 8; n++) mx = fmaxf(mx, x[n]);
-    mx = fmaxf(m, max_quarters(mx));
+    mx = fmaxf(m, max_quarters(mx) * scale2);
     if (__ballot(mx != m)) {
-      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+      const float f = __builtin_amdgcn_exp2f(m - mx);  // every block has a slot in use: mx is a number
 #pragma unroll
       for (int e = 0; e < ND; e++) o[e] *= f;
       den *= f;
       m = mx;
     }
     // numerators, slot pairs (t = 0, 1) as pair_of gives the values'
-    half8v pv;
+    half8v pv, pl;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      pv[2 * i] = rn_h(x[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i] - m));
-      pv[2 * i + 1] = rn_h(x[4 + i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[4 + i] - m));
+    for (int n = 0; n < 8; n++) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(x[4 * (n & 1) + (n >> 1)], scale2, -m));
+      pv[n] = rn_h(p);
+      pl[n] = rn_h(p - (float)pv[n]);
     }
     den = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pv, den, 0, 0, 0);
+    den = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl, den, 0, 0, 0);
     auto values = [&](auto gc) {
       constexpr int g = decltype(gc)::value;
       half2v s2[4], m2[4];
-      s2[0] = __builtin_bit_cast(half2v, row16_bcast<4 * g>(vpar.x));
-      s2[1] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 1>(vpar.x));
-      s2[2] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 2>(vpar.x));
-      s2[3] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 3>(vpar.x));
-      m2[0] = __builtin_bit_cast(half2v, row16_bcast<4 * g>(vpar.y));
-      m2[1] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 1>(vpar.y));
-      m2[2] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 2>(vpar.y));
-      m2[3] = __builtin_bit_cast(half2v, row16_bcast<4 * g + 3>(vpar.y));
+      auto of_slot = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const uint2 p = row16_bcast<4 * g + i>(vpar);
+        s2[i] = __builtin_bit_cast(half2v, p.x);
+        m2[i] = __builtin_bit_cast(half2v, p.y);
+      };
+      of_slot(std::integral_constant<int, 0>{});
+      of_slot(std::integral_constant<int, 1>{});
+      of_slot(std::integral_constant<int, 2>{});
+      of_slot(std::integral_constant<int, 3>{});
 #pragma unroll
       for (int e = 2 * g; e < 2 * g + 2; e++) {
         half8v a;
@@ -527,6 +602,7 @@ __global__ __launch_bounds__(64 * kMaxWaves4, 2) void kv4_attention_kernel(
           a[2 * i + 1] = v2.y;
         }
         o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pv, o[e], 0, 0, 0);
+        o[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[e], 0, 0, 0);
       }
     };
     values(std::integral_constant<int, 0>{});
@@ -722,7 +798,9 @@ extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_
   int64_t max_pos = sinks < 0 ? slots : INT32_MAX;
   if (rope_cos) max_pos = std::min(max_pos, rope_rows);
   const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
-  const float scale2 = scale * 1.44269504f;
+  // (a negative scale: the queries' sign, so that the largest product has the largest score)
+  const float scale2 = fabsf(scale) * 1.44269504f;
+  if (scale < 0.0f) q_scale = -q_scale;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(Hkv * sp.hb), (unsigned)B, (unsigned)sp.ns);
   const size_t lds = (size_t)sp.nw * kHeads * (D + 2) * 4;
