@@ -798,9 +798,10 @@ extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_
   int64_t max_pos = sinks < 0 ? slots : INT32_MAX;
   if (rope_cos) max_pos = std::min(max_pos, rope_rows);
   const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
-  // (a negative scale: the queries' sign, so that the largest product has the largest score)
-  const float scale2 = fabsf(scale) * 1.44269504f;
-  if (scale < 0.0f) q_scale = -q_scale;
+  // the kernel's is above 0, so that the largest product has the largest score and a
+  // masked one, -inf, stays it: a negative scale's sign and a zero go to the queries
+  const float scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
+  if (!(scale > 0.0f)) q_scale = scale == 0.0f ? 0.0f : -q_scale;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(Hkv * sp.hb), (unsigned)B, (unsigned)sp.ns);
   const size_t lds = (size_t)sp.nw * kHeads * (D + 2) * 4;

@@ -26,8 +26,8 @@ struct WindowArgs {
   const int* starts;
   uint16_t* out;
   int H, G, M, N, window, sinks, blocks, items, per;
-  float c;  // |scale| log2(e)
-  uint32_t flip;  // sign bits of a negative scale, for the queries
+  float c;  // |scale| log2(e), above 0: a masked score, -inf, times it stays that
+  uint32_t keep, flip;  // for the queries' bits: none for a scale of 0, the sign of a negative one
 };
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
@@ -116,7 +116,8 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
 #pragma unroll
     for (int s = 0; s < D / 16; s++) {
       uint4 x = *reinterpret_cast<const uint4*>(qp + 16 * s);
-      x.x ^= a.flip, x.y ^= a.flip, x.z ^= a.flip, x.w ^= a.flip;
+#pragma unroll
+      for (int i = 0; i < 4; i++) (&x.x)[i] = ((&x.x)[i] & a.keep) ^ a.flip;
       qv[s] = __builtin_bit_cast(half8v, x);
     }
   }
@@ -344,7 +345,8 @@ extern "C" int aq_window_attention(const void* q, const void* k, const void* v, 
   a.N = (int)N;
   a.window = (int)std::min<int64_t>(window, N);
   a.sinks = (int)std::min<int64_t>(sinks, N);
-  a.c = fabsf(scale) * 1.44269504f;
+  a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
+  a.keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.blocks = (int)aq::ceil_div(M, kQ);
   const int64_t items = B * H * a.blocks;

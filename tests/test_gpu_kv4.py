@@ -92,16 +92,19 @@ def _attention_ref(q, cache, last, scale):
     H, D = q.shape
     G = H // k.shape[0]
     k, v, q = k.repeat_interleave(G, 0), v.repeat_interleave(G, 0), q.double()
+    ks = ks[:, :last + 1]
     s = (k * q[:, None]).sum(-1) * scale
     w = torch.softmax(s, -1)
     want = (w[..., None] * v).sum(1)
-    # keys and values rounded to fp16 (2^-11 each, subnormals 2^-25), numerators
-    # rounded to fp16 above and below the fraction (2^-11, or 2^-25 of the
-    # largest), the output once; f32 sums and the exponential: 2^-17 in all
-    ds = (2.0 ** -11 + 2.0 ** -17) * ((k.abs() * q.abs()[:, None]).sum(-1) * abs(scale)).amax(-1)
-    ds = ds + 2.0 ** -25 * q.abs().sum(-1) * abs(scale)
+    # scores from sums in f32 of the codes raised by 1024, times the group's scale (8
+    # roundings of 2^-24 of at most 1039 s sum |q|, under 2^-11 s sum |q|), and of the
+    # minima's part and the exponential: 2^-17 of the terms; values rounded to fp16
+    # (2^-11; the numerators are two numbers, 2^-22 or 2^-25 of the largest), the
+    # output once
+    top = ks.double().amax((1, 2)).repeat_interleave(G, 0)
+    ds = (2.0 ** -17 * (k.abs() * q.abs()[:, None]).sum(-1).amax(-1) + 2.0 ** -11 * top * q.abs().sum(-1)) * abs(scale)
     wv = (w[..., None] * v.abs()).sum(1)
-    bound = (torch.expm1(2 * ds)[:, None] + 3 * 2.0 ** -11 + 2.0 ** -17) * wv + 2.0 ** -24 * v.abs().sum(1)
+    bound = (torch.expm1(2 * ds)[:, None] + 2.0 ** -11 + 2.0 ** -17) * wv + 2.0 ** -24 * v.abs().sum(1)
     bound = bound + 2.0 ** -11 * want.abs() + 2.0 ** -24
     return want, bound
 
@@ -183,6 +186,24 @@ def test_shared_position_and_bounds():
     one = DC.kv4_attention(q, kn, vn, cache, torch.tensor([7], device=DEV), scale=0.125, slots=10)
     two = DC.kv4_attention(q, kn, vn, cache, torch.tensor([7, 7], device=DEV), scale=0.125, slots=10)
     assert torch.equal(one, two)
+
+
+def test_scales():
+    """A negative scale is that of the negated queries; with 0 every slot counts alike."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    B, H, Hkv, D, slots = 2, 6, 3, 64, 90
+    cache = DC.kv4_buffers(B, Hkv, slots, D, DEV)
+    DC.kv4_store(_rnd(g, B, Hkv, 80, D), _rnd(g, B, Hkv, 80, D), cache, slots=slots)
+    q, kn, vn = _rnd(g, B, H, D), _rnd(g, B, Hkv, D), _rnd(g, B, Hkv, D)
+    pos = torch.tensor([80, 50], device=DEV)
+    a = DC.kv4_attention(q, kn, vn, cache, pos, scale=-0.2, slots=slots)
+    assert torch.equal(a, DC.kv4_attention(-q, kn, vn, cache, pos, scale=0.2, slots=slots))
+    got = DC.kv4_attention(q, kn, vn, cache, pos, scale=0.0, slots=slots)
+    v = R.values(*R.unpack(cache, slots)[1]).repeat_interleave(H // Hkv, 1)
+    for b, p in enumerate(pos.tolist()):
+        seen = v[b, :, :p + 1]
+        bound = 2.0 ** -10 * seen.abs().mean(1) + 2.0 ** -11 * seen.mean(1).abs() + 2.0 ** -24
+        assert ((got[b].cpu().double() - seen.mean(1)).abs() <= bound).all()
 
 
 def test_steps_in_a_graph():

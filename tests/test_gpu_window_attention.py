@@ -67,6 +67,18 @@ def test_windows(M, N, window, sinks):
     _check(1, 2, 1, M, N, 128, window, sinks, seed=M)
 
 
+def test_scales():
+    """A negative scale is that of the negated queries; with 0 every key seen counts alike."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    for D in (64, 128):
+        q, k, v = _rnd(g, 2, 4, 150, D), _rnd(g, 2, 2, 150, D), _rnd(g, 2, 2, 150, D)
+        starts = torch.tensor([0, 30], dtype=torch.int32, device=DEV)
+        kw = dict(window=70, sinks=3, starts=starts)
+        assert torch.equal(window_attention(q, k, v, scale=-0.2, **kw), window_attention(-q, k, v, scale=0.2, **kw))
+        want, bound = _reference(q, k, v, 70, 3, 0.0, starts)
+        assert ((window_attention(q, k, v, scale=0.0, **kw).double() - want).abs() <= bound).all()
+
+
 def test_left_padding():
     """Sequences that begin late, rows of which see nothing, one of them empty."""
     got = _check(5, 4, 2, 200, 200, 64, 40, 4, starts=[0, 1, 70, 199, 200], seed=5)
