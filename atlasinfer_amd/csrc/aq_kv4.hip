@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Cache4 c, int slots, int 
                                                        uint16_t* __restrict__ v) {
   constexpr int TPR = D / 8, RPS = 256 / TPR;
   const int t = threadIdx.x, blk = blockIdx.x, nblk = (slots + kSlotBlock - 1) / kSlotBlock;
-  const int64_t head = blockIdx.y;
+  const int64_t head = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
   const uint8_t* kc = c.kc + (head * nblk + blk) * (kSlotBlock * D / 2);
   const uint16_t* kp = c.kp + (head * nblk + blk) * (kSlotBlock * (D / 32) * 2);
   const uint8_t* vc = c.vc + (head * nblk + blk) * (16 * D);
@@ -754,10 +754,9 @@ extern "C" int aq_kv4_load(const void* k_codes, const void* k_params, const void
   AQ_CHECK_ARG(k && v, "aq_kv4_load: null pointer");
   if (const int rc = check_cache4("aq_kv4_load", k_codes, k_params, v_codes, v_params, B, Hkv, D, slots)) return rc;
   AQ_CHECK_ARG(count > 0 && count <= slots, "aq_kv4_load: %lld of %lld slots", (long long)count, (long long)slots);
-  AQ_CHECK_ARG(B * Hkv <= 65535, "aq_kv4_load: %lld heads in all (at most 65535)", (long long)(B * Hkv));
   AQ_CHECK_ARG((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "aq_kv4_load: k and v must be 16-byte aligned");
   const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
-  const dim3 grid((unsigned)aq::ceil_div(count, kSlotBlock), (unsigned)(B * Hkv));
+  const dim3 grid((unsigned)aq::ceil_div(count, kSlotBlock), (unsigned)Hkv, (unsigned)B);
   if (D == 64)
     hipLaunchKernelGGL((kv4_load_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, c, (int)slots, (int)count, (uint16_t*)k, (uint16_t*)v);
   else

@@ -92,6 +92,21 @@ def _strides(t: torch.Tensor):
     return _lib.ptr_array(t.stride()[:3], ctypes.c_int64)
 
 
+def _prompt_arguments(what, k, v, lengths, start, B, Hkv, D, slots, sinks, dev):
+    """Checks of a prompt's tensors and place; its length."""
+    S = k.shape[2] if k.dim() == 4 else -1
+    if k.shape != (B, Hkv, S, D) or v.shape != k.shape:
+        _refuse(f"{what}: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
+    if not (k.dtype == v.dtype == torch.float16 and k.device == dev and v.device == dev):
+        _refuse(f"{what}: k and v must be fp16 on {dev}")
+    if lengths is not None and not (lengths.dtype == torch.int64 and lengths.shape == (B,) and lengths.is_contiguous()
+                                    and lengths.device == dev):
+        _refuse(f"{what}: lengths must be contiguous int64 [{B}] on {dev}")
+    if start < 0 or (sinks is None and start + S > slots):
+        _refuse(f"{what}: positions {start} .. {start + S - 1} in {slots} slots")
+    return S
+
+
 def kv4_store(k: torch.Tensor, v: torch.Tensor, cache, start: int = 0, lengths: Optional[torch.Tensor] = None,
               slots: Optional[int] = None, sinks: Optional[int] = None) -> None:
     """Quantize positions start .. start + S - 1 (k, v fp16 [B, Hkv, S, D], any
@@ -99,16 +114,7 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, cache, start: int = 0, lengths: 
     (int64 [B]).  ``sinks``: the cache is a window (None: it is not, and the
     positions must fit)."""
     B, Hkv, D, slots, dev = _kv4_sizes(cache, slots)
-    S = k.shape[2] if k.dim() == 4 else -1
-    if k.shape != (B, Hkv, S, D) or v.shape != k.shape:
-        _refuse(f"kv4_store: k {tuple(k.shape)}, v {tuple(v.shape)} for a cache of [{B}, {Hkv}, *, {D}]")
-    if not (k.dtype == v.dtype == torch.float16 and k.device == dev and v.device == dev):
-        _refuse(f"kv4_store: k and v must be fp16 on {dev}")
-    if lengths is not None and not (lengths.dtype == torch.int64 and lengths.shape == (B,) and lengths.is_contiguous()
-                                    and lengths.device == dev):
-        _refuse(f"kv4_store: lengths must be int64 [{B}] on {dev}")
-    if start < 0 or (sinks is None and start + S > slots):
-        _refuse(f"kv4_store: positions {start} .. {start + S - 1} in {slots} slots")
+    S = _prompt_arguments("kv4_store", k, v, lengths, start, B, Hkv, D, slots, sinks, dev)
     sk = _sinks(sinks, slots)
     if S == 0:
         return
@@ -273,13 +279,12 @@ class DecodeCache:
         if self.bits == 4:
             kv4_store(k, v, self.buffers, start, lengths, self.slots, self.sinks)
             return
-        S = k.shape[2]
-        if start < 0 or (self.sinks is None and start + S > self.slots):
-            _refuse(f"DecodeCache: positions {start} .. {start + S - 1} in {self.slots} slots")
+        dev = self.buffers[0].device
+        S = _prompt_arguments("DecodeCache.store", k, v, lengths, start, self.batch, self.kv_heads, self.head_dim,
+                              self.slots, self.sinks, dev)
         if S == 0:
             return
         # the newest position of each slot, by sequence when their lengths differ
-        dev = self.buffers[0].device
         slot = torch.arange(self.slots, device=dev)[None]
         end = start + (torch.full((1, 1), S, device=dev) if lengths is None else lengths.clamp(0, S).view(-1, 1))
         p = slot
@@ -298,6 +303,8 @@ class DecodeCache:
         if self.bits == 4:
             return kv4_load(self.buffers, count, self.slots)
         n = self.slots if count is None else count
+        if not 0 <= n <= self.slots:
+            _refuse(f"DecodeCache.load: {n} of {self.slots} slots")
         return self.buffers[0][:, :, :n].clone(), self.buffers[1][:, :, :n].clone()
 
     def attend(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pos: torch.Tensor, *, scale: float,

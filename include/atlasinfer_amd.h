@@ -486,12 +486,14 @@ int aq_kv4_load(const void* k_codes, const void* k_params, const void* v_codes, 
  * aq_window_decode_attention over a 4-bit cache: the step's key (rotated) and
  * value are quantized into their slot as aq_kv4_store does it, then
  *   out[b, h, :] = fp16(softmax(scale q . k) v)
- * over the slots in use, as the values they stand for (each rounded to fp16;
- * scores and sums in f32, the softmax's numerators rounded to fp16).  H any
- * multiple of Hkv.  q, k_new, v_new, pos, q_scale, rope_* and which sequences
- * are run: as there, q, k_new, v_new, out and the tables 16-byte aligned; workspace: aq_kv4_attention_workspace bytes (may be 0,
- * then NULL will do; -1 for sizes it cannot take), 16-byte aligned, no initial
- * contents; calls that overlap in time must not share one.
+ * over the slots in use, as the values they stand for (keys exactly, values
+ * rounded to fp16; scores and sums in f32, the softmax's numerators to 22 bits).
+ * H any multiple of Hkv.  q, k_new, v_new, pos, q_scale, rope_* and which
+ * sequences are run: as there; q, k_new, v_new, out and the tables 16-byte
+ * aligned.
+ *   workspace  aq_kv4_attention_workspace bytes (may be 0, then NULL will do; -1
+ *          for sizes it cannot take), 16-byte aligned, no initial contents; calls
+ *          that overlap in time must not share one.
  */
 int64_t aq_kv4_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t slots);
 int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* k_codes, void* k_params, void* v_codes,
