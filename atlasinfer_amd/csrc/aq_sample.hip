@@ -16,25 +16,32 @@
 // and errors of 2^-24 in the sums would choose another token in one row of a
 // hundred where tens of thousands are kept.
 //
-// One workgroup takes a row.  A full sort is never made:
+// One workgroup takes a row (long rows of few are split, see below).  A full sort is
+// never made:
 //   max      one pass, 16 bytes a thread and load, packed maxima
 //   top-k    (k <= 512) of the 1024 threads' own maxima the k-th largest is a
 //            key that at least k tokens reach; the tokens that do (k and a few,
-//            for logits in any order) go to a list in LDS
-//   top-p    a histogram of masses over the keys' first 11 bits has the bin in
-//            which the running mass reaches p; the next pass sums what lies above
-//            it and lists what lies inside
-//   the cut  of a list of up to 256 by comparing its members with each other (four
-//            threads each); else by descending the keys' bits, 11 at a time, with
-//            histograms of counts and masses in LDS, over the list or, where it
-//            overflows (ties, large k), the row
-//   token    kept masses by segments of 1 KiB, summed in the exact pass or from
-//            the list; one wave goes through the segment that the number falls in
+//            for logits in any order) go to a list in LDS, which is the whole rest
+//            where it has up to 256
+//   cuts     2048 bins by how far a logit lies below the maximum, counts and
+//            masses: the bin in which the running count reaches k, or the running
+//            mass p, then the order of its members.  Up to 256 are compared with each
+//            other, four threads a member; more (ties, high temperatures) are ordered
+//            by the bits of their keys, 11 at a time, with the same histograms.
+//            (Bins by the keys' own first bits fall on the few exponents that most
+//            logits share: nearly every row went through all bits, top-p of 256 fp32
+//            rows of 32000 took 53 us, here 48; of one fp16 row of 50272 40, here 34.)
+//   token    kept masses by segments of 1 KiB, summed in the pass that lists the
+//            bin's members; one wave goes through the segment that the number falls in
 //
+// Bound by instructions: an exponential is 30 of them, a pass over 32 tokens a thread
+// 10 to 15 us, and what every call does once (finding a bin, ordering a list, the last
+// segment) 2 to 4 us a step; reading the row is a tenth of it.
 // Passes are short loops over the row in memory (the L2 has it after the first):
 // with every element of a thread unrolled, and kept in registers, the kernel was
 // 20 000 instructions long, ran once through them and took 25 us for a greedy row
-// of 50272, most of it waiting for instructions.
+// of 50272, most of it waiting for instructions.  (Four tokens at a time in a thread: no
+// faster, 5 us slower where it spilled.)
 #include "aq_common.h"
 
 namespace {
@@ -103,21 +110,36 @@ __device__ __forceinline__ uint32_t keys_of_word(uint32_t w) {
 // exp((x - mx) / T) in units of 2^-42, rounded to a whole number: 2^(n / 512)
 // 2^(r / 512) with y = n + r, y = (x - mx) c, c = 512 log2(e) / T, from a table of
 // 2^(j / 512 + 42) and a polynomial of degree 3 (|r| <= 1/2: relative error 1e-14).
-// Adding 1.5 2^52 rounds y to n and leaves n in the low bits; its upper part goes to
-// the exponent; adding 2^52 rounds the result.  (rndne, cvt and ldexp in 64 bits
-// take four times as long as an addition.)  Where y is not a number (x is not, or
-// -inf at T = inf) or below -512 x 60, the result is 0.
+// Adding 1.5 2^52 to y rounds it to n and leaves n in the low bits; its upper part
+// goes to the exponent; the last product is added to 2^52, which rounds it and
+// leaves it in the low bits.  (Conversions between 64 bits and whole numbers, and
+// rndne and ldexp, take four times as long as an addition.)  x is taken from lo
+// on, where the weight is 2^-60 or less, and -inf and NaN with it.
 struct Weigh {
   double mx, c;
   const double* table;
-  __device__ __forceinline__ double operator()(float x) const {
+  float lo, hi;
+  bool endless;  // a row with infinities: these weigh 1 and every number nothing
+  __device__ __forceinline__ uint64_t operator()(float x) const {
     constexpr double a = 0.0013538030870311431, a2 = a * a / 2, a3 = a * a * a / 6;  // ln 2 / 512
-    const double y = fmin(fmax(((double)x - mx) * c, -30720.0), 0.0);
-    const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
+    constexpr double k = 6755399441055744.0, one = 4503599627370496.0;
+    if (endless) x = x == INFINITY ? hi : lo;
+    x = __builtin_amdgcn_fmed3f(x, lo, hi);
+    const double d = (double)x - mx, t = fma(d, c, k), r = fma(d, c, k - t);
     const int n = (int)__builtin_bit_cast(uint64_t, t);
-    const double v = table[n & (kTable - 1)] * fma(r, fma(r, fma(r, a3, a2), a), 1.0);
-    const uint64_t b = __builtin_bit_cast(uint64_t, v) + ((uint64_t)(uint32_t)((n >> 9) << 20) << 32);
-    return (__builtin_bit_cast(double, b) + 4503599627370496.0) - 4503599627370496.0;
+    const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)]) + ((uint64_t)(uint32_t)((n >> 9) << 20) << 32);
+    const double v = fma(__builtin_bit_cast(double, e), fma(r, fma(r, fma(r, a3, a2), a), 1.0), one);
+    return __builtin_bit_cast(uint64_t, v) - __builtin_bit_cast(uint64_t, one);
+  }
+};
+
+// Bins by how far below the maximum a logit lies, 43.1 halvings of its weight in
+// all: bin kBins - 1 has the largest, and what bin 0 has (from 43 halvings on) weighs
+// 0.  Subtraction, product and conversion never turn an order around.
+struct Bins {
+  float mx, q;  // q = 2047 / (43.1 ln 2 T)
+  __device__ __forceinline__ float place(float x) const {  // NaN as -inf; inf - inf is a maximum
+    return fmaxf((mx - fmaxf(x, -INFINITY)) * q, 0.0f);
   }
 };
 
@@ -140,12 +162,21 @@ __device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
   return v;
 }
 
+// The thread's index, worked out where it is used: kept over the loops, what
+// follows from it took more registers than there are (the kernel then spilled 100 and
+// ran 5 to 15 us longer, writing them out).
+__device__ __forceinline__ int tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // Inclusive prefix sum over the workgroup; *total its whole sum.
 __device__ __forceinline__ uint64_t block_scan_u64(uint64_t v, uint64_t* lds, uint64_t* total) {
-  const int w = threadIdx.x >> 6;
+  const int w = tid() >> 6;
   v = wave_scan_u64(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) lds[w] = v;
+  if ((tid() & 63) == 63) lds[w] = v;
   __syncthreads();
   uint64_t before = 0, all = 0;
 #pragma unroll
@@ -166,9 +197,10 @@ struct Shared {
   double table[kTable];
   uint64_t sorted_mass[kSmallList];
   uint32_t sorted_index[kSmallList];
+  uint2 members[kSmallList];
   uint64_t red[kWaves];
   uint64_t found_mass;
-  uint32_t found_bin, found_count, n_list, segment, seg_rank, token;
+  uint32_t found_bin, found_count, n_list, n_members, segment, seg_rank, token;
   uint64_t seg_before;
 };
 
@@ -185,12 +217,12 @@ __device__ __forceinline__ uint64_t reach(float p, uint64_t m) {
 
 // The bin, from the highest down, in which the running count (by_mass: the
 // running mass) reaches `most` (0: that of the bins' whole mass and p), and what
-// lies above it.  The caller knows that one does.
+// lies above it; bin 0 and everything if none does.
 __device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& most, float p) {
-  const int t = threadIdx.x;
+  const int t = tid();
   const int b0 = kBins - 1 - 2 * t, b1 = b0 - 1;  // this thread's
   const uint64_t m0 = s.mass[b0], m1 = s.mass[b1], c0 = s.count[b0], c1 = s.count[b1];
-  uint64_t bm = 0, bc = 0;
+  uint64_t bm = 0, bc = 0, am = 0, ac = 0;
 #pragma unroll 1
   for (int i = 0; i < 2; i++) {  // both scans by the same instructions: they run once, most time goes to fetching them
     const uint64_t v = i ? c0 + c1 : m0 + m1;
@@ -198,11 +230,14 @@ __device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& mos
     const uint64_t before = block_scan_u64(v, s.red, &all) - v;
     if (i) {
       bc = before;
+      ac = all;
     } else {
       bm = before;
+      am = all;
       if (most == 0) most = reach(p, all);
     }
   }
+  if ((by_mass ? am : ac) < most) return {0, (uint32_t)ac, am};
   // a bin is the one if what lies above it does not reach `most` and with it does
   auto take = [&](int bin, uint64_t mb, uint64_t cb, uint64_t m, uint64_t c) {
     const uint64_t lo = by_mass ? mb : cb, hi = by_mass ? mb + m : cb + c;
@@ -222,7 +257,7 @@ __device__ __forceinline__ Found find_bin(Shared& s, bool by_mass, uint64_t& mos
 // The highest key edge (of the first 11 bits) that at least k of the threads'
 // keys reach; s.count is the scratch.
 __device__ __forceinline__ uint32_t edge_of_kth(Shared& s, uint32_t key, int bits, uint32_t k) {
-  const int t = threadIdx.x, w = t >> 6;
+  const int t = tid(), w = t >> 6;
   uint32_t* red = reinterpret_cast<uint32_t*>(s.red);
   s.count[t] = 0;
   s.count[t + kThreads] = 0;
@@ -257,12 +292,12 @@ struct Row {
   const uint8_t* x;
   const uint4* pieces;
   int V, skip, np, inside, outside, c0, c1;
-  uint4 head, tail;
+  uint4* ends;  // in LDS: the pieces that reach over the row's ends
 
   // NaNs, which count as -inf
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu); }
 
-  __device__ __forceinline__ Row(const void* logits, int64_t row, int64_t stride, int V_) : V(V_) {
+  __device__ __forceinline__ Row(const void* logits, int64_t row, int64_t stride, int V_, uint4* ends_) : V(V_), ends(ends_) {
     x = (const uint8_t*)logits + row * stride * (L::kBits / 8);
     skip = (int)((uintptr_t)x % 16) / (L::kBits / 8);
     pieces = reinterpret_cast<const uint4*>(x - skip * (L::kBits / 8));
@@ -270,16 +305,15 @@ struct Row {
     // pieces inside .. outside - 1 lie in the row as a whole
     inside = skip ? 1 : 0;
     outside = (V + skip) / E;
-    take(0, np);
+    c0 = 0;
+    c1 = np;
+    const int t = tid();
+    if (t < 2) ends[t] = edge(t ? np - 1 : 0);
+    __syncthreads();
   }
   __device__ __forceinline__ void take(int from, int to) {
     c0 = from;
     c1 = to;
-    // the pieces that reach over the row's ends, in the threads that have them
-    head = tail = none();
-    const int t = threadIdx.x;
-    if (skip && c0 == 0 && t == 0) head = edge(0);
-    if (outside < np && np - 1 >= c0 && np - 1 < c1 && t == (np - 1 - c0) % kThreads) tail = edge(np - 1);
   }
   __device__ __forceinline__ uint4 edge(int c) const {  // the elements that there are
     uint4 r = none();
@@ -294,13 +328,10 @@ struct Row {
       }
     return r;
   }
-  // any piece, in any thread
-  __device__ __forceinline__ uint4 piece(int c) const { return c >= inside && c < outside ? pieces[c] : c < np ? edge(c) : none(); }
-  // one of the thread's own
   __device__ __forceinline__ uint4 load(int c) const {
     uint4 v = inside < outside ? pieces[min(max(c, inside), outside - 1)] : none();
-    if (c >= outside) v = c == np - 1 ? tail : none();
-    if (c < inside) v = head;
+    if (c >= outside) v = c == np - 1 ? ends[1] : none();
+    if (c < inside) v = ends[0];
     return v;
   }
   // f(piece, its 16 bytes) for every piece, in order within a thread; the next
@@ -309,9 +340,9 @@ struct Row {
   // part's, as nothing).
   template <class F>
   __device__ __forceinline__ void each_piece(F f) const {
-    uint4 next = load(c0 + threadIdx.x);
+    uint4 next = load(c0 + tid());
 #pragma unroll 1
-    for (int c = c0 + threadIdx.x; c - (int)threadIdx.x < c1; c += kThreads) {
+    for (int c = c0 + tid(); c - tid() < c1; c += kThreads) {
       const uint4 v = c < c1 ? next : none();
       next = load(c + kThreads);
       f(c, v);
@@ -358,12 +389,12 @@ struct Row {
   __device__ __forceinline__ uint32_t largest(uint64_t* lds, uint32_t (&keys)[8], uint32_t* best) const {
     uint32_t own = 0;
 #pragma unroll 1
-    for (int c = c0 + threadIdx.x; c - (int)threadIdx.x < c1; c += 8 * kThreads) own = max(own, largest_of_eight(c, keys));
+    for (int c = c0 + tid(); c - tid() < c1; c += 8 * kThreads) own = max(own, largest_of_eight(c, keys));
     uint32_t b = own;
 #pragma unroll
     for (int d = 32; d; d >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, d, 64));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = b;
+    if ((tid() & 63) == 0) lds[tid() >> 6] = b;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kWaves; i++) b = max(b, (uint32_t)lds[i]);
@@ -378,17 +409,26 @@ struct PartsOfRow {
   uint64_t seg_mass[kMaxSegments];
   uint2 list[kList];
   uint32_t best[kMaxParts];
-  uint32_t n_list, pad[3];
+  uint64_t most, above;  // the mass that top-p reaches, the mass above the bin in which it does
+  uint32_t n_list, bin, pad[2];
 };
 
 __device__ __forceinline__ Weigh weigh_from(float mx, float T, const double* table) {
-  // 512 log2(e) / T; of a row with infinities, these weigh 1 (as what is above
-  // the maximum would) and every number nothing
-  const bool endless = mx == INFINITY;
-  return Weigh{endless ? 1e39 : (double)mx, endless ? 1.0 : 738.6598609514740 / (double)T, table};
+  if (mx == INFINITY) return Weigh{1.0, 30720.0, table, 0.0f, 1.0f, true};
+  double c = 738.6598609514740 / (double)fminf(T, 1e34f);  // 512 log2(e) / T
+  float lo = fmaxf((float)((double)mx - 30720.0 / c), -3.4028235e38f);
+  if (!(lo < mx)) {  // T is far below the logits' steps: the next one weighs nothing
+    lo = nextafterf(mx, -INFINITY);
+    c = 30720.0 / ((double)mx - (double)lo);
+  }
+  return Weigh{(double)mx, c, table, lo, mx, false};
 }
+__device__ __forceinline__ uint64_t whole_of(float min_p) {  // the least weight that min-p leaves
+  return min_p > 0.0f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * kOne) : 0;
+}
+__device__ __forceinline__ Bins bins_from(float mx, float T) { return Bins{mx, 68.52f / fminf(T, 1e34f)}; }
 __device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable) * kOne;
+  if (tid() < kTable) table[tid()] = exp2((double)tid() / kTable) * kOne;
 }
 
 __device__ __forceinline__ void append(Shared& s, int V, int i, uint32_t key) {
@@ -397,29 +437,31 @@ __device__ __forceinline__ void append(Shared& s, int V, int i, uint32_t key) {
   if (at < kList) s.list[at] = make_uint2(key, (uint32_t)i);
 }
 
-// Masses of keys above `hi` by segment (of w >= wmin), to seg_mass.  LISTING: keys
-// from `lo` to `hi` go to the list; else the keys equal to hi are counted by
-// segment.
+// Masses (of w >= wmin) by segment, to seg_mass.  LISTING: of what lies in the bins
+// above `bin` (counted from the top); what lies in it goes to the list.  Else of the
+// keys above `cut`; those equal to it are counted by segment.
 template <int FMT, bool LISTING>
-__device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, const Weigh& weigh, double wmin, uint32_t lo,
-                                             uint32_t hi, uint64_t* seg_mass) {
+__device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, const Weigh& weigh, uint64_t wmin,
+                                             const Bins& bins, float bin, uint32_t cut, uint64_t* seg_mass) {
   row.each_piece([&](int c, const uint4& v) {
-    double sum = 0.0;
+    uint64_t sum = 0;
     uint32_t ties = 0;
     row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-      if (__ballot(key > hi)) {  // the exponential only where a lane asks for it
-        const double w = weigh(Logit<FMT>::value(bits));
-        sum += key > hi && w >= wmin ? w : 0.0;
+      const float x = Logit<FMT>::value(bits), at = LISTING ? bins.place(x) : 0.0f;
+      const bool above = LISTING ? at < bin : key > cut;
+      if (__ballot(above)) {  // the exponential only where a lane asks for it
+        const uint64_t w = weigh(x);
+        sum += above && w >= wmin ? w : 0;
       }
       if (LISTING) {
-        if (key >= lo && key <= hi && c < row.c1) append(s, row.V, i, key);
+        if (!above && at < bin + 1.0f && c < row.c1) append(s, row.V, i, key);
       } else {
-        ties += (uint32_t)__popcll(__ballot(key == hi && (uint32_t)i < (uint32_t)row.V));
+        ties += (uint32_t)__popcll(__ballot(key == cut && (uint32_t)i < (uint32_t)row.V));
       }
     });
-    sum = wave_group_sum_f64<64>(sum);  // 2^9 whole numbers of up to 2^42: exact
-    if ((threadIdx.x & 63) == 0 && c < row.c1) {  // 64 pieces are a segment
-      seg_mass[c >> 6] = (uint64_t)sum;
+    sum = wave_scan_u64(sum);
+    if ((tid() & 63) == 63 && c - 63 < row.c1) {  // 64 pieces are a segment
+      seg_mass[c >> 6] = sum;
       if (!LISTING) s.seg_ties[c >> 6] = ties;
     }
   });
@@ -428,7 +470,7 @@ __device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, con
 
 __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
+  for (int i = tid(); i < kBins; i += kThreads) {
     s.mass[i] = 0;
     s.count[i] = 0;
   }
@@ -441,8 +483,8 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
 // exponential is needed; the others are left to sample_kernel whole.
 
 template <int FMT>
-__device__ __forceinline__ Row<FMT> part_of(const void* logits, int V, int64_t stride, int per) {
-  Row<FMT> row(logits, blockIdx.y, stride, V);
+__device__ __forceinline__ Row<FMT> part_of(const void* logits, int V, int64_t stride, int per, uint4* ends) {
+  Row<FMT> row(logits, blockIdx.y, stride, V, ends);
   row.take((int)blockIdx.x * per, min((int)(blockIdx.x + 1) * per, row.np));
   return row;
 }
@@ -458,14 +500,15 @@ template <int FMT>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(const void* __restrict__ logits, int V, int64_t stride,
                                                               int per, Settings set, PartsOfRow* __restrict__ ws) {
   __shared__ uint64_t red[kWaves];
+  __shared__ uint4 ends[2];
   if (!in_parts(set, blockIdx.y, V)) return;
-  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per, ends);
   PartsOfRow& w = ws[blockIdx.y];
   uint32_t best, keys8[8];
   row.largest(red, keys8, &best);
-  if (threadIdx.x == 0) w.best[blockIdx.x] = best;
-  for (int i = blockIdx.x * kThreads + threadIdx.x; i < kBins; i += gridDim.x * kThreads) w.mass[i] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) w.n_list = 0;
+  if (tid() == 0) w.best[blockIdx.x] = best;
+  for (int i = blockIdx.x * kThreads + tid(); i < kBins; i += gridDim.x * kThreads) w.mass[i] = 0;
+  if (blockIdx.x == 0 && tid() == 0) w.n_list = 0;
 }
 
 __device__ __forceinline__ uint32_t best_of(const PartsOfRow& w, int parts) {
@@ -474,31 +517,34 @@ __device__ __forceinline__ uint32_t best_of(const PartsOfRow& w, int parts) {
   return b;
 }
 
-// The part's masses by the keys' first 11 bits, added to the row's.
+// The part's masses by bins, added to the row's.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const void* __restrict__ logits, int V, int64_t stride,
                                                                int per, Settings set, PartsOfRow* __restrict__ ws) {
   __shared__ uint64_t mass[kBins];
   __shared__ double table[kTable];
+  __shared__ uint4 ends[2];
   const int b = blockIdx.y;
   const float p = set.p ? set.p[b] : set.p0, T = set.t ? set.t[b] : set.t0;
   if (!in_parts(set, b, V) || !(p < 1.0f)) return;
-  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per, ends);
   PartsOfRow& w = ws[b];
   const float mx = Logit<FMT>::value_of_key(best_of(w, gridDim.x));
   if (mx == -INFINITY) return;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = 0;
+  for (int i = tid(); i < kBins; i += kThreads) mass[i] = 0;
   fill_table(table);
   __syncthreads();
   const Weigh weigh = weigh_from(mx, T, table);
+  const Bins bins = bins_from(mx, T);
   row.each_piece([&](int c, const uint4& v) {
-    row.each_element(c, v, [&](int, uint32_t bits, uint32_t key) {
-      const uint64_t m = (uint64_t)weigh(Logit<FMT>::value(bits));
-      if (m) atomicAdd((unsigned long long*)&mass[key >> (Logit<FMT>::kBits - 11)], (unsigned long long)m);
+    row.each_element(c, v, [&](int, uint32_t bits, uint32_t) {
+      const float x = Logit<FMT>::value(bits), at = bins.place(x);
+      if (at < kBins - 1.0f)
+        atomicAdd((unsigned long long*)&mass[kBins - 1 - (int)at], weigh(x));
     });
   });
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kThreads)
+  for (int i = tid(); i < kBins; i += kThreads)
     if (mass[i]) atomicAdd((unsigned long long*)&w.mass[i], (unsigned long long)mass[i]);
 }
 
@@ -510,16 +556,17 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* _
                                                                    PartsOfRow* __restrict__ ws) {
   __shared__ Shared s;
   __shared__ uint32_t at;
-  const int b = blockIdx.y, t = threadIdx.x;
+  __shared__ uint4 ends[2];
+  const int b = blockIdx.y, t = tid();
   const float p = set.p ? set.p[b] : set.p0, T = set.t ? set.t[b] : set.t0, mp = set.m ? set.m[b] : set.m0;
   if (!in_parts(set, b, V)) return;
-  const Row<FMT> row = part_of<FMT>(logits, V, stride, per);
+  const Row<FMT> row = part_of<FMT>(logits, V, stride, per, ends);
   PartsOfRow& w = ws[b];
   const float mx = Logit<FMT>::value_of_key(best_of(w, gridDim.x));
   if (mx == -INFINITY) return;
   fill_table(s.table);
   if (t == 0) s.n_list = 0;
-  uint32_t lo = 1, hi = 0;  // no list, everything above
+  float bin = INFINITY;  // no list, everything above
   if (p < 1.0f) {
     for (int i = t; i < kBins; i += kThreads) {
       s.mass[i] = w.mass[i];
@@ -527,12 +574,17 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* _
     }
     __syncthreads();
     uint64_t most = 0;
-    lo = find_bin(s, true, most, p).bin << (Logit<FMT>::kBits - 11);
-    hi = lo | ((1u << (Logit<FMT>::kBits - 11)) - 1);
+    const Found f = find_bin(s, true, most, p);
+    bin = (float)(kBins - 1 - (int)f.bin);
+    if (blockIdx.x == 0 && t == 0) {
+      w.most = most;
+      w.above = f.mass;
+      w.bin = f.bin;
+    }
   }
   __syncthreads();
-  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) * kOne : 0.0;
-  sum_segments<FMT, true>(s, row, weigh_from(mx, T, s.table), wmin, lo, hi, w.seg_mass);
+  const uint64_t wmin = whole_of(mp);
+  sum_segments<FMT, true>(s, row, weigh_from(mx, T, s.table), wmin, bins_from(mx, T), bin, 0, w.seg_mass);
   const uint32_t n = s.n_list;  // more than there is room for is counted all the same
   if (t == 0) at = atomicAdd(&w.n_list, n);
   __syncthreads();
@@ -547,33 +599,35 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   typedef Logit<FMT> L;
   constexpr int B = L::kBits, E = L::kPer;
   __shared__ Shared s;
-  const int t = threadIdx.x, row = blockIdx.x, ln = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int t = tid(), row = blockIdx.x;
   const float T = set.t ? set.t[row] : set.t0, p = set.p ? set.p[row] : set.p0, mp = set.m ? set.m[row] : set.m0;
   const int k = set.k ? set.k[row] : set.k0;
-  const Row<FMT> r(logits, row, stride, V);
+  __shared__ uint4 ends[2];
+  const Row<FMT> r(logits, row, stride, V, ends);
   const int skip = r.skip, np = r.np;
 
   // ---- the largest key, each thread's own on the way
-  if (t == 0) {
-    s.n_list = 0;
-    s.token = 0;
-  }
+  if (t == 0) s.n_list = 0;
+  // a row whose parts have been summed: what they left
+  const PartsOfRow* done = parts > 1 && in_parts(set, row, V) && best_of(ws[row], parts) > L::kLowest ? ws + row : nullptr;
   for (int i = t; i < kMaxSegments; i += kThreads) {
-    s.seg_mass[i] = 0;
+    s.seg_mass[i] = done && i < (np + 63) / 64 ? done->seg_mass[i] : 0;
     s.seg_ties[i] = 0;
   }
-  // of a row whose parts have been summed: their largest
-  const PartsOfRow* done = parts > 1 && in_parts(set, row, V) && best_of(ws[row], parts) > L::kLowest ? ws + row : nullptr;
+  if (done && p < 1.0f) {
+    if (t == 0) s.n_list = done->n_list;
+    for (int i = t; i < (int)min(done->n_list, (uint32_t)kList); i += kThreads) s.list[i] = done->list[i];
+  }
   uint32_t own = 0, best, keys8[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (done)
     best = best_of(*done, parts);
   else
     own = r.largest(s.red, keys8, &best);
+  best = __builtin_amdgcn_readfirstlane(best);
   const float mx = L::value_of_key(best);
   const Weigh weigh = weigh_from(mx, T, s.table);
   const bool greedy = !(T > 0.0f) || mx == -INFINITY;  // also a row without a token to choose: its first
-  const double wmin = mp > 0.0f ? fmin((double)mp, 1.0) * kOne : 0.0;
+  const uint64_t wmin = whole_of(mp);
   if (greedy) {
     if (t == 0) s.token = 0xFFFFFFFFu;
     __syncthreads();
@@ -602,7 +656,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   // The whole rest for a list of at most 256 that holds the first k: four
   // threads a member count what comes before it.
   auto small_list = [&] {
-    const int n = (int)s.n_list, i = t >> 2;
+    const int n = (int)s.n_list, t = tid(), i = t >> 2, ln = t & 63;
     const uint2 me = i < n ? s.list[i] : make_uint2(0, 0);
     uint32_t r = 0;
 #pragma unroll 4
@@ -612,7 +666,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     }
     r += xlane_partner_u32<1>(r);
     r += xlane_partner_u32<2>(r);
-    const uint64_t w = i < n ? (uint64_t)weigh(L::value_of_key(me.x)) : 0;
+    const uint64_t w = i < n ? weigh(L::value_of_key(me.x)) : 0;
     if (i < n && (t & 3) == 0) {
       s.sorted_mass[r] = w;
       s.sorted_index[r] = me.y;
@@ -633,7 +687,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     sum = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const bool in = 4 * ln + e < last && at < most && (double)m[e] >= wmin;
+      const bool in = 4 * ln + e < last && at < most && m[e] >= wmin;
       at += m[e];
       stay += in;
       sum += in ? m[e] : 0;
@@ -650,104 +704,188 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   };
 
   Cut cut = {0, 0};  // everything
-  bool from_list = false, summed = false;
+  bool from_list = false, summed = false, binned = false;
   uint64_t mass = 0;
+  const Bins bins = bins_from(mx, T);
+  // f(index, key) for the list's members or the row's tokens
+  auto each = [&](auto f) {
+    if (from_list) {
+      const int n = (int)s.n_list;
+#pragma unroll 1
+      for (int i = tid(); i < n; i += kThreads) f((int)s.list[i].y, s.list[i].x);
+    } else {
+      r.each_piece([&](int c, const uint4& v) { r.each_element(c, v, [&](int i, uint32_t, uint32_t key) { f(i, key); }); });
+    }
+  };
+  if (by_k && k <= kMaxListK) {
+    const int t = tid();
+    const uint32_t least = edge_of_kth(s, own, B, (uint32_t)k);
+    if (own >= least) {  // a thread whose largest is less has none
+#pragma unroll 1
+      for (int c = t; c < np; c += 8 * kThreads) {
+        if (np > 8 * kThreads) r.largest_of_eight(c, keys8);
+        uint32_t which = 0;  // of eight pieces those that have one
+#pragma unroll
+        for (int n = 0; n < 8; n++) which |= (keys8[n] >= least ? 1u : 0u) << n;
+        for (; which; which &= which - 1) {
+          const int d = c + __builtin_ctz(which) * kThreads;
+          r.each_element(d, r.load(d), [&](int i, uint32_t, uint32_t key) {
+            if (key >= least) append(s, V, i, key);
+          });
+        }
+      }
+    }
+    __syncthreads();
+    from_list = s.n_list <= kList;
+    if (s.n_list <= kSmallList) {
+      small_list();
+      return;
+    }
+  }
+
   // the cut of the first k, then that of the mass p of these
 #pragma unroll 1
   for (int stage = 0; stage < 2; stage++) {
     const bool by_mass = stage == 1;
     if (by_mass ? !by_p : !by_k) continue;
     uint64_t most = by_mass ? (by_k ? reach(p, mass) : 0) : (uint64_t)k;
-    if (!by_mass && k <= kMaxListK) {
-      const uint32_t least = edge_of_kth(s, own, B, (uint32_t)k);
-      if (own >= least) {  // a thread whose largest is less has none
+    // the bin in which the running count (by_mass: the running mass) reaches `most`;
+    // then, unless its members are few, the bits of their keys, 11 at a time
+    float bin = 0.0f;
+    uint32_t key = 0, above = 0, ties = 0;  // the last key kept, how many of it
+    uint64_t above_mass = 0;
+    bool all = false;
 #pragma unroll 1
-        for (int c = t; c < np; c += 8 * kThreads) {
-          if (np > 8 * kThreads) r.largest_of_eight(c, keys8);
-          uint32_t which = 0;  // of eight pieces those that have one
-#pragma unroll
-          for (int n = 0; n < 8; n++) which |= (keys8[n] >= least ? 1u : 0u) << n;
-          for (; which; which &= which - 1) {
-            const int d = c + __builtin_ctz(which) * kThreads;
-            r.each_element(d, r.load(d), [&](int i, uint32_t, uint32_t key) {
-              if (key >= least) append(s, V, i, key);
-            });
-          }
-        }
-      }
-      __syncthreads();
-      from_list = s.n_list <= kList;
-      if (s.n_list <= kSmallList) {
-        small_list();
-        return;
-      }
-    }
-
-    // descend the keys' bits, 11 at a time, to the key at which the running
-    // count (by_mass: the running mass) reaches `most`, over the list or the row
-    uint32_t prefix = 0, above = 0;
-    uint64_t above_mass = 0, each = 0;
-#pragma unroll 1
-    for (int shift = B; shift > 0;) {
-      const int bits = min(11, shift), next = shift - bits;
-      clear_bins(s);
-      const bool first = shift == B;
-      auto see = [&](uint32_t key) {
-        if (!first && key >> (shift & 31) != prefix) return;
-        const uint32_t bin = (key >> next) & ((1u << bits) - 1);
-        atomicAdd(&s.count[bin], 1u);
-        const uint64_t w = (uint64_t)weigh(L::value_of_key(key));
-        if (w) atomicAdd((unsigned long long*)&s.mass[bin], (unsigned long long)w);
-      };
+    for (int shift = B + 11; shift > 0;) {
+      const bool first = shift > B;
+      const int bits = min(11, shift), next = shift - bits, t = tid(), ln = t & 63;
+      Found f;
       if (first && done) {
-        for (int i = t; i < kBins; i += kThreads) s.mass[i] = done->mass[i];
-      } else if (from_list) {
-        const int n = (int)s.n_list;
-        for (int i = t; i < n; i += kThreads) see(s.list[i].x);
+        most = done->most;
+        f = {done->bin, 0, done->above};
       } else {
-        r.each_piece([&](int c, const uint4& v) { r.each_element(c, v, [&](int, uint32_t, uint32_t key) { see(key); }); });
+        if (!first || !binned) {
+          clear_bins(s);
+          each([&](int i, uint32_t y) {
+            const float x = L::value_of_key(y), at = bins.place(x);
+            if (!(at < kBins - 1.0f) || (uint32_t)i >= (uint32_t)V) return;  // the rest weighs nothing
+            if (!first && !(at >= bin && at < bin + 1.0f && (shift == B || y >> (shift & 31) == key))) return;
+            const uint32_t to = first ? kBins - 1 - (uint32_t)at : (y >> next) & ((1u << bits) - 1);
+            if (by_k || !first) atomicAdd(&s.count[to], 1u);
+            atomicAdd((unsigned long long*)&s.mass[to], weigh(x));
+          });
+          __syncthreads();
+        }
+        binned = first;
+        uint64_t left = first ? most : most - (by_mass ? above_mass : above);
+        f = find_bin(s, by_mass, left, p);
+        if (first) most = left;
       }
-      __syncthreads();
-      uint64_t left = most - (by_mass ? above_mass : above);
-      const Found f = find_bin(s, by_mass, left, p);
-      if (first) most = left;
       above += f.count;
       above_mass += f.mass;
-      prefix = first ? f.bin : prefix << bits | f.bin;
       shift = next;
-      if (shift == 0) each = s.mass[f.bin] / s.count[f.bin];  // of one of the ties
-      if (first && by_mass && !by_k) {
-        if (done) {
-          if (t == 0) s.n_list = done->n_list;
-          for (int i = t; i < (int)min(done->n_list, (uint32_t)kList); i += kThreads) s.list[i] = done->list[i];
-          __syncthreads();
-        } else {
-          sum_segments<FMT, true>(s, r, weigh, wmin, prefix << next, prefix << next | ((1u << next) - 1), s.seg_mass);
+      if (!first) {
+        key = key << bits | f.bin;
+        if (shift == 0) {
+          const uint64_t each_mass = s.mass[f.bin] / s.count[f.bin];  // of one of the ties
+          ties = by_mass ? (uint32_t)((most - above_mass + each_mass - 1) / each_mass) : (uint32_t)(most - above);
+          above_mass += ties * each_mass;
         }
-        summed = from_list = s.n_list <= kList;
+        continue;
       }
+      if (f.bin == 0) {  // the first k have everything that weighs something
+        all = true;
+        break;
+      }
+      bin = (float)(kBins - 1 - (int)f.bin);
+      // its members: the list, or `members`
+      if (t == 0) s.n_members = 0;
+      __syncthreads();
+      const uint2* members = s.members;
+      uint32_t n;
+      if (by_mass && !by_k) {
+        if (!done) sum_segments<FMT, true>(s, r, weigh, wmin, bins, bin, 0, s.seg_mass);
+        members = s.list;
+        n = s.n_list;
+        summed = from_list = n <= kList;
+      } else {
+        each([&](int i, uint32_t key) {
+          const float place = bins.place(L::value_of_key(key));
+          if (place >= bin && place < bin + 1.0f && (uint32_t)i < (uint32_t)V) {
+            const uint32_t at = atomicAdd(&s.n_members, 1u);
+            if (at < kSmallList) s.members[at] = make_uint2(key, (uint32_t)i);
+          }
+        });
+        __syncthreads();
+        n = s.n_members;
+      }
+
+      if (n > kSmallList) continue;
+      // by comparing the members with each other, four threads each
+      const int i = t >> 2;
+      const uint2 me = i < (int)n ? members[i] : make_uint2(0, 0);
+      uint32_t rank = 0;
+#pragma unroll 4
+      for (int j = t & 3; j < (int)n; j += 4) {
+        const uint2 o = members[j];
+        rank += (o.x > me.x) | ((o.x == me.x) & (o.y < me.y));
+      }
+      rank += xlane_partner_u32<1>(rank);
+      rank += xlane_partner_u32<2>(rank);
+      if (i < (int)n && (t & 3) == 0) {
+        s.sorted_mass[rank] = weigh(L::value_of_key(me.x));
+        s.sorted_index[rank] = me.x;
+      }
+      __syncthreads();
+      // every wave by itself, four of the sorted members a lane: how many lie before
+      // the one that reaches `most`
+      uint64_t m[4], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        m[e] = 4 * ln + e < (int)n ? s.sorted_mass[4 * ln + e] : 0;
+        sum += m[e];
+      }
+      uint64_t at = above_mass + wave_scan_u64(sum) - sum;
+      int before = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        at += m[e];
+        before += 4 * ln + e < (int)n - 1 && (by_mass ? at < most : above + 4 * ln + e + 1 < most);
+      }
+      before = __builtin_amdgcn_readlane(wave_incl_scan_i32<64>(before), 63);
+      key = s.sorted_index[before];
+      sum = 0;
+      int same = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const bool in = 4 * ln + e <= before;
+        sum += in ? m[e] : 0;
+        same += in && s.sorted_index[4 * ln + e] == key;
+      }
+      above_mass += __shfl(wave_scan_u64(sum), 63, 64);
+      ties = (uint32_t)__builtin_amdgcn_readlane(wave_incl_scan_i32<64>(same), 63);
+      __syncthreads();
+      break;
+    }
+    if (all) {
+      mass = above_mass;
+      continue;
     }
     if (!by_mass) {
-      cut = {prefix, (uint32_t)k - above};
-      mass = above_mass + cut.ties * each;
-    } else {
-      const uint32_t n = (uint32_t)((most - above_mass + each - 1) / each);
-      if (prefix > cut.key)
-        cut = {prefix, n};
-      else if (prefix == cut.key)
-        cut.ties = min(cut.ties, n);
+      cut = {key, ties};
+      mass = above_mass;
+    } else if (key > cut.key) {
+      cut = {key, ties};
+    } else if (key == cut.key) {
+      cut.ties = min(cut.ties, ties);
     }
   }
 
   // ---- kept masses and ties by segment
-  const double ecut = cut.key ? weigh(L::value_of_key(cut.key)) : 0.0;
-  const uint64_t wcut = ecut >= wmin ? (uint64_t)ecut : 0;
+  uint64_t wcut = cut.key ? weigh(L::value_of_key(cut.key)) : 0;
+  if (wcut < wmin) wcut = 0;
   __syncthreads();
-  if (done && (!by_p || summed)) {
-    summed = true;
-    for (int i = t; i < (np + 63) / 64; i += kThreads) s.seg_mass[i] = done->seg_mass[i];
-    __syncthreads();
-  }
+  if (done && !by_p) summed = true;
   if (from_list) {
     for (int i = t; i < (int)s.n_list; i += kThreads) {
       const uint2 y = s.list[i];
@@ -755,12 +893,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       if (y.x == cut.key) {
         atomicAdd(&s.seg_ties[seg], 1u);
       } else if (y.x > cut.key) {
-        const double w = weigh(L::value_of_key(y.x));
-        if (w >= wmin) atomicAdd((unsigned long long*)&s.seg_mass[seg], (unsigned long long)w);
+        const uint64_t w = weigh(L::value_of_key(y.x));
+        if (w >= wmin) atomicAdd((unsigned long long*)&s.seg_mass[seg], w);
       }
     }
   } else if (!summed) {
-    sum_segments<FMT, false>(s, r, weigh, wmin, 0, cut.key, s.seg_mass);
+    sum_segments<FMT, false>(s, r, weigh, wmin, bins, 0.0f, cut.key, s.seg_mass);
   }
   __syncthreads();
 
@@ -800,17 +938,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   }
   __syncthreads();
   // ---- the token: one wave, a piece a lane
-  if (wave == 0) {
-    const int c = (int)s.segment * 64 + ln;
-    const uint4 v = r.piece(c);
+  if (t < 64) {
+    const int c = (int)s.segment * 64 + t;
+    const uint4 v = r.load(c);
     uint32_t ties = 0;
     r.each_element(c, v, [&](int i, uint32_t, uint32_t key) { ties += key == cut.key && (uint32_t)i < (uint32_t)V; });
     const uint32_t rank = s.seg_rank + (uint32_t)wave_scan_u64(ties) - ties;
     auto mass_of = [&](int i, uint32_t bits, uint32_t key, uint32_t& n) -> uint64_t {
       if ((uint32_t)i >= (uint32_t)V || key < cut.key) return 0;
       if (key == cut.key) return n++ < cut.ties ? wcut : 0;
-      const double d = weigh(L::value(bits));
-      return d >= wmin ? (uint64_t)d : 0;
+      const uint64_t w = weigh(L::value(bits));
+      return w >= wmin ? w : 0;
     };
     uint64_t sum = 0;
     uint32_t n = rank;
@@ -831,7 +969,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 
 // Workgroups a row is split into: enough to fill the GPU, 1024 pieces each at
 // least, for rows that have 2048 (top-p of 64 rows of 128256: one workgroup each
-// 106 us, four 58; of one row in fp32 118 us and, in 31, 46).  One setting of top-k for all rows rules the split out.
+// 106 us, four 56; of one row in fp32 118 us and, in 31, 38).  One setting of top-k
+// for all rows rules the split out.
 static int parts_of(int64_t B, int64_t V, int dtype, bool top_k) {
   const int64_t per = dtype == AQ_F32 ? 4 : 8, pieces = V / per;
   if (top_k || pieces < 2048) return 1;

@@ -514,8 +514,9 @@ int aq_kv4_attention(const void* q, const void* k_new, const void* v_new, void* 
  * the first one always.  tokens[b] is the first kept token, by index, at which
  * the running mass of the kept ones exceeds u[b] times their whole mass (u >= 1:
  * the last).  temperature <= 0, or a row without a logit above -inf: the largest
- * logit, the lowest index of equal ones.  NaN counts as -inf; logits of +inf
- * share the whole mass.  Masses are sums of w rounded to 2^-42.
+ * logit, the lowest index of equal ones; temperatures above 1e34 count as 1e34.
+ * NaN counts as -inf; logits of +inf share the whole mass.  Masses are sums of w
+ * rounded to 2^-42.
  *   logits  dtype AQ_F16, AQ_BF16 or AQ_F32 [B, V], rows `stride` elements apart,
  *           V <= 262144
  *   u       f32 [B], in [0, 1)      tokens  int64 [B] (out)
