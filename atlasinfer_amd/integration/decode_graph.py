@@ -41,8 +41,9 @@ Options (on the GPU path with an fp16 model):
 
 * ``sampling=True``: the token is sampled (``sample_tokens``: temperature, top-k,
   top-p, min-p) instead of the largest logit's.  The settings are device memory,
-  one per sequence, and so are the random numbers, one per sequence and step
-  drawn ahead, so a captured graph takes new ones.
+  one per sequence, and so are the random numbers, one per sequence and step,
+  drawn ahead by ``set_sampling`` or for a prompt, so a captured graph takes new
+  ones.
 * ``kv_bits=4``: keys and values are kept in 4 bits (``DecodeCache``): 5/16 of
   the memory and of the bytes a step reads.  The prompt itself attends to its own
   keys and values as they are.
@@ -146,6 +147,7 @@ class GraphDecoder:
             self.v = [torch.zeros(B, self.Hkv, L, self.D, dtype=self.dtype, device=dev) for _ in self.layers]
         if sampling:
             self.u = torch.zeros(L, B, dtype=torch.float32, device=dev)  # a number per token and sequence
+            self._generator, self._fresh = None, False  # whose they are; whether a sequence has not used them yet
             self.settings = dict(temperature=torch.ones(B, device=dev), top_k=torch.zeros(B, dtype=torch.int32, device=dev),
                                  top_p=torch.ones(B, device=dev), min_p=torch.zeros(B, device=dev))
         if self.kind == "llama":
@@ -463,15 +465,21 @@ class GraphDecoder:
     def set_sampling(self, temperature=None, top_k=None, top_p=None, min_p=None, generator=None) -> None:
         """New settings (a number, or one per sequence; None: as they are; at first
         the whole distribution at temperature 1) and fresh random numbers for the
-        tokens to come, from ``generator`` (torch's default one of the device)."""
+        tokens to come, from ``generator`` (torch's default one of the device), which
+        later prompts draw theirs from too."""
         if not self.sampling:
             raise ValueError("GraphDecoder: built without sampling=True")
         for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             if value is not None:
                 t = self.settings[name]
                 t.copy_(torch.as_tensor(value, device=self.dev).to(t.dtype).expand(self.B))
-        dev = self.dev if generator is None else generator.device
-        self.u.copy_(torch.rand(self.u.shape, generator=generator, device=dev))
+        self._generator = generator
+        self._draw()
+
+    def _draw(self) -> None:
+        g = self._generator
+        self.u.copy_(torch.rand(self.u.shape, generator=g, device=self.dev if g is None else g.device))
+        self._fresh = True
 
     @staticmethod
     def _argmax(logits):
@@ -513,6 +521,10 @@ class GraphDecoder:
             raise ValueError(f"prefill: batch {B} (decoder built for {self.B}), prompt {S} (cache {self.L})")
         if self.use_graph and not self.captured:
             self._capture()
+        if self.sampling:
+            if not self._fresh:
+                self._draw()
+            self._fresh = False
         from transformers import DynamicCache
         cache = DynamicCache()
         with contextlib.nullcontext() if self.window is None else window_prompts(self.model, self.window, self.sinks):
@@ -544,6 +556,7 @@ class GraphDecoder:
         if self.S + self._n >= self.L:
             raise RuntimeError(f"GraphDecoder: cache of {self.L} positions is full")
         self._n += 1
+        self._fresh = False
         if self.use_graph:
             self.graph.replay()
             return self.logits

@@ -160,3 +160,28 @@ def test_cache_sizes_and_refusals():
         with window_prompts(m, 8):
             raise RuntimeError
     assert m.config._attn_implementation == "sdpa"
+
+
+def test_every_prompt_draws_its_numbers():
+    """set_sampling's numbers serve the prompt that follows; prompts without it, and
+    the first one, draw their own, from the last generator."""
+    gd = GraphDecoder(_model("llama"), batch=2, max_len=24, sampling=True)
+    ids = torch.randint(0, 512, (2, 5), device=DEV)
+    gd.prefill(ids)
+    one = gd.u.clone()
+    assert one.min() >= 0 and one.max() < 1 and one.unique().numel() > 40
+    gd.step()
+    gd.set_sampling(temperature=1.2, generator=torch.Generator().manual_seed(3))
+    two = gd.u.clone()
+    assert torch.equal(two.cpu(), torch.rand(24, 2, generator=torch.Generator().manual_seed(3)))
+    gd.step()  # takes them, so that the next prompt may not
+    g = torch.Generator().manual_seed(3)
+    torch.rand(24, 2, generator=g)
+    gd.prefill(ids)
+    assert torch.equal(gd.u.cpu(), torch.rand(24, 2, generator=g))
+    gd.set_sampling(generator=torch.Generator().manual_seed(4))
+    three = gd.u.clone()
+    gd.prefill(ids)
+    assert torch.equal(gd.u, three)
+    gd.prefill(ids)
+    assert not torch.equal(gd.u, three)
