@@ -86,6 +86,10 @@ __device__ __forceinline__ uint32_t quantize8(const uint16_t (&h)[8], uint16_t* 
 // elements a thread and step, keys first.  A slot takes the newest of the
 // given positions that belongs to it; slots without one keep what they hold.
 // The codes of the values are turned in LDS.
+// Bound by its instructions, about 90 a thread for 8 elements (the vector units are
+// four fifths busy): 4 sequences x 8 heads x 8192 positions of 128, 134 MB read and 42
+// written, 49 us, 3.6 TB/s.  (Heads next to each other in the grid, several blocks a
+// workgroup with the next one's rows on the way, extremes by pairs: all the same.)
 template <int D>
 __global__ __launch_bounds__(256) void kv4_store_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                         int64_t ksb, int64_t ksh, int64_t kss, int64_t vsb, int64_t vsh,
@@ -169,7 +173,8 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(const uint16_t* __restri
   }
 }
 
-// Slots [0, count) back in fp16: fp16(s c + m), the product exact in f32.
+// Slots [0, count) back in fp16: fp16(s c + m), the product exact in f32.  Bound by
+// HBM: the case above, 42 MB read and 134 written, 27 us, 6.5 TB/s.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_load_kernel(Cache4 c, int slots, int count, uint16_t* __restrict__ k,
                                                        uint16_t* __restrict__ v) {
