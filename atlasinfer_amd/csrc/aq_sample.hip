@@ -30,7 +30,7 @@
 //            by the bits of their keys, 11 at a time, with the same histograms.
 //            (Bins by the keys' own first bits fall on the few exponents that most
 //            logits share: nearly every row went through all bits, top-p of 256 fp32
-//            rows of 32000 took 53 us, here 48; of one fp16 row of 50272 40, here 34.)
+//            rows of 32000 took 53 us, here 46; of one fp16 row of 50272 40, here 35.)
 //   token    kept masses by segments of 1 KiB, summed in the pass that lists the
 //            bin's members; one wave goes through the segment that the number falls in
 //
@@ -116,30 +116,45 @@ __device__ __forceinline__ uint32_t keys_of_word(uint32_t w) {
 // rndne and ldexp, take four times as long as an addition.)  x is taken from lo
 // on, where the weight is 2^-60 or less, and -inf and NaN with it.
 struct Weigh {
+  static constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52
   double mx, c;
   const double* table;
   float lo, hi;
   bool endless;  // a row with infinities: these weigh 1 and every number nothing
-  __device__ __forceinline__ uint64_t operator()(float x) const {
+  // d = x - mx and t = y + 1.5 2^52
+  __device__ __forceinline__ void step(float x, double* d, double* t) const {
+    if (endless) {
+      asm volatile("");  // a branch, which few rows take
+      x = x == INFINITY ? hi : lo;
+    }
+    *d = (double)__builtin_amdgcn_fmed3f(x, lo, hi) - mx;
+    *t = fma(*d, c, kMagic);
+  }
+  __device__ __forceinline__ uint64_t weight(double d, double t) const {
     constexpr double a = 0.0013538030870311431, a2 = a * a / 2, a3 = a * a * a / 6;  // ln 2 / 512
-    constexpr double k = 6755399441055744.0, one = 4503599627370496.0;
-    if (endless) x = x == INFINITY ? hi : lo;
-    x = __builtin_amdgcn_fmed3f(x, lo, hi);
-    const double d = (double)x - mx, t = fma(d, c, k), r = fma(d, c, k - t);
+    constexpr double one = 4503599627370496.0;
+    const double r = fma(d, c, kMagic - t);
     const int n = (int)__builtin_bit_cast(uint64_t, t);
     const uint64_t e = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)]) + ((uint64_t)(uint32_t)((n >> 9) << 20) << 32);
     const double v = fma(__builtin_bit_cast(double, e), fma(r, fma(r, fma(r, a3, a2), a), 1.0), one);
     return __builtin_bit_cast(uint64_t, v) - __builtin_bit_cast(uint64_t, one);
   }
-};
-
-// Bins by how far below the maximum a logit lies, 43.1 halvings of its weight in
-// all: bin kBins - 1 has the largest, and what bin 0 has (from 43 halvings on) weighs
-// 0.  Subtraction, product and conversion never turn an order around.
-struct Bins {
-  float mx, q;  // q = 2047 / (43.1 ln 2 T)
-  __device__ __forceinline__ float place(float x) const {  // NaN as -inf; inf - inf is a maximum
-    return fmaxf((mx - fmaxf(x, -INFINITY)) * q, 0.0f);
+  // The bin, by how far below the maximum x lies: kBins - 1 has the largest, and what
+  // bin 0 has (n <= -22065, 43 halvings and more) weighs 0.  Never turns an order
+  // around, as n does not.
+  static __device__ __forceinline__ int bin_of(double t) {
+    const int n = (int)__builtin_bit_cast(uint64_t, t);
+    return max(kBins - 1 - ((-n * 95) >> 10), 0);
+  }
+  __device__ __forceinline__ uint64_t operator()(float x) const {
+    double d, t;
+    step(x, &d, &t);
+    return weight(d, t);
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    double d, t;
+    step(x, &d, &t);
+    return bin_of(t);
   }
 };
 
@@ -426,7 +441,6 @@ __device__ __forceinline__ Weigh weigh_from(float mx, float T, const double* tab
 __device__ __forceinline__ uint64_t whole_of(float min_p) {  // the least weight that min-p leaves
   return min_p > 0.0f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * kOne) : 0;
 }
-__device__ __forceinline__ Bins bins_from(float mx, float T) { return Bins{mx, 68.52f / fminf(T, 1e34f)}; }
 __device__ __forceinline__ void fill_table(double* table) {
   if (tid() < kTable) table[tid()] = exp2((double)tid() / kTable) * kOne;
 }
@@ -438,27 +452,34 @@ __device__ __forceinline__ void append(Shared& s, int V, int i, uint32_t key) {
 }
 
 // Masses (of w >= wmin) by segment, to seg_mass.  LISTING: of what lies in the bins
-// above `bin` (counted from the top); what lies in it goes to the list.  Else of the
-// keys above `cut`; those equal to it are counted by segment.
+// above `bin`; what lies in it goes to the list (bin 0 does not).  Else of the keys
+// above `cut`; those equal to it are counted by segment.
 template <int FMT, bool LISTING>
 __device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, const Weigh& weigh, uint64_t wmin,
-                                             const Bins& bins, float bin, uint32_t cut, uint64_t* seg_mass) {
+                                             int bin, uint32_t cut, uint64_t* seg_mass) {
   row.each_piece([&](int c, const uint4& v) {
     uint64_t sum = 0;
     uint32_t ties = 0;
+    bool hit = false;
     row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-      const float x = Logit<FMT>::value(bits), at = LISTING ? bins.place(x) : 0.0f;
-      const bool above = LISTING ? at < bin : key > cut;
+      double d, t;
+      weigh.step(Logit<FMT>::value(bits), &d, &t);
+      const int at = LISTING ? Weigh::bin_of(t) : 0;
+      const bool above = LISTING ? at > bin : key > cut;
       if (__ballot(above)) {  // the exponential only where a lane asks for it
-        const uint64_t w = weigh(x);
+        const uint64_t w = weigh.weight(d, t);
         sum += above && w >= wmin ? w : 0;
       }
       if (LISTING) {
-        if (!above && at < bin + 1.0f && c < row.c1) append(s, row.V, i, key);
+        hit |= at == bin;
       } else {
         ties += (uint32_t)__popcll(__ballot(key == cut && (uint32_t)i < (uint32_t)row.V));
       }
     });
+    if (LISTING && bin && hit && c < row.c1)
+      row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
+        if (weigh.bin(Logit<FMT>::value(bits)) == bin) append(s, row.V, i, key);
+      });
     sum = wave_scan_u64(sum);
     if ((tid() & 63) == 63 && c - 63 < row.c1) {  // 64 pieces are a segment
       seg_mass[c >> 6] = sum;
@@ -535,12 +556,12 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const void* __res
   fill_table(table);
   __syncthreads();
   const Weigh weigh = weigh_from(mx, T, table);
-  const Bins bins = bins_from(mx, T);
   row.each_piece([&](int c, const uint4& v) {
     row.each_element(c, v, [&](int, uint32_t bits, uint32_t) {
-      const float x = Logit<FMT>::value(bits), at = bins.place(x);
-      if (at < kBins - 1.0f)
-        atomicAdd((unsigned long long*)&mass[kBins - 1 - (int)at], weigh(x));
+      double d, t;
+      weigh.step(Logit<FMT>::value(bits), &d, &t);
+      const int at = Weigh::bin_of(t);
+      if (at) atomicAdd((unsigned long long*)&mass[at], weigh.weight(d, t));
     });
   });
   __syncthreads();
@@ -566,7 +587,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* _
   if (mx == -INFINITY) return;
   fill_table(s.table);
   if (t == 0) s.n_list = 0;
-  float bin = INFINITY;  // no list, everything above
+  int bin = 0;  // no list: everything that weighs something lies above
   if (p < 1.0f) {
     for (int i = t; i < kBins; i += kThreads) {
       s.mass[i] = w.mass[i];
@@ -575,7 +596,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* _
     __syncthreads();
     uint64_t most = 0;
     const Found f = find_bin(s, true, most, p);
-    bin = (float)(kBins - 1 - (int)f.bin);
+    bin = (int)f.bin;
     if (blockIdx.x == 0 && t == 0) {
       w.most = most;
       w.above = f.mass;
@@ -584,7 +605,7 @@ __global__ __launch_bounds__(kThreads) void sample_segments_kernel(const void* _
   }
   __syncthreads();
   const uint64_t wmin = whole_of(mp);
-  sum_segments<FMT, true>(s, row, weigh_from(mx, T, s.table), wmin, bins_from(mx, T), bin, 0, w.seg_mass);
+  sum_segments<FMT, true>(s, row, weigh_from(mx, T, s.table), wmin, bin, 0, w.seg_mass);
   const uint32_t n = s.n_list;  // more than there is room for is counted all the same
   if (t == 0) at = atomicAdd(&w.n_list, n);
   __syncthreads();
@@ -706,7 +727,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
   Cut cut = {0, 0};  // everything
   bool from_list = false, summed = false, binned = false;
   uint64_t mass = 0;
-  const Bins bins = bins_from(mx, T);
   // f(index, key) for the list's members or the row's tokens
   auto each = [&](auto f) {
     if (from_list) {
@@ -751,7 +771,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
     uint64_t most = by_mass ? (by_k ? reach(p, mass) : 0) : (uint64_t)k;
     // the bin in which the running count (by_mass: the running mass) reaches `most`;
     // then, unless its members are few, the bits of their keys, 11 at a time
-    float bin = 0.0f;
+    int bin = 0;
     uint32_t key = 0, above = 0, ties = 0;  // the last key kept, how many of it
     uint64_t above_mass = 0;
     bool all = false;
@@ -767,12 +787,14 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         if (!first || !binned) {
           clear_bins(s);
           each([&](int i, uint32_t y) {
-            const float x = L::value_of_key(y), at = bins.place(x);
-            if (!(at < kBins - 1.0f) || (uint32_t)i >= (uint32_t)V) return;  // the rest weighs nothing
-            if (!first && !(at >= bin && at < bin + 1.0f && (shift == B || y >> (shift & 31) == key))) return;
-            const uint32_t to = first ? kBins - 1 - (uint32_t)at : (y >> next) & ((1u << bits) - 1);
+            double d, t;
+            weigh.step(L::value_of_key(y), &d, &t);
+            const int at = Weigh::bin_of(t);
+            if (!at || (uint32_t)i >= (uint32_t)V) return;  // the rest weighs nothing
+            if (!first && !(at == bin && (shift == B || y >> (shift & 31) == key))) return;
+            const uint32_t to = first ? (uint32_t)at : (y >> next) & ((1u << bits) - 1);
             if (by_k || !first) atomicAdd(&s.count[to], 1u);
-            atomicAdd((unsigned long long*)&s.mass[to], weigh(x));
+            atomicAdd((unsigned long long*)&s.mass[to], weigh.weight(d, t));
           });
           __syncthreads();
         }
@@ -797,21 +819,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
         all = true;
         break;
       }
-      bin = (float)(kBins - 1 - (int)f.bin);
+      bin = (int)f.bin;
       // its members: the list, or `members`
       if (t == 0) s.n_members = 0;
       __syncthreads();
       const uint2* members = s.members;
       uint32_t n;
       if (by_mass && !by_k) {
-        if (!done) sum_segments<FMT, true>(s, r, weigh, wmin, bins, bin, 0, s.seg_mass);
+        if (!done) sum_segments<FMT, true>(s, r, weigh, wmin, bin, 0, s.seg_mass);
         members = s.list;
         n = s.n_list;
         summed = from_list = n <= kList;
       } else {
         each([&](int i, uint32_t key) {
-          const float place = bins.place(L::value_of_key(key));
-          if (place >= bin && place < bin + 1.0f && (uint32_t)i < (uint32_t)V) {
+          if (weigh.bin(L::value_of_key(key)) == bin && (uint32_t)i < (uint32_t)V) {
             const uint32_t at = atomicAdd(&s.n_members, 1u);
             if (at < kSmallList) s.members[at] = make_uint2(key, (uint32_t)i);
           }
@@ -898,7 +919,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
       }
     }
   } else if (!summed) {
-    sum_segments<FMT, false>(s, r, weigh, wmin, bins, 0.0f, cut.key, s.seg_mass);
+    sum_segments<FMT, false>(s, r, weigh, wmin, 0, cut.key, s.seg_mass);
   }
   __syncthreads();
 
@@ -969,7 +990,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 
 // Workgroups a row is split into: enough to fill the GPU, 1024 pieces each at
 // least, for rows that have 2048 (top-p of 64 rows of 128256: one workgroup each
-// 106 us, four 56; of one row in fp32 118 us and, in 31, 38).  One setting of top-k
+// 106 us, four 55; of one row in fp32 118 us and, in 31, 38).  One setting of top-k
 // for all rows rules the split out.
 static int parts_of(int64_t B, int64_t V, int dtype, bool top_k) {
   const int64_t per = dtype == AQ_F32 ? 4 : 8, pieces = V / per;
