@@ -313,24 +313,27 @@ __device__ __forceinline__ uint2 row16_bcast(uint2 x) {
 __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_f32<6>(xlane_level_max_f32<5>(x)); }
 
 // Workgroup (j, b, z) takes key/value head j (and head tile) of sequence b and
-// blocks z nt .. of its slots; wave w every nw-th of them.  One step is a block
-// of 32 slots: scores of 2 x 16 slots against up to 16 query heads
-// (mfma 16 x 16 x 32, keys as rows, so that a lane's results are 2 x 4 slots of
-// one head), the running softmax of a head in the four lanes that hold it, the
+// blocks z nt .. of its slots; wave w every nw-th of them.  The last spans, which
+// short sequences do not have, come first: the workgroups that have nothing to do are
+// gone before the GPU runs empty (lengths of 1 to 16384: 92 us, first spans first 95).
+// One step is a block of 32 slots: scores of 2 x 16 slots against up to 16 query
+// heads (mfma 16 x 16 x 32, keys as rows, so that a lane's results are 2 x 4 slots
+// of one head), the running softmax of a head in the four lanes that hold it, the
 // numerators as the second product's operand, which they are without an exchange,
 // and the values' rows.
 //   Scores: the products of one group's codes, whole numbers as fp16, with the
 // query are exact to f32 and scaled there; the minima meet the sums of the query
 // in a product of f32 (16 x 16 x 4).  Keys rounded to fp16 (a fused multiply-add a
 // pair, the scales then inside the product) gave 4.2e-4 of the result against 2.1e-4
-// of the output's own rounding, at 89 us for the long case below instead of 95.
+// of the output's own rounding, at 89 us for the long case below where this took 95.
 //   Numerators are two fp16 numbers each, the second what the first leaves over: with
 // one alone the error is 3.0e-4 and 91 us.  With both 2.6e-4: what is left beside
 // the output's rounding is that of the values s c + m to fp16, once each (fma).  The
 // denominator is the product of the same numerators with ones.
 // Bound by HBM and by the instructions together: a step of 32 slots of D = 128 is 290
 // vector and 29 matrix instructions a wave for 5 KiB (32 sequences x 8 heads of up to
-// 16384 slots, half of them in use: 336 MB in 95 us, 3.5 TB/s).
+// 16384 slots, half of them in use: 336 MB in 92 us, 3.7 TB/s; all of 8192: 77, 4.4; the
+// loads alone take 68).
 template <int D>
 __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, Cache4 c,
@@ -341,7 +344,8 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
   constexpr int ND = D / 16;   // row tiles of the output
   const int t = threadIdx.x, ln = t & 63, nw = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int j = blockIdx.x / hb, h0 = blockIdx.x % hb * kHeads, b = blockIdx.y, z = blockIdx.z;
+  const int j = blockIdx.x / hb, h0 = blockIdx.x % hb * kHeads, b = blockIdx.y;
+  const int z = ns - 1 - (int)blockIdx.z;
   const int G = H / Hkv, heads = min(kHeads, G - h0);
   const int64_t pos = pos_p[(int64_t)b * pos_stride];
   if (pos < 0 || pos >= max_pos) return;
