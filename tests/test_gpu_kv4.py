@@ -267,3 +267,24 @@ def test_refusals():
     with pytest.raises(ValueError):
         DC.kv4_buffers(1, 1, 10, 96, DEV)
     DC.kv4_store(h(2, 2, 0, 64), h(2, 2, 0, 64), cache, slots=40)  # nothing to do
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_positions_of_31_bits(bits):
+    """Positions far past a window take the slots of the near ones they are equal to
+    modulo it; the last one that is run is 2^31 - 2."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    B, H, Hkv, D, slots, sinks = 2, 4, 2, 128, 75, 5
+    k, v = _rnd(g, B, Hkv, slots, D), _rnd(g, B, Hkv, slots, D)
+    q, kn, vn = _rnd(g, B, H, D), _rnd(g, B, Hkv, D), _rnd(g, B, Hkv, D)
+    far = torch.tensor([2 ** 31 - 2, 2 ** 31 - 1000], device=DEV)
+    near = sinks + (far - sinks) % (slots - sinks) + 3 * (slots - sinks)
+    caches = [DC.DecodeCache(B, Hkv, slots, D, bits=bits, sinks=sinks, device=DEV) for _ in range(3)]
+    for c in caches:
+        c.store(k, v)
+    outs = [c.attend(q, kn, vn, p, scale=0.1) for c, p in zip(caches, (far, near))]
+    assert torch.equal(*outs)
+    assert all(torch.equal(a, b) for a, b in zip(caches[0].buffers, caches[1].buffers))
+    out = torch.full((B, H, D), 3.0, dtype=torch.float16, device=DEV)
+    caches[2].attend(q, kn, vn, torch.tensor([2 ** 31 - 1], device=DEV), scale=0.1, out=out)
+    assert (out == 3.0).all()
