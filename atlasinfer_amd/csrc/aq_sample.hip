@@ -995,7 +995,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const void* __restrict
 static int parts_of(int64_t B, int64_t V, int dtype, bool top_k) {
   const int64_t per = dtype == AQ_F32 ? 4 : 8, pieces = V / per;
   if (top_k || pieces < 2048) return 1;
-  return (int)std::min<int64_t>(std::min<int64_t>(kMaxParts, 256 / B), pieces / 1024);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxParts, 256 / B), pieces / 1024));
 }
 
 extern "C" int64_t aq_sample_workspace(int64_t B, int64_t V, int dtype, int32_t top_k0) {

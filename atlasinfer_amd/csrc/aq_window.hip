@@ -353,7 +353,8 @@ extern "C" int aq_window_attention(const void* q, const void* k, const void* v, 
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   a.blocks = (int)aq::ceil_div(M, kQ);
   const int64_t items = B * H * a.blocks;
-  AQ_CHECK_ARG(items <= (1 << 30), "aq_window_attention: %lld blocks of queries", (long long)items);
+  // (a grid has fewer than 2^32 threads)
+  AQ_CHECK_ARG(items <= (1 << 24) - 8, "aq_window_attention: %lld blocks of queries", (long long)items);
   a.items = (int)items;
   a.per = (int)aq::ceil_div(items, 8);
   const dim3 grid((unsigned)(8 * a.per));

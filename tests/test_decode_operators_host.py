@@ -65,8 +65,9 @@ def test_sample_workspace_rule(lib):
     assert one > 0 and one % 16 == 0
     # rows of 2048 pieces of 16 bytes, where there are too few rows for the GPU and no top-k
     for args, parts in (((64, 128256, 0, 0), True), ((128, 128256, 0, 0), True), ((129, 128256, 0, 0), False),
-                        ((1, 2048 * 8, 1, 0), True), ((1, 2048 * 8 - 1, 1, 0), False), ((1, 2048 * 4, 2, 0), True),
-                        ((1, 128256, 0, 50), False), ((1, 128256, 0, 128256), True), ((1, 128256, 0, -1), True)):
+                        ((257, 128256, 0, 0), False), ((65535, 128256, 0, 0), False), ((1, 2048 * 8, 1, 0), True),
+                        ((1, 2048 * 8 - 1, 1, 0), False), ((1, 2048 * 4, 2, 0), True), ((1, 128256, 0, 50), False),
+                        ((1, 128256, 0, 128256), True), ((1, 128256, 0, -1), True)):
         assert size(*args) == (args[0] * one if parts else 0), args
 
 
@@ -167,6 +168,7 @@ def test_window_attention_refusals(lib):
         c.bad("multiples of 8", **{x: _strides(*t)})
     for x, far in itertools.product(("ks", "vs"), (-64, (1 << 23) + 8)):
         c.bad("2^23", **{x: _strides(0, 0, far)})
+    c.bad("blocks of queries", B=65535, H=512, Hkv=1, M=1, N=1)
     for x in ("q", "k", "v", "out"):
         c.bad("16-byte aligned", **{x: ODD})
     c.bad("16-byte aligned", starts=ctypes.c_void_p(4098))

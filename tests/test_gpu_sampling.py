@@ -206,3 +206,13 @@ def test_refusals():
         with pytest.raises(ValueError):
             sample_tokens(*args, **kw)
     assert sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+def test_more_long_rows_than_workgroups_fit():
+    """More than 256 rows are never split, however long."""
+    g = torch.Generator(device=DEV).manual_seed(21)
+    x = torch.randn(300, 17000, generator=g, device=DEV).half()
+    u = torch.rand(300, generator=g, device=DEV)
+    got = sample_tokens(x, u, 0.9, 0, 0.8)
+    parts = torch.cat([sample_tokens(x[i:i + 75], u[i:i + 75], 0.9, 0, 0.8) for i in range(0, 300, 75)])
+    assert torch.equal(got, parts)
