@@ -460,7 +460,6 @@ __device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, con
   row.each_piece([&](int c, const uint4& v) {
     uint64_t sum = 0;
     uint32_t ties = 0;
-    bool hit = false;
     row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
       double d, t;
       weigh.step(Logit<FMT>::value(bits), &d, &t);
@@ -471,15 +470,11 @@ __device__ __forceinline__ void sum_segments(Shared& s, const Row<FMT>& row, con
         sum += above && w >= wmin ? w : 0;
       }
       if (LISTING) {
-        hit |= at == bin;
+        if (bin && at == bin && c < row.c1) append(s, row.V, i, key);
       } else {
         ties += (uint32_t)__popcll(__ballot(key == cut && (uint32_t)i < (uint32_t)row.V));
       }
     });
-    if (LISTING && bin && hit && c < row.c1)
-      row.each_element(c, v, [&](int i, uint32_t bits, uint32_t key) {
-        if (weigh.bin(Logit<FMT>::value(bits)) == bin) append(s, row.V, i, key);
-      });
     sum = wave_scan_u64(sum);
     if ((tid() & 63) == 63 && c - 63 < row.c1) {  // 64 pieces are a segment
       seg_mass[c >> 6] = sum;
