@@ -94,6 +94,9 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
   // runs of neighbouring items to an XCD (they share keys and values in its L2)
   const int item = (int)(blockIdx.x & 7) * a.per + (int)(blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= a.per || item >= a.items) return;
+  // cleared before any wave may set one, which is before the loop's first barrier
+  if (t < NS) bad[t] = 0;
+  __syncthreads();
   // heads of a group next to each other, late blocks (more keys) first
   const int g = item % a.G, qb = a.blocks - 1 - item / a.G % a.blocks, u = item / a.G / a.blocks;
   const int hkv = a.H / a.G, b = u / hkv, j = u % hkv, head = j * a.G + g, q0 = qb * kQ;
@@ -172,7 +175,6 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
 #pragma unroll
   for (int e = 0; e < 2; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
 
-  if (t < NS) bad[t] = 0;
   for (int i = 0; i < min(NS - 1, tiles); i++) load(i);
   for (int i = 0; i < tiles; i++) {
     const int k0 = tile_at(i) * kK;

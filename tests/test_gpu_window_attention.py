@@ -227,3 +227,21 @@ def test_prompt_then_steps(bits):
                     if bits == 4:
                         want = R.values(*R.quantize(want.cpu())).half().to(DEV)
                     assert ((x[b, :, R.slot_of(p, slots, sinks)] - want).abs() <= 2e-3 * want.abs()).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [64, 100, 300])
+def test_unseen_values_of_the_first_tile(D, N):
+    """Infinities and NaN in the rows that each of the waves loads of the first tile, in
+    many heads at once: queries before them do not see them."""
+    g = torch.Generator(device=DEV).manual_seed(N)
+    B, H = 8, 16
+    q, k, v = _rnd(g, B, H, N, D), _rnd(g, B, H, N, D), _rnd(g, B, H, N, D)
+    first = torch.tensor([3, 17, 31, 33, 47, 49, 62, 63], device=DEV)  # by sequence
+    for b, at in enumerate(first.tolist()):
+        v[b, :, at, b::5] = [float("nan"), float("inf"), -float("inf")][b % 3]
+    for window, sinks in ((N, 0), (20, 4)):
+        got = window_attention(q, k, v, window=window, sinks=sinks).double()
+        want, bound = _reference(q, k, v, window, sinks, D ** -0.5, None)
+        before = (torch.arange(N, device=DEV)[None] < first[:, None])[..., None, None]
+        assert (((got - want).abs() <= bound) | ~before).all()
