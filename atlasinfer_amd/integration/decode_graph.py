@@ -50,7 +50,8 @@ Options (on the GPU path with an fp16 model):
 * ``window``, ``sinks``: attention through a sliding window, the first ``sinks``
   positions staying visible; the cache holds just these, so ``max_len`` bounds
   positions but not memory.  A model whose configuration has a sliding window
-  shorter than ``max_len`` gets that window by itself.
+  shorter than ``max_len`` gets that window by itself; a window given here takes
+  its place, for the prompt as for the steps.
 
 Limits: equal-length prompts without padding (batch rows share ``pos``), no
 beam search.
@@ -104,10 +105,12 @@ class GraphDecoder:
             self.H = cfg.num_attention_heads
             self.Hkv = self.H
             self.D = cfg.hidden_size // self.H
+            configured = None
         else:
             self.layers = list(model.model.layers)
-            if window is None and getattr(cfg, "sliding_window", None) not in (None, 0):
-                window = cfg.sliding_window
+            configured = getattr(cfg, "sliding_window", None) or None
+            if window is None:
+                window = configured
             self.H = cfg.num_attention_heads
             self.Hkv = getattr(cfg, "num_key_value_heads", None) or self.H
             self.D = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.H
@@ -129,12 +132,15 @@ class GraphDecoder:
             raise ValueError("GraphDecoder: sinks without a window")
         # the window, None where it reaches back to the first position anyway
         self.window = window if window is not None and sinks + window < L else None
+        # a prompt goes through the model's own forward as it is only where that applies
+        # no window either; it applies the configured one, whatever is asked for here
+        self._own_prompt = self.window is None and (configured is None or configured >= L)
         self.sinks, self.kv_bits, self.sampling = sinks, kv_bits, sampling
         if kv_bits not in (4, 16):
             raise ValueError(f"GraphDecoder: kv_bits {kv_bits} (4 or 16)")
-        if not self.fused and (self.window is not None or kv_bits != 16 or sampling):
-            raise NotImplementedError("GraphDecoder: a sliding window shorter than max_len, kv_bits=4 and sampling need "
-                                      "an fp16 model on a HIP device, head size 64 or 128")
+        if not self.fused and (not self._own_prompt or kv_bits != 16 or sampling):
+            raise NotImplementedError("GraphDecoder: a sliding window shorter than max_len (asked for or configured), "
+                                      "kv_bits=4 and sampling need an fp16 model on a HIP device, head size 64 or 128")
         self.caches = None
         if self.window is not None or kv_bits != 16:
             slots, keep = (L, None) if self.window is None else (sinks + self.window, sinks)
@@ -527,7 +533,7 @@ class GraphDecoder:
             self._fresh = False
         from transformers import DynamicCache
         cache = DynamicCache()
-        with contextlib.nullcontext() if self.window is None else window_prompts(self.model, self.window, self.sinks):
+        with contextlib.nullcontext() if self._own_prompt else window_prompts(self.model, self.window, self.sinks):
             out = self.model(input_ids=input_ids.to(self.dev), past_key_values=cache, use_cache=True)
         for li in range(len(self.layers)):
             kl, vl = cache.layers[li].keys, cache.layers[li].values  # [B, Hkv, S, D]

@@ -125,3 +125,19 @@ def test_window_prompts_reach_the_attention(monkeypatch):
         assert seen == [((2, 4, 11, 32), (2, heads, 11, 32), w, s, scale) for w, s in [(100, 0)] * 2 + [(3, 1)] * 2]
         assert (same - whole).abs().max() < 1e-5 and (short - whole).abs().max() > 1e-4
         assert torch.allclose(short[:, :4], whole[:, :4], atol=1e-5)  # these see everything through window and sink
+
+
+def test_a_longer_window_than_the_configured_one_needs_the_gpu_path():
+    """Where the steps would see every position but the model's own forward applies
+    its configured window to the prompt, the torch form of the step is refused."""
+    m = _model("mistral")
+    m.config.sliding_window = 4
+    for kw in (dict(window=64), dict(window=30, sinks=2), dict(sinks=28)):
+        with pytest.raises(NotImplementedError):
+            GraphDecoder(m, batch=1, max_len=32, graph=False, **kw)
+    assert GraphDecoder(m, batch=1, max_len=4, graph=False, window=9).window is None
+    m.config.sliding_window = None
+    ids = torch.randint(0, 256, (1, 20))
+    with torch.no_grad():
+        ref = m.generate(ids, attention_mask=torch.ones_like(ids), max_new_tokens=5, do_sample=False)
+    assert torch.equal(GraphDecoder(m, batch=1, max_len=32, graph=False, window=64).generate(ids, 5), ref)

@@ -185,3 +185,35 @@ def test_every_prompt_draws_its_numbers():
     assert torch.equal(gd.u, three)
     gd.prefill(ids)
     assert not torch.equal(gd.u, three)
+
+
+@pytest.mark.parametrize("options", [dict(window=64), dict(window=100, sinks=2), dict(sinks=52), dict(window=40, sinks=24),
+                                     dict(window=64, kv_bits=4)])
+def test_a_window_that_reaches_max_len_replaces_the_configured_one(options):
+    """A Mistral with a configured window, decoded with one that reaches back to the
+    first position: the prompt, longer than the configured window, sees every position
+    before it as the steps do."""
+    from transformers import AttentionInterface
+    from transformers.masking_utils import AttentionMaskInterface
+    m = _model("mistral", 4, sliding_window=12)
+    ids = torch.randint(0, 512, (2, 30), device=DEV)
+    four = options.get("kv_bits") == 4
+    name = f"ref_whole_{four}"
+    AttentionInterface.register(name, _reference_attention(None, 0, four))
+    AttentionMaskInterface.register(name, lambda *a, **k: None)
+    before = m.config._attn_implementation
+    m.config.sliding_window = None  # HF's cache would keep the window alone
+    m.set_attn_implementation(name)
+    with torch.no_grad():
+        ref = m.generate(ids, attention_mask=torch.ones_like(ids), max_new_tokens=20, do_sample=False,
+                         return_dict_in_generate=True, output_logits=True)
+    m.set_attn_implementation(before)
+    m.config.sliding_window = 12
+    gd = GraphDecoder(m, 2, 64, **options)
+    assert gd.window is None
+    gd.prefill(ids)
+    assert m.config._attn_implementation == before
+    for t in range(1, 20):
+        gd.tok.copy_(ref.sequences[:, 30 + t - 1])
+        got, want = gd.step().float(), ref.logits[t].float()
+        assert ((got - want).abs().amax(-1) <= 2e-2 * want.abs().amax(-1)).all(), t
