@@ -120,12 +120,16 @@ struct Weigh {
   double mx, c;
   const double* table;
   float lo, hi;
-  bool endless;  // a row with infinities: these weigh 1 and every number nothing
+  // 0: a row with infinities: these weigh 1 and every number nothing; 1/2: one of large
+  // negative numbers, taken by their halves (exact), mx, lo and hi too, so that there are
+  // numbers below the lowest that weighs something; 1: every other (then `other` is 0)
+  float factor;
+  int other;
   // d = x - mx and t = y + 1.5 2^52
   __device__ __forceinline__ void step(float x, double* d, double* t) const {
-    if (endless) {
+    if (other) {
       asm volatile("");  // a branch, which few rows take
-      x = x == INFINITY ? hi : lo;
+      x = x == INFINITY ? hi : x * factor;
     }
     *d = (double)__builtin_amdgcn_fmed3f(x, lo, hi) - mx;
     *t = fma(*d, c, kMagic);
@@ -429,14 +433,19 @@ struct PartsOfRow {
 };
 
 __device__ __forceinline__ Weigh weigh_from(float mx, float T, const double* table) {
-  if (mx == INFINITY) return Weigh{1.0, 30720.0, table, 0.0f, 1.0f, true};
-  double c = 738.6598609514740 / (double)fminf(T, 1e34f);  // 512 log2(e) / T
-  float lo = fmaxf((float)((double)mx - 30720.0 / c), -3.4028235e38f);
-  if (!(lo < mx)) {  // T is far below the logits' steps: the next one weighs nothing
-    lo = nextafterf(mx, -INFINITY);
-    c = 30720.0 / ((double)mx - (double)lo);
+  if (mx == INFINITY) return Weigh{1.0, 30720.0, table, 0.0f, 1.0f, 0.0f, 1};
+  // lo lies at least 60 halvings below the maximum and is a finite number: for rows
+  // below half the lowest of fp32 by way of their halves (T counts as 1e34 at most)
+  const float f = mx < -1.7014118e38f ? 0.5f : 1.0f;
+  const double m = f * mx, t = (double)f * (double)fminf(T, 1e34f);
+  double c = 738.6598609514740 / t;  // 512 log2(e) / T
+  float lo = (float)(m - 41.588830833596719 * t);
+  if (!((m - (double)lo) * c >= 30720.0)) {
+    asm volatile("");  // a branch: lo was rounded up; T may be far below the logits' steps, the next one weighs nothing
+    lo = nextafterf(lo, -INFINITY);
+    c = fmin(c, 92160.0 / (m - (double)lo));
   }
-  return Weigh{(double)mx, c, table, lo, mx, false};
+  return Weigh{m, c, table, lo, (float)m, f, __builtin_amdgcn_readfirstlane(f != 1.0f)};  // mx is the row's
 }
 __device__ __forceinline__ uint64_t whole_of(float min_p) {  // the least weight that min-p leaves
   return min_p > 0.0f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * kOne) : 0;

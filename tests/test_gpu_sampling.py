@@ -1,5 +1,7 @@
 """aq_sample against a plain form in 64 bits: every filter, ties, rows that
 leave nothing, all types, ragged sizes, settings per row, graphs."""
+import math
+
 import pytest
 import torch
 
@@ -216,3 +218,55 @@ def test_more_long_rows_than_workgroups_fit():
     got = sample_tokens(x, u, 0.9, 0, 0.8)
     parts = torch.cat([sample_tokens(x[i:i + 75], u[i:i + 75], 0.9, 0, 0.8) for i in range(0, 300, 75)])
     assert torch.equal(got, parts)
+
+
+@pytest.mark.parametrize("V", [1001, 32000, 50273])
+def test_rows_of_the_lowest_numbers(V):
+    """Rows whose largest logit is the lowest number fp32 has, or near it (what
+    masking with finfo.min leaves): -inf, NaN and what lies before and behind the row
+    weigh nothing there either."""
+    low, inf = torch.finfo(torch.float32).min, float("inf")
+    x = torch.full((5, V), low)
+    x[1, ::3] = -inf
+    x[2] = -inf
+    x[2, [V // 3, V - 2]] = low
+    x[3] = torch.linspace(low, low * 0.999, V)
+    x[3, ::4] = float("nan")
+    x[4, 7:] = -inf
+    wide = torch.zeros(5, V + 3, device=DEV)
+    wide[:, 1:V + 1] = x.to(DEV)
+    y = wide[:, 1:V + 1]
+    for u0 in (0.0, 0.37, 0.99999):
+        u = torch.full((5,), u0, device=DEV)
+        for t in (0.01, 1.0, 2e33, inf):  # 2e33: the numbers of row 3 differ in weight
+            for k, p, m in [(0, 1.0, 0.0), (0, 0.7, 0.0), (700, 1.0, 0.0), (5, 0.6, 0.1), (0, 1.0, 0.5)]:
+                got = sample_tokens(y, u, t, k, p, m)
+                # temperatures above 1e34 count as 1e34, weights below 2^-43 round to nothing
+                # (the running mass exceeds 0 at the first that does not)
+                tt = min(f32(t), f32(1e34))
+                z = x.double().nan_to_num(nan=-inf, neginf=-inf)
+                z = torch.where((z - z.amax(-1, keepdim=True)) / tt < -43 * math.log(2.0), -inf, z)
+                want = reference(z, u, [tt] * 5, [k] * 5, [f32(p)] * 5, [f32(m)] * 5)
+                assert torch.equal(got.cpu(), want), (u0, t, k, p, m)
+
+
+def test_lowest_numbers_of_bf16():
+    V, low = 9001, torch.finfo(torch.bfloat16).min
+    x = torch.full((2, V), low)
+    x[1, 5:] = -float("inf")
+    for t in (1.0, 1e34):
+        got = sample_tokens(x.bfloat16().to(DEV), torch.full((2,), 0.6, device=DEV), t)
+        assert torch.equal(got.cpu(), reference(x, torch.full((2,), 0.6), [f32(t)] * 2, [0] * 2, [1.0] * 2, [0.0] * 2))
+
+
+def test_tiny_temperatures():
+    """Temperatures of a fraction of the step between fp32 numbers: what lies below
+    the largest number weighs nothing, -inf among it."""
+    x = torch.full((1, 3000), -float("inf"), device=DEV)
+    x[0, 1234] = 1.0
+    u = torch.full((1,), 0.9999999, device=DEV)
+    for steps in (0.3, 0.9, 1.1, 1.3, 1.45, 1.6, 3.0):
+        t = steps * 2.0 ** -24 / 41.6  # the distance at which weights end, in steps below 1
+        for p in (1.0, 0.9):
+            assert sample_tokens(x, u, t, 0, p).item() == 1234, (steps, p)
+            assert sample_tokens(x, torch.zeros_like(u), t, 0, p).item() == 1234, (steps, p)
