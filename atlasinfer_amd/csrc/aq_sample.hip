@@ -438,7 +438,7 @@ __device__ __forceinline__ Weigh weigh_from(float mx, float T, const double* tab
   // below half the lowest of fp32 by way of their halves (T counts as 1e34 at most)
   const float f = mx < -1.7014118e38f ? 0.5f : 1.0f;
   const double m = f * mx, t = (double)f * (double)fminf(T, 1e34f);
-  double c = 738.6598609514740 / t;  // 512 log2(e) / T
+  double c = 738.65986093514927 / t;  // 512 log2(e) / T
   float lo = (float)(m - 41.588830833596719 * t);
   if (!((m - (double)lo) * c >= 30720.0)) {
     asm volatile("");  // a branch: lo was rounded up; T may be far below the logits' steps, the next one weighs nothing

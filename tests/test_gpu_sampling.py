@@ -270,3 +270,14 @@ def test_tiny_temperatures():
         for p in (1.0, 0.9):
             assert sample_tokens(x, u, t, 0, p).item() == 1234, (steps, p)
             assert sample_tokens(x, torch.zeros_like(u), t, 0, p).item() == 1234, (steps, p)
+
+
+@pytest.mark.parametrize("n,d,t", [(7, 7.161129951477051, 3.6800928115844727), (3, 15.558229446411133, 14.161710739135742),
+                                   (3, 12.468780517578125, 11.349573135375977), (2, 4.920184135437012, 7.098325252532959),
+                                   (7, 14.07146167755127, 7.2313008308410645)])
+def test_weights_at_a_border(n, d, t):
+    """n tokens d below the largest, with n exp(-d / t) = 1 + e, e from 7e-12 to 1.4e-11:
+    at u = 1/2 the last of them is the token, by a margin of e / 2, which is 15 to 30 units
+    of 2^-42; their roundings are n / 2 units at most."""
+    x = torch.tensor([[-d] * n + [0.0]], device=DEV)
+    assert sample_tokens(x, torch.full((1,), 0.5, device=DEV), t).item() == n - 1
