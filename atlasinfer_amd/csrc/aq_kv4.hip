@@ -27,6 +27,7 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint16_t ushort2v __attribute__((ext_vector_type(2)));
 
 constexpr int kSlotBlock = 32;
 constexpr uint16_t kNaN16 = 0x7E00;
@@ -232,6 +233,7 @@ constexpr int kMaxWaves4 = 8;
 constexpr int64_t kOneSpan4 = 16, kFirstSpan4 = 4, kLongSpan4 = 32;
 constexpr int64_t kMaxSpans4 = 64, kMaxGroups4 = 1024;
 constexpr int kHeads = 16;  // query heads a workgroup takes: a tile's columns
+constexpr float kCodeUnit = 1.0f / (1 << 24);  // of the codes in the scores' product
 
 struct Split4 {
   int64_t nt, ns, nw, hb, part_floats, bytes;  // blocks a span, spans, waves, head tiles
@@ -272,11 +274,12 @@ __device__ __forceinline__ half2v pair_of(uint32_t w, int n, uint32_t magic) {
   return __builtin_bit_cast(half2v, (w & 0x000F000Fu) | magic) - big;
 }
 
-// The same pair with 1024 (n even) or 64 (n odd: a nibble four bits up counts 1 each
-// under that exponent) left in, one instruction a pair.
-__device__ __forceinline__ uint32_t raised_pair_of(uint32_t w, int n, uint32_t magic, uint32_t magic64) {
-  if (n & 2) w >>= 8;
-  return n & 1 ? (w & 0x00F000F0u) | magic64 : (w & 0x000F000Fu) | magic;
+// The same pair as it is: a nibble in the lowest bits is a subnormal number, 2^-24
+// times the nibble, which the matrix instructions take like any other.
+// (The highest nibbles come by one shift of both halves of the word.)
+__device__ __forceinline__ uint32_t small_pair_of(uint32_t w, int n) {
+  if (n == 3) return __builtin_bit_cast(uint32_t, __builtin_bit_cast(ushort2v, w) >> (uint16_t)12);
+  return (w >> (4 * n)) & 0x000F000Fu;
 }
 
 // Words n of the lanes (l, r), r = lane / 16, a group of keys each (D = 128: group r
@@ -321,9 +324,12 @@ __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_
 // of one head), the running softmax of a head in the four lanes that hold it, the
 // numerators as the second product's operand, which they are without an exchange,
 // and the values' rows.
-//   Scores: the products of one group's codes, whole numbers as fp16, with the
-// query are exact to f32 and scaled there; the minima meet the sums of the query
-// in a product of f32 (16 x 16 x 4).  Keys rounded to fp16 (a fused multiply-add a
+//   Scores: the products of one group's codes, whole numbers times 2^-24 as fp16,
+// with the query are exact to f32 and scaled there; the minima meet the sums of the
+// query (times 2^-24 too) in a product of f32 (16 x 16 x 4).  (Codes raised by 1024 and
+// 64, one instruction a pair fewer, whose share was taken away again after the product:
+// for queries far from zero on average, as biases make them, scores were off by 2e-2.)
+// Keys rounded to fp16 (a fused multiply-add a
 // pair, the scales then inside the product) gave 4.2e-4 of the result against 2.1e-4
 // of the output's own rounding, at 89 us for the long case below where this took 95.
 //   Numerators are two fp16 numbers each, the second what the first leaves over: with
@@ -444,23 +450,20 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
   __syncthreads();
 
   // the queries as the scores' second operand: head l, elements 32 kk +
-  // 8 word_of(r) + the order in which pair_of gives a word's nibbles; what the
-  // nibbles' 1024 and 64 add to the products of group r, and the sum of the queries
-  // over it, which the keys' minima multiply
+  // 8 word_of(r) + the order in which pair_of gives a word's nibbles; the sum of the
+  // queries over group r, which the keys' minima multiply, in the codes' unit
   half8v qv[NK];
-  float lift = 0.0f, qsum = 0.0f;
+  float qsum = 0.0f;
 #pragma unroll
   for (int kk = 0; kk < NK; kk++) {
-    half8v offs, ones;
+    half8v ones;
 #pragma unroll
     for (int n = 0; n < 8; n++) {
       qv[kk][n] = bits_to_h(qs[l][32 * kk + 8 * word_of<D>(r) + (n >> 1) + 4 * (n & 1)]);
-      offs[n] = (f16)(n & 2 ? -64.0f : -1024.0f);
       ones[n] = (f16)1.0f;
     }
-    const float a = __builtin_amdgcn_mfma_f32_16x16x32_f16(offs, qv[kk], float4v{0, 0, 0, 0}, 0, 0, 0)[0];
     const float b = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, qv[kk], float4v{0, 0, 0, 0}, 0, 0, 0)[0];
-    if (r == kk) lift = a, qsum = b;
+    if (r == kk) qsum = b * kCodeUnit;
   }
 
   float4v o[ND], den;
@@ -468,8 +471,8 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
   for (int e = 0; e < ND; e++) o[e] = float4v{0, 0, 0, 0};
   den = float4v{0, 0, 0, 0};
   float m = -INFINITY;
-  uint32_t magic = 0x64006400u, magic64 = 0x54005400u;
-  asm volatile("" : "+v"(magic), "+v"(magic64));
+  uint32_t magic = 0x64006400u;
+  asm volatile("" : "+v"(magic));
   half8v ones;
 #pragma unroll
   for (int n = 0; n < 8; n++) ones[n] = (f16)1.0f;
@@ -520,8 +523,8 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
       if (s0 + 4 * r + i > last) vpar.x &= 0xFFFF0000u, vpar.y &= 0xFFFF0000u;
       if (s0 + 16 + 4 * r + i > last) vpar.x &= 0xFFFFu, vpar.y &= 0xFFFFu;
     }
-    // q . (s c + m) = sum over groups of s (q . (c + lift)) - s (q . lift) + m sum(q):
-    // products of whole numbers with q, scaled in f32
+    // q . (s c + m) = sum over groups of s (q . c) + m sum(q): products of whole numbers
+    // with q, scaled in f32
     float4v acc[2];
     float s_of[2];
 #pragma unroll
@@ -529,7 +532,6 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
       groups_apart<D>(y.k[tt]);
       s_of[tt] = (float)bits_to_h((uint16_t)y.kscale[tt]);
       acc[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)bits_to_h((uint16_t)(y.kpar[tt] >> 16)), qsum, float4v{0, 0, 0, 0}, 0, 0, 0);
-      acc[tt] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)bits_to_h((uint16_t)y.kpar[tt]), lift, acc[tt], 0, 0, 0);
     }
     auto group = [&](auto gc) {
       constexpr int g = decltype(gc)::value;
@@ -538,7 +540,7 @@ __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attentio
       for (int tt = 0; tt < 2; tt++) {
         u32x4 a;
 #pragma unroll
-        for (int n = 0; n < 4; n++) a[n] = raised_pair_of(y.k[tt][g], n, magic, magic64);
+        for (int n = 0; n < 4; n++) a[n] = small_pair_of(y.k[tt][g], n);
         d[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, a), qv[g], float4v{0, 0, 0, 0}, 0, 0, 0);
       }
       auto of_slot = [&](auto ic) {
@@ -808,7 +810,7 @@ extern "C" int aq_kv4_attention(const void* q, const void* k_new, const void* v_
   const Cache4 c = {(uint8_t*)k_codes, (uint16_t*)k_params, (uint8_t*)v_codes, (uint16_t*)v_params};
   // the kernel's is above 0, so that the largest product has the largest score and a
   // masked one, -inf, stays it: a negative scale's sign and a zero go to the queries
-  const float scale2 = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
+  const float scale2 = (scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f) / kCodeUnit;
   if (!(scale > 0.0f)) q_scale = scale == 0.0f ? 0.0f : -q_scale;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(Hkv * sp.hb), (unsigned)B, (unsigned)sp.ns);

@@ -288,3 +288,45 @@ def test_positions_of_31_bits(bits):
     out = torch.full((B, H, D), 3.0, dtype=torch.float16, device=DEV)
     caches[2].attend(q, kn, vn, torch.tensor([2 ** 31 - 1], device=DEV), scale=0.1, out=out)
     assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mean", [3.0, 10.0])
+@pytest.mark.parametrize("slots", [2, 700])
+def test_scores_of_biased_queries(D, mean, slots):
+    """Queries far from zero on average, as biases of their projection make them:
+    two slots of near scores and values 1 and -1, whose output is tanh of half the
+    scores' difference, so that it shows their errors and hardly its own rounding."""
+    g = torch.Generator(device=DEV).manual_seed(D + int(mean))
+    B, H, Hkv = 24, 8, 2
+    q = mean + 0.25 * torch.randint(-1, 2, (B, H, D), generator=g, device=DEV)
+    q[torch.rand(B, H, D, generator=g, device=DEV) < 0.8] = mean
+    q = q.half()  # whole multiples of 1/4
+    # groups of codes 0 .. 15, the lowest of them 0: the minimum is 0, the scale from 1.3 to 2
+    codes = torch.randint(0, 16, (B, Hkv, D // 32, 32), generator=g, device=DEV).float()
+    codes[..., 0], codes[..., 1] = 0.0, 15.0
+    k0 = codes * (1.3 + 0.7 * torch.rand(B, Hkv, D // 32, 1, generator=g, device=DEV))
+    k1 = k0[..., torch.randperm(32, generator=g, device=DEV)]
+    k0, k1 = k0.half().view(B, Hkv, 1, D), k1.half().view(B, Hkv, D)
+    one = torch.ones(B, Hkv, D, dtype=torch.float16, device=DEV)
+    cache = DC.kv4_buffers(B, Hkv, slots, D, DEV)
+    DC.kv4_store(k0, one[:, :, None], cache, slots=slots)
+    got = DC.kv4_attention(q, k1, -one, cache, torch.ones(1, dtype=torch.int64, device=DEV), scale=D ** -0.5,
+                           slots=slots).cpu().double()
+    (c, s, m), values = R.unpack(cache, slots)
+    assert (m[:, :, :2] == 0).all()
+    k = R.values(c, s, m)[:, :, :2].repeat_interleave(H // Hkv, 1)
+    assert torch.equal(R.values(*values)[:, :, :2], torch.tensor([1.0, -1.0]).double().view(1, 1, 2, 1).expand(B, Hkv, 2, D))
+    score = (k * q.cpu().double()[:, :, None]).sum(-1) * D ** -0.5  # [B, H, 2], all terms positive
+    delta = score[..., 0] - score[..., 1]
+    assert delta.abs().max() < 12
+    # sums of codes times quarters are exact, so a score has the roundings of up to four
+    # products and sums with the scales, 2^-24 of the score each, and of the exponent's
+    # argument, 2^-24 of it: 5 2^-24 of both scores; scale and log2(e) round, 2^-23 of the
+    # difference; half of that reaches the output, and the weights' roundings (2^-20 of 1)
+    # and its own
+    off = 5 * 2.0 ** -24 * score.sum(-1) + 2.0 ** -23 * delta.abs()
+    want = torch.tanh(0.5 * delta)
+    bound = 0.5 * off + 2.0 ** -20 + 2.0 ** -11 * want.abs() + 2.0 ** -25
+    err = (got - want[..., None]).abs()
+    assert (err <= bound[..., None]).all(), (err / bound[..., None]).max()
