@@ -573,10 +573,13 @@ class GraphDecoder:
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, **sampling) -> torch.Tensor:
         """Prompt + ``max_new_tokens`` tokens, [B, S + max_new_tokens]: greedy, or
         of a decoder built with ``sampling=True`` sampled with fresh random numbers,
-        ``sampling`` being set_sampling's arguments."""
+        ``sampling`` being set_sampling's arguments (without ``generator`` the last
+        one's goes on)."""
         S = input_ids.shape[1]
         if S + max_new_tokens > self.L:
             raise ValueError(f"generate: {S} + {max_new_tokens} positions exceed the cache ({self.L})")
+        if self.sampling:
+            sampling.setdefault("generator", self._generator)
         if self.sampling or sampling:
             self.set_sampling(**sampling)
         self.prefill(input_ids)

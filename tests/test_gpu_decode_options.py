@@ -217,3 +217,22 @@ def test_a_window_that_reaches_max_len_replaces_the_configured_one(options):
         gd.tok.copy_(ref.sequences[:, 30 + t - 1])
         got, want = gd.step().float(), ref.logits[t].float()
         assert ((got - want).abs().amax(-1) <= 2e-2 * want.abs().amax(-1)).all(), t
+
+
+def test_generate_keeps_the_generator():
+    """A generator given once serves every generate that names no other."""
+    gd = GraphDecoder(_model("llama"), batch=2, max_len=24, sampling=True)
+    ids = torch.randint(0, 512, (2, 5), device=DEV)
+    gd.set_sampling(temperature=1.3, generator=torch.Generator().manual_seed(7))
+    g = torch.Generator().manual_seed(7)
+    torch.rand(24, 2, generator=g)
+    for kw in ({}, dict(top_k=9), {}):
+        gd.generate(ids, 6, **kw)
+        assert torch.equal(gd.u.cpu(), torch.rand(24, 2, generator=g)), kw
+    gd.generate(ids, 6, generator=torch.Generator().manual_seed(8))
+    assert torch.equal(gd.u.cpu(), torch.rand(24, 2, generator=torch.Generator().manual_seed(8)))
+    gd.generate(ids, 6, generator=None)  # back to torch's default one
+    assert not torch.equal(gd.u.cpu(), torch.rand(24, 2, generator=g))
+    a = gd.u.clone()
+    gd.generate(ids, 6)
+    assert not torch.equal(gd.u, a)
