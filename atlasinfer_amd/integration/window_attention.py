@@ -62,13 +62,27 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
 
 _NAME = "atlas_window"  # this attention's name among HF's
-_current = threading.local()  # (window, sinks) of the innermost window_prompts
+_local = threading.local()  # .open: the thread's open contexts, the innermost last
+_switch = threading.Lock()  # held while a model's attention is changed
+
+
+class _Context:
+    def __init__(self, config, window, sinks, before):
+        self.config, self.window, self.sinks, self.before = config, window, sinks, before
+
+
+def _open():
+    if not hasattr(_local, "open"):
+        _local.open = []
+    return _local.open
 
 
 def _attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
     """HF's attention interface: [B, H, M, D] and [B, Hkv, N, D] to [B, M, H, D]."""
-    window, sinks = _current.value
-    return window_attention(query, key, value, window=window, sinks=sinks, scale=scaling), None
+    for c in reversed(_open()):
+        if c.config is module.config:
+            return window_attention(query, key, value, window=c.window, sinks=c.sinks, scale=scaling), None
+    raise RuntimeError("window_prompts: the model runs in a thread that has not entered the context it is in")
 
 
 @contextlib.contextmanager
@@ -76,16 +90,26 @@ def window_prompts(model, window: Optional[int], sinks: int = 0):
     """Within the context ``model``'s forward (HF OPT, Llama or Mistral, fp16 on a
     HIP device) attends through a sliding window with sinks, whatever its
     configuration says; prompts without padding (the attention mask is not
-    looked at)."""
+    looked at).  Contexts of a model nest, the innermost counts.  A model's
+    attention is its threads' in common, so while one thread is in a context of it
+    another can neither enter one nor run it (RuntimeError)."""
     from transformers import AttentionInterface
     from transformers.masking_utils import AttentionMaskInterface
     AttentionInterface.register(_NAME, _attention)
     AttentionMaskInterface.register(_NAME, lambda *args, **kwargs: None)  # no dense mask is made
-    before, outer = model.config._attn_implementation, getattr(_current, "value", None)
-    _current.value = (window, sinks)
-    model.set_attn_implementation(_NAME)
+    mine, config = _open(), model.config
+    with _switch:
+        outer = next((c for c in mine if c.config is config), None)
+        before = outer.before if outer is not None else config._attn_implementation
+        if outer is None and before == _NAME:
+            raise RuntimeError("window_prompts: the model is in another thread's context")
+        model.set_attn_implementation(_NAME)
+        context = _Context(config, window, sinks, before)
+        mine.append(context)
     try:
         yield model
     finally:
-        model.set_attn_implementation(before)
-        _current.value = outer
+        with _switch:
+            mine.remove(context)
+            if all(c.config is not config for c in mine):
+                model.set_attn_implementation(before)

@@ -141,3 +141,63 @@ def test_a_longer_window_than_the_configured_one_needs_the_gpu_path():
     with torch.no_grad():
         ref = m.generate(ids, attention_mask=torch.ones_like(ids), max_new_tokens=5, do_sample=False)
     assert torch.equal(GraphDecoder(m, batch=1, max_len=32, graph=False, window=64).generate(ids, 5), ref)
+
+
+def test_window_prompts_nest_and_keep_to_their_thread(monkeypatch):
+    """The innermost context counts, in whatever order they end; two models at once;
+    another thread is refused, and the model is left as it was."""
+    import threading
+    from atlasinfer_amd.integration import window_attention as W
+    seen = []
+
+    def plain(q, k, v, window, sinks, scale):
+        seen.append((window, sinks))
+        return q.transpose(1, 2).contiguous()
+
+    monkeypatch.setattr(W, "window_attention", plain)
+    a, b = _model("llama"), _model("mistral")
+    before = a.config._attn_implementation
+    ids = torch.randint(0, 256, (1, 5))
+
+    def ran(m):
+        seen.clear()
+        with torch.no_grad():
+            m(input_ids=ids)
+        assert len(set(seen)) <= 1
+        return seen[0] if seen else None
+
+    def elsewhere(f):
+        out = []
+
+        def run():
+            try:
+                out.append(f())
+            except Exception as e:
+                out.append(e)
+        t = threading.Thread(target=run)
+        t.start()
+        t.join()
+        return out[0]
+
+    def enter(m):
+        with W.window_prompts(m, 9):
+            return ran(m)
+
+    with W.window_prompts(a, 3, 1):
+        assert ran(a) == (3, 1) and ran(b) is None
+        with W.window_prompts(b, 4), W.window_prompts(a, 5):
+            assert ran(a) == (5, 0) and ran(b) == (4, 0)
+        assert ran(a) == (3, 1) and ran(b) is None
+        assert isinstance(elsewhere(lambda: ran(a)), RuntimeError)
+        assert isinstance(elsewhere(lambda: enter(a)), RuntimeError)
+        assert elsewhere(lambda: enter(b)) == (9, 0)  # another model
+        assert ran(a) == (3, 1) and ran(b) is None
+    assert ran(a) is None and a.config._attn_implementation == b.config._attn_implementation == before
+    assert elsewhere(lambda: enter(a)) == (9, 0)
+    one, two = W.window_prompts(a, 3), W.window_prompts(a, 4)
+    one.__enter__()
+    two.__enter__()
+    one.__exit__(None, None, None)
+    assert ran(a) == (4, 0)
+    two.__exit__(None, None, None)
+    assert ran(a) is None and a.config._attn_implementation == before
