@@ -260,17 +260,23 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
     }
     if (!all && bad[i & (NS - 1)] == i + 1) {
       // an infinity or NaN among the values of a tile that the mask cuts: the
-      // terms one by one, leaving out those of weight zero
+      // terms one by one, leaving out those of keys that the query does not see (a
+      // weight may also have rounded to zero: times infinity that is NaN, as in the
+      // products below)
       // (the sums pass an empty asm here, so that what the compiler does for this
       // loop's sake, copying them, it does here and not on the common path)
 #pragma unroll
       for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
+      int from = max(qpos - a.window + 1, start) - k0, sink0 = start - k0;
+      uint32_t near_n = (uint32_t)max(qpos - k0 - from + 1, 0), sink_n = (uint32_t)max(min(a.sinks, qpos - start + 1), 0);
+      asm volatile("" : "+v"(from), "+v"(sink0), "+v"(near_n), "+v"(sink_n));
 #pragma unroll 1
       for (int key = 0; key < kK; key++) {
         const int y = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
         uint32_t w = p[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) w = e == n ? p[e] : w;
+        const bool seen = (uint32_t)(key - from) < near_n || (uint32_t)(key - sink0) < sink_n;
         const float wf = __shfl((float)bits_to_h((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * y, 64);
 #pragma unroll
         for (int e = 0; e < D / 32; e++)
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
           for (int z = 0; z < 16; z++) {
             const int d = 32 * e + 8 * (z >> 2) + 4 * h + (z & 3);
             const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + TB + v_place<D>(key, d >> 3) + (d & 7) * 2);
-            if (wf != 0.0f) o[e][z] = fmaf(wf, (float)bits_to_h(vd), o[e][z]);
+            if (seen) o[e][z] = fmaf(wf, (float)bits_to_h(vd), o[e][z]);
           }
       }
       continue;

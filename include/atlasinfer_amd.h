@@ -442,7 +442,8 @@ int aq_window_decode_attention(const void* q, const void* k_new, const void* v_n
  *   D = 64 or 128, H a multiple of Hkv, M <= N < 2^24, window >= 1 (N or more:
  *   causal), sinks >= 0; q, k, v, out 16-byte aligned
  * What a key or value that a query does not see holds, infinities and NaN
- * included, does not reach its output.
+ * included, does not reach its output; a value that it sees and that is not finite
+ * makes its element of the output not finite, however little it weighs.
  */
 int aq_window_attention(const void* q, const void* k, const void* v, int64_t B, int64_t H, int64_t Hkv, int64_t M,
                         int64_t N, int64_t D, const int64_t* q_strides, const int64_t* k_strides,

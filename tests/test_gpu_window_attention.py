@@ -245,3 +245,23 @@ def test_unseen_values_of_the_first_tile(D, N):
         want, bound = _reference(q, k, v, window, sinks, D ** -0.5, None)
         before = (torch.arange(N, device=DEV)[None] < first[:, None])[..., None, None]
         assert (((got - want).abs() <= bound) | ~before).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("window,sinks", [(300, 0), (40, 0), (40, 11)])
+def test_seen_values_that_are_not_finite(D, bad, window, sinks):
+    """One of weight e^-32 or less, which rounds to zero beside the others' in fp16: it
+    reaches every query that sees it, in tiles that the mask cuts and in whole ones, and
+    no other."""
+    N, at = 300, 10
+    g = torch.Generator(device=DEV).manual_seed(D)
+    q = 1.0 + 0.1 * _rnd(g, 2, 2, N, D)
+    k, v = 0.1 * _rnd(g, 2, 2, N, D), _rnd(g, 2, 2, N, D)
+    k[:, :, at] = -4.0  # -4 D of 1 / sqrt(D): -32 for D = 64
+    v[:, :, at, 3] = bad
+    got = window_attention(q, k, v, window=window, sinks=sinks)
+    i = torch.arange(N, device=DEV)
+    sees = (i >= at) & ((i - at < window) | (at < sinks))
+    assert not got[:, sees][..., 3].isfinite().any()
+    assert got[:, ~sees].isfinite().all() and got[..., :3].isfinite().all() and got[..., 4:].isfinite().all()
