@@ -301,7 +301,9 @@ __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) 
   }
   l = xlane_level_sum_f32<6>(l);
   if (qi < a.M) {
-    const float f = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a query that sees nothing answers zero
+    // a query that sees nothing answers zero; one that sees a key, its own among them, and
+    // only scores of -inf (l is 0) NaN, as the softmax of these
+    const float f = qpos >= start ? (l == 0.0f ? NAN : 1.0f / l) : 0.0f;
     uint16_t* op = a.out + (((int64_t)b * a.M + qi) * a.H + head) * D + 4 * h;
 #pragma unroll
     for (int e = 0; e < D / 32; e++)

@@ -265,3 +265,20 @@ def test_seen_values_that_are_not_finite(D, bad, window, sinks):
     sees = (i >= at) & ((i - at < window) | (at < sinks))
     assert not got[:, sees][..., 3].isfinite().any()
     assert got[:, ~sees].isfinite().all() and got[..., :3].isfinite().all() and got[..., 4:].isfinite().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_of_minus_infinity(D):
+    """They weigh nothing beside others; a query that sees only such has no softmax
+    (NaN), unlike one that sees nothing (zeros)."""
+    N, n = 200, 70
+    g = torch.Generator(device=DEV).manual_seed(D)
+    q, k, v = _rnd(g, 2, 2, N, D).abs() + 0.1, _rnd(g, 2, 1, N, D), _rnd(g, 2, 1, N, D)
+    k[:, :, :n] = -float("inf")
+    starts = torch.tensor([0, 20], dtype=torch.int32, device=DEV)
+    for window, sinks in ((300, 0), (90, 3)):
+        got = window_attention(q, k, v, window=window, sinks=sinks, starts=starts)
+        assert got[0, :n].isnan().all() and got[1, 20:n].isnan().all() and (got[1, :20] == 0).all()
+        # sinks are among the first n keys: the rest see what begins at n
+        want, bound = _reference(q, k, v, window, 0, D ** -0.5, starts.clamp(min=n))
+        assert ((got.double() - want).abs() <= bound)[:, n:].all()
