@@ -318,7 +318,7 @@ __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_
 // Workgroup (j, b, z) takes key/value head j (and head tile) of sequence b and
 // blocks z nt .. of its slots; wave w every nw-th of them.  The last spans, which
 // short sequences do not have, come first: the workgroups that have nothing to do are
-// gone before the GPU runs empty (lengths of 1 to 16384: 92 us, first spans first 95).
+// gone before the GPU runs empty (lengths of 1 to 16384: with first spans first 3 us more).
 // One step is a block of 32 slots: scores of 2 x 16 slots against up to 16 query
 // heads (mfma 16 x 16 x 32, keys as rows, so that a lane's results are 2 x 4 slots
 // of one head), the running softmax of a head in the four lanes that hold it, the
@@ -331,15 +331,15 @@ __device__ __forceinline__ float max_quarters(float x) { return xlane_level_max_
 // for queries far from zero on average, as biases make them, scores were off by 2e-2.)
 // Keys rounded to fp16 (a fused multiply-add a
 // pair, the scales then inside the product) gave 4.2e-4 of the result against 2.1e-4
-// of the output's own rounding, at 89 us for the long case below where this took 95.
+// of the output's own rounding, at 88 us for the long case below, no less.
 //   Numerators are two fp16 numbers each, the second what the first leaves over: with
-// one alone the error is 3.0e-4 and 91 us.  With both 2.6e-4: what is left beside
+// one alone the error is 3.0e-4, the long case 4 us shorter.  With both 2.6e-4: what is left beside
 // the output's rounding is that of the values s c + m to fp16, once each (fma).  The
 // denominator is the product of the same numerators with ones.
-// Bound by HBM and by the instructions together: a step of 32 slots of D = 128 is 290
-// vector and 29 matrix instructions a wave for 5 KiB (32 sequences x 8 heads of up to
-// 16384 slots, half of them in use: 336 MB in 92 us, 3.7 TB/s; all of 8192: 77, 4.4; the
-// loads alone take 68).
+// Bound by HBM and by the instructions together: a step of 32 slots of D = 128 is 310
+// vector and 28 matrix instructions a wave for 5 KiB (32 sequences x 8 heads of up to
+// 16384 slots, half of them in use: 336 MB in 88.5 us, 3.8 TB/s; all of 8192, two caches
+// in turn: 87, 3.9; 32 x 32 heads of 64: 167, 4.0).
 template <int D>
 __global__ __launch_bounds__(64 * kMaxWaves4, D == 64 ? 4 : 3) void kv4_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, Cache4 c,

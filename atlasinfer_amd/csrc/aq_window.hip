@@ -78,9 +78,10 @@ __device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((
 //   sums     of the rounded numerators (v_dot2), so that rounding them does not
 //            shift the mean
 // Bound by the matrix unit and the softmax's exponentials together: 32 heads of 128
-// over 8 key/value heads, 8192 positions, a window of 4096 with 4 sinks: 480 us, 859
+// over 8 key/value heads, 8192 positions, a window of 4096 with 4 sinks: 483 us, 854
 // TFLOP/s of the two products (the library's fp16 product of 8192^3: 1144); 32 heads
-// of 64, 1017 positions, a window of 256: 15 us, three rounds of tiles a workgroup.
+// of 64, 1017 positions, a window of 256: 15 us, one round of workgroups of up to
+// seven tiles each, one wave a SIMD.
 template <int D>
 __global__ __launch_bounds__(256, 2) void window_attention_kernel(WindowArgs a) {
   constexpr int NC = D / 8;                    // 16-byte pieces of a row

@@ -5,7 +5,8 @@ The reference decodes with HF ``generate`` (examples/run_atlas_inference.py
 vocabulary and torch's multinomial.  ``sample_tokens`` does it in the library
 (``aq_sample``) from one given random number per sequence, so a step can be
 captured in a HIP graph and the same numbers give the same tokens;
-``GraphDecoder.generate(do_sample=True)`` uses it.
+``GraphDecoder(..., sampling=True)`` uses it, with generate's ``temperature``,
+``top_k``, ``top_p`` and ``min_p``.
 """
 from __future__ import annotations
 

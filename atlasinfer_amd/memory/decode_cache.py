@@ -18,7 +18,7 @@ below are the same on buffers of the caller's own.  Positions are device
 memory, one for all sequences or one each, so that a captured HIP graph
 replays a step; a sequence whose position is out of range (negative, past the
 rotary tables, past a cache without a window) is left out: its row of the
-result and its cache stay as they were.
+result and its cache stay as they were (without ``out`` that row is undefined).
 """
 from __future__ import annotations
 
@@ -275,7 +275,8 @@ class DecodeCache:
 
     def store(self, k: torch.Tensor, v: torch.Tensor, start: int = 0, lengths: Optional[torch.Tensor] = None) -> None:
         """Write positions start .. start + S - 1 (k, v fp16 [B, Hkv, S, D]), of
-        sequence b the first ``lengths[b]`` of them."""
+        sequence b the first ``lengths[b]`` of them.  In 16 bits by torch operations
+        over all slots, with temporaries of the cache's size."""
         if self.bits == 4:
             kv4_store(k, v, self.buffers, start, lengths, self.slots, self.sinks)
             return

@@ -408,9 +408,9 @@ int64_t aq_decode_attention_workspace(int64_t B, int64_t H, int64_t Hkv, int64_t
 
 /*
  * aq_decode_attention over a cache that keeps a sliding window of positions
- * and the first few (the attention of models with a window, and of endless
- * generation; no counterpart in the reference, whose cache keeps every
- * position).  The cache's L slots hold the first `sinks` positions and the last
+ * and the first few (the attention of models with a window; the cache stops
+ * growing there, positions run on to 2^31 - 2 or the rotary tables' end; no
+ * counterpart in the reference, whose cache keeps every position).  The cache's L slots hold the first `sinks` positions and the last
  * L - sinks (a window of L - sinks, the step's own position included): position
  * p is in slot p while p < L, then in slot sinks + (p - sinks) mod (L - sinks).
  * Keys are rotated at their position before they are cached, so the order of
@@ -434,7 +434,8 @@ int aq_window_decode_attention(const void* q, const void* k_new, const void* v_n
  * over a dense mask).  Query i (0 .. M - 1) stands at position N - M + i; it sees
  * key j when start <= j <= its position and (position - j < window or
  * j - start < sinks), start = starts[b] (a left-padded batch) or 0.
- *   out[b, i, h, :] = fp16(softmax(scale q . k) v)  (zeros where it sees nothing)
+ *   out[b, i, h, :] = fp16(softmax(scale q . k) v)  (zeros where it sees nothing,
+ *   NaN where every score that it sees is -inf)
  * Scores, softmax and sums in f32, the softmax's numerators rounded to fp16.
  *   q      fp16 [B, H, M, D]    k, v  fp16 [B, Hkv, N, D], by strides
  *          (elements, {batch, head, position}, multiples of 8; D contiguous)
