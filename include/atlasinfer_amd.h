@@ -436,7 +436,9 @@ int aq_window_decode_attention(const void* q, const void* k_new, const void* v_n
  * j - start < sinks), start = starts[b] (a left-padded batch) or 0.
  *   out[b, i, h, :] = fp16(softmax(scale q . k) v)  (zeros where it sees nothing,
  *   NaN where every score that it sees is -inf)
- * Scores, softmax and sums in f32, the softmax's numerators rounded to fp16.
+ * Scores, softmax and sums in f32, the softmax's numerators rounded to fp16.  Scores
+ * (scale q . k) up to 2^26 in magnitude: past that the maximum's rounding to f32, which
+ * every exponent shares, is itself an exponent that overflows.
  *   q      fp16 [B, H, M, D]    k, v  fp16 [B, Hkv, N, D], by strides
  *          (elements, {batch, head, position}, multiples of 8; D contiguous)
  *   starts int32 [B] or NULL    out   fp16 [B, M, H, D]
@@ -490,6 +492,8 @@ int aq_kv4_load(const void* k_codes, const void* k_params, const void* v_codes, 
  *   out[b, h, :] = fp16(softmax(scale q . k) v)
  * over the slots in use, as the values they stand for (keys exactly, values
  * rounded to fp16; scores and sums in f32, the softmax's numerators to 22 bits).
+ * Scores (scale q . k) up to 2^30 in magnitude, for the reason given at
+ * aq_window_attention.
  * H any multiple of Hkv.  q, k_new, v_new, pos, q_scale, rope_* and which
  * sequences are run: as there; q, k_new, v_new, out and the tables 16-byte
  * aligned.
