@@ -40,7 +40,7 @@ FLAGS = [
 # accumulators in ordinary VGPRs (the accumulator-register form made the
 # compiler shuffle accumulators between register files inside the K loop)
 FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-              for f in ("aq_qlinear.hip", "aq_qlinear_mid.hip", "aq_kv4.hip", "aq_window.hip")}
+              for f in ("aq_qlinear.hip", "aq_qlinear_mid.hip", "aq_kv4.hip", "aq_window.hip", "aq_paged_attention.hip")}
 
 
 def _compile(src: str) -> str:

@@ -1,0 +1,486 @@
+// aq_paged_attention.hip -- attention of new tokens of several sequences over
+// a paged cache.
+//
+// out = softmax(scale q k^T + mask) v in one pass over the keys that a block of
+// queries can see: with the running maximum m of a query's scores and the sums
+// l = sum e^(s - m), o = sum e^(s - m) v so far, a tile of keys with maximum m'
+// scales l and o by e^(m - max(m, m')) and adds its own terms.  Parts of the keys
+// taken by different workgroups meet the same way (paged_merge_kernel).
+//
+// The G query heads that share a key/value head are rows of one block: row r of
+// a sequence's n G rows is its new token r / G, head r % G of the group.
+#include "aq_paged.h"
+
+namespace {
+
+using namespace paged;
+
+constexpr int kQ = 128;  // rows a workgroup, 32 a wave
+constexpr int kK = 64;   // keys a tile
+constexpr float kGrow = 8.0f;
+
+struct AttendArgs {
+  Batch b;
+  const uint16_t *q, *k, *v;
+  int64_t qs[2];  // elements between rows, heads
+  uint16_t* out;
+  float* part;    // [T, H, spans, D + 2]: sums, then the maximum and the denominator
+  int H, G, Hkv, window, sinks, items, per;
+  int span, spans;  // tiles a workgroup, workgroups a block
+  float c;  // |scale| log2(e), above 0: a masked score, -inf, times it stays that
+  uint32_t keep, flip;  // for the queries' bits: none for a scale of 0, the sign of a negative one
+};
+
+// 16 bytes a lane from a buffer's byte `off` straight to LDS, at dst + 16 lane;
+// zeros past the buffer's end.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (void*)dst, 16, off, 0, 0, 0);
+}
+
+// Four rows of 16 numbers of 16 bits in LDS, 8 bytes given by each of 16 lanes
+// in order: lane i gets column i.
+__device__ __forceinline__ u32x2 read_turned(const uint8_t* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_u8*)p));
+}
+
+// The larger of m and the magnitudes of eight numbers, as pairs of bits.
+__device__ __forceinline__ u16x2 magnitudes8(u16x2 m, uint4 x) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+  return m;
+}
+
+// Rows of a sequence, and the tiles of keys that a block of them sees: tiles
+// 0 .. na - 1 hold the sinks, then come b0 .. b0 + tiles - na - 1.
+struct Block {
+  int first, n, len, r0;  // the sequence's first row, its new tokens, its length; the block's first row
+  int lo, hi;             // positions of the block's first and last row
+  int b0, na, tiles, sink_end;
+};
+
+// s: the sequence; r0: the block's first of its rows, of `rows`.
+__device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, int rows, Block& k) {
+  k.first = a.b.start(s);
+  k.n = max(a.b.start(s + 1) - k.first, 0);
+  k.len = a.b.lengths[s];
+  k.r0 = r0;
+  if (r0 >= k.n * a.G || k.n > k.len || k.n > a.b.max_new || k.len > a.b.max_length) return false;
+  k.lo = k.len - k.n + r0 / a.G;
+  k.hi = k.len - k.n + min(r0 + rows - 1, k.n * a.G - 1) / a.G;
+  const int near = max(k.lo - a.window + 1, 0);
+  k.b0 = near / kK;
+  k.sink_end = min(a.sinks, k.hi + 1);
+  k.na = k.sink_end > 0 ? min((k.sink_end - 1) / kK + 1, k.b0) : 0;
+  k.tiles = k.na + k.hi / kK - k.b0 + 1;
+  return true;
+}
+
+// The sequence that block `blk` belongs to, -1 for none: sequence s's blocks
+// are starts[s] G / 128 + s and on (as many as its rows can need, or one more).
+__device__ __forceinline__ int find_sequence(const AttendArgs& a, int blk, int ln, int& first) {
+  for (int s0 = 0; s0 < a.b.S; s0 += 64) {
+    const int s = min(s0 + ln, a.b.S - 1);
+    const int f = a.b.start(s) * a.G / kQ + s, e = a.b.start(s + 1) * a.G / kQ + s + 1;
+    const uint64_t hit = __ballot(f <= blk && blk < e && s == s0 + ln);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      first = __builtin_amdgcn_readlane(f, at);
+      return s0 + at;
+    }
+  }
+  return -1;
+}
+
+// A tile's rows lie in LDS one after the other, 16-byte pieces permuted within
+// each so that the reads below meet every bank equally: piece c of key r at place
+// c ^ (r & 7) of a key row, pairs of pieces c / 2 at (c / 2) ^ (r & 3) of a value row.
+template <int D>
+__device__ __forceinline__ int k_place(int r, int c) { return r * (D * 2) + (c ^ (r & 7)) * 16; }
+template <int D>
+__device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) * 16; }
+
+// One workgroup: 128 rows of a key/value head, 32 a wave; tiles of 64 keys and
+// values go straight from their pages to LDS (a wave loads 16 rows of each, which
+// lie in one page).
+//   scores   transposed, s^T = k q^T (mfma 32 x 32 x 16): a lane has 32 scores of
+//            one row, another lane the other 32
+//   softmax  p = e^(s - m) with m the maximum when it last moved: it moves only
+//            when a score passes it by 2^8, which spares scaling the sums nearly always
+//   values   o^T = v^T p^T: the numerators, rounded to 16 bits, are the operand as
+//            they are; the values come out of their rows transposed
+//   sums     of the rounded numerators, so that rounding them does not shift the mean
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
+  constexpr int NC = D / 8;                    // 16-byte pieces of a row
+  constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
+  constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave: 16 rows
+  constexpr int NS = D == 64 ? 4 : 2;          // stages: 64 KiB
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * 2 * TB];  // keys and values of each stage
+  __shared__ int bad[NS];
+  const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  // runs of neighbouring items to an XCD (they share keys and values in its L2)
+  const int item = (int)(blockIdx.x & 7) * a.per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= a.per || item >= a.items) return;
+  const int blocks = a.items / a.Hkv;
+  const int j = item / blocks, blk = blocks - 1 - item % blocks;  // late blocks (more keys) first
+  int blk0;
+  const int seq = find_sequence(a, blk, ln, blk0);
+  if (seq < 0) return;
+  Block B;
+  if (!find_block(a, seq, (blk - blk0) * kQ, kQ, B)) return;
+  const int t0 = (int)blockIdx.y * a.span, t1 = min(t0 + a.span, B.tiles);
+  if (t0 >= t1) return;
+  // cleared before any wave may set one, which is before the loop's first barrier
+  if (t < NS) bad[t] = 0;
+  __syncthreads();
+  const int lo = B.lo, hi = B.hi, sink_end = B.sink_end;
+  auto tile_at = [&](int i) { return i < B.na ? i : B.b0 + i - B.na; };
+
+  const int row = B.r0 + wave * 32 + c, last_row = B.n * a.G - 1;  // this lane's row
+  const int tok = min(row, last_row) / a.G, head = j * a.G + (min(row, last_row) - tok * a.G);
+  const int qpos = B.len - B.n + tok;
+  u32x4 qv[D / 16];
+  {
+    const uint16_t* qp = a.q + (int64_t)(B.first + tok) * a.qs[0] + head * a.qs[1] + 8 * h;
+#pragma unroll
+    for (int s = 0; s < D / 16; s++) {
+      u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = (x[i] & a.keep) ^ a.flip;
+      qv[s] = x;
+    }
+  }
+  float16v o[D / 32];
+#pragma unroll
+  for (int e = 0; e < D / 32; e++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[e][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  // positions of the wave's rows
+  const int wlo = B.len - B.n + min(B.r0 + wave * 32, last_row) / a.G;
+  const int whi = B.len - B.n + min(B.r0 + wave * 32 + 31, last_row) / a.G;
+  const float grow = kGrow / a.c;
+
+  // this lane's part of the loads: piece n of the wave covers rows of its 16
+  int ko[PN], vo[PN];
+#pragma unroll
+  for (int n = 0; n < PN; n++) {
+    const int r = n * (64 / NC) + ln / NC, pc = ln % NC;
+    ko[n] = r * (D * 2) + (pc ^ (r & 7)) * 16;
+    vo[n] = r * (D * 2) + ((((pc >> 1) ^ (r & 3)) << 1) | (pc & 1)) * 16;
+  }
+  const int* table = a.b.table + (int64_t)seq * a.b.W;
+  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i, read a tile ahead
+    const int k0 = tile_at(i) * kK + wave * 16;
+    return i < t1 && k0 < B.len ? table[k0 >> a.b.shift] : -1;
+  };
+  int next_page = page_at(t0);
+  auto load = [&](int i) {
+    const int k0 = tile_at(i) * kK + wave * 16;
+    uint8_t* st = lds + (i & (NS - 1)) * (2 * TB) + wave * PN * 1024;
+    // rows past the last, and those of a page outside the cache, read as zeros
+    const int page = __builtin_amdgcn_readfirstlane(next_page);
+    const bool there = (unsigned)page < (unsigned)a.b.pages;
+    const int bytes = there ? max(min(B.len - k0, 16), 0) * (D * 2) : 0;
+    const int64_t at = (((((int64_t)(there ? page : 0) * a.Hkv + j) << a.b.shift) + (k0 & ((1 << a.b.shift) - 1)))) * D;
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k + at), (short)0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + at), (short)0, bytes, 0x00020000);
+#pragma unroll
+    for (int n = 0; n < PN; n++) load_to_lds(kr, st + n * 1024, ko[n]);
+#pragma unroll
+    for (int n = 0; n < PN; n++) load_to_lds(vr, st + TB + n * 1024, vo[n]);
+    next_page = page_at(i + 1);
+  };
+  // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h (e & 3;
+  // e + 4 lies 128 bytes on); values of keys 4 h + r, 16 elements of 32 e (e & 1)
+  int kf[4], vf[2];
+#pragma unroll
+  for (int e = 0; e < 4; e++) kf[e] = k_place<D>(c, 2 * e + h);
+  const int r4 = (ln >> 2) & 3;
+#pragma unroll
+  for (int e = 0; e < 2; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
+
+  for (int i = t0; i < min(t0 + NS - 1, t1); i++) load(i);
+  for (int i = t0; i < t1; i++) {
+    const int k0 = tile_at(i) * kK;
+    const uint8_t* st = lds + (i & (NS - 1)) * (2 * TB);
+    // this wave's part of the tile is there (and the page numbers read since)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const bool cut = !(k0 + kK - 1 <= lo && k0 > hi - a.window);
+    if (cut) {
+      // a tile that the mask cuts for some row: whether its values are finite
+      u16x2 x = 0;
+#pragma unroll
+      for (int n = 0; n < PN; n++) x = magnitudes8(x, *reinterpret_cast<const uint4*>(st + TB + (wave * PN + n) * 1024 + ln * 16));
+      if (__ballot(max(x.x, x.y) >= T::kInf) && ln == 0) bad[i & (NS - 1)] = i + 1;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's part; the tile before is done with
+    if (i + NS - 1 < t1) load(i + NS - 1);
+    // whether this wave's rows see none, all or some of the tile
+    if (k0 > whi || (k0 + kK - 1 <= wlo - a.window && k0 >= sink_end)) continue;
+    const bool all = k0 + kK - 1 <= wlo && k0 > whi - a.window;
+    float16v x[2];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) x[s][e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D / 16; e++) {
+        const u32x4 f = *reinterpret_cast<const u32x4*>(st + kf[e & 3] + (e >> 2) * 128 + s * 32 * (D * 2));
+        x[s] = T::mfma32(f, qv[e], x[s]);
+      }
+    }
+    if (!all) {
+      // a key is seen when it lies in one of two ranges: near the row's position,
+      // or among the sinks, both up to that position (each a subtraction, an
+      // unsigned comparison and a selection)
+      const int last = qpos - k0 - 4 * h, from = max(last - a.window + 1, -k0 - 4 * h);
+      const int sink0 = -k0 - 4 * h;
+      const uint32_t near_n = (uint32_t)max(last - from + 1, 0);
+      const uint32_t sink_n = (uint32_t)max(min(a.sinks, last - sink0 + 1), 0);
+      if (k0 < sink_end) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
+            const float y = (uint32_t)(key - sink0) < sink_n ? x[s][e] : -INFINITY;
+            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : y;
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
+            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : -INFINITY;
+          }
+      }
+    }
+    float mx = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+    for (int e = 1; e < 16; e++) mx = fmaxf(fmaxf(mx, x[0][e]), x[1][e]);  // v_max3
+    if (__ballot(mx > m + grow)) {
+      mx = xlane_level_max_f32<6>(mx);  // both lanes of a row move alike
+      const float n = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - n) * a.c);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) o[e] *= f;
+      m = n;
+    }
+    const float base = m == -INFINITY ? 0.0f : -m * a.c;
+    uint32_t p[16];  // the numerators in pairs: p[4 n .. 4 n + 3] are the operand of 16 keys
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const int y = 2 * e & 15;
+      p[e] = T::pack(__builtin_amdgcn_exp2f(fmaf(x[e >> 3][y], a.c, base)),
+                     __builtin_amdgcn_exp2f(fmaf(x[e >> 3][y + 1], a.c, base)));
+      l = T::add2(p[e], l);
+    }
+    if (!all && bad[i & (NS - 1)] == i + 1) {
+      // an infinity or NaN among the values of a tile that the mask cuts: the
+      // terms one by one, leaving out those of keys that the row does not see
+      // (the sums pass an empty asm here, so that what the compiler does for this
+      // loop's sake, copying them, it does here and not on the common path)
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
+      int from = max(qpos - a.window + 1, 0) - k0, sink0 = -k0;
+      uint32_t near_n = (uint32_t)max(qpos - k0 - from + 1, 0), sink_n = (uint32_t)max(min(a.sinks, qpos + 1), 0);
+      asm volatile("" : "+v"(from), "+v"(sink0), "+v"(near_n), "+v"(sink_n));
+#pragma unroll 1
+      for (int key = 0; key < kK; key++) {
+        const int y = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
+        uint32_t w = p[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) w = e == n ? p[e] : w;
+        const bool seen = (uint32_t)(key - from) < near_n || (uint32_t)(key - sink0) < sink_n;
+        const float wf = __shfl(T::to_f32((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * y, 64);
+#pragma unroll
+        for (int e = 0; e < D / 32; e++)
+#pragma unroll
+          for (int z = 0; z < 16; z++) {
+            const int d = 32 * e + 8 * (z >> 2) + 4 * h + (z & 3);
+            const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + TB + v_place<D>(key, d >> 3) + (d & 7) * 2);
+            if (seen) o[e][z] = fmaf(wf, T::to_f32(vd), o[e][z]);
+          }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) {
+        // keys 16 s + 4 h + 0 .. 3, then 8 on: the order in which a lane has the numerators
+        const uint8_t* f = st + TB + vf[e & 1] + (e >> 1) * 128 + s * 16 * (D * 2);
+        const u32x2 w0 = read_turned(f), w1 = read_turned(f + 8 * (D * 2));
+        o[e] = T::mfma32(u32x4{w0.x, w0.y, w1.x, w1.y}, u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}, o[e]);
+      }
+  }
+  l = xlane_level_sum_f32<6>(l);
+  if (row > last_row) return;
+  const int64_t at = (int64_t)(B.first + tok) * a.H + head;
+  if (B.tiles > a.span) {  // one of several spans: sums, maximum and denominator as they are
+    float* pp = a.part + (at * a.spans + blockIdx.y) * (D + 2) + 4 * h;
+#pragma unroll
+    for (int e = 0; e < D / 32; e++)
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int z = 0; z < 4; z++) pp[32 * e + 8 * n + z] = o[e][4 * n + z];
+    if (h == 0) {
+      pp[D] = m;
+      pp[D + 1] = l;
+    }
+    return;
+  }
+  // a row that sees only scores of -inf (l is 0) answers NaN, as the softmax of these
+  const float f = l == 0.0f ? NAN : 1.0f / l;
+  uint16_t* op = a.out + at * D + 4 * h;
+#pragma unroll
+  for (int e = 0; e < D / 32; e++)
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+      *reinterpret_cast<uint2*>(op + 32 * e + 8 * n) =
+          make_uint2(T::pack(o[e][4 * n] * f, o[e][4 * n + 1] * f), T::pack(o[e][4 * n + 2] * f, o[e][4 * n + 3] * f));
+}
+
+// The spans of a row joined, a wave a row (token and head).
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
+  const int ln = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int t = (int)(at / a.H), head = (int)(at % a.H);
+  if (t >= a.b.T) return;
+  // the row's sequence, and the block that it was in
+  int seq = -1;
+  for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
+    const int s = min(s0 + ln, a.b.S - 1);
+    const uint64_t hit = __ballot(a.b.start(s) <= t && t < a.b.start(s + 1) && s == s0 + ln);
+    if (hit) seq = s0 + __builtin_ctzll(hit);
+  }
+  if (seq < 0) return;
+  const int r = (t - a.b.start(seq)) * a.G + head % a.G;
+  Block B;
+  if (!find_block(a, seq, r / kQ * kQ, kQ, B) || B.tiles <= a.span) return;
+  const int spans = (B.tiles + a.span - 1) / a.span;
+  const float* pp = a.part + at * a.spans * (D + 2);
+  float m = -INFINITY;
+  for (int s = 0; s < spans; s++) m = fmaxf(m, pp[s * (D + 2) + D]);
+  float l = 0.0f, o[D / 64];
+#pragma unroll
+  for (int e = 0; e < D / 64; e++) o[e] = 0.0f;
+  for (int s = 0; s < spans; s++) {
+    const float* x = pp + s * (D + 2);
+    const float ms = x[D];
+    // a span with scores of -inf only has sums of zero, or the NaN of what it saw
+    const float f = ms == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((ms - m) * a.c);
+    l = fmaf(x[D + 1], f, l);
+#pragma unroll
+    for (int e = 0; e < D / 64; e++) o[e] = fmaf(x[ln * (D / 64) + e], f, o[e]);
+  }
+  const float f = l == 0.0f ? NAN : 1.0f / l;
+  uint16_t* op = a.out + at * D + ln * (D / 64);
+  if (D == 128)
+    *reinterpret_cast<uint32_t*>(op) = T::pack(o[0] * f, o[D / 64 - 1] * f);
+  else
+    *op = T::from_f32(o[0] * f);
+}
+
+// How the keys are split.  `span` tiles a workgroup, the longest sequence in
+// `spans` of them.
+struct Plan {
+  int64_t blocks, items, per, span, spans, bytes;
+};
+
+Plan plan(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_length) {
+  Plan p;
+  const int64_t G = H / Hkv;
+  p.blocks = S == 1 ? aq::ceil_div(T * G, kQ) : T * G / kQ + S;
+  p.items = p.blocks * Hkv;
+  p.per = aq::ceil_div(p.items, 8);
+  const int64_t tiles = aq::ceil_div(max_length, kK) + 1;
+  p.spans = std::max<int64_t>(1, std::min<int64_t>(512 / p.items, aq::ceil_div(tiles, 8)));
+  p.span = aq::ceil_div(tiles, p.spans);
+  p.spans = aq::ceil_div(tiles, p.span);
+  p.bytes = p.spans > 1 ? T * H * p.spans * (D + 2) * 4 : 0;
+  return p;
+}
+
+bool sizes_ok(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_length) {
+  return (D == 64 || D == 128) && T > 0 && T < (1 << 24) && S > 0 && S <= 65535 && Hkv > 0 && H > 0 && H <= 1024 &&
+         H % Hkv == 0 && max_new > 0 && max_length > 0 && max_length <= INT32_MAX - 2 * kK && T * (H / Hkv) < (1 << 30);
+}
+
+template <class T, int D>
+void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
+  if (p.spans > 1)
+    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)aq::ceil_div((int64_t)a.b.T * a.H, 4)), dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" int64_t aq_paged_attention_workspace(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new,
+                                                int64_t max_length) {
+  return sizes_ok(T, S, H, Hkv, D, max_new, max_length) ? plan(T, S, H, Hkv, D, max_length).bytes : -1;
+}
+
+extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                                  const int64_t* q_strides, const void* k_cache, const void* v_cache, int64_t pages,
+                                  int64_t page_size, const int32_t* starts, const int32_t* lengths, int64_t S,
+                                  const int32_t* table, int64_t W, int64_t max_new, int64_t max_length, int64_t window,
+                                  int64_t sinks, float scale, void* workspace, int64_t ws_bytes, void* out, void* stream) {
+  const char* me = "aq_paged_attention";
+  AQ_CHECK_ARG(q && q_strides && k_cache && v_cache && starts && lengths && table && out, "%s: null pointer", me);
+  AQ_CHECK_ARG(dtype == AQ_F16 || dtype == AQ_BF16, "%s: dtype %d (fp16 and bf16 supported)", me, dtype);
+  AQ_CHECK_ARG(D == 64 || D == 128, "%s: head dim %lld (64 or 128 supported)", me, (long long)D);
+  AQ_CHECK_ARG(Hkv > 0 && H > 0 && H <= 1024 && H % Hkv == 0, "%s: H (%lld) must be a multiple of Hkv (%lld)", me, (long long)H,
+               (long long)Hkv);
+  AQ_CHECK_ARG(sizes_ok(T, S, H, Hkv, D, max_new, max_length),
+               "%s: sizes out of range (%lld rows, %lld sequences, at most %lld new, %lld positions of one)", me, (long long)T,
+               (long long)S, (long long)max_new, (long long)max_length);
+  AQ_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+               "%s: page size %lld (a power of two from 16 to 1024)", me, (long long)page_size);
+  AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W * page_size <= INT32_MAX && max_length <= W * page_size,
+               "%s: %lld pages, %lld of a sequence for %lld positions", me, (long long)pages, (long long)W, (long long)max_length);
+  AQ_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %lld, %lld sinks", me, (long long)window, (long long)sinks);
+  AQ_CHECK_ARG(q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0, "%s: strides must be multiples of 8", me);
+  AQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16 == 0 &&
+                   ((uintptr_t)starts | (uintptr_t)lengths | (uintptr_t)table) % 4 == 0,
+               "%s: q, the caches and out must be 16-byte aligned", me);
+  const Plan p = plan(T, S, H, Hkv, D, max_length);
+  AQ_CHECK_ARG(p.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= p.bytes),
+               "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me, (long long)ws_bytes, (long long)p.bytes);
+  // (a grid has fewer than 2^32 threads)
+  AQ_CHECK_ARG(p.items <= (1 << 24) / p.spans - 8, "%s: %lld blocks of rows", me, (long long)p.items);
+  AttendArgs a;
+  a.b = paged::Batch{starts, lengths, table, (int)T, (int)S, (int)W, (int)pages, __builtin_ctz((unsigned)page_size),
+                     (int)std::min<int64_t>(max_new, T), (int)max_length};
+  a.q = (const uint16_t*)q;
+  a.k = (const uint16_t*)k_cache;
+  a.v = (const uint16_t*)v_cache;
+  a.qs[0] = q_strides[0];
+  a.qs[1] = q_strides[1];
+  a.out = (uint16_t*)out;
+  a.part = (float*)workspace;
+  a.H = (int)H;
+  a.G = (int)(H / Hkv);
+  a.Hkv = (int)Hkv;
+  a.window = (int)std::min<int64_t>(window, max_length);
+  a.sinks = (int)std::min<int64_t>(sinks, max_length);
+  a.items = (int)p.items;
+  a.per = (int)p.per;
+  a.span = (int)p.span;
+  a.spans = (int)p.spans;
+  a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
+  a.keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  if (dtype == AQ_F16)
+    D == 64 ? launch<Half, 64>(a, p, (hipStream_t)stream) : launch<Half, 128>(a, p, (hipStream_t)stream);
+  else
+    D == 64 ? launch<Bf16, 64>(a, p, (hipStream_t)stream) : launch<Bf16, 128>(a, p, (hipStream_t)stream);
+  AQ_LAUNCH_CHECK(me);
+  return AQ_OK;
+}

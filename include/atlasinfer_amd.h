@@ -540,6 +540,64 @@ int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t strid
               int64_t ws_bytes, void* stream);
 
 /*
+ * A paged key/value cache and packed batches of new tokens (no counterpart in the
+ * reference, whose cache keeps a tensor per layer and sequence,
+ * atlasinfer_core/memory/unified_memory_manager.py:111-563).  Keys and values are
+ * [pages, Hkv, page_size, D] in fp16 or bf16 each (dtype AQ_F16, AQ_BF16, the
+ * type of q, k, v and out too), page_size a power of two from 16 to 1024, D = 64 or
+ * 128.  Position p of sequence s is in page table[s][p / page_size], slot
+ * p % page_size.  A call takes the T new tokens of S sequences as packed rows:
+ *   starts   int32 [S + 1]  sequence s has rows starts[s] .. starts[s + 1] - 1 (none is
+ *            fine), n of them; starts ascend
+ *   lengths  int32 [S]  its positions after them: the rows stand at lengths[s] - n and on
+ *   table    int32 [S, W]  read up to lengths[s] only; sequences may share pages
+ * all in device memory, so a captured graph takes new ones, and on the host
+ *   max_new, max_length  at least the largest n and length, max_length <= W page_size
+ * T < 2^24, S <= 65535, H <= 1024.  A sequence with more new rows than max_new or than
+ * positions, or longer than max_length, is left out, rows before starts[0] and from
+ * starts[S] on too: their rows of q_out and out stay as they were.  A page outside
+ * 0 .. pages - 1 is not written, and read as zeros.
+ *
+ * aq_paged_store writes the rows' keys and values to their places, turning the
+ * first `rotary` elements of keys and queries to their positions on the way: the pairs
+ * x, y at elements i and i + rotary / 2 (interleaved = 0) or 2 i and 2 i + 1 (1) become
+ *   factor (x cos a - y sin a), factor (y cos a + x sin a),  a = position frequencies[i]
+ * (angles reduced in 64 bits, products in f32, one rounding).
+ *   q   [T, H, D] or NULL (H = 0), k, v [T, Hkv, D]: by strides {row, head} in
+ *       elements, multiples of 8; 16-byte aligned
+ *   frequencies  f32 [rotary / 2], or NULL with rotary = 0; rotary a multiple of 16
+ *   q_out  [T, H, D], not q
+ * Rows that share a place (tables with the same page for two sequences' new tokens)
+ * are written in no order.
+ *
+ * aq_paged_attention: query head h of a row at position p sees the keys j <= p of its
+ * sequence with p - j < window or j < sinks (window >= max_length: all of them),
+ *   out[t, h, :] = softmax(scale q . k) v
+ * Scores, softmax and sums in f32, the softmax's numerators rounded to the data's type;
+ * scores up to 2^26 in magnitude, for the reason given at aq_window_attention.  What a key
+ * or value that a row does not see holds, infinities and NaN included, does not reach
+ * its output; a seen value that is not finite makes its element of the output not
+ * finite; a row whose seen scores are all -inf answers NaN.
+ *   q   [T, H, D] by strides {row, head}, multiples of 8; H a multiple of Hkv
+ *   out [T, H, D]; q, out and the caches 16-byte aligned
+ *   workspace  aq_paged_attention_workspace bytes (may be 0, then NULL will do; -1 for
+ *       sizes it cannot take), 16-byte aligned, no initial contents; calls that
+ *       overlap in time must not share one
+ */
+int aq_paged_store(const void* q, const void* k, const void* v, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D,
+                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* starts,
+                   const int32_t* lengths, int64_t S, const int32_t* table, int64_t W, int64_t max_new,
+                   int64_t max_length, const float* frequencies, int64_t rotary, int interleaved, float factor,
+                   void* q_out, void* k_cache, void* v_cache, int64_t pages, int64_t page_size, void* stream);
+int64_t aq_paged_attention_workspace(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new,
+                                     int64_t max_length);
+int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
+                       const void* k_cache, const void* v_cache, int64_t pages, int64_t page_size,
+                       const int32_t* starts, const int32_t* lengths, int64_t S, const int32_t* table, int64_t W,
+                       int64_t max_new, int64_t max_length, int64_t window, int64_t sinks, float scale,
+                       void* workspace, int64_t ws_bytes, void* out, void* stream);
+
+/*
  * Residual add and normalisation of `rows` rows of n fp16 (n a multiple of
  * 8, at most 16384), one launch.  With delta: x = fp16(x + delta), in place
  * (the residual stream).  Then y = norm(x):
