@@ -84,6 +84,9 @@ SIGNATURES = {
     "aq_sample": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_float,
                                  ctypes.c_int32, ctypes.c_float, ctypes.c_float, _P, _P, _I64, _P]),
     "aq_sample_workspace": (_I64, [_I64, _I64, ctypes.c_int, ctypes.c_int32]),
+    "aq_token_logprobs_workspace": (_I64, [_I64, _I64, ctypes.c_int, _I64]),
+    "aq_token_logprobs": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64,
+                                         _P]),
     "aq_qlinear_decode": (ctypes.c_int, [_P, _I64, _I64, ctypes.c_int, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                          _P, _P, ctypes.c_int,
                                          _P, _P, _P, ctypes.c_float, _P, _P, _P]),

@@ -598,6 +598,34 @@ int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t H
                        void* workspace, int64_t ws_bytes, void* out, void* stream);
 
 /*
+ * Log probabilities of given tokens (no counterpart in the reference, which hands
+ * logits to HF generate, examples/run_atlas_inference.py:244-264).  Of each row x
+ * of logits, with m = max x and Z = sum exp(x_i - m):
+ *   logprobs[b]   = x_t - m - log Z, t = tokens[b]
+ *   entropies[b]  = -sum p_i log p_i
+ *   ranks[b]      = how many tokens stand before t in the order of falling logit,
+ *                   equal ones by index (0: t is the first)
+ *   top_tokens[b, i], top_logprobs[b, i]  = the first `top` of that order
+ * NaN counts as -inf; logits of +inf share the whole mass; a row without a logit above
+ * -inf has NaN for probabilities and its entropy.  A token outside 0 .. V - 1 has logprob
+ * NaN and rank -1.  Sums in f32.
+ *   logits   dtype AQ_F16, AQ_BF16 or AQ_F32 [B, V], rows `stride` elements apart,
+ *            V <= 262144, B <= 65535
+ *   tokens   int64 [B]     top  0 .. 64, at most V
+ *   logprobs, entropies f32 [B], ranks int64 [B], top_logprobs f32 [B, top],
+ *            top_tokens int64 [B, top]
+ *   workspace  aq_token_logprobs_workspace bytes (may be 0, then NULL will do; -1 for
+ *            sizes it cannot take), 16-byte aligned, no initial contents; calls that
+ *            overlap in time must not share one.  It lets several workgroups share a
+ *            long row; with less, or NULL, one workgroup takes each (ranks and tokens
+ *            are the same, sums are added in another order).
+ */
+int64_t aq_token_logprobs_workspace(int64_t B, int64_t V, int dtype, int64_t top);
+int aq_token_logprobs(const void* logits, int dtype, int64_t B, int64_t V, int64_t stride, const int64_t* tokens,
+                      int64_t top, float* logprobs, float* entropies, int64_t* ranks, float* top_logprobs,
+                      int64_t* top_tokens, void* workspace, int64_t ws_bytes, void* stream);
+
+/*
  * Residual add and normalisation of `rows` rows of n fp16 (n a multiple of
  * 8, at most 16384), one launch.  With delta: x = fp16(x + delta), in place
  * (the residual stream).  Then y = norm(x):
