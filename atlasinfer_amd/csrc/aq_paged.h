@@ -63,6 +63,13 @@ struct Bf16 {
 // The packed batch.  Device numbers are not trusted: rows are cut to 0 .. T, a
 // sequence that contradicts the host's bounds is left out, a page outside the
 // cache is neither read nor written.
+typedef const __attribute__((address_space(4))) int const_int;
+
+// p[i] for an i that all lanes of a wave share, by the scalar unit.
+__device__ __forceinline__ int scalar_int(const int* p, int64_t i) {
+  return ((const_int*)(uintptr_t)p)[i];
+}
+
 struct Batch {
   const int *starts, *lengths, *table;
   int T, S, W, pages, shift;  // rows, sequences, table entries a sequence, pages, log2(page size)

@@ -31,11 +31,30 @@ struct AttendArgs {
   uint32_t keep, flip;  // for the queries' bits: none for a scale of 0, the sign of a negative one
 };
 
-// 16 bytes a lane from a buffer's byte `off` straight to LDS, at dst + 16 lane;
-// zeros past the buffer's end.
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint8_t* dst, int off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (void*)dst, 16, off, 0, 0, 0);
+// A buffer of `bytes` at p, for loads that read zeros past its end.
+__device__ __forceinline__ u32x4 buffer_of(const uint16_t* p, int bytes) {
+  return u32x4{(uint32_t)(uintptr_t)p, (uint32_t)((uintptr_t)p >> 32) & 0xFFFFu, (uint32_t)bytes, 0x00020000u};
 }
+
+// N times 16 bytes a lane from a buffer's bytes off[n] straight to LDS, to
+// dst + 1024 n + 16 lane.  In assembly, since the compiler, which knows of such
+// loads, waits for all of them before it reads from LDS anything that it cannot
+// tell apart: the waits are the caller's (s_waitcnt vmcnt).  The buffer's registers
+// may have been written by the vector unit just before: five wait states.
+template <int N>
+__device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t dst, const int (&off)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    if (n == 0)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off[0]), "s"(r)
+                   : "m0", "memory");
+    else
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst + 1024 * n), "v"(off[n]), "s"(r)
+                   : "m0", "memory");
+  }
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_u8*)p; }
 
 // Four rows of 16 numbers of 16 bits in LDS, 8 bytes given by each of 16 lanes
 // in order: lane i gets column i.
@@ -59,11 +78,12 @@ struct Block {
   int b0, na, tiles, sink_end;
 };
 
-// s: the sequence; r0: the block's first of its rows, of `rows`.
+// s: the sequence; r0: the block's first of its rows, of `rows`; all the same in
+// every lane.
 __device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, int rows, Block& k) {
-  k.first = a.b.start(s);
-  k.n = max(a.b.start(s + 1) - k.first, 0);
-  k.len = a.b.lengths[s];
+  k.first = min(max(scalar_int(a.b.starts, s), 0), a.b.T);
+  k.n = max(min(max(scalar_int(a.b.starts, s + 1), 0), a.b.T) - k.first, 0);
+  k.len = scalar_int(a.b.lengths, s);
   k.r0 = r0;
   if (r0 >= k.n * a.G || k.n > k.len || k.n > a.b.max_new || k.len > a.b.max_length) return false;
   k.lo = k.len - k.n + r0 / a.G;
@@ -86,7 +106,7 @@ __device__ __forceinline__ int find_sequence(const AttendArgs& a, int blk, int l
     if (hit) {
       const int at = __builtin_ctzll(hit);
       first = __builtin_amdgcn_readlane(f, at);
-      return s0 + at;
+      return __builtin_amdgcn_readfirstlane(s0 + at);
     }
   }
   return -1;
@@ -172,25 +192,23 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
     vo[n] = r * (D * 2) + ((((pc >> 1) ^ (r & 3)) << 1) | (pc & 1)) * 16;
   }
   const int* table = a.b.table + (int64_t)seq * a.b.W;
-  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i, read a tile ahead
-    const int k0 = tile_at(i) * kK + wave * 16;
-    return i < t1 && k0 < B.len ? table[k0 >> a.b.shift] : -1;
+  const int last_page = (B.len - 1) >> a.b.shift;
+  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i, read a tile ahead (rows past the last: any)
+    const int k0 = tile_at(min(i, t1 - 1)) * kK + wave * 16;
+    return scalar_int(table, min(k0 >> a.b.shift, last_page));
   };
   int next_page = page_at(t0);
   auto load = [&](int i) {
     const int k0 = tile_at(i) * kK + wave * 16;
-    uint8_t* st = lds + (i & (NS - 1)) * (2 * TB) + wave * PN * 1024;
+    const uint32_t st = lds_offset(lds) + (i & (NS - 1)) * (2 * TB) + wave * PN * 1024;
     // rows past the last, and those of a page outside the cache, read as zeros
-    const int page = __builtin_amdgcn_readfirstlane(next_page);
+    const int page = next_page;
     const bool there = (unsigned)page < (unsigned)a.b.pages;
-    const int bytes = there ? max(min(B.len - k0, 16), 0) * (D * 2) : 0;
+    // (a median is taken by the vector unit)
+    const int bytes = there ? __builtin_amdgcn_readfirstlane(max(min(B.len - k0, 16), 0)) * (D * 2) : 0;
     const int64_t at = (((((int64_t)(there ? page : 0) * a.Hkv + j) << a.b.shift) + (k0 & ((1 << a.b.shift) - 1)))) * D;
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.k + at), (short)0, bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void*)(a.v + at), (short)0, bytes, 0x00020000);
-#pragma unroll
-    for (int n = 0; n < PN; n++) load_to_lds(kr, st + n * 1024, ko[n]);
-#pragma unroll
-    for (int n = 0; n < PN; n++) load_to_lds(vr, st + TB + n * 1024, vo[n]);
+    load_to_lds<PN>(buffer_of(a.k + at, bytes), st, ko);
+    load_to_lds<PN>(buffer_of(a.v + at, bytes), st + TB, vo);
     next_page = page_at(i + 1);
   };
   // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h (e & 3;
@@ -206,8 +224,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   for (int i = t0; i < t1; i++) {
     const int k0 = tile_at(i) * kK;
     const uint8_t* st = lds + (i & (NS - 1)) * (2 * TB);
-    // this wave's part of the tile is there (and the page numbers read since)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // this wave's part of the tile is there; the NS - 2 tiles after it may be on their way
+    if (i + NS - 2 < t1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * PN) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     const bool cut = !(k0 + kK - 1 <= lo && k0 > hi - a.window);
     if (cut) {
       // a tile that the mask cuts for some row: whether its values are finite
@@ -350,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
   const int ln = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = (int)(at / a.H), head = (int)(at % a.H);
   if (t >= a.b.T) return;
   // the row's sequence, and the block that it was in
@@ -358,10 +379,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
   for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
     const int s = min(s0 + ln, a.b.S - 1);
     const uint64_t hit = __ballot(a.b.start(s) <= t && t < a.b.start(s + 1) && s == s0 + ln);
-    if (hit) seq = s0 + __builtin_ctzll(hit);
+    if (hit) seq = __builtin_amdgcn_readfirstlane(s0 + __builtin_ctzll(hit));
   }
   if (seq < 0) return;
-  const int r = (t - a.b.start(seq)) * a.G + head % a.G;
+  const int r = (t - min(max(scalar_int(a.b.starts, seq), 0), a.b.T)) * a.G + head % a.G;
   Block B;
   if (!find_block(a, seq, r / kQ * kQ, kQ, B) || B.tiles <= a.span) return;
   const int spans = (B.tiles + a.span - 1) / a.span;
