@@ -17,6 +17,7 @@ using namespace paged;
 
 constexpr int kQ = 128;  // rows a workgroup, 32 a wave
 constexpr int kK = 64;   // keys a tile
+constexpr int kFewRows = 32;  // rows of a sequence that the kernel for few takes at most
 constexpr float kGrow = 8.0f;
 
 struct AttendArgs {
@@ -24,12 +25,21 @@ struct AttendArgs {
   const uint16_t *q, *k, *v;
   int64_t qs[2];  // elements between rows, heads
   uint16_t* out;
-  float* part;    // [T, H, spans, D + 2]: sums, then the maximum and the denominator
+  float* part;    // [T, H, slots, D], sums, then [T, H, slots, 2], maxima and denominators
   int H, G, Hkv, window, sinks, items, per;
-  int span, spans;  // tiles a workgroup, workgroups a block
+  int few;                 // sequences of up to so many rows are the first kernel's, the others the second's
+  int few_span, few_spans; // steps a workgroup of the first kernel, workgroups a sequence
+  int span, spans;         // tiles a workgroup of the second, workgroups a block
+  int slots;               // the larger number of spans
   float c;  // |scale| log2(e), above 0: a masked score, -inf, times it stays that
   uint32_t keep, flip;  // for the queries' bits: none for a scale of 0, the sign of a negative one
 };
+
+// Maxima and denominators of the spans.
+template <int D>
+__device__ __forceinline__ float2* ends_of(const AttendArgs& a) {
+  return reinterpret_cast<float2*>(a.part + (int64_t)a.b.T * a.H * a.slots * D);
+}
 
 // A buffer of `bytes` at p, for loads that read zeros past its end.
 __device__ __forceinline__ u32x4 buffer_of(const uint16_t* p, int bytes) {
@@ -70,7 +80,7 @@ __device__ __forceinline__ u16x2 magnitudes8(u16x2 m, uint4 x) {
   return m;
 }
 
-// Rows of a sequence, and the tiles of keys that a block of them sees: tiles
+// Rows of a sequence, and the tiles of `keys` keys that a block of them sees: tiles
 // 0 .. na - 1 hold the sinks, then come b0 .. b0 + tiles - na - 1.
 struct Block {
   int first, n, len, r0;  // the sequence's first row, its new tokens, its length; the block's first row
@@ -80,6 +90,7 @@ struct Block {
 
 // s: the sequence; r0: the block's first of its rows, of `rows`; all the same in
 // every lane.
+template <int KEYS>
 __device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, int rows, Block& k) {
   k.first = min(max(scalar_int(a.b.starts, s), 0), a.b.T);
   k.n = max(min(max(scalar_int(a.b.starts, s + 1), 0), a.b.T) - k.first, 0);
@@ -89,10 +100,10 @@ __device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, i
   k.lo = k.len - k.n + r0 / a.G;
   k.hi = k.len - k.n + min(r0 + rows - 1, k.n * a.G - 1) / a.G;
   const int near = max(k.lo - a.window + 1, 0);
-  k.b0 = near / kK;
+  k.b0 = near / KEYS;
   k.sink_end = min(a.sinks, k.hi + 1);
-  k.na = k.sink_end > 0 ? min((k.sink_end - 1) / kK + 1, k.b0) : 0;
-  k.tiles = k.na + k.hi / kK - k.b0 + 1;
+  k.na = k.sink_end > 0 ? min((k.sink_end - 1) / KEYS + 1, k.b0) : 0;
+  k.tiles = k.na + k.hi / KEYS - k.b0 + 1;
   return true;
 }
 
@@ -119,6 +130,13 @@ template <int D>
 __device__ __forceinline__ int k_place(int r, int c) { return r * (D * 2) + (c ^ (r & 7)) * 16; }
 template <int D>
 __device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) * 16; }
+
+// The same for the values of the kernel for few rows, whose lanes read 16 rows at
+// once: pairs of pieces at (c / 2) ^ (r & 7), or ^ (r / 2 & 3) where two rows fill the banks.
+template <int D>
+__device__ __forceinline__ int few_place(int r, int c) {
+  return r * (D * 2) + ((((c >> 1) ^ (D == 128 ? r & 7 : (r >> 1) & 3)) << 1) | (c & 1)) * 16;
+}
 
 // One workgroup: 128 rows of a key/value head, 32 a wave; tiles of 64 keys and
 // values go straight from their pages to LDS (a wave loads 16 rows of each, which
@@ -149,7 +167,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   const int seq = find_sequence(a, blk, ln, blk0);
   if (seq < 0) return;
   Block B;
-  if (!find_block(a, seq, (blk - blk0) * kQ, kQ, B)) return;
+  if (!find_block<kK>(a, seq, (blk - blk0) * kQ, kQ, B) || B.n * a.G <= a.few) return;
   const int t0 = (int)blockIdx.y * a.span, t1 = min(t0 + a.span, B.tiles);
   if (t0 >= t1) return;
   // cleared before any wave may set one, which is before the loop's first barrier
@@ -343,17 +361,14 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   if (row > last_row) return;
   const int64_t at = (int64_t)(B.first + tok) * a.H + head;
   if (B.tiles > a.span) {  // one of several spans: sums, maximum and denominator as they are
-    float* pp = a.part + (at * a.spans + blockIdx.y) * (D + 2) + 4 * h;
+    const int64_t slot = at * a.slots + blockIdx.y;
+    float* pp = a.part + slot * D + 4 * h;
 #pragma unroll
     for (int e = 0; e < D / 32; e++)
 #pragma unroll
       for (int n = 0; n < 4; n++)
-#pragma unroll
-        for (int z = 0; z < 4; z++) pp[32 * e + 8 * n + z] = o[e][4 * n + z];
-    if (h == 0) {
-      pp[D] = m;
-      pp[D + 1] = l;
-    }
+        *reinterpret_cast<float4*>(pp + 32 * e + 8 * n) = make_float4(o[e][4 * n], o[e][4 * n + 1], o[e][4 * n + 2], o[e][4 * n + 3]);
+    if (h == 0) ends_of<D>(a)[slot] = make_float2(m, l);
     return;
   }
   // a row that sees only scores of -inf (l is 0) answers NaN, as the softmax of these
@@ -367,13 +382,257 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
           make_uint2(T::pack(o[e][4 * n] * f, o[e][4 * n + 1] * f), T::pack(o[e][4 * n + 2] * f, o[e][4 * n + 3] * f));
 }
 
-// The spans of a row joined, a wave a row (token and head).
+constexpr int kStep = 32;  // keys a wave takes at a time below
+
+// Sequences of few rows (a token or some): one workgroup a span of a sequence's and
+// key/value head's keys, all its rows (NR groups of 16) in every wave, the waves
+// taking 32 keys in turn.
+//   keys     straight to the registers that the product reads: lane 16 g + i has
+//            elements 8 g + 32 e .. of key i
+//   scores   transposed, s^T = k q^T (mfma 16 x 16 x 32): lane 16 g + r has those of
+//            keys 4 g + 0 .. 3 and 16 + 4 g + 0 .. 3 with row r
+//   values   by whole rows through registers to the wave's own part of LDS, from
+//            where they come transposed as the operand of o^T = v^T p^T, in the
+//            order of keys in which the numerators are at hand
+// The next keys are asked for when the scores' products have taken the last ones, the
+// next values when the last ones are in LDS.
+template <class T, int D, int NR>
+__global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
+  constexpr int NC = D / 8;             // 16-byte pieces of a row
+  constexpr int RL = 64 / NC;           // rows a load of values
+  constexpr int NV = kStep / RL;        // loads of values a step
+  constexpr int VB = kStep * D * 2;     // bytes of a step's values
+  constexpr int RS = D + 4;             // floats of a row of sums in LDS, so that rows spread over the banks
+  constexpr int SUMS = 4 * NR * 16 * RS * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[SUMS > 4 * VB ? SUMS : 4 * VB];
+  __shared__ float2 ends[4][NR * 16];
+  const int t = threadIdx.x, ln = t & 63, i16 = ln & 15, g = ln >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
+  Block B;
+  if (!find_block<kStep>(a, seq, 0, NR * 16, B) || B.n * a.G > a.few) return;
+  const int t0 = (int)blockIdx.y * a.few_span, t1 = min(t0 + a.few_span, B.tiles);
+  if (t0 >= t1) return;
+  const int rows = B.n * a.G;
+  auto step_at = [&](int i) { return (i < B.na ? i : B.b0 + i - B.na) * kStep; };
+
+  // this lane's rows: token and head, and the queries
+  int qpos[NR];
+  u32x4 qv[NR][D / 32];
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+    const int r = min(16 * n + i16, rows - 1), tok = r / a.G;
+    qpos[n] = B.len - B.n + tok;
+    const uint16_t* qp = a.q + (int64_t)(B.first + tok) * a.qs[0] + (j * a.G + r - tok * a.G) * a.qs[1] + 8 * g;
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) {
+      u32x4 x = *reinterpret_cast<const u32x4*>(qp + 32 * e);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = (x[i] & a.keep) ^ a.flip;
+      qv[n][e] = x;
+    }
+  }
+  float4v o[NR][D / 16];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; e++) o[n][e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float grow = kGrow / a.c;
+
+  const int* table = a.b.table + (int64_t)seq * a.b.W;
+  const int last_page = (B.len - 1) >> a.b.shift, in_page = (1 << a.b.shift) - 1;
+  // the buffers of 16 rows from k0 on, which lie in one page; rows past the last, and
+  // those of a page outside the cache, read as zeros
+  auto buffer = [&](const uint16_t* base, int k0) {
+    const int page = scalar_int(table, min(k0 >> a.b.shift, last_page));
+    const bool there = (unsigned)page < (unsigned)a.b.pages;
+    const int bytes = there ? __builtin_amdgcn_readfirstlane(max(min(B.len - k0, 16), 0)) * (D * 2) : 0;
+    const int64_t at = ((((int64_t)(there ? page : 0) * a.Hkv + j) << a.b.shift) + (k0 & in_page)) * D;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + at), (short)0, bytes, 0x00020000);
+  };
+  u32x4 kv[2][D / 32], vv[NV];
+  const int k_off = i16 * (D * 2) + g * 16, v_off = ln * 16;
+  auto load_keys = [&](int k0) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const __amdgpu_buffer_rsrc_t r = buffer(a.k, k0 + 16 * x);
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) kv[x][e] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off + 64 * e, 0, 0);
+    }
+  };
+  auto load_values = [&](int k0) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const __amdgpu_buffer_rsrc_t r = buffer(a.v, k0 + 16 * x);
+#pragma unroll
+      for (int n = 0; n < NV / 2; n++) vv[x * (NV / 2) + n] = __builtin_amdgcn_raw_buffer_load_b128(r, v_off + 1024 * n, 0, 0);
+    }
+  };
+  uint8_t* vs = lds + wave * VB;
+  int vw[2], vf;  // LDS offsets of the values' pieces (even and odd loads) and of this lane's part of a fragment
+#pragma unroll
+  for (int n = 0; n < 2; n++) vw[n] = few_place<D>(n * RL + ln / NC, ln % NC) - n * 1024;
+  const int fr = 4 * g + (i16 >> 2);
+
+  int k0 = step_at(min(t0 + wave, t1 - 1));
+  if (t0 + wave < t1) {
+    load_keys(k0);
+    load_values(k0);
+  }
+  for (int i = t0 + wave; i < t1; i += 4) {
+    const int next = i + 4 < t1 ? step_at(i + 4) : -1;
+    const bool all = k0 + kStep - 1 <= B.lo && k0 > B.hi - a.window;
+    bool bad = false;
+    if (!all) {
+      // a step that the mask cuts for some row: whether its values are finite
+      u16x2 x = 0;
+#pragma unroll
+      for (int n = 0; n < NV; n++) x = magnitudes8(x, make_uint4(vv[n][0], vv[n][1], vv[n][2], vv[n][3]));
+      bad = __ballot(max(x.x, x.y) >= T::kInf) != 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NV; n++) *reinterpret_cast<u32x4*>(vs + vw[n & 1] + n * 1024) = vv[n];
+    if (next >= 0) load_values(next);
+    float4v x[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        x[n][y] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) x[n][y] = T::mfma16(kv[y][e], qv[n][e], x[n][y]);
+      }
+    if (next >= 0) load_keys(next);
+    uint32_t p[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+      if (!all) {
+        const int from = qpos[n] - a.window;
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int key = k0 + 16 * y + 4 * g + e;
+            const bool near = key > from, sink = key < a.sinks;
+            if (key > qpos[n] || !(near || sink)) x[n][y][e] = -INFINITY;
+          }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(x[n][0][0], x[n][0][1]), fmaxf(x[n][0][2], x[n][0][3])),
+                       fmaxf(fmaxf(x[n][1][0], x[n][1][1]), fmaxf(x[n][1][2], x[n][1][3])));
+      if (__ballot(mx > m[n] + grow)) {
+        mx = xlane_level_max_f32<6>(xlane_level_max_f32<5>(mx));  // the four lanes of a row move alike
+        const float z = fmaxf(m[n], mx), f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - z) * a.c);
+        l[n] *= f;
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) o[n][e] *= f;
+        m[n] = z;
+      }
+      const float base = m[n] == -INFINITY ? 0.0f : -m[n] * a.c;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[n][e] = T::pack(__builtin_amdgcn_exp2f(fmaf(x[n][e >> 1][2 * e & 3], a.c, base)),
+                          __builtin_amdgcn_exp2f(fmaf(x[n][e >> 1][(2 * e & 3) + 1], a.c, base)));
+        l[n] = T::add2(p[n][e], l[n]);
+      }
+    }
+    if (bad) {
+      // an infinity or NaN among the values of a step that the mask cuts: the terms one
+      // by one, leaving out those of keys that the row does not see
+#pragma unroll 1
+      for (int key = 0; key < kStep; key++) {
+        const int y = key >> 4, from_g = (key >> 2) & 3, e = key & 3;
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+          const uint32_t w0 = y ? p[n][2] : p[n][0], w1 = y ? p[n][3] : p[n][1], w = e & 2 ? w1 : w0;
+          const float wf = __shfl(T::to_f32((uint16_t)(e & 1 ? w >> 16 : w)), i16 + 16 * from_g, 64);
+          const int at = k0 + key;
+          const bool seen = at <= qpos[n] && (at > qpos[n] - a.window || at < a.sinks);
+#pragma unroll
+          for (int d = 0; d < D / 16; d++)
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+              const int el = 16 * d + 4 * g + z;
+              const uint16_t vd = *reinterpret_cast<const uint16_t*>(vs + few_place<D>(key, el >> 3) + (el & 7) * 2);
+              if (seen) o[n][d][z] = fmaf(wf, T::to_f32(vd), o[n][d][z]);
+            }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < D / 16; e++) {
+        vf = few_place<D>(fr, 2 * e + ((i16 & 3) >> 1)) + (i16 & 1) * 8;
+        const u32x2 w0 = read_turned(vs + vf), w1 = read_turned(vs + vf + 16 * D * 2);
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+          o[n][e] = T::mfma16(u32x4{w0.x, w0.y, w1.x, w1.y}, u32x4{p[n][0], p[n][1], p[n][2], p[n][3]}, o[n][e]);
+      }
+    }
+    k0 = next;
+  }
+
+  // the waves' sums joined
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int n = 0; n < NR; n++) {
+    l[n] = xlane_level_sum_f32<6>(xlane_level_sum_f32<5>(l[n]));
+    const int r = 16 * n + i16;
+    if (g == 0) ends[wave][r] = make_float2(m[n], l[n]);
+#pragma unroll
+    for (int e = 0; e < D / 16; e++)
+      *reinterpret_cast<float4v*>(sums + (wave * NR * 16 + r) * RS + 16 * e + 4 * g) = o[n][e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < (NR * 16 * NC + 255) / 256; n++) {
+    const int r = (t + 256 * n) / NC, d = (t + 256 * n) % NC * 8;
+    if (r >= rows) continue;
+    float mx = -INFINITY, den = 0.0f, acc[8];
+#pragma unroll
+    for (int w = 0; w < 4; w++) mx = fmaxf(mx, ends[w][r].x);
+#pragma unroll
+    for (int z = 0; z < 8; z++) acc[z] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float2 y = ends[w][r];
+      // a wave with scores of -inf only has sums of zero, or the NaN of what it saw
+      const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - mx) * a.c);
+      den = fmaf(y.y, f, den);
+      const float* x = sums + (w * NR * 16 + r) * RS + d;
+#pragma unroll
+      for (int z = 0; z < 8; z++) acc[z] = fmaf(x[z], f, acc[z]);
+    }
+    const int tok = r / a.G, head = j * a.G + r - tok * a.G;
+    const int64_t at = (int64_t)(B.first + tok) * a.H + head;
+    if (B.tiles > a.few_span) {
+      const int64_t slot = at * a.slots + blockIdx.y;
+      *reinterpret_cast<float4*>(a.part + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(a.part + slot * D + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (d == 0) ends_of<D>(a)[slot] = make_float2(mx, den);
+    } else {
+      // a row that sees only scores of -inf (den is 0) answers NaN, as the softmax of these
+      const float f = den == 0.0f ? NAN : 1.0f / den;
+      *reinterpret_cast<uint4*>(a.out + at * D + d) =
+          make_uint4(T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f), T::pack(acc[4] * f, acc[5] * f),
+                     T::pack(acc[6] * f, acc[7] * f));
+    }
+  }
+}
+
+// The spans of a row joined, a wave a row (token and head): lane s has the maximum
+// and denominator of span s (there are up to 64).
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
   const int ln = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = (int)(at / a.H), head = (int)(at % a.H);
   if (t >= a.b.T) return;
+  // (read before it is known how many there are: what is none is not looked at)
+  float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
   // the row's sequence, and the block that it was in
   int seq = -1;
   for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
@@ -382,50 +641,76 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
     if (hit) seq = __builtin_amdgcn_readfirstlane(s0 + __builtin_ctzll(hit));
   }
   if (seq < 0) return;
-  const int r = (t - min(max(scalar_int(a.b.starts, seq), 0), a.b.T)) * a.G + head % a.G;
+  const int first = min(max(scalar_int(a.b.starts, seq), 0), a.b.T);
+  const int r = (t - first) * a.G + head % a.G;
   Block B;
-  if (!find_block(a, seq, r / kQ * kQ, kQ, B) || B.tiles <= a.span) return;
-  const int spans = (B.tiles + a.span - 1) / a.span;
-  const float* pp = a.part + at * a.spans * (D + 2);
-  float m = -INFINITY;
-  for (int s = 0; s < spans; s++) m = fmaxf(m, pp[s * (D + 2) + D]);
-  float l = 0.0f, o[D / 64];
-#pragma unroll
-  for (int e = 0; e < D / 64; e++) o[e] = 0.0f;
-  for (int s = 0; s < spans; s++) {
-    const float* x = pp + s * (D + 2);
-    const float ms = x[D];
-    // a span with scores of -inf only has sums of zero, or the NaN of what it saw
-    const float f = ms == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((ms - m) * a.c);
-    l = fmaf(x[D + 1], f, l);
-#pragma unroll
-    for (int e = 0; e < D / 64; e++) o[e] = fmaf(x[ln * (D / 64) + e], f, o[e]);
+  int spans = 1;
+  if ((min(max(scalar_int(a.b.starts, seq + 1), 0), a.b.T) - first) * a.G <= a.few) {
+    if (find_block<kStep>(a, seq, 0, kFewRows, B)) spans = (B.tiles + a.few_span - 1) / a.few_span;
+  } else if (find_block<kK>(a, seq, r / kQ * kQ, kQ, B)) {
+    spans = (B.tiles + a.span - 1) / a.span;
   }
-  const float f = l == 0.0f ? NAN : 1.0f / l;
-  uint16_t* op = a.out + at * D + ln * (D / 64);
+  if (spans <= 1) return;
+  if (ln >= spans) y = make_float2(-INFINITY, 0.0f);
+  const float m = wave_group_max_f32<64>(y.x);
+  // a span with scores of -inf only has sums of zero, or the NaN of what it saw
+  const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - m) * a.c);
+  const float l = wave_group_sum_f32<64>(y.y * f);
+  constexpr int E = D / 64;
+  float o[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = 0.0f;
+  const float* pp = a.part + at * a.slots * D + ln * E;
+#pragma unroll 8
+  for (int s = 0; s < spans; s++) {
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = fmaf(pp[(int64_t)s * D + e], w, o[e]);
+  }
+  const float inv = l == 0.0f ? NAN : 1.0f / l;
+  uint16_t* op = a.out + at * D + ln * E;
   if (D == 128)
-    *reinterpret_cast<uint32_t*>(op) = T::pack(o[0] * f, o[D / 64 - 1] * f);
+    *reinterpret_cast<uint32_t*>(op) = T::pack(o[0] * inv, o[E - 1] * inv);
   else
-    *op = T::from_f32(o[0] * f);
+    *op = T::from_f32(o[0] * inv);
 }
 
-// How the keys are split.  `span` tiles a workgroup, the longest sequence in
-// `spans` of them.
+// Which kernels run, and how the keys are split: sequences of up to `few` rows by
+// the first kernel (nr groups of 16 rows), in spans of few_span steps, the others by
+// the second in spans of `span` tiles.
 struct Plan {
-  int64_t blocks, items, per, span, spans, bytes;
+  int nr;       // 0: the first kernel does not run
+  bool many;    // whether the second runs
+  int64_t few, few_span, few_spans, blocks, items, per, span, spans, slots, bytes;
 };
 
-Plan plan(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_length) {
-  Plan p;
-  const int64_t G = H / Hkv;
-  p.blocks = S == 1 ? aq::ceil_div(T * G, kQ) : T * G / kQ + S;
-  p.items = p.blocks * Hkv;
-  p.per = aq::ceil_div(p.items, 8);
-  const int64_t tiles = aq::ceil_div(max_length, kK) + 1;
-  p.spans = std::max<int64_t>(1, std::min<int64_t>(512 / p.items, aq::ceil_div(tiles, 8)));
-  p.span = aq::ceil_div(tiles, p.spans);
-  p.spans = aq::ceil_div(tiles, p.span);
-  p.bytes = p.spans > 1 ? T * H * p.spans * (D + 2) * 4 : 0;
+Plan plan(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new, int64_t max_length) {
+  Plan p = {};
+  const int64_t G = H / Hkv, most = std::min(max_new, T) * G;  // rows of a sequence
+  if (most <= kFewRows)
+    p.nr = most <= 16 ? 1 : 2;
+  else if (S > 1 && G <= kFewRows)
+    p.nr = G <= 16 ? 1 : 2;
+  p.few = 16 * p.nr;
+  p.many = most > p.few;
+  p.few_spans = p.spans = 1;
+  if (p.nr) {
+    const int64_t steps = aq::ceil_div(max_length, kStep) + 1, pairs = S * Hkv;
+    p.few_spans = std::max<int64_t>(1, std::min<int64_t>({1024 / pairs, aq::ceil_div(steps, 4), 64}));
+    p.few_span = aq::ceil_div(steps, p.few_spans);
+    p.few_spans = aq::ceil_div(steps, p.few_span);
+  }
+  if (p.many) {
+    p.blocks = S == 1 ? aq::ceil_div(T * G, kQ) : T * G / kQ + S;
+    p.items = p.blocks * Hkv;
+    p.per = aq::ceil_div(p.items, 8);
+    const int64_t tiles = aq::ceil_div(max_length, kK) + 1;
+    p.spans = std::max<int64_t>(1, std::min<int64_t>({512 / p.items, aq::ceil_div(tiles, 8), 64}));
+    p.span = aq::ceil_div(tiles, p.spans);
+    p.spans = aq::ceil_div(tiles, p.span);
+  }
+  p.slots = std::max(p.spans, p.few_spans);
+  p.bytes = p.slots > 1 ? T * H * p.slots * (D + 2) * 4 : 0;
   return p;
 }
 
@@ -436,8 +721,12 @@ bool sizes_ok(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t m
 
 template <class T, int D>
 void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
-  if (p.spans > 1)
+  const dim3 few((unsigned)(a.b.S * a.Hkv), (unsigned)p.few_spans);
+  if (p.nr == 1) hipLaunchKernelGGL((paged_few_kernel<T, D, 1>), few, dim3(256), 0, stream, a);
+  if (p.nr == 2) hipLaunchKernelGGL((paged_few_kernel<T, D, 2>), few, dim3(256), 0, stream, a);
+  if (p.many)
+    hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
+  if (p.slots > 1)
     hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)aq::ceil_div((int64_t)a.b.T * a.H, 4)), dim3(256), 0, stream, a);
 }
 
@@ -445,7 +734,7 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
 
 extern "C" int64_t aq_paged_attention_workspace(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new,
                                                 int64_t max_length) {
-  return sizes_ok(T, S, H, Hkv, D, max_new, max_length) ? plan(T, S, H, Hkv, D, max_length).bytes : -1;
+  return sizes_ok(T, S, H, Hkv, D, max_new, max_length) ? plan(T, S, H, Hkv, D, max_new, max_length).bytes : -1;
 }
 
 extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D,
@@ -471,11 +760,12 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   AQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16 == 0 &&
                    ((uintptr_t)starts | (uintptr_t)lengths | (uintptr_t)table) % 4 == 0,
                "%s: q, the caches and out must be 16-byte aligned", me);
-  const Plan p = plan(T, S, H, Hkv, D, max_length);
+  const Plan p = plan(T, S, H, Hkv, D, max_new, max_length);
   AQ_CHECK_ARG(p.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me, (long long)ws_bytes, (long long)p.bytes);
   // (a grid has fewer than 2^32 threads)
-  AQ_CHECK_ARG(p.items <= (1 << 24) / p.spans - 8, "%s: %lld blocks of rows", me, (long long)p.items);
+  AQ_CHECK_ARG(p.items <= (1 << 24) / p.spans - 8 && S * Hkv <= (1 << 24) / p.few_spans && T * H <= (1 << 25),
+               "%s: %lld rows of %lld heads, %lld sequences", me, (long long)T, (long long)H, (long long)S);
   AttendArgs a;
   a.b = paged::Batch{starts, lengths, table, (int)T, (int)S, (int)W, (int)pages, __builtin_ctz((unsigned)page_size),
                      (int)std::min<int64_t>(max_new, T), (int)max_length};
@@ -493,8 +783,12 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   a.sinks = (int)std::min<int64_t>(sinks, max_length);
   a.items = (int)p.items;
   a.per = (int)p.per;
+  a.few = (int)p.few;
+  a.few_span = (int)p.few_span;
+  a.few_spans = (int)p.few_spans;
   a.span = (int)p.span;
   a.spans = (int)p.spans;
+  a.slots = (int)p.slots;
   a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
   a.keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
