@@ -75,12 +75,13 @@ SIGNATURES = {
     "aq_kv4_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "aq_kv4_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                         ctypes.c_float, ctypes.c_float, _P, _P, _I64, _P, _I64, _P, _P]),
-    "aq_paged_store": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P,
-                                      _I64, _I64, _I64, _P, _I64, ctypes.c_int, ctypes.c_float, _P, _P, _P, _I64,
-                                      _I64, _P]),
+    "aq_paged_store": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                      _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, ctypes.c_int, ctypes.c_float,
+                                      _P, _P, _P, _I64, _I64, _P]),
     "aq_paged_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
-    "aq_paged_attention": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P,
-                                          _I64, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P, _P]),
+    "aq_paged_attention": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _P,
+                                          _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_float, _P, _I64, _P,
+                                          _P]),
     "aq_sample": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_float,
                                  ctypes.c_int32, ctypes.c_float, ctypes.c_float, _P, _P, _I64, _P]),
     "aq_sample_workspace": (_I64, [_I64, _I64, ctypes.c_int, ctypes.c_int32]),

@@ -623,34 +623,11 @@ __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
   }
 }
 
-// The spans of a row joined, a wave a row (token and head): lane s has the maximum
-// and denominator of span s (there are up to 64).
+// The spans of a row (token and head, `at` of them) joined by a wave: lane s has the
+// maximum and denominator of span s (y; there are up to 64).
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
+__device__ __forceinline__ void merge_row(const AttendArgs& a, int64_t at, int spans, float2 y) {
   const int ln = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = (int)(at / a.H), head = (int)(at % a.H);
-  if (t >= a.b.T) return;
-  // (read before it is known how many there are: what is none is not looked at)
-  float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
-  // the row's sequence, and the block that it was in
-  int seq = -1;
-  for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
-    const int s = min(s0 + ln, a.b.S - 1);
-    const uint64_t hit = __ballot(a.b.start(s) <= t && t < a.b.start(s + 1) && s == s0 + ln);
-    if (hit) seq = __builtin_amdgcn_readfirstlane(s0 + __builtin_ctzll(hit));
-  }
-  if (seq < 0) return;
-  const int first = min(max(scalar_int(a.b.starts, seq), 0), a.b.T);
-  const int r = (t - first) * a.G + head % a.G;
-  Block B;
-  int spans = 1;
-  if ((min(max(scalar_int(a.b.starts, seq + 1), 0), a.b.T) - first) * a.G <= a.few) {
-    if (find_block<kStep>(a, seq, 0, kFewRows, B)) spans = (B.tiles + a.few_span - 1) / a.few_span;
-  } else if (find_block<kK>(a, seq, r / kQ * kQ, kQ, B)) {
-    spans = (B.tiles + a.span - 1) / a.span;
-  }
-  if (spans <= 1) return;
   if (ln >= spans) y = make_float2(-INFINITY, 0.0f);
   const float m = wave_group_max_f32<64>(y.x);
   // a span with scores of -inf only has sums of zero, or the NaN of what it saw
@@ -673,6 +650,46 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
     *reinterpret_cast<uint32_t*>(op) = T::pack(o[0] * inv, o[E - 1] * inv);
   else
     *op = T::from_f32(o[0] * inv);
+}
+
+// For the first kernel, a workgroup a sequence and key/value head, as there.
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_few_merge_kernel(AttendArgs a) {
+  const int ln = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
+  Block B;
+  if (!find_block<kStep>(a, seq, 0, kFewRows, B) || B.n * a.G > a.few) return;
+  const int spans = (B.tiles + a.few_span - 1) / a.few_span;
+  if (spans <= 1) return;
+  for (int r = wave; r < B.n * a.G; r += 4) {
+    const int tok = r / a.G;
+    const int64_t at = (int64_t)(B.first + tok) * a.H + j * a.G + r - tok * a.G;
+    merge_row<T, D>(a, at, spans, ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)]);
+  }
+}
+
+// For the second, a wave a row.
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
+  const int ln = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = (int)(at / a.H), head = (int)(at % a.H);
+  if (t >= a.b.T) return;
+  // (read before it is known how many there are: what is none is not looked at)
+  const float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
+  // the row's sequence, and the block that it was in
+  int seq = -1;
+  for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
+    const int s = min(s0 + ln, a.b.S - 1);
+    const uint64_t hit = __ballot(a.b.start(s) <= t && t < a.b.start(s + 1) && s == s0 + ln);
+    if (hit) seq = __builtin_amdgcn_readfirstlane(s0 + __builtin_ctzll(hit));
+  }
+  if (seq < 0) return;
+  const int r = (t - min(max(scalar_int(a.b.starts, seq), 0), a.b.T)) * a.G + head % a.G;
+  Block B;
+  if (!find_block<kK>(a, seq, r / kQ * kQ, kQ, B) || B.n * a.G <= a.few) return;
+  const int spans = (B.tiles + a.span - 1) / a.span;
+  if (spans > 1) merge_row<T, D>(a, at, spans, y);
 }
 
 // Which kernels run, and how the keys are split: sequences of up to `few` rows by
@@ -726,7 +743,8 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.nr == 2) hipLaunchKernelGGL((paged_few_kernel<T, D, 2>), few, dim3(256), 0, stream, a);
   if (p.many)
     hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
-  if (p.slots > 1)
+  if (p.few_spans > 1) hipLaunchKernelGGL((paged_few_merge_kernel<T, D>), dim3(few.x), dim3(256), 0, stream, a);
+  if (p.spans > 1)
     hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)aq::ceil_div((int64_t)a.b.T * a.H, 4)), dim3(256), 0, stream, a);
 }
 
@@ -738,12 +756,12 @@ extern "C" int64_t aq_paged_attention_workspace(int64_t T, int64_t S, int64_t H,
 }
 
 extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D,
-                                  const int64_t* q_strides, const void* k_cache, const void* v_cache, int64_t pages,
+                                  int64_t q_row, int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages,
                                   int64_t page_size, const int32_t* starts, const int32_t* lengths, int64_t S,
                                   const int32_t* table, int64_t W, int64_t max_new, int64_t max_length, int64_t window,
                                   int64_t sinks, float scale, void* workspace, int64_t ws_bytes, void* out, void* stream) {
   const char* me = "aq_paged_attention";
-  AQ_CHECK_ARG(q && q_strides && k_cache && v_cache && starts && lengths && table && out, "%s: null pointer", me);
+  AQ_CHECK_ARG(q && k_cache && v_cache && starts && lengths && table && out, "%s: null pointer", me);
   AQ_CHECK_ARG(dtype == AQ_F16 || dtype == AQ_BF16, "%s: dtype %d (fp16 and bf16 supported)", me, dtype);
   AQ_CHECK_ARG(D == 64 || D == 128, "%s: head dim %lld (64 or 128 supported)", me, (long long)D);
   AQ_CHECK_ARG(Hkv > 0 && H > 0 && H <= 1024 && H % Hkv == 0, "%s: H (%lld) must be a multiple of Hkv (%lld)", me, (long long)H,
@@ -756,7 +774,7 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W * page_size <= INT32_MAX && max_length <= W * page_size,
                "%s: %lld pages, %lld of a sequence for %lld positions", me, (long long)pages, (long long)W, (long long)max_length);
   AQ_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %lld, %lld sinks", me, (long long)window, (long long)sinks);
-  AQ_CHECK_ARG(q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0, "%s: strides must be multiples of 8", me);
+  AQ_CHECK_ARG(q_row % 8 == 0 && q_head % 8 == 0, "%s: strides must be multiples of 8", me);
   AQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) % 16 == 0 &&
                    ((uintptr_t)starts | (uintptr_t)lengths | (uintptr_t)table) % 4 == 0,
                "%s: q, the caches and out must be 16-byte aligned", me);
@@ -772,8 +790,8 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   a.q = (const uint16_t*)q;
   a.k = (const uint16_t*)k_cache;
   a.v = (const uint16_t*)v_cache;
-  a.qs[0] = q_strides[0];
-  a.qs[1] = q_strides[1];
+  a.qs[0] = q_row;
+  a.qs[1] = q_head;
   a.out = (uint16_t*)out;
   a.part = (float*)workspace;
   a.H = (int)H;

@@ -111,14 +111,14 @@ __global__ __launch_bounds__(kThreads) void paged_store_kernel(StoreArgs a) {
 }  // namespace
 
 extern "C" int aq_paged_store(const void* q, const void* k, const void* v, int dtype, int64_t T, int64_t H, int64_t Hkv,
-                              int64_t D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                              const int32_t* starts, const int32_t* lengths, int64_t S, const int32_t* table, int64_t W,
+                              int64_t D, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
+                              int64_t v_head, const int32_t* starts, const int32_t* lengths, int64_t S, const int32_t* table, int64_t W,
                               int64_t max_new, int64_t max_length, const float* frequencies, int64_t rotary,
                               int interleaved, float factor, void* q_out, void* k_cache, void* v_cache, int64_t pages,
                               int64_t page_size, void* stream) {
   const char* me = "aq_paged_store";
-  AQ_CHECK_ARG(k && v && k_strides && v_strides && starts && lengths && table && k_cache && v_cache, "%s: null pointer", me);
-  AQ_CHECK_ARG((q == nullptr) == (H == 0) && (q == nullptr || (q_out && q_strides)), "%s: q, its strides and q_out come with H", me);
+  AQ_CHECK_ARG(k && v && starts && lengths && table && k_cache && v_cache, "%s: null pointer", me);
+  AQ_CHECK_ARG((q == nullptr) == (H == 0) && (q == nullptr) == (q_out == nullptr), "%s: q and q_out come with H", me);
   AQ_CHECK_ARG(dtype == AQ_F16 || dtype == AQ_BF16, "%s: dtype %d (fp16 and bf16 supported)", me, dtype);
   AQ_CHECK_ARG(D == 64 || D == 128, "%s: head dim %lld (64 or 128 supported)", me, (long long)D);
   AQ_CHECK_ARG(T > 0 && T < (1 << 24) && S > 0 && S <= 65535 && H >= 0 && H <= 1024 && Hkv > 0 && Hkv <= 1024,
@@ -131,9 +131,7 @@ extern "C" int aq_paged_store(const void* q, const void* k, const void* v, int d
                (long long)max_new, (long long)max_length);
   AQ_CHECK_ARG(rotary >= 0 && rotary <= D && rotary % 16 == 0 && (rotary == 0) == (frequencies == nullptr),
                "%s: %lld rotary elements (a multiple of 16 up to D, with their frequencies)", me, (long long)rotary);
-  for (int i = 0; i < 2; i++)
-    AQ_CHECK_ARG((!q || q_strides[i] % 8 == 0) && k_strides[i] % 8 == 0 && v_strides[i] % 8 == 0,
-                 "%s: strides must be multiples of 8", me);
+  AQ_CHECK_ARG((q_row | q_head | k_row | k_head | v_row | v_head) % 8 == 0, "%s: strides must be multiples of 8", me);
   AQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 &&
                    ((uintptr_t)starts | (uintptr_t)lengths | (uintptr_t)table | (uintptr_t)frequencies) % 4 == 0,
                "%s: q, k, v, q_out and the caches must be 16-byte aligned", me);
@@ -143,11 +141,12 @@ extern "C" int aq_paged_store(const void* q, const void* k, const void* v, int d
   a.q = (const uint16_t*)q;
   a.k = (const uint16_t*)k;
   a.v = (const uint16_t*)v;
-  for (int i = 0; i < 2; i++) {
-    a.qs[i] = q ? q_strides[i] : 0;
-    a.ks[i] = k_strides[i];
-    a.vs[i] = v_strides[i];
-  }
+  a.qs[0] = q_row;
+  a.qs[1] = q_head;
+  a.ks[0] = k_row;
+  a.ks[1] = k_head;
+  a.vs[0] = v_row;
+  a.vs[1] = v_head;
   a.q_out = (uint16_t*)q_out;
   a.k_cache = (uint16_t*)k_cache;
   a.v_cache = (uint16_t*)v_cache;

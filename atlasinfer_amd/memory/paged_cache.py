@@ -16,7 +16,6 @@ HIP graph replays with new lengths and pages; only its shapes and the bounds
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -153,10 +152,6 @@ def _cache(what, cache, batch):
     return k, v, Hkv, P, D
 
 
-def _strides(t: torch.Tensor):
-    return _lib.ptr_array(t.stride()[:2], ctypes.c_int64)
-
-
 def _no_gradients(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} records no gradients: call it under torch.no_grad()")
@@ -205,8 +200,8 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, cache: Sequence[torch.Tensor],
     starts, lengths, S, table, W, max_new, max_length = batch._args
     with _lib.on_device(dev):
         _lib.check(_lib.load().aq_paged_store(
-            _lib.ptr(q), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, None if q is None else _strides(q),
-            _strides(k), _strides(v), starts, lengths, S, table, W, max_new, max_length, _lib.ptr(freq), R, int(inter),
+            _lib.ptr(q), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, *(q.stride()[:2] if H else (0, 0)),
+            *k.stride()[:2], *v.stride()[:2], starts, lengths, S, table, W, max_new, max_length, _lib.ptr(freq), R, int(inter),
             factor, _lib.ptr(q_out), kc.data_ptr(), vc.data_ptr(), kc.shape[0], P, _lib.stream_of(dev)), "aq_paged_store")
     return q_out
 
@@ -256,8 +251,8 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
         workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     with _lib.on_device(dev):
-        _lib.check(L.aq_paged_attention(q.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, _strides(q), kc.data_ptr(),
-                                        vc.data_ptr(), kc.shape[0], P, starts, lengths, S, table, W, max_new, max_length,
+        _lib.check(L.aq_paged_attention(q.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, *q.stride()[:2],
+                                        kc.data_ptr(), vc.data_ptr(), kc.shape[0], P, starts, lengths, S, table, W, max_new, max_length,
                                         min(window, _INT_MAX), min(sinks, _INT_MAX), scale, ws, size, out.data_ptr(),
                                         _lib.stream_of(dev)), "aq_paged_attention")
     return out

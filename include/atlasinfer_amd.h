@@ -563,8 +563,8 @@ int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t strid
  * x, y at elements i and i + rotary / 2 (interleaved = 0) or 2 i and 2 i + 1 (1) become
  *   factor (x cos a - y sin a), factor (y cos a + x sin a),  a = position frequencies[i]
  * (angles reduced in 64 bits, products in f32, one rounding).
- *   q   [T, H, D] or NULL (H = 0), k, v [T, Hkv, D]: by strides {row, head} in
- *       elements, multiples of 8; 16-byte aligned
+ *   q   [T, H, D] or NULL (H = 0), k, v [T, Hkv, D]: by strides *_row and
+ *       *_head in elements, multiples of 8; 16-byte aligned
  *   frequencies  f32 [rotary / 2], or NULL with rotary = 0; rotary a multiple of 16
  *   q_out  [T, H, D], not q
  * Rows that share a place (tables with the same page for two sequences' new tokens)
@@ -578,21 +578,21 @@ int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t strid
  * or value that a row does not see holds, infinities and NaN included, does not reach
  * its output; a seen value that is not finite makes its element of the output not
  * finite; a row whose seen scores are all -inf answers NaN.
- *   q   [T, H, D] by strides {row, head}, multiples of 8; H a multiple of Hkv
+ *   q   [T, H, D] by strides, multiples of 8; H a multiple of Hkv
  *   out [T, H, D]; q, out and the caches 16-byte aligned
  *   workspace  aq_paged_attention_workspace bytes (may be 0, then NULL will do; -1 for
  *       sizes it cannot take), 16-byte aligned, no initial contents; calls that
  *       overlap in time must not share one
  */
 int aq_paged_store(const void* q, const void* k, const void* v, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D,
-                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int32_t* starts,
-                   const int32_t* lengths, int64_t S, const int32_t* table, int64_t W, int64_t max_new,
+                   int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                   const int32_t* starts, const int32_t* lengths, int64_t S, const int32_t* table, int64_t W, int64_t max_new,
                    int64_t max_length, const float* frequencies, int64_t rotary, int interleaved, float factor,
                    void* q_out, void* k_cache, void* v_cache, int64_t pages, int64_t page_size, void* stream);
 int64_t aq_paged_attention_workspace(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_new,
                                      int64_t max_length);
-int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
-                       const void* k_cache, const void* v_cache, int64_t pages, int64_t page_size,
+int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H, int64_t Hkv, int64_t D, int64_t q_row,
+                       int64_t q_head, const void* k_cache, const void* v_cache, int64_t pages, int64_t page_size,
                        const int32_t* starts, const int32_t* lengths, int64_t S, const int32_t* table, int64_t W,
                        int64_t max_new, int64_t max_length, int64_t window, int64_t sinks, float scale,
                        void* workspace, int64_t ws_bytes, void* out, void* stream);
