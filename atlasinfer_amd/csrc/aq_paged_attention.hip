@@ -56,11 +56,9 @@ __device__ __forceinline__ void load_to_lds(u32x4 r, uint32_t dst, const int (&o
 #pragma unroll
   for (int n = 0; n < N; n++) {
     if (n == 0)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off[0]), "s"(r)
-                   : "m0", "memory");
+      asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(dst), "v"(off[0]), "s"(r) : "memory");
     else
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst + 1024 * n), "v"(off[n]), "s"(r)
-                   : "m0", "memory");
+      asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(dst + 1024 * n), "v"(off[n]), "s"(r) : "memory");
   }
 }
 
@@ -398,14 +396,15 @@ constexpr int kStep = 32;  // keys a wave takes at a time below
 // next values when the last ones are in LDS.
 template <class T, int D, int NR>
 __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
+  constexpr int NW = 4;                 // waves
   constexpr int NC = D / 8;             // 16-byte pieces of a row
   constexpr int RL = 64 / NC;           // rows a load of values
   constexpr int NV = kStep / RL;        // loads of values a step
   constexpr int VB = kStep * D * 2;     // bytes of a step's values
   constexpr int RS = D + 4;             // floats of a row of sums in LDS, so that rows spread over the banks
-  constexpr int SUMS = 4 * NR * 16 * RS * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[SUMS > 4 * VB ? SUMS : 4 * VB];
-  __shared__ float2 ends[4][NR * 16];
+  constexpr int SUMS = NW * NR * 16 * RS * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[SUMS > NW * VB ? SUMS : NW * VB];
+  __shared__ float2 ends[NW][NR * 16];
   const int t = threadIdx.x, ln = t & 63, i16 = ln & 15, g = ln >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
@@ -483,8 +482,8 @@ __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
     load_keys(k0);
     load_values(k0);
   }
-  for (int i = t0 + wave; i < t1; i += 4) {
-    const int next = i + 4 < t1 ? step_at(i + 4) : -1;
+  for (int i = t0 + wave; i < t1; i += NW) {
+    const int next = i + NW < t1 ? step_at(i + NW) : -1;
     const bool all = k0 + kStep - 1 <= B.lo && k0 > B.hi - a.window;
     bool bad = false;
     if (!all) {
@@ -588,16 +587,16 @@ __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < (NR * 16 * NC + 255) / 256; n++) {
-    const int r = (t + 256 * n) / NC, d = (t + 256 * n) % NC * 8;
+  for (int n = 0; n < (NR * 16 * NC + 64 * NW - 1) / (64 * NW); n++) {
+    const int r = (t + 64 * NW * n) / NC, d = (t + 64 * NW * n) % NC * 8;
     if (r >= rows) continue;
     float mx = -INFINITY, den = 0.0f, acc[8];
 #pragma unroll
-    for (int w = 0; w < 4; w++) mx = fmaxf(mx, ends[w][r].x);
+    for (int w = 0; w < NW; w++) mx = fmaxf(mx, ends[w][r].x);
 #pragma unroll
     for (int z = 0; z < 8; z++) acc[z] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < NW; w++) {
       const float2 y = ends[w][r];
       // a wave with scores of -inf only has sums of zero, or the NaN of what it saw
       const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - mx) * a.c);
@@ -652,20 +651,60 @@ __device__ __forceinline__ void merge_row(const AttendArgs& a, int64_t at, int s
     *op = T::from_f32(o[0] * inv);
 }
 
-// For the first kernel, a workgroup a sequence and key/value head, as there.
+// For the first kernel, a workgroup a row: 16 bytes a lane, the spans dealt to
+// groups of D / 4 lanes, whose sums meet in LDS.  Everything is asked for at once,
+// before it is known how many spans there are: what is none is not looked at.
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_few_merge_kernel(AttendArgs a) {
-  const int ln = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
+  constexpr int N = 256 / (D / 4);  // groups
+  __shared__ float4 sums[N][D / 4];
+  const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv, r = blockIdx.y;
+  const int t = threadIdx.x, ln = t & 63, grp = t / (D / 4), d = t % (D / 4);
   Block B;
-  if (!find_block<kStep>(a, seq, 0, kFewRows, B) || B.n * a.G > a.few) return;
+  if (!find_block<kStep>(a, seq, 0, kFewRows, B) || B.n * a.G > a.few || r >= B.n * a.G) return;
+  const int tok = r / a.G;
+  const int64_t at = (int64_t)(B.first + tok) * a.H + j * a.G + r - tok * a.G;
+  float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
+  const float4* pp = reinterpret_cast<const float4*>(a.part + at * a.slots * D) + d;
+  constexpr int U = 4;
+  float4 x[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) x[u] = pp[(int64_t)min(grp + N * u, a.slots - 1) * (D / 4)];
   const int spans = (B.tiles + a.few_span - 1) / a.few_span;
   if (spans <= 1) return;
-  for (int r = wave; r < B.n * a.G; r += 4) {
-    const int tok = r / a.G;
-    const int64_t at = (int64_t)(B.first + tok) * a.H + j * a.G + r - tok * a.G;
-    merge_row<T, D>(a, at, spans, ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)]);
+  if (ln >= spans) y = make_float2(-INFINITY, 0.0f);
+  const float m = wave_group_max_f32<64>(y.x);
+  // a span with scores of -inf only has sums of zero, or the NaN of what it saw
+  const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - m) * a.c);
+  const float l = wave_group_sum_f32<64>(y.y * f);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s0 = grp; s0 - grp < spans; s0 += N * U) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int s = s0 + N * u;
+      const float w = __shfl(f, min(s, 63), 64);
+      if (s0 != grp && s < spans) x[u] = pp[(int64_t)s * (D / 4)];
+      if (s < spans) {
+        o.x = fmaf(x[u].x, w, o.x);
+        o.y = fmaf(x[u].y, w, o.y);
+        o.z = fmaf(x[u].z, w, o.z);
+        o.w = fmaf(x[u].w, w, o.w);
+      }
+    }
   }
+  sums[grp][d] = o;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int n = 1; n < N; n++) {
+    const float4 z = sums[n][d];
+    o.x += z.x;
+    o.y += z.y;
+    o.z += z.z;
+    o.w += z.w;
+  }
+  const float inv = l == 0.0f ? NAN : 1.0f / l;
+  *reinterpret_cast<uint2*>(a.out + at * D + 4 * d) = make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
 }
 
 // For the second, a wave a row.
@@ -697,6 +736,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
 // the second in spans of `span` tiles.
 struct Plan {
   int nr;       // 0: the first kernel does not run
+  int64_t few_rows;  // rows of a sequence and key/value head there, at most
   bool many;    // whether the second runs
   int64_t few, few_span, few_spans, blocks, items, per, span, spans, slots, bytes;
 };
@@ -712,8 +752,17 @@ Plan plan(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_n
   p.many = most > p.few;
   p.few_spans = p.spans = 1;
   if (p.nr) {
+    p.few_rows = std::min(most, p.few);
     const int64_t steps = aq::ceil_div(max_length, kStep) + 1, pairs = S * Hkv;
-    p.few_spans = std::max<int64_t>(1, std::min<int64_t>({1024 / pairs, aq::ceil_div(steps, 4), 64}));
+    // One span where it is short (up to 12 steps, three a wave: 300 positions of one
+    // sequence 7.1 us, 7.5 split and merged; 500 9.2 and 7.8) or the sequences and heads
+    // are many (256 of 4000 positions 91 us, 96 in two spans each), but for long ones,
+    // whose lengths differ more (256 of up to 16384: 220 us, 187 in 8 spans); else 512
+    // workgroups (64 of 4000: 26.0, 26.9 with 1024; 8 of 16000 17.4) of a step a wave at
+    // least.
+    if (steps <= 12 || pairs > 512) p.few_spans = 1;
+    else if (pairs >= 256) p.few_spans = steps <= 160 ? 1 : std::min<int64_t>(aq::ceil_div(steps, 64), 64);
+    else p.few_spans = std::min<int64_t>({512 / pairs, aq::ceil_div(steps, 4), 64});
     p.few_span = aq::ceil_div(steps, p.few_spans);
     p.few_spans = aq::ceil_div(steps, p.few_span);
   }
@@ -743,7 +792,8 @@ void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   if (p.nr == 2) hipLaunchKernelGGL((paged_few_kernel<T, D, 2>), few, dim3(256), 0, stream, a);
   if (p.many)
     hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
-  if (p.few_spans > 1) hipLaunchKernelGGL((paged_few_merge_kernel<T, D>), dim3(few.x), dim3(256), 0, stream, a);
+  if (p.few_spans > 1)
+    hipLaunchKernelGGL((paged_few_merge_kernel<T, D>), dim3(few.x, (unsigned)p.few_rows), dim3(256), 0, stream, a);
   if (p.spans > 1)
     hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3((unsigned)aq::ceil_div((int64_t)a.b.T * a.H, 4)), dim3(256), 0, stream, a);
 }
