@@ -3,28 +3,30 @@
 //
 // With m = max x, Z = sum e^(x_i - m) and E = sum e^(x_i - m) (x_i - m):
 //   log p_t = x_t - m - log Z,   entropy = -sum p log p = log Z - E / Z
-// in one pass: where the running maximum m grows by d, Z and E so far become
-// Z e^-d and (E - d Z) e^-d.  Parts of a row meet the same way.
+// in one pass, each lane with a maximum of its own: where it grows by d, Z and E so
+// far become Z e^-d and (E - d Z) e^-d.  Lanes, and parts of a row, meet the same way.
 //
 // The alternatives need no sort of the row.  In each wave, the n-th largest of the
 // lanes' maxima is a value that n elements at least reach; the largest of the
-// waves' values cuts the row to a short list (a few times n), gathered by the
-// lanes whose maxima reach it and ranked by counting.
+// waves' values cuts the row to a short list (about four times n), which is ranked by
+// counting.
 #include "aq_common.h"
 
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kList = 1024;
+constexpr int kHeld = 8;   // pieces that a thread keeps (in LDS): 2048 a workgroup
+constexpr int kList = 256;  // places of a wave's list
 constexpr int kMaxTop = 64, kMaxParts = 32;
 constexpr int kMaxVocab = 1 << 18;
-constexpr float kLog2e = 1.4426950408889634f;
-// What the pass over a row takes everything below, -inf and NaN too, for: no
-// weight beside a logit above it (and rows without one are looked at again).
-constexpr float kLow = -1e30f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Logits that the pass over a row can weigh; a part whose largest is not between
+// these is looked at again, number by number.
+constexpr float kLow = -1e30f, kHigh = 1e30f;
 
 typedef unsigned long long u64;
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 struct Sums {
   float m, z, e;
@@ -75,6 +77,22 @@ __device__ __forceinline__ float next_below(float x) {
   return of_key(k == 0x7FFFFFFFu ? k - 1 : k);  // below 0 comes -0, which is the same
 }
 
+// Logit i of a row that starts on any element, i the same for all lanes: the scalar
+// unit reads the word that holds it.
+template <int FMT>
+__device__ __forceinline__ float scalar_logit(const uint8_t* x, int64_t i) {
+  typedef const __attribute__((address_space(4))) uint32_t const_u32;
+  const uintptr_t at = (uintptr_t)x + i * Type<FMT>::kSize;
+  const uint32_t w = *(const_u32*)(at & ~(uintptr_t)3);
+  if (FMT == AQ_F32) return __builtin_bit_cast(float, w);
+  const uint16_t b = (uint16_t)(w >> (8 * (at & 2)));
+  return FMT == AQ_BF16 ? __builtin_bit_cast(float, (uint32_t)b << 16) : (float)bits_to_h(b);
+}
+__device__ __forceinline__ int64_t scalar_token(const int64_t* tokens, int row) {
+  typedef const __attribute__((address_space(4))) int64_t const_i64;
+  return ((const_i64*)(uintptr_t)tokens)[row];
+}
+
 // Part of a row: whole 16-byte pieces p0 .. p1 - 1, and up to 2 E - 2 single
 // elements before the first and behind the last of the row's.
 template <int FMT>
@@ -109,17 +127,8 @@ struct Part {
     const uint16_t b = reinterpret_cast<const uint16_t*>(x)[i];
     return FMT == AQ_BF16 ? __builtin_bit_cast(float, (uint32_t)b << 16) : (float)bits_to_h(b);
   }
-  // f(value, index) for this thread's elements, in order of index but for the single one
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    const int t = threadIdx.x;
-    if (t < singles) f(value(single(t)), single(t));
-    for (int p = p0 + t; p < p1; p += kThreads) {
-      const uint4 w = pieces[p];
-#pragma unroll
-      for (int i = 0; i < T::E; i++) f(T::get(w, i), lead + p * T::E + i);
-    }
-  }
+  // element i, the same for all lanes, by the scalar unit
+  __device__ __forceinline__ float scalar_value(int i) const { return scalar_logit<FMT>(x, i); }
 };
 
 __device__ __forceinline__ int wave_sum_i32(int v) {
@@ -128,177 +137,259 @@ __device__ __forceinline__ int wave_sum_i32(int v) {
 }
 
 struct Shared {
-  u64 list[kList];
+  uint4 held[kHeld * kThreads];
+  __attribute__((aligned(16))) u64 list[kWaves][kList];
+  u64 top[kMaxTop];
   Sums sums[kWaves];
+  float largest[kWaves];
   uint32_t cut[kWaves];
-  int scan[kWaves];
+  int count[kWaves];
   u64 best[kWaves];
-  int count;
 };
 
-// Sums of two sets of elements joined.  -inf: an empty one, or one of only -inf;
-// two of +inf count alike.
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = a.m == r.m ? 0.0f : a.m - r.m, db = b.m == r.m ? 0.0f : b.m - r.m;
-  const float fa = __builtin_amdgcn_exp2f(da * kLog2e), fb = __builtin_amdgcn_exp2f(db * kLog2e);
-  r.z = a.z * fa + b.z * fb;
-  r.e = (fa > 0.0f ? fmaf(da, a.z, a.e) * fa : 0.0f) + (fb > 0.0f ? fmaf(db, b.z, b.e) * fb : 0.0f);
-  r.before = a.before + b.before;
-  return r;
+// f(value, index, whether it is one) for this thread's elements, the wave's lanes
+// together; `there`: the part's pieces are in s.held.
+template <int FMT, class F>
+__device__ __forceinline__ void each(const Shared& s, const Part<FMT>& r, bool there, F f) {
+  typedef Type<FMT> T;
+  const int t = threadIdx.x, first = __builtin_amdgcn_readfirstlane(t & ~63);
+  if (first < r.singles) f(t < r.singles ? r.value(r.single(t)) : -INFINITY, r.single(t), t < r.singles);
+  if (there) {
+#pragma unroll 1
+    for (int p = r.p0 + first, u = 0; p < r.p1; p += kThreads, u++) {
+      const uint4 w = s.held[t + u * kThreads];
+      const int at = p + (t & 63);
+#pragma unroll
+      for (int i = 0; i < T::E; i++) f(T::get(w, i), r.lead + at * T::E + i, at < r.p1);
+    }
+  } else {
+#pragma unroll 1
+    for (int p = r.p0 + first; p < r.p1; p += kThreads) {
+      const int at = p + (t & 63);
+      const uint4 w = at < r.p1 ? r.pieces[at] : T::none();
+#pragma unroll
+      for (int i = 0; i < T::E; i++) f(T::get(w, i), r.lead + at * T::E + i, at < r.p1);
+    }
+  }
 }
 
-__device__ __forceinline__ float shfl_xor_f32(float x, int d) { return __shfl_xor(x, d, 64); }
+// The largest over the workgroup.
+__device__ __forceinline__ float block_max(Shared& s, float x) {
+  x = wave_group_max_f32<64>(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.largest[threadIdx.x >> 6] = x;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) x = fmaxf(x, s.largest[w]);
+  return x;
+}
 
-__device__ __forceinline__ Sums block_join(Shared& s, Sums v) {
-  for (int d = 1; d < 64; d *= 2) {
-    const Sums o = {shfl_xor_f32(v.m, d), shfl_xor_f32(v.z, d), shfl_xor_f32(v.e, d), 0};
-    const int n = v.before;
-    v = (threadIdx.x & d) ? join(o, v) : join(v, o);  // the same order in both lanes
-    v.before = n;
-  }
-  v.before = wave_sum_i32(v.before);
+// z, e and before (a wave's count in each of its lanes) summed over the workgroup.
+__device__ __forceinline__ Sums block_sum(Shared& s, Sums v) {
+  v.z = wave_group_sum_f32<64>(v.z);
+  v.e = wave_group_sum_f32<64>(v.e);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) s.sums[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = s.sums[0];
+  v.z = v.e = 0.0f;
+  v.before = 0;
 #pragma unroll
-  for (int w = 1; w < kWaves; w++) v = join(v, s.sums[w]);
+  for (int w = 0; w < kWaves; w++) {
+    v.z += s.sums[w].z;
+    v.e += s.sums[w].e;
+    v.before += s.sums[w].before;
+  }
   return v;
 }
 
-// The same sums number by number, for parts with a +inf, without a logit above
-// kLow, or of a token whose logit is not above kLow.
-template <int FMT>
-__device__ __forceinline__ Sums exact_sums(Shared& s, const Part<FMT>& r, float own, int token) {
-  float m = -INFINITY;
-  r.each([&](float x, int) { m = fmaxf(m, x); });
-  m = wave_group_max_f32<64>(m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.sums[threadIdx.x >> 6].m = m;
-  __syncthreads();
+// How many of n numbers (a multiple of 32) are larger than e, counted by four
+// neighbouring lanes, which all have e.
+__device__ __forceinline__ int count_above(const u64* list, int n, u64 e) {
+  int above = 0;
+#pragma unroll 1
+  for (int i = 2 * (threadIdx.x & 3); i < n; i += 32) {
+    u64x2 x[4];
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) m = fmaxf(m, s.sums[w].m);
+    for (int u = 0; u < 4; u++) x[u] = *reinterpret_cast<const u64x2*>(list + i + 8 * u);
+#pragma unroll
+    for (int u = 0; u < 4; u++) above += (x[u].x > e) + (x[u].y > e);
+  }
+  above += __builtin_amdgcn_mov_dpp(above, 0xB1, 0xF, 0xF, false);  // quad_perm [1,0,3,2]
+  return above + __builtin_amdgcn_mov_dpp(above, 0x4E, 0xF, 0xF, false);  // [2,3,0,1]
+}
+
+// Sums number by number, for parts that the pass over them cannot weigh, or of a
+// token whose logit is not above kLow: e^(x - m) with the largest exactly 1, +inf too.
+template <int FMT>
+__device__ __forceinline__ Sums exact_sums(Shared& s, const Part<FMT>& r, bool there, float own, int token) {
+  float m = -INFINITY;
+  each(s, r, there, [&](float x, int, bool) { m = fmaxf(m, x); });
+  m = block_max(s, m);
   Sums v = {m, 0.0f, 0.0f, 0};
-  r.each([&](float x, int i) {
+  each(s, r, there, [&](float x, int i, bool in) {
     x = fmaxf(x, -INFINITY);
-    v.before += x > own || (x == own && i < token);
-    if (x == -INFINITY) return;
-    const float d = x == m ? 0.0f : x - m, w = __builtin_amdgcn_exp2f(d * kLog2e);
+    v.before += __popcll(__ballot(in && (x > own || (x == own && i < token))));
+    const float d = x == m ? 0.0f : x - m, w = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(d * kLog2e);
     v.z += w;
     v.e += w > 0.0f ? w * d : 0.0f;
   });
-  return block_join(s, v);
+  return block_sum(s, v);
 }
 
-// The `n` first elements of the part, by falling value and then by index, in
-// s.list (fewer if it has fewer); mine: this thread's largest, has: whether it has any.
+// The `n` first elements of the part, by falling value and then by index, in s.top
+// (fewer if it has fewer); mine: this thread's largest, has: whether it has any.
 template <int FMT>
-__device__ __forceinline__ int part_top(Shared& s, const Part<FMT>& r, int n, float mine, bool has) {
+__device__ __forceinline__ int part_top(Shared& s, const Part<FMT>& r, bool there, int n, float mine, bool has) {
   typedef Type<FMT> T;
-  const int t = threadIdx.x, wave = t >> 6;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t key = has ? key_of(mine) : 0u;
-  // the largest value that n of the wave's lanes reach (0: fewer have any); the low
-  // bits of 16-bit numbers are all alike
-  constexpr int kLowest = FMT == AQ_F32 ? 0 : FMT == AQ_BF16 ? 16 : 13;
+  // the largest value that n of the wave's lanes reach (0: fewer have any), two bits
+  // at a time; the low bits of 16-bit numbers are all alike
+  constexpr int kLowest = FMT == AQ_F32 ? 0 : FMT == AQ_BF16 ? 16 : 12;
   uint32_t cut = 0;
-  for (int bit = 31; bit >= kLowest; bit--) {
-    const uint32_t c = cut | 1u << bit;
-    if (__popcll(__ballot(key >= c)) >= n) cut = c;
+#pragma unroll 1
+  for (int bit = 30; bit >= kLowest; bit -= 2) {
+    const uint32_t c1 = cut | 1u << bit, c2 = cut | 2u << bit, c3 = cut | 3u << bit;
+    const int k1 = __popcll(__ballot(key >= c1)), k2 = __popcll(__ballot(key >= c2)), k3 = __popcll(__ballot(key >= c3));
+    cut = k3 >= n ? c3 : k2 >= n ? c2 : k1 >= n ? c1 : cut;
   }
   if (cut && !(cut >> 31)) cut |= (1u << kLowest) - 1;
   __syncthreads();
   if ((t & 63) == 0) s.cut[wave] = cut;
-  if (t == 0) s.count = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; w++) cut = max(cut, s.cut[w]);
-  auto gather = [&](uint32_t low) {  // what has keys of `low` and above; where a lane has none it does not look
-    if (key >= low)
-      r.each([&](float x, int i) {
-        if (key_of(x) >= low) {
-          const int at = atomicAdd(&s.count, 1);
-          if (at < kList) s.list[at] = entry_of(x, i);
-        }
-      });
-    __syncthreads();
-    const int c = s.count;
-    __syncthreads();
-    return c;
-  };
-  int c = gather(cut);
-  if (c > kList) {  // many at the cut: those above it, then the first ones at it, by index
-    if (t == 0) s.count = 0;
-    __syncthreads();
-    c = gather(cut + 1);
-    if (c < n) {
-      auto place = [&](int mask, int base) {  // elements base + i of this thread for the bits i
-        const int k = __popc(mask);
-        const int inc = wave_incl_scan_i32<64>(k);
-        if ((t & 63) == 63) s.scan[wave] = inc;
-        __syncthreads();
-        int at = c + inc - k, all = 0;
+  // Each wave lists its elements with keys of `low` and above (where it has one); the
+  // second time, where very many are equal to the cut, those above it.
+  int c = 0, before = 0;
+  bool over = false;
+#pragma unroll 1
+  for (uint32_t low = cut; low <= cut + 1; low++) {
+    const float least = low > key_of(-INFINITY) ? of_key(low) : -INFINITY;
+    int k = 0;
+    auto list = [&](float x, int i, bool in) {
+      const bool take = in && fmaxf(x, -INFINITY) >= least;
+      const uint64_t mask = __ballot(take);
+      const int at = k + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+      if (take && at < kList) s.list[wave][at] = entry_of(x, i);
+      k += __popcll(mask);
+    };
+    uint64_t reach = __ballot(key >= low);
+    if (!there) {
+      if (reach) each(s, r, there, list);
+    } else {
+      // lane by lane of those whose maxima reach it, an element of its pieces a lane
+      // (two lanes at once for numbers of 32 bits): a tenth of the time that every
+      // lane's walk over its own takes
+      if (wave == 0 && r.singles) list(t < r.singles ? r.value(r.single(t)) : -INFINITY, r.single(min(t, r.singles - 1)), t < r.singles);
+      constexpr int kAtOnce = 64 / (kHeld * T::E);
+      const int ln = t & 63, u = ln / T::E % kHeld, el = ln % T::E, half = ln / (kHeld * T::E);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(s.held) + (wave * 64 + u * kThreads) * 16 + el * T::kSize;
+#pragma unroll 1
+      while (reach) {
+        constexpr int U = 4;
+        int src[U];
+        float x[U];
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-          at += w < wave ? s.scan[w] : 0;
-          all += s.scan[w];
+        for (int n = 0; n < U; n++) {
+          src[n] = reach ? __builtin_ctzll(reach) : -1;
+          reach &= reach - 1;
+          if (kAtOnce == 2) {
+            const int other = reach ? __builtin_ctzll(reach) : -1;
+            reach &= reach - 1;
+            src[n] = half ? other : src[n];
+          }
+          const uint8_t* at = from + max(src[n], 0) * 16;
+          if (FMT == AQ_F32) x[n] = *reinterpret_cast<const float*>(at);
+          else if (FMT == AQ_BF16) x[n] = __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(at) << 16);
+          else x[n] = (float)bits_to_h(*reinterpret_cast<const uint16_t*>(at));
         }
-        for (int m = mask; m && at < n; m &= m - 1) s.list[at++] = (u64)cut << 32 | (uint32_t)~(base + __builtin_ctz(m));
-        c = min(c + all, n);
-        __syncthreads();
-      };
-      const int head = r.first ? r.lead : 0;
-      place(t < head && key_of(r.value(t)) == cut, t);
-      for (int p = r.p0; p < r.p1 && c < n; p += kThreads) {
-        int mask = 0;
-        if (p + t < r.p1) {
-          const uint4 w = r.pieces[p + t];
 #pragma unroll
-          for (int i = 0; i < T::E; i++) mask |= (key_of(T::get(w, i)) == cut) << i;
+        for (int n = 0; n < U; n++) {
+          const int piece = r.p0 + wave * 64 + src[n] + u * kThreads;
+          list(x[n], r.lead + piece * T::E + el, src[n] >= 0 && piece < r.p1);
         }
-        place(mask, r.lead + (p + t) * T::E);
       }
-      if (r.last && c < n) place(t < r.V - r.tail0 && key_of(r.value(min(r.tail0 + t, r.V - 1))) == cut, r.tail0 + t);
     }
+    __syncthreads();
+    if ((t & 63) == 0) s.count[wave] = k;
+    __syncthreads();
+    c = before = 0;
+    over = false;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      before += w < wave ? s.count[w] : 0;
+      c += s.count[w];
+      over |= s.count[w] > kList;
+    }
+    if (!over) break;
   }
-  if (c > kList) {  // a few lanes hold very many large ones: one by one
+  if (over) {  // a few lanes hold very many large ones: one by one
     u64 below = ~0ull;
+#pragma unroll 1
     for (c = 0; c < n; c++) {
       u64 best = 0;
-      r.each([&](float x, int i) {
+      each(s, r, there, [&](float x, int i, bool in) {
         const u64 e = entry_of(x, i);
-        if (e < below && e > best) best = e;
+        if (in && e < below && e > best) best = e;
       });
+#pragma unroll 1
       for (int d = 1; d < 64; d *= 2) best = max(best, (u64)__shfl_xor((unsigned long long)best, d, 64));
       __syncthreads();
       if ((t & 63) == 0) s.best[wave] = best;
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < kWaves; w++) best = max(best, s.best[w]);
-      if (t == 0) s.list[c] = best;
+      if (t == 0) s.top[c] = best;
       below = best;
     }
     __syncthreads();
     return c;
   }
-  // ranked by counting
-  u64 mineq[kList / kThreads];
-  int place[kList / kThreads];
+  // the waves' lists as one, where the pieces were; behind it zeros, which nothing is below
+  u64* list = reinterpret_cast<u64*>(s.held);
+  const int mine_n = s.count[wave];
+  for (int i = t & 63; i < mine_n; i += 64) list[before + i] = s.list[wave][i];
+  if (c < n) {
+    // the first ones at the cut, by index
+    const int head = r.first ? r.lead : 0;
+    auto place = [&](int mask, int base) {  // elements base + i of this thread for the bits i
+      const int k = __popc(mask);
+      const int inc = wave_incl_scan_i32<64>(k);
+      __syncthreads();
+      if ((t & 63) == 63) s.count[wave] = inc;
+      __syncthreads();
+      int to = c + inc - k, all = 0;
 #pragma unroll
-  for (int k = 0; k < kList / kThreads; k++) {
-    place[k] = kList;
-    if (t + k * kThreads < c) {
-      mineq[k] = s.list[t + k * kThreads];
-      int at = 0;
-      for (int i = 0; i < c; i++) at += s.list[i] > mineq[k];
-      place[k] = at;
+      for (int w = 0; w < kWaves; w++) {
+        to += w < wave ? s.count[w] : 0;
+        all += s.count[w];
+      }
+      for (int m = mask; m && to < n; m &= m - 1) list[to++] = (u64)cut << 32 | (uint32_t)~(base + __builtin_ctz(m));
+      c = min(c + all, n);
+    };
+    place(t < head && key_of(r.value(t)) == cut, t);
+#pragma unroll 1
+    for (int p = r.p0; p < r.p1 && c < n; p += kThreads) {
+      int mask = 0;
+      if (p + t < r.p1) {
+        const uint4 w = r.pieces[p + t];
+#pragma unroll
+        for (int i = 0; i < T::E; i++) mask |= (key_of(T::get(w, i)) == cut) << i;
+      }
+      place(mask, r.lead + (p + t) * T::E);
     }
+    if (r.last && c < n) place(t < r.V - r.tail0 && key_of(r.value(min(r.tail0 + t, r.V - 1))) == cut, r.tail0 + t);
   }
+  const int padded = (c + 31) & ~31;
+  if (t < padded - c) list[c + t] = 0;
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kList / kThreads; k++)
-    if (place[k] < n) s.list[place[k]] = mineq[k];
+#pragma unroll 1
+  for (int k = 0; k < c; k += kThreads / 4) {  // four lanes an element
+    const u64 e = list[min(k + t / 4, c - 1)];
+    const int at = count_above(list, padded, e);
+    if (at < n) s.top[at] = e;
+  }
   __syncthreads();
   return min(c, n);
 }
@@ -323,124 +414,135 @@ template <int FMT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   typedef Type<FMT> T;
   __shared__ Shared s;
-  const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x;
+  const int row = blockIdx.y, part = blockIdx.x, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Part<FMT> r(a, row, part);
-  const int64_t token64 = a.tokens[row];
+  // a thread's pieces, and its single element, are asked for at once
+  uint4 held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; u++) held[u] = r.p0 + t + u * kThreads < r.p1 ? r.pieces[r.p0 + t + u * kThreads] : T::none();
+  const float single = t < r.singles ? r.value(r.single(t)) : -INFINITY;
+  const int64_t token64 = scalar_token(a.tokens, row);
   const bool valid = token64 >= 0 && token64 < a.V;
   const int token = valid ? (int)token64 : 0;
-  const float own = fmaxf(r.value(token), -INFINITY);
+  const float own = fmaxf(r.scalar_value(token), -INFINITY);
   const float own_low = next_below(own);
   const int own_piece = token < r.lead ? -1 : (token - r.lead) / T::E;
 
-  Sums v = {kLow, 0.0f, 0.0f, 0};
-  float mine = -INFINITY;  // the largest as it is
-  auto add = [&](float x, bool before) {
-    mine = fmaxf(mine, x);
-    v.before += before;
-    x = fmaxf(x, kLow);
-    const float m = fmaxf(v.m, x), d = v.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-    const float w = __builtin_amdgcn_exp2f((x - m) * kLog2e);
-    v.e = fmaf(d, v.z, v.e) * f + w * (x - m);
-    v.z = v.z * f + w;
-    v.m = m;
+  // Exponents of 2: t = x log2(e) - m2, m2 about m log2(e), which every term shares, so
+  // that its rounding is put right at the end.  Counts are the wave's, by the
+  // scalar unit.
+  float m = kLow, m2 = kLow * kLog2e, mine = -INFINITY;  // mine: the largest as it is
+  Sums v = {0.0f, 0.0f, 0.0f, 0};
+  auto weigh = [&](float x) {
+    const float y = fmaxf(fmaf(x, kLog2e, -m2), -150.0f), w = __builtin_amdgcn_exp2f(y);  // NaN, -inf: 0
+    v.z += w;
+    v.e = fmaf(w, y, v.e);
   };
-  if (t < r.singles) {
-    const int i = r.single(t);
-    const float x = r.value(i);
-    add(x, x > own || (x == own && i < token));
+  auto raise = [&](float largest) {
+    mine = fmaxf(mine, largest);
+    m = fmaxf(m, largest);
+    const float n2 = m * kLog2e, d = m2 - n2, f = __builtin_amdgcn_exp2f(d);
+    v.e = fmaf(d, v.z, v.e) * f;
+    v.z *= f;
+    m2 = n2;
+  };
+  const bool there = r.p1 - r.p0 <= kHeld * kThreads;
+#pragma unroll
+  for (int u = 0; u < kHeld; u++) s.held[t + u * kThreads] = held[u];
+  if (wave == 0 && r.singles) {
+    raise(single);
+    if (t < r.singles) weigh(single);
+    v.before += __popcll(__ballot(t < r.singles && (single > own || (single == own && r.single(t) < token))));
   }
-  constexpr int U = 4;  // pieces in flight
-  for (int p = r.p0 + t; p < r.p1; p += U * kThreads) {
-    uint4 w[U];
+  auto add = [&](const uint4& w, int p) {
+    float x[T::E], largest = -INFINITY;
+    // before the token's piece, elements equal to it stand before it too
+    const float limit = p < own_piece ? own_low : own;
 #pragma unroll
-    for (int u = 0; u < U; u++) w[u] = p + u * kThreads < r.p1 ? r.pieces[p + u * kThreads] : T::none();
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      float x[T::E];
-      // before the token's piece, elements equal to it stand before it too
-      const float limit = p + u * kThreads < own_piece ? own_low : own;
-#pragma unroll
-      for (int i = 0; i < T::E; i++) {
-        x[i] = T::get(w[u], i);
-        mine = fmaxf(mine, x[i]);
-        x[i] = fmaxf(x[i], kLow);
-        v.before += x[i] > limit;
-      }
-      float m = v.m;
-#pragma unroll
-      for (int i = 0; i < T::E; i++) m = fmaxf(m, x[i]);
-      const float d = v.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-      v.e = fmaf(d, v.z, v.e) * f;
-      v.z *= f;
-      v.m = m;
-#pragma unroll
-      for (int i = 0; i < T::E; i++) {
-        const float y = x[i] - m, z = __builtin_amdgcn_exp2f(y * kLog2e);
-        v.z += z;
-        v.e = fmaf(z, y, v.e);
-      }
+    for (int i = 0; i < T::E; i++) {
+      x[i] = T::get(w, i);
+      largest = fmaxf(largest, x[i]);
     }
+    raise(largest);
+#pragma unroll
+    for (int i = 0; i < T::E; i++) {
+      weigh(x[i]);
+      v.before += __popcll(__ballot(x[i] > limit));
+    }
+  };
+#pragma unroll 1
+  for (int u = 0; u < kHeld && r.p0 + wave * 64 + u * kThreads < r.p1; u++) add(s.held[t + u * kThreads], r.p0 + t + u * kThreads);
+#pragma unroll 1
+  for (int p = r.p0 + wave * 64 + kHeld * kThreads; p < r.p1; p += kThreads) {
+    const int at = p + (t & 63);
+    add(at < r.p1 ? r.pieces[at] : T::none(), at);
   }
   // elements of the token's own piece that are equal to it and stand before it
-  if (own_piece >= r.p0 && own_piece < r.p1 && (own_piece - r.p0) % kThreads == t)
-    for (int i = r.lead + own_piece * T::E; i < token; i++) v.before += r.value(i) == own;
+  if (own_piece >= r.p0 && own_piece < r.p1 && (own_piece - r.p0) % kThreads / 64 == wave)
+    for (int i = r.lead + own_piece * T::E; i < token; i++) v.before += r.scalar_value(i) == own;
   const bool has = t < r.singles || r.p0 + t < r.p1;
-  v = block_join(s, v);
-  // (also where there is nothing: an empty part joins as one of -inf)
-  if (!(v.m > kLow && v.m < INFINITY) || !(own > kLow)) v = exact_sums(s, r, own, token);
-  const int c = a.top ? part_top(s, r, a.top, mine, has) : 0;
+  const float all = block_max(s, m);
+  if (!(all > kLow && all < kHigh) || !(own > kLow)) {  // (nothing at all, too: it counts as -inf)
+    v = exact_sums(s, r, there, own, token);
+  } else {
+    m = all;
+    const float n2 = m * kLog2e, d = m2 - n2, f = __builtin_amdgcn_exp2f(d);
+    v.e = fmaf(d, v.z, v.e) * f;
+    v.z *= f;
+    v = block_sum(s, v);
+    // from n2 to the maximum itself, which is off by the rounding of their product
+    const float off = fmaf(m, kLog2e, -n2), g = __builtin_amdgcn_exp2f(-off);
+    v.e = (v.e - off * v.z) * g * kLn2;
+    v.z *= g;
+    v.m = m;
+  }
+  const int c = a.top ? part_top(s, r, there, a.top, mine, has) : 0;
   if (a.parts == 1) {
     const float log_z = logf(v.z);
     write_row(a, row, v, own, valid, log_z);
-    if (t < c) write_top(a, row, t, s.list[t], v, log_z);
+    if (t < c) write_top(a, row, t, s.top[t], v, log_z);
     return;
   }
   const int64_t at = (int64_t)row * a.parts + part;
   if (t == 0) a.sums[at] = v;
-  if (t < a.top) a.lists[at * a.top + t] = t < c ? s.list[t] : 0;
+  if (t < a.top) a.lists[at * a.top + t] = t < c ? s.top[t] : 0;
 }
 
-// The parts of a row joined, a workgroup a row.
+// The parts of a row joined, a workgroup a row; lane p has the sums of part p.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void logprobs_merge_kernel(Args a) {
-  __shared__ u64 list[kMaxParts * kMaxTop];
-  const int row = blockIdx.x, t = threadIdx.x;
+  __shared__ __attribute__((aligned(16))) u64 list[kMaxParts * kMaxTop];
+  const int row = blockIdx.x, t = threadIdx.x, ln = t & 63;
   const int n = a.parts * a.top;
+  const Sums mine = a.sums[(int64_t)row * a.parts + min(ln, a.parts - 1)];
   for (int i = t; i < n; i += kThreads) list[i] = a.lists[(int64_t)row * n + i];
-  Sums v = a.sums[(int64_t)row * a.parts];
-  for (int p = 1; p < a.parts; p++) v = join(v, a.sums[(int64_t)row * a.parts + p]);
-  const float log_z = logf(v.z);
-  const int64_t token = a.tokens[row];
+  if (t < 32 && n + t < kMaxParts * kMaxTop) list[n + t] = 0;
+  const int64_t token = scalar_token(a.tokens, row);
   const bool valid = token >= 0 && token < a.V;
-  const uint8_t* x = a.logits + row * a.stride + (valid ? token : 0) * Type<FMT>::kSize;
-  float own = 0.0f;
-  if (FMT == AQ_F32)
-    own = *reinterpret_cast<const float*>(x);
-  else
-    own = FMT == AQ_BF16 ? __builtin_bit_cast(float, (uint32_t)*reinterpret_cast<const uint16_t*>(x) << 16)
-                         : (float)bits_to_h(*reinterpret_cast<const uint16_t*>(x));
-  write_row(a, row, v, fmaxf(own, -INFINITY), valid, log_z);
+  const float own = fmaxf(scalar_logit<FMT>(a.logits + row * a.stride, valid ? token : 0), -INFINITY);
+  Sums v = ln < a.parts ? mine : Sums{-INFINITY, 0.0f, 0.0f, 0};
+  const float m = wave_group_max_f32<64>(v.m), d = v.m == m ? 0.0f : v.m - m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+  v.e = wave_group_sum_f32<64>(f > 0.0f ? fmaf(d, v.z, v.e) * f : 0.0f);
+  v.z = wave_group_sum_f32<64>(v.z * f);
+  v.before = wave_sum_i32(v.before);
+  v.m = m;
+  const float log_z = logf(v.z);
+  write_row(a, row, v, own, valid, log_z);
   __syncthreads();
-  for (int i = t; i < n; i += kThreads) {
-    const u64 e = list[i];
-    if (!e) continue;
-    int at = 0;  // in each list, those before it
-    for (int p = 0; p < a.parts && at < a.top; p++) {
-      int lo = 0, hi = a.top;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (list[p * a.top + mid] > e) lo = mid + 1;
-        else hi = mid;
-      }
-      at += lo;
-    }
-    if (at < a.top) write_top(a, row, at, e, v, log_z);
+  const int padded = (n + 31) & ~31;
+#pragma unroll 1
+  for (int k = 0; k < n; k += kThreads / 4) {  // four lanes an entry
+    const u64 e = list[min(k + t / 4, n - 1)];
+    const int at = count_above(list, padded, e);
+    if (e && at < a.top && (t & 3) == 0 && k + t / 4 < n) write_top(a, row, at, e, v, log_z);
   }
 }
 
+// Parts whose pieces the threads can hold (up to 32 of 2048), and more for few rows: as
+// many as make 512 workgroups, of 512 pieces each at least.
 int parts_of(int64_t B, int64_t V, int dtype) {
   const int64_t pieces = V * (dtype == AQ_F32 ? 4 : 2) / 16;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / B, pieces / 512, kMaxParts}));
+  return (int)std::max<int64_t>({1, aq::ceil_div(pieces, kHeld * kThreads), std::min<int64_t>({512 / B, pieces / 512, kMaxParts})});
 }
 
 bool sizes_ok(int64_t B, int64_t V, int dtype, int64_t top) {
