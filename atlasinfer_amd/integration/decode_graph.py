@@ -52,13 +52,20 @@ Options (on the GPU path with an fp16 model):
   positions but not memory.  A model whose configuration has a sliding window
   shorter than ``max_len`` gets that window by itself; a window given here takes
   its place, for the prompt as for the steps.
+* ``page_size``: the cache is paged (``paged_cache``): prompts may differ in length,
+  go in packed, ``chunk`` rows at a time, and each sequence holds pages for its own
+  positions only, from a pool of ``pages`` a layer.  ``score`` gives the log
+  probabilities of given texts' tokens.
+* ``logprobs=n``: of every token that is chosen the log probability, rank, the
+  entropy it was chosen at and the n most likely tokens (``token_logprobs``), in
+  ``chosen``.
 
-Limits: equal-length prompts without padding (batch rows share ``pos``), no
-beam search.
+Limits: without ``page_size`` equal-length prompts without padding (batch rows share
+``pos``); no beam search.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import List, Optional, Sequence, Union
 
 import contextlib
 import ctypes
@@ -68,6 +75,9 @@ import torch.nn.functional as F
 
 from .. import _lib
 from ..memory.decode_cache import DecodeCache
+from ..memory.paged_cache import (PagedBatch, Rotary, paged_attention, paged_attention_workspace, paged_buffers,
+                                  paged_store)
+from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .sampling import sample_tokens
 from .window_attention import window_prompts
 
@@ -84,12 +94,16 @@ def _kind(model) -> str:
 class GraphDecoder:
     """Decode of ``model`` for ``batch`` sequences of up to ``max_len``
     positions (prompt + new tokens), one HIP graph replay per token: greedy, or
-    sampled with ``sampling=True``; ``kv_bits`` 16 or 4, ``window`` and ``sinks``:
-    the cache.  ``graph=False`` runs the same step eagerly (no capture), which is
-    also how it runs on a CPU."""
+    sampled with ``sampling=True``; ``kv_bits`` 16 or 4, ``window`` and ``sinks``,
+    ``page_size`` and ``pages`` (of a layer; None: enough for ``batch`` times
+    ``max_len``): the cache; ``logprobs``: alternatives kept of each token.
+    ``graph=False`` runs the same step eagerly (no capture), which is also how it
+    runs on a CPU."""
 
     def __init__(self, model, batch: int, max_len: int, graph: bool = True, *, kv_bits: int = 16,
-                 window: Optional[int] = None, sinks: int = 0, sampling: bool = False):
+                 window: Optional[int] = None, sinks: int = 0, sampling: bool = False,
+                 page_size: Optional[int] = None, pages: Optional[int] = None, chunk: int = 2048,
+                 logprobs: Optional[int] = None):
         self.model = model
         self.kind = _kind(model)
         cfg = model.config
@@ -125,7 +139,7 @@ class GraphDecoder:
         # on the GPU: the attention of a step in one HIP kernel
         # (aq_decode_attention), q/k/v and gate/up in one grouped launch each
         self.fused = (self.dev.type == "cuda" and self.dtype == torch.float16 and self.D in (64, 128)
-                      and self.H % self.Hkv == 0 and self.H // self.Hkv in (1, 2, 4, 8))
+                      and self.H % self.Hkv == 0 and (self.H // self.Hkv in (1, 2, 4, 8) or page_size is not None))
         if window is not None and (window < 1 or sinks < 0):
             raise ValueError(f"GraphDecoder: window {window}, {sinks} sinks")
         if window is None and sinks:
@@ -138,11 +152,23 @@ class GraphDecoder:
         self.sinks, self.kv_bits, self.sampling = sinks, kv_bits, sampling
         if kv_bits not in (4, 16):
             raise ValueError(f"GraphDecoder: kv_bits {kv_bits} (4 or 16)")
-        if not self.fused and (not self._own_prompt or kv_bits != 16 or sampling):
+        if not self.fused and (not self._own_prompt or kv_bits != 16 or sampling or page_size is not None
+                               or logprobs is not None):
             raise NotImplementedError("GraphDecoder: a sliding window shorter than max_len (asked for or configured), "
-                                      "kv_bits=4 and sampling need an fp16 model on a HIP device, head size 64 or 128")
+                                      "kv_bits=4, sampling, page_size and logprobs need an fp16 model on a HIP device, "
+                                      "head size 64 or 128")
+        if page_size is None and pages is not None:
+            raise ValueError("GraphDecoder: pages without a page_size")
+        if page_size is not None and kv_bits != 16:
+            raise ValueError("GraphDecoder: pages hold fp16 (kv_bits 16)")
+        if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, cfg.vocab_size):
+            raise ValueError(f"GraphDecoder: {logprobs} alternatives (0 .. {MAX_TOP})")
+        self.paged, self.logprobs = page_size is not None, logprobs
         self.caches = None
-        if self.window is not None or kv_bits != 16:
+        if self.paged:
+            self._page_state(page_size, pages, chunk)
+            self.k = self.v = None
+        elif self.window is not None or kv_bits != 16:
             slots, keep = (L, None) if self.window is None else (sinks + self.window, sinks)
             self.caches = [DecodeCache(B, self.Hkv, slots, self.D, bits=kv_bits, sinks=keep, device=dev)
                            for _ in self.layers]
@@ -156,7 +182,12 @@ class GraphDecoder:
             self._generator, self._fresh = None, False  # whose they are; whether a sequence has not used them yet
             self.settings = dict(temperature=torch.ones(B, device=dev), top_k=torch.zeros(B, dtype=torch.int32, device=dev),
                                  top_p=torch.ones(B, device=dev), min_p=torch.zeros(B, device=dev))
-        if self.kind == "llama":
+        if logprobs is not None:
+            f32, i64 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.long, device=dev)
+            # of the tokens in ``out``, at the same places
+            self.chosen = TokenLogprobs(torch.zeros(B, L, **f32), torch.zeros(B, L, **f32), torch.zeros(B, L, **i64),
+                                        torch.zeros(B, L, logprobs, **f32), torch.zeros(B, L, logprobs, **i64))
+        if self.kind == "llama" and not self.paged:
             rot = model.model.rotary_emb
             pos_ids = torch.arange(L, device=dev)[None]
             with torch.no_grad():
@@ -171,8 +202,12 @@ class GraphDecoder:
             # the attention kernel's per-span partial results: one workspace
             # for every layer (the layers' calls follow each other on one
             # stream)
-            nb = (self._lib.aq_decode_attention_workspace(B, self.H, self.Hkv, self.D, L) if self.caches is None
-                  else self.caches[0].workspace_bytes(self.H))
+            if self.paged:
+                nb = paged_attention_workspace(B, self.H, self.Hkv, self.D, self._steps)
+            elif self.caches is not None:
+                nb = self.caches[0].workspace_bytes(self.H)
+            else:
+                nb = self._lib.aq_decode_attention_workspace(B, self.H, self.Hkv, self.D, L)
             if nb < 0:
                 raise ValueError("aq_decode_attention_workspace refused these sizes")
             self.ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)
@@ -183,13 +218,156 @@ class GraphDecoder:
         self.b1 = self.folded and B == 1
         self.bm = self.folded and B > 1
 
+    # ------------------------------------------------------------ pages
+
+    def _page_state(self, page_size: int, pages: Optional[int], chunk: int) -> None:
+        """The pool of pages, the table of the sequences' and the batch of a step."""
+        B, dev = self.B, self.dev
+        width = -(-self.L // page_size)
+        if pages is None:
+            pages = B * width
+        if not 0 < chunk <= 65535:
+            raise ValueError(f"GraphDecoder: chunks of {chunk} rows (1 .. 65535)")
+        self.page_size, self.pages, self.chunk = page_size, pages, chunk
+        self.caches = [paged_buffers(pages, self.Hkv, page_size, self.D, self.dtype, dev) for _ in self.layers]
+        self._rotary = None
+        if self.kind == "llama":
+            rot = self.model.model.rotary_emb
+            kind = getattr(rot, "rope_type", "default")
+            if kind not in ("default", "linear", "llama3", "yarn"):  # others change with the length
+                raise NotImplementedError(f"GraphDecoder: page_size with rotary positions of type {kind!r}")
+            self._rotary = Rotary(rot.inv_freq.detach().float().to(dev).contiguous(), False,
+                                float(getattr(rot, "attention_scaling", 1.0)))
+        # positions of each sequence, the step's token included: page 0 until a prompt has come
+        self.lengths = torch.ones(B, dtype=torch.int32, device=dev)
+        self.table = torch.zeros(B, width, dtype=torch.int32, device=dev)
+        self.pos = torch.zeros(B, dtype=torch.long, device=dev)
+        self._steps = PagedBatch(torch.arange(B + 1, dtype=torch.int32, device=dev), self.lengths, self.table, 1, self.L)
+        self._release()
+
+    def _release(self) -> None:
+        """Every page back to the pool."""
+        self._free = list(range(self.pages - 1, -1, -1))
+        self._held: List[List[int]] = [[] for _ in range(self.B)]
+        self._len = [0] * self.B
+
+    def _device(self, values, dtype) -> torch.Tensor:
+        """Host numbers on the device without waiting for it (each copy from page-locked memory of its own)."""
+        return torch.tensor(values, dtype=dtype, pin_memory=True).to(self.dev, non_blocking=True)
+
+    def _reserve(self, lengths: Sequence[int], ahead: int = 0) -> None:
+        """Pages for the first lengths[b] positions of every sequence, and where one
+        is short, as far as the pool reaches, for ``ahead`` more of each."""
+        P = self.page_size
+        need = [-(-n // P) for n in lengths]
+        if all(len(h) >= n for h, n in zip(self._held, need)):
+            return
+        if sum(max(0, n - len(h)) for h, n in zip(self._held, need)) > len(self._free):
+            raise RuntimeError(f"GraphDecoder: {self.pages} pages of {P} positions are too few")
+        for wanted in (need, [-(-min(n + ahead, self.L) // P) for n in lengths]):
+            for h, n in zip(self._held, wanted):
+                while len(h) < n and self._free:
+                    h.append(self._free.pop())
+        width = self.table.shape[1]
+        self.table.copy_(self._device([h + [0] * (width - len(h)) for h in self._held], torch.int32))
+
+    def _passes(self, counts: Sequence[int]):
+        """The prompts' rows, ``chunk`` at a time in the sequences' order: the new
+        rows of every sequence in each pass."""
+        done = [0] * self.B
+        while done != list(counts):
+            room, news = self.chunk, [0] * self.B
+            for b, n in enumerate(counts):
+                news[b] = min(n - done[b], room)
+                room -= news[b]
+            yield list(done), news
+            done = [d + n for d, n in zip(done, news)]
+
+    def _rows(self, prompts, done, news):
+        """A pass through the layers: the final norm's output [rows, hidden] of
+        ``news`` tokens of every prompt after the first ``done``, their keys and
+        values in the pages."""
+        m, dev = self.model, self.dev
+        starts = [0]
+        for n in news:
+            starts.append(starts[-1] + n)
+        # sequences without rows take no part (their lengths may be 0)
+        batch = PagedBatch(self._device(starts, torch.int32),
+                           self._device([d + n for d, n in zip(done, news)], torch.int32), self.table, max(news),
+                           max(d + n for d, n in zip(done, news)))
+        tokens = torch.cat([p[d:d + n] for p, d, n in zip(prompts, done, news) if n])
+        if self.kind == "opt":
+            dec = m.model.decoder
+            at = torch.cat([torch.arange(d, d + n, device=dev) for d, n in zip(done, news) if n])
+            x = dec.embed_tokens(tokens) + dec.embed_positions.weight.index_select(0, at + 2)
+            final = dec.final_layer_norm
+        else:
+            x, final = m.model.embed_tokens(tokens), m.model.norm
+        x, delta = x.contiguous(), None
+        for li, layer in enumerate(self.layers):
+            x, delta = self._layer_fused(li, layer, x, delta, batch)
+        return self._addnorm(x, delta, final)
+
+    def _prompts(self, input_ids) -> List[torch.Tensor]:
+        """The prompts as 1-D tensors on the device, checked."""
+        prompts = [torch.as_tensor(p).to(self.dev, torch.long) for p in input_ids]
+        if len(prompts) != self.B or any(p.dim() != 1 or p.numel() == 0 or p.numel() >= self.L for p in prompts):
+            raise ValueError(f"prefill: {len(prompts)} prompts of {[tuple(p.shape) for p in prompts][:8]} tokens "
+                             f"(decoder built for {self.B} of 1 to {self.L - 1})")
+        return prompts
+
+    @torch.no_grad()
+    def score(self, texts: Sequence[torch.Tensor], top: int = 0) -> List[TokenLogprobs]:
+        """Of each text (1-D tokens, 1 .. max_len of them, any number of texts) the log
+        probabilities of its tokens from the second on, each given those before it, with
+        ranks, entropies and the ``top`` most likely tokens in its place.  The decoder's
+        sequences are given up."""
+        if not self.paged:
+            raise NotImplementedError("GraphDecoder.score needs page_size")
+        texts = [torch.as_tensor(p).to(self.dev, torch.long) for p in texts]
+        if any(p.dim() != 1 or not 0 < p.numel() <= self.L for p in texts):
+            raise ValueError(f"score: texts of 1 to {self.L} tokens each")
+        self._end()
+        out = []
+        for lo in range(0, len(texts), self.B):
+            group = texts[lo:lo + self.B]
+            group = group + [group[0][:0]] * (self.B - len(group))
+            self._release()
+            self._reserve([p.numel() for p in group])
+            found = [[] for _ in group]
+            for done, news in self._passes([p.numel() for p in group]):
+                x = self._rows(group, done, news)
+                # a row's target is the next token; a text's last row has none
+                target = torch.cat([F.pad(p[d + 1:d + n + 1], (0, max(0, d + n + 1 - p.numel())), value=-1)
+                                    for p, d, n in zip(group, done, news) if n])
+                got = token_logprobs(self.model.lm_head(x), target, top)
+                at = 0
+                for b, (p, d, n) in enumerate(zip(group, done, news)):
+                    keep = n - (d + n == p.numel() and n > 0)
+                    found[b].append([t[at:at + keep] for t in got])
+                    at += n
+            out += [TokenLogprobs(*(torch.cat(t) for t in zip(*f))) for f, p in zip(found, group) if p.numel()]
+        self._release()
+        return out
+
+    def _end(self) -> None:
+        """No sequence is being decoded: a step is refused until the next prompt."""
+        self.S, self._n = self.L, 0
+
     # ------------------------------------------------------------ one step
 
-    def _attend_fused(self, li: int, q, k, v, scale: float, q_scale: float, rope: bool):
+    def _attend_fused(self, li: int, q, k, v, scale: float, q_scale: float, rope: bool, batch=None):
         """aq_decode_attention: q [B, H, D] scaled by q_scale (rounded to
         fp16) and, with ``rope``, q and the new key k [B, Hkv, D] rotated at
         pos; k, v written at pos; attention over positions 0..pos."""
         B, H, Hkv, D = self.B, self.H, self.Hkv, self.D
+        if self.paged:  # the rows of ``batch``, or a step
+            ws = self.ws if batch is None else None
+            batch = self._steps if batch is None else batch
+            turned = paged_store(k, v, self.caches[li], batch, q=q if rope else None, rope=self._rotary if rope else None)
+            o = paged_attention(turned if rope else q, self.caches[li], batch, scale=scale * q_scale, window=self.window,
+                                sinks=self.sinks if self.window is not None else 0, workspace=ws)
+            return o.view(-1, H * D)
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         if self.caches is not None:
             return self.caches[li].attend(q, k, v, self.pos, scale=scale, q_scale=q_scale,
@@ -337,24 +515,25 @@ class GraphDecoder:
         g, u = self._normed([mlp.gate_proj, mlp.up_proj], x1, layer.post_attention_layernorm)
         return self._qdec([mlp.down_proj], g, u=u, res=[x1])[0]
 
-    def _layer_fused(self, li, layer, x, delta):
-        """One layer on the GPU path: the residual stream x [B, hidden] is
+    def _layer_fused(self, li, layer, x, delta, batch=None):
+        """One layer on the GPU path: the residual stream x [B, hidden] (or the
+        packed rows of ``batch``) is
         updated in place by the norm launches (x += the previous layer's
         output delta, then x += this layer's attention output); returns x
         and the MLP output, which the next norm adds."""
-        B, H, Hkv, D = self.B, self.H, self.Hkv, self.D
+        B, H, Hkv, D = x.shape[0], self.H, self.Hkv, self.D
         at = layer.self_attn
         if self.kind == "opt":
             h = self._addnorm(x, delta, layer.self_attn_layer_norm)
             q, k, v = self._linears([at.q_proj, at.k_proj, at.v_proj], h)
             o = self._attend_fused(li, q.view(B, H, D), k.view(B, Hkv, D), v.view(B, Hkv, D), 1.0, at.scaling,
-                                   rope=False)
+                                   rope=False, batch=batch)
             h = self._addnorm(x, at.out_proj(o), layer.final_layer_norm)
             return x, layer.fc2(layer.activation_fn(layer.fc1(h)))
         h = self._addnorm(x, delta, layer.input_layernorm)
         q, k, v = self._linears([at.q_proj, at.k_proj, at.v_proj], h)
         o = self._attend_fused(li, q.view(B, H, D), k.view(B, Hkv, D), v.view(B, Hkv, D), at.scaling, 1.0,
-                               rope=True)
+                               rope=True, batch=batch)
         h = self._addnorm(x, at.o_proj(o), layer.post_attention_layernorm)
         g, u = self._linears([layer.mlp.gate_proj, layer.mlp.up_proj], h)
         return x, layer.mlp.down_proj(self._silu_mul(layer.mlp.act_fn, g, u))
@@ -458,15 +637,22 @@ class GraphDecoder:
         self.tok.copy_(nxt)
         self.out.index_copy_(1, self.slot, nxt.view(self.B, 1))
         self.pos.add_(1)
+        if self.paged:
+            self.lengths.add_(1)
         self.slot.add_(1)
         return logits
 
     def _choose(self, logits, slot):
         """The next tokens: the largest logits', or sampled with the random
         numbers of output slot ``slot`` (device int64 [1])."""
-        if not self.sampling:
-            return self._argmax(logits)
-        return sample_tokens(logits, self.u.index_select(0, slot).view(self.B), **self.settings)
+        if self.sampling:
+            nxt = sample_tokens(logits, self.u.index_select(0, slot).view(self.B), **self.settings)
+        else:
+            nxt = self._argmax(logits)
+        if self.logprobs is not None:
+            for kept, new in zip(self.chosen, token_logprobs(logits, nxt, self.logprobs)):
+                kept.index_copy_(1, slot, new.unsqueeze(1))
+        return nxt
 
     def set_sampling(self, temperature=None, top_k=None, top_p=None, min_p=None, generator=None) -> None:
         """New settings (a number, or one per sequence; None: as they are; at first
@@ -519,18 +705,63 @@ class GraphDecoder:
         self.captured = True
 
     @torch.no_grad()
-    def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
-        """Run the prompt [B, S] through the model's own forward, fill the
-        static cache and set tok / pos / slot; returns the first new token."""
-        B, S = input_ids.shape
-        if B != self.B or S >= self.L:
-            raise ValueError(f"prefill: batch {B} (decoder built for {self.B}), prompt {S} (cache {self.L})")
+    def prefill(self, input_ids: Union[torch.Tensor, Sequence[torch.Tensor]]) -> torch.Tensor:
+        """Run the prompts [B, S] (with ``page_size`` also B 1-D tensors of any
+        lengths) through the model, fill the cache and set tok / pos / slot; returns
+        the first new tokens."""
+        if self.paged:
+            prompts = self._prompts(input_ids)
+            S = max(p.numel() for p in prompts)
+        else:
+            B, S = input_ids.shape
+            if B != self.B or S >= self.L:
+                raise ValueError(f"prefill: batch {B} (decoder built for {self.B}), prompt {S} (cache {self.L})")
         if self.use_graph and not self.captured:
             self._capture()
         if self.sampling:
             if not self._fresh:
                 self._draw()
             self._fresh = False
+        if self.paged:
+            logits = self._paged_prefill(prompts)
+        else:
+            logits = self._own_prefill(input_ids)
+            self.pos.fill_(S)
+        self.slot.zero_()
+        first = self._choose(logits, self.slot)
+        self.tok.copy_(first)
+        self.out.zero_()
+        self.out[:, 0].copy_(first)
+        self.slot.fill_(1)
+        self.S, self._n = S, 0
+        return first
+
+    def _paged_prefill(self, prompts):
+        """The prompts in, packed; the logits of their last rows [B, V]."""
+        counts = [p.numel() for p in prompts]
+        self._end()
+        self._release()
+        self._reserve(counts)
+        last = None
+        for done, news in self._passes(counts):
+            x = self._rows(prompts, done, news)
+            if last is None:
+                last = x.new_empty(self.B, x.shape[1])
+            at = 0
+            for b, n in enumerate(news):
+                at += n
+                if n and done[b] + n == counts[b]:
+                    last[b] = x[at - 1]
+        self._len = counts
+        n = self._device(counts, torch.long)
+        self.pos.copy_(n)
+        self.lengths.copy_(n + 1)
+        return self.model.lm_head(last)
+
+    def _own_prefill(self, input_ids):
+        """The prompts through the model's own forward, their keys and values into the
+        static cache; the last position's logits."""
+        S = input_ids.shape[1]
         from transformers import DynamicCache
         cache = DynamicCache()
         with contextlib.nullcontext() if self._own_prompt else window_prompts(self.model, self.window, self.sinks):
@@ -542,15 +773,7 @@ class GraphDecoder:
                 continue
             self.k[li][:, :, :S].copy_(kl)
             self.v[li][:, :, :S].copy_(vl)
-        self.slot.zero_()
-        first = self._choose(out.logits[:, -1], self.slot)
-        self.tok.copy_(first)
-        self.out.zero_()
-        self.out[:, 0].copy_(first)
-        self.pos.fill_(S)
-        self.slot.fill_(1)
-        self.S, self._n = S, 0
-        return first
+        return out.logits[:, -1]
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
@@ -561,6 +784,8 @@ class GraphDecoder:
         # output at slot 1 + n, both below L
         if self.S + self._n >= self.L:
             raise RuntimeError(f"GraphDecoder: cache of {self.L} positions is full")
+        if self.paged:  # pages that the step writes, and some more, so that most steps need none
+            self._reserve([n + self._n + 1 for n in self._len], ahead=4 * self.page_size)
         self._n += 1
         self._fresh = False
         if self.use_graph:
@@ -570,12 +795,15 @@ class GraphDecoder:
         return self.logits
 
     @torch.no_grad()
-    def generate(self, input_ids: torch.Tensor, max_new_tokens: int, **sampling) -> torch.Tensor:
-        """Prompt + ``max_new_tokens`` tokens, [B, S + max_new_tokens]: greedy, or
-        of a decoder built with ``sampling=True`` sampled with fresh random numbers,
-        ``sampling`` being set_sampling's arguments (without ``generator`` the last
-        one's goes on)."""
-        S = input_ids.shape[1]
+    def generate(self, input_ids: Union[torch.Tensor, Sequence[torch.Tensor]], max_new_tokens: int, **sampling):
+        """Prompt + ``max_new_tokens`` tokens, [B, S + max_new_tokens] (of prompts given
+        as a list, with ``page_size``, a list): greedy, or of a decoder built with
+        ``sampling=True`` sampled with fresh random numbers, ``sampling`` being
+        set_sampling's arguments (without ``generator`` the last one's goes on)."""
+        several = not isinstance(input_ids, torch.Tensor)
+        if several and not self.paged:
+            raise ValueError("generate: prompts of several lengths need page_size")
+        S = max((len(p) for p in input_ids), default=0) if several else input_ids.shape[1]
         if S + max_new_tokens > self.L:
             raise ValueError(f"generate: {S} + {max_new_tokens} positions exceed the cache ({self.L})")
         if self.sampling:
@@ -585,4 +813,7 @@ class GraphDecoder:
         self.prefill(input_ids)
         for _ in range(max_new_tokens - 1):
             self.step()
-        return torch.cat([input_ids.to(self.dev), self.out[:, :max_new_tokens]], dim=1)
+        new = self.out[:, :max_new_tokens]
+        if several:
+            return [torch.cat([torch.as_tensor(p).to(self.dev, torch.long), n]) for p, n in zip(input_ids, new)]
+        return torch.cat([input_ids.to(self.dev), new], dim=1)
