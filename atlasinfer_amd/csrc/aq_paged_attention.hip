@@ -121,13 +121,17 @@ __device__ __forceinline__ int find_sequence(const AttendArgs& a, int blk, int l
   return -1;
 }
 
-// A tile's rows lie in LDS one after the other, 16-byte pieces permuted within
-// each so that the reads below meet every bank equally: piece c of key r at place
-// c ^ (r & 7) of a key row, pairs of pieces c / 2 at (c / 2) ^ (r & 3) of a value row.
+// A tile's rows lie in LDS one after the other, 16-byte pieces permuted within each
+// so that the reads below meet every bank equally.  Keys, 16 rows at once: piece c of
+// row r at c ^ (r & 15), for D = 64, where two rows fill the banks, c ^ (r / 2 & 7).
+// Values, 64 bytes of 4 rows at once: pairs of pieces at (c / 2) ^ 2 (r & 3), for
+// D = 64 (c / 2) ^ 2 (r / 2 & 1).
 template <int D>
-__device__ __forceinline__ int k_place(int r, int c) { return r * (D * 2) + (c ^ (r & 7)) * 16; }
+__device__ __forceinline__ int k_place(int r, int c) { return r * (D * 2) + (c ^ (D == 128 ? r & 15 : (r >> 1) & 7)) * 16; }
 template <int D>
-__device__ __forceinline__ int v_place(int r, int c) { return r * (D * 2) + ((((c >> 1) ^ (r & 3)) << 1) | (c & 1)) * 16; }
+__device__ __forceinline__ int v_place(int r, int c) {
+  return r * (D * 2) + ((((c >> 1) ^ (2 * (D == 128 ? r & 3 : (r >> 1) & 1))) << 1) | (c & 1)) * 16;
+}
 
 // The same for the values of the kernel for few rows, whose lanes read 16 rows at
 // once: pairs of pieces at (c / 2) ^ (r & 7), or ^ (r / 2 & 3) where two rows fill the banks.
@@ -138,22 +142,30 @@ __device__ __forceinline__ int few_place(int r, int c) {
 
 // One workgroup: 128 rows of a key/value head, 32 a wave; tiles of 64 keys and
 // values go straight from their pages to LDS (a wave loads 16 rows of each, which
-// lie in one page).
-//   scores   transposed, s^T = k q^T (mfma 32 x 32 x 16): a lane has 32 scores of
-//            one row, another lane the other 32
+// lie in one page), and are taken in halves of 32 keys:
+//   scores   transposed, s^T = k q^T (mfma 32 x 32 x 16): a lane has 16 scores of
+//            one row, another lane the other 16
 //   softmax  p = e^(s - m) with m the maximum when it last moved: it moves only
 //            when a score passes it by 2^8, which spares scaling the sums nearly always
 //   values   o^T = v^T p^T: the numerators, rounded to 16 bits, are the operand as
 //            they are; the values come out of their rows transposed
 //   sums     of the rounded numerators, so that rounding them does not shift the mean
+// The products of the next half's scores stand beside the exponentials of this one's
+// in the code, so that the matrix unit works under them: one after the other (and
+// waves of two workgroups on a SIMD hardly filled the gaps: matrix unit 41 % and
+// vector unit 48 % busy) a prompt of 8192, 32 heads of 128, took 614 us.
+// Keys are a half ahead of values, so they have buffers and barriers of their own:
+//   E(i), before tile i's first half: everyone is done with the values of tile i - 1,
+//         those of i + 1 are asked for; those of i are there
+//   M(i), before its second half: everyone is done with the keys of tile i, those of
+//         i + 2 are asked for; those of i + 1 are there
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   constexpr int NC = D / 8;                    // 16-byte pieces of a row
   constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
   constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave: 16 rows
-  constexpr int NS = D == 64 ? 4 : 2;          // stages: 64 KiB
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * 2 * TB];  // keys and values of each stage
-  __shared__ int bad[NS];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys of even and odd tiles, values
+  __shared__ int bad[2];
   const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // runs of neighbouring items to an XCD (they share keys and values in its L2)
@@ -168,11 +180,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   if (!find_block<kK>(a, seq, (blk - blk0) * kQ, kQ, B) || B.n * a.G <= a.few) return;
   const int t0 = (int)blockIdx.y * a.span, t1 = min(t0 + a.span, B.tiles);
   if (t0 >= t1) return;
-  // cleared before any wave may set one, which is before the loop's first barrier
-  if (t < NS) bad[t] = 0;
+  // cleared before any wave may set one, which is before the first barrier below
+  if (t < 2) bad[t] = -1;
   __syncthreads();
-  const int lo = B.lo, hi = B.hi, sink_end = B.sink_end;
-  auto tile_at = [&](int i) { return i < B.na ? i : B.b0 + i - B.na; };
+  const int lo = B.lo, hi = B.hi;
+  auto tile_at = [&](int i) { return (i < B.na ? i : B.b0 + i - B.na) * kK; };
 
   const int row = B.r0 + wave * 32 + c, last_row = B.n * a.G - 1;  // this lane's row
   const int tok = min(row, last_row) / a.G, head = j * a.G + (min(row, last_row) - tok * a.G);
@@ -204,72 +216,58 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
 #pragma unroll
   for (int n = 0; n < PN; n++) {
     const int r = n * (64 / NC) + ln / NC, pc = ln % NC;
-    ko[n] = r * (D * 2) + (pc ^ (r & 7)) * 16;
-    vo[n] = r * (D * 2) + ((((pc >> 1) ^ (r & 3)) << 1) | (pc & 1)) * 16;
+    ko[n] = k_place<D>(r, pc);  // (the places are their own inverse)
+    vo[n] = v_place<D>(r, pc);
   }
   const int* table = a.b.table + (int64_t)seq * a.b.W;
   const int last_page = (B.len - 1) >> a.b.shift;
-  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i, read a tile ahead (rows past the last: any)
-    const int k0 = tile_at(min(i, t1 - 1)) * kK + wave * 16;
-    return scalar_int(table, min(k0 >> a.b.shift, last_page));
+  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i (past the last: any)
+    return scalar_int(table, min((tile_at(min(i, t1 - 1)) + wave * 16) >> a.b.shift, last_page));
   };
-  int next_page = page_at(t0);
-  auto load = [&](int i) {
-    const int k0 = tile_at(i) * kK + wave * 16;
-    const uint32_t st = lds_offset(lds) + (i & (NS - 1)) * (2 * TB) + wave * PN * 1024;
+  auto load = [&](const uint16_t* base, int i, int page, uint32_t dst, const int (&off)[PN]) {
+    const int k0 = tile_at(i) + wave * 16;
     // rows past the last, and those of a page outside the cache, read as zeros
-    const int page = next_page;
     const bool there = (unsigned)page < (unsigned)a.b.pages;
     // (a median is taken by the vector unit)
     const int bytes = there ? __builtin_amdgcn_readfirstlane(max(min(B.len - k0, 16), 0)) * (D * 2) : 0;
     const int64_t at = (((((int64_t)(there ? page : 0) * a.Hkv + j) << a.b.shift) + (k0 & ((1 << a.b.shift) - 1)))) * D;
-    load_to_lds<PN>(buffer_of(a.k + at, bytes), st, ko);
-    load_to_lds<PN>(buffer_of(a.v + at, bytes), st + TB, vo);
-    next_page = page_at(i + 1);
+    load_to_lds<PN>(buffer_of(base + at, bytes), dst + (i & 1) * TB + wave * PN * 1024, off);
   };
-  // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h (e & 3;
-  // e + 4 lies 128 bytes on); values of keys 4 h + r, 16 elements of 32 e (e & 1)
-  int kf[4], vf[2];
+  const uint32_t k_lds = lds_offset(lds), v_lds = k_lds + 2 * TB;
+  // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h; values of
+  // keys 4 h + r, 16 elements of 32 e
+  int kf[D / 16], vf[D / 32];
 #pragma unroll
-  for (int e = 0; e < 4; e++) kf[e] = k_place<D>(c, 2 * e + h);
+  for (int e = 0; e < D / 16; e++) kf[e] = k_place<D>(c, 2 * e + h);
   const int r4 = (ln >> 2) & 3;
 #pragma unroll
-  for (int e = 0; e < 2; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
+  for (int e = 0; e < D / 32; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
 
-  for (int i = t0; i < min(t0 + NS - 1, t1); i++) load(i);
-  for (int i = t0; i < t1; i++) {
-    const int k0 = tile_at(i) * kK;
-    const uint8_t* st = lds + (i & (NS - 1)) * (2 * TB);
-    // this wave's part of the tile is there; the NS - 2 tiles after it may be on their way
-    if (i + NS - 2 < t1)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * 2 * PN) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool cut = !(k0 + kK - 1 <= lo && k0 > hi - a.window);
-    if (cut) {
-      // a tile that the mask cuts for some row: whether its values are finite
-      u16x2 x = 0;
+  // Fragments of half y of tile i: its keys, its values (16 s + 4 h + 0 .. 3, then 8 on:
+  // the order in which a lane has the numerators).
+  u32x4 kr[D / 16];
+  u32x2 vr[D / 32][2];
+  auto read_keys = [&](int i, int y) {
+    const uint8_t* st = lds + (i & 1) * TB + y * 32 * (D * 2);
 #pragma unroll
-      for (int n = 0; n < PN; n++) x = magnitudes8(x, *reinterpret_cast<const uint4*>(st + TB + (wave * PN + n) * 1024 + ln * 16));
-      if (__ballot(max(x.x, x.y) >= T::kInf) && ln == 0) bad[i & (NS - 1)] = i + 1;
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's part; the tile before is done with
-    if (i + NS - 1 < t1) load(i + NS - 1);
-    // whether this wave's rows see none, all or some of the tile
-    if (k0 > whi || (k0 + kK - 1 <= wlo - a.window && k0 >= sink_end)) continue;
-    const bool all = k0 + kK - 1 <= wlo && k0 > whi - a.window;
-    float16v x[2];
+    for (int e = 0; e < D / 16; e++) kr[e] = *reinterpret_cast<const u32x4*>(st + kf[e]);
+  };
+  auto read_values = [&](int i, int y, int s) {
+    const uint8_t* st = lds + 2 * TB + (i & 1) * TB + (32 * y + 16 * s) * (D * 2);
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
+    for (int e = 0; e < D / 32; e++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) x[s][e] = 0.0f;
+      for (int n = 0; n < 2; n++) vr[e][n] = read_turned(st + vf[e] + 8 * n * (D * 2));
+  };
+  auto products = [&](float16v& x) {
 #pragma unroll
-      for (int e = 0; e < D / 16; e++) {
-        const u32x4 f = *reinterpret_cast<const u32x4*>(st + kf[e & 3] + (e >> 2) * 128 + s * 32 * (D * 2));
-        x[s] = T::mfma32(f, qv[e], x[s]);
-      }
-    }
-    if (!all) {
+    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; e++) x = T::mfma32(kr[e], qv[e], x);
+  };
+  // what the mask leaves of scores from key k0 on, and the maximum moved where they pass it
+  auto settle = [&](int k0, float16v& x) {
+    if (!(k0 + 31 <= wlo && k0 > whi - a.window)) {
       // a key is seen when it lies in one of two ranges: near the row's position,
       // or among the sinks, both up to that position (each a subtraction, an
       // unsigned comparison and a selection)
@@ -277,28 +275,17 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
       const int sink0 = -k0 - 4 * h;
       const uint32_t near_n = (uint32_t)max(last - from + 1, 0);
       const uint32_t sink_n = (uint32_t)max(min(a.sinks, last - sink0 + 1), 0);
-      if (k0 < sink_end) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
-            const float y = (uint32_t)(key - sink0) < sink_n ? x[s][e] : -INFINITY;
-            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : y;
-          }
-      } else {
-#pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) {
-            const int key = 32 * s + 8 * (e >> 2) + (e & 3);
-            x[s][e] = (uint32_t)(key - from) < near_n ? x[s][e] : -INFINITY;
-          }
+      for (int e = 0; e < 16; e++) {
+        const int key = 8 * (e >> 2) + (e & 3);
+        const float y = (uint32_t)(key - sink0) < sink_n ? x[e] : -INFINITY;
+        x[e] = (uint32_t)(key - from) < near_n ? x[e] : y;
       }
     }
-    float mx = fmaxf(x[0][0], x[1][0]);
+    float mx = x[0];
 #pragma unroll
-    for (int e = 1; e < 16; e++) mx = fmaxf(fmaxf(mx, x[0][e]), x[1][e]);  // v_max3
+    for (int e = 1; e < 15; e += 2) mx = fmaxf(fmaxf(mx, x[e]), x[e + 1]);  // v_max3
+    mx = fmaxf(mx, x[15]);
     if (__ballot(mx > m + grow)) {
       mx = xlane_level_max_f32<6>(mx);  // both lanes of a row move alike
       const float n = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - n) * a.c);
@@ -307,53 +294,119 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
       for (int e = 0; e < D / 32; e++) o[e] *= f;
       m = n;
     }
+  };
+  // numerators of scores x: p[4 n .. 4 n + 3] are the operand of 16 keys
+  auto numerators = [&](const float16v& x, u32x8& p) {
     const float base = m == -INFINITY ? 0.0f : -m * a.c;
-    uint32_t p[16];  // the numerators in pairs: p[4 n .. 4 n + 3] are the operand of 16 keys
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      const int y = 2 * e & 15;
-      p[e] = T::pack(__builtin_amdgcn_exp2f(fmaf(x[e >> 3][y], a.c, base)),
-                     __builtin_amdgcn_exp2f(fmaf(x[e >> 3][y + 1], a.c, base)));
+    for (int e = 0; e < 8; e++) {
+      p[e] = T::pack(__builtin_amdgcn_exp2f(fmaf(x[2 * e], a.c, base)), __builtin_amdgcn_exp2f(fmaf(x[2 * e + 1], a.c, base)));
       l = T::add2(p[e], l);
     }
-    if (!all && bad[i & (NS - 1)] == i + 1) {
-      // an infinity or NaN among the values of a tile that the mask cuts: the
-      // terms one by one, leaving out those of keys that the row does not see
-      // (the sums pass an empty asm here, so that what the compiler does for this
-      // loop's sake, copying them, it does here and not on the common path)
+  };
+  auto sums = [&](int s, const u32x8& p) {
 #pragma unroll
-      for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
-      int from = max(qpos - a.window + 1, 0) - k0, sink0 = -k0;
-      uint32_t near_n = (uint32_t)max(qpos - k0 - from + 1, 0), sink_n = (uint32_t)max(min(a.sinks, qpos + 1), 0);
-      asm volatile("" : "+v"(from), "+v"(sink0), "+v"(near_n), "+v"(sink_n));
+    for (int e = 0; e < D / 32; e++)
+      o[e] = T::mfma32(u32x4{vr[e][0].x, vr[e][0].y, vr[e][1].x, vr[e][1].y},
+                       u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}, o[e]);
+  };
+  // The same where an infinity or NaN is among the values of a tile that the mask cuts:
+  // the terms one by one, leaving out those of keys that the row does not see.
+  auto careful_sums = [&](int i, int y, const u32x8& p) {
+    // (the sums pass an empty asm here, so that what the compiler does for this
+    // loop's sake, copying them, it does here and not on the common path)
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
+    const uint8_t* st = lds + 2 * TB + (i & 1) * TB;
+    const int k0 = tile_at(i) + y * 32;
 #pragma unroll 1
-      for (int key = 0; key < kK; key++) {
-        const int y = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
-        uint32_t w = p[0];
+    for (int key = 0; key < 32; key++) {
+      const int z = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
+      const uint32_t w = p[n];
+      const int at = k0 + key;
+      const bool seen = at <= qpos && (at > qpos - a.window || at < a.sinks);
+      const float wf = __shfl(T::to_f32((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * z, 64);
 #pragma unroll
-        for (int e = 1; e < 16; e++) w = e == n ? p[e] : w;
-        const bool seen = (uint32_t)(key - from) < near_n || (uint32_t)(key - sink0) < sink_n;
-        const float wf = __shfl(T::to_f32((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * y, 64);
+      for (int e = 0; e < D / 32; e++)
 #pragma unroll
-        for (int e = 0; e < D / 32; e++)
-#pragma unroll
-          for (int z = 0; z < 16; z++) {
-            const int d = 32 * e + 8 * (z >> 2) + 4 * h + (z & 3);
-            const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + TB + v_place<D>(key, d >> 3) + (d & 7) * 2);
-            if (seen) o[e][z] = fmaf(wf, T::to_f32(vd), o[e][z]);
-          }
-      }
-      continue;
+        for (int u = 0; u < 16; u++) {
+          const int d = 32 * e + 8 * (u >> 2) + 4 * h + (u & 3);
+          const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + v_place<D>(y * 32 + key, d >> 3) + (d & 7) * 2);
+          if (seen) o[e][u] = fmaf(wf, T::to_f32(vd), o[e][u]);
+        }
     }
+  };
+
+  // in the order of E and M: keys, values, keys
+  int page1 = page_at(t0), page2 = page_at(t0 + 1);
+  load(a.k, t0, page1, k_lds, ko);
+  load(a.v, t0, page1, v_lds, vo);
+  if (t0 + 1 < t1) {
+    load(a.k, t0 + 1, page2, k_lds, ko);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PN) : "memory");
+  } else {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
+  }
+  asm volatile("s_barrier" ::: "memory");  // the first keys are there
+  float16v x, x1;
+  read_keys(t0, 0);
+  products(x);
+  settle(tile_at(t0), x);
+  for (int i = t0; i < t1; i++) {
+    const int k0 = tile_at(i);
+    // E(i)
+    if (i + 1 < t1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const bool cut = !(k0 + kK - 1 <= lo && k0 > hi - a.window);
+    if (cut) {
+      // a tile that the mask cuts for some row: whether its values are finite
+      u16x2 z = 0;
 #pragma unroll
-    for (int s = 0; s < 4; s++)
-#pragma unroll
-      for (int e = 0; e < D / 32; e++) {
-        // keys 16 s + 4 h + 0 .. 3, then 8 on: the order in which a lane has the numerators
-        const uint8_t* f = st + TB + vf[e & 1] + (e >> 1) * 128 + s * 16 * (D * 2);
-        const u32x2 w0 = read_turned(f), w1 = read_turned(f + 8 * (D * 2));
-        o[e] = T::mfma32(u32x4{w0.x, w0.y, w1.x, w1.y}, u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}, o[e]);
-      }
+      for (int n = 0; n < PN; n++)
+        z = magnitudes8(z, *reinterpret_cast<const uint4*>(lds + 2 * TB + (i & 1) * TB + (wave * PN + n) * 1024 + ln * 16));
+      if (__ballot(max(z.x, z.y) >= T::kInf) && ln == 0) bad[i & 1] = i;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (i + 1 < t1) load(a.v, i + 1, page2, v_lds, vo);
+    const bool careful = cut && bad[i & 1] == i;
+    u32x8 p;
+    read_keys(i, 1);
+    read_values(i, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);  // (they are on their way under what follows)
+    products(x1);
+    numerators(x, p);
+    if (careful) {
+      careful_sums(i, 0, p);
+    } else {
+      sums(0, p);
+      read_values(i, 0, 1);
+      sums(1, p);
+    }
+    settle(k0 + 32, x1);
+    // M(i)
+    if (i + 1 < t1)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (i + 2 < t1) {
+      page2 = page_at(i + 2);
+      load(a.k, i + 2, page2, k_lds, ko);
+    }
+    // (behind the last tile, scores of keys that nobody looks at)
+    read_keys(i + 1, 0);
+    read_values(i, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    products(x);
+    numerators(x1, p);
+    if (careful) {
+      careful_sums(i, 1, p);
+    } else {
+      sums(0, p);
+      read_values(i, 1, 1);
+      sums(1, p);
+    }
+    if (i + 1 < t1) settle(tile_at(i + 1), x);
   }
   l = xlane_level_sum_f32<6>(l);
   if (row > last_row) return;
