@@ -78,6 +78,13 @@ __device__ __forceinline__ u16x2 magnitudes8(u16x2 m, uint4 x) {
   return m;
 }
 
+// Two numbers, those that are not finite as zeros.
+template <class T>
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+  const uint32_t lo = (x & 0x7FFF) >= T::kInf ? 0 : x & 0xFFFF, hi = ((x >> 16) & 0x7FFF) >= T::kInf ? 0 : x & 0xFFFF0000u;
+  return lo | hi;
+}
+
 // Rows of a sequence, and the tiles of `keys` keys that a block of them sees: tiles
 // 0 .. na - 1 hold the sinks, then come b0 .. b0 + tiles - na - 1.
 struct Block {
@@ -151,21 +158,17 @@ __device__ __forceinline__ int few_place(int r, int c) {
 //            they are; the values come out of their rows transposed
 //   sums     of the rounded numerators, so that rounding them does not shift the mean
 // The products of the next half's scores stand beside the exponentials of this one's
-// in the code, so that the matrix unit works under them: one after the other (and
-// waves of two workgroups on a SIMD hardly filled the gaps: matrix unit 41 % and
-// vector unit 48 % busy) a prompt of 8192, 32 heads of 128, took 614 us.
-// Keys are a half ahead of values, so they have buffers and barriers of their own:
-//   E(i), before tile i's first half: everyone is done with the values of tile i - 1,
-//         those of i + 1 are asked for; those of i are there
-//   M(i), before its second half: everyone is done with the keys of tile i, those of
-//         i + 2 are asked for; those of i + 1 are there
+// in the code, so that the matrix unit works under them, and a half's keys are in
+// registers a half before they are needed.  So when everyone comes to a tile's one
+// barrier, its keys and the last tile's values are done with; what takes their places
+// in LDS, the keys of two tiles on and the values of the next, has a tile's time.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   constexpr int NC = D / 8;                    // 16-byte pieces of a row
   constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
   constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave: 16 rows
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys of even and odd tiles, values
-  __shared__ int bad[2];
+  __shared__ int bad;  // whether a tile that the mask cuts had an infinity or NaN among its values
   const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // runs of neighbouring items to an XCD (they share keys and values in its L2)
@@ -180,11 +183,10 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   if (!find_block<kK>(a, seq, (blk - blk0) * kQ, kQ, B) || B.n * a.G <= a.few) return;
   const int t0 = (int)blockIdx.y * a.span, t1 = min(t0 + a.span, B.tiles);
   if (t0 >= t1) return;
-  // cleared before any wave may set one, which is before the first barrier below
-  if (t < 2) bad[t] = -1;
-  __syncthreads();
+  if (t == 0) bad = 0;  // (before any wave may set it, which is behind the first barrier)
   const int lo = B.lo, hi = B.hi;
   auto tile_at = [&](int i) { return (i < B.na ? i : B.b0 + i - B.na) * kK; };
+  auto cut = [&](int k0) { return !(k0 + kK - 1 <= lo && k0 > hi - a.window); };  // whether some row does not see all of it
 
   const int row = B.r0 + wave * 32 + c, last_row = B.n * a.G - 1;  // this lane's row
   const int tok = min(row, last_row) / a.G, head = j * a.G + (min(row, last_row) - tok * a.G);
@@ -234,30 +236,27 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
     load_to_lds<PN>(buffer_of(base + at, bytes), dst + (i & 1) * TB + wave * PN * 1024, off);
   };
   const uint32_t k_lds = lds_offset(lds), v_lds = k_lds + 2 * TB;
-  // LDS offsets of this lane's fragments: keys of row c, pieces 2 e + h; values of
-  // keys 4 h + r, 16 elements of 32 e
-  int kf[D / 16], vf[D / 32];
-#pragma unroll
-  for (int e = 0; e < D / 16; e++) kf[e] = k_place<D>(c, 2 * e + h);
-  const int r4 = (ln >> 2) & 3;
-#pragma unroll
-  for (int e = 0; e < D / 32; e++) vf[e] = v_place<D>(4 * h + r4, 2 * (2 * e + ((ln >> 4) & 1)) + ((ln & 3) >> 1)) + (ln & 1) * 8;
+  // LDS offsets of this lane's first fragments: keys of row c, pieces 2 e + h; values of
+  // keys 4 h + r, 16 elements of 32 e.  The others' are these with 32 e and 64 e
+  // exclusive or (worked out where they are used: kept, they took registers that
+  // there are not).
+  const int kf = k_place<D>(c, h), vf = v_place<D>(4 * h + ((ln >> 2) & 3), 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1)) + (ln & 1) * 8;
 
   // Fragments of half y of tile i: its keys, its values (16 s + 4 h + 0 .. 3, then 8 on:
   // the order in which a lane has the numerators).
   u32x4 kr[D / 16];
   u32x2 vr[D / 32][2];
   auto read_keys = [&](int i, int y) {
-    const uint8_t* st = lds + (i & 1) * TB + y * 32 * (D * 2);
+    const int at = kf + (i & 1) * TB + y * 32 * (D * 2);
 #pragma unroll
-    for (int e = 0; e < D / 16; e++) kr[e] = *reinterpret_cast<const u32x4*>(st + kf[e]);
+    for (int e = 0; e < D / 16; e++) kr[e] = *reinterpret_cast<const u32x4*>(lds + (at ^ (32 * e)));
   };
   auto read_values = [&](int i, int y, int s) {
-    const uint8_t* st = lds + 2 * TB + (i & 1) * TB + (32 * y + 16 * s) * (D * 2);
+    const int at = vf + 2 * TB + (i & 1) * TB + (32 * y + 16 * s) * (D * 2);
 #pragma unroll
     for (int e = 0; e < D / 32; e++)
 #pragma unroll
-      for (int n = 0; n < 2; n++) vr[e][n] = read_turned(st + vf[e] + 8 * n * (D * 2));
+      for (int n = 0; n < 2; n++) vr[e][n] = read_turned(lds + (at ^ (64 * e)) + 8 * n * (D * 2));
   };
   auto products = [&](float16v& x) {
 #pragma unroll
@@ -310,103 +309,88 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
       o[e] = T::mfma32(u32x4{vr[e][0].x, vr[e][0].y, vr[e][1].x, vr[e][1].y},
                        u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}, o[e]);
   };
-  // The same where an infinity or NaN is among the values of a tile that the mask cuts:
-  // the terms one by one, leaving out those of keys that the row does not see.
-  auto careful_sums = [&](int i, int y, const u32x8& p) {
-    // (the sums pass an empty asm here, so that what the compiler does for this
-    // loop's sake, copying them, it does here and not on the common path)
-#pragma unroll
-    for (int e = 0; e < D / 32; e++) asm volatile("" : "+v"(o[e]));
-    const uint8_t* st = lds + 2 * TB + (i & 1) * TB;
-    const int k0 = tile_at(i) + y * 32;
-#pragma unroll 1
-    for (int key = 0; key < 32; key++) {
-      const int z = (key >> 2) & 1, n = (key >> 4) * 4 + ((key >> 3) & 1) * 2 + ((key >> 1) & 1);  // its half wave, pair
-      const uint32_t w = p[n];
-      const int at = k0 + key;
-      const bool seen = at <= qpos && (at > qpos - a.window || at < a.sinks);
-      const float wf = __shfl(T::to_f32((uint16_t)(key & 1 ? w >> 16 : w)), c + 32 * z, 64);
-#pragma unroll
-      for (int e = 0; e < D / 32; e++)
-#pragma unroll
-        for (int u = 0; u < 16; u++) {
-          const int d = 32 * e + 8 * (u >> 2) + 4 * h + (u & 3);
-          const uint16_t vd = *reinterpret_cast<const uint16_t*>(st + v_place<D>(y * 32 + key, d >> 3) + (d & 7) * 2);
-          if (seen) o[e][u] = fmaf(wf, T::to_f32(vd), o[e][u]);
-        }
-    }
-  };
-
-  // in the order of E and M: keys, values, keys
-  int page1 = page_at(t0), page2 = page_at(t0 + 1);
-  load(a.k, t0, page1, k_lds, ko);
-  load(a.v, t0, page1, v_lds, vo);
+  int page = page_at(t0), next_page = page_at(t0 + 1);
+  load(a.k, t0, page, k_lds, ko);
+  load(a.v, t0, page, v_lds, vo);
   if (t0 + 1 < t1) {
-    load(a.k, t0 + 1, page2, k_lds, ko);
+    load(a.k, t0 + 1, next_page, k_lds, ko);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PN) : "memory");
   } else {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
   }
-  asm volatile("s_barrier" ::: "memory");  // the first keys are there
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the first keys are there
   float16v x, x1;
   read_keys(t0, 0);
   products(x);
+  read_keys(t0, 1);
   settle(tile_at(t0), x);
   for (int i = t0; i < t1; i++) {
     const int k0 = tile_at(i);
-    // E(i)
-    if (i + 1 < t1)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool cut = !(k0 + kK - 1 <= lo && k0 > hi - a.window);
-    if (cut) {
-      // a tile that the mask cuts for some row: whether its values are finite
-      u16x2 z = 0;
+    // this wave's part of the values of this tile and the keys of the next is there
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (cut(k0)) {
+      // The mask cuts the tile for some row: infinities and NaN among its values count as
+      // zeros here, so that a weight of zero leaves them out, and reach the rows that
+      // see them at the end.
 #pragma unroll
-      for (int n = 0; n < PN; n++)
-        z = magnitudes8(z, *reinterpret_cast<const uint4*>(lds + 2 * TB + (i & 1) * TB + (wave * PN + n) * 1024 + ln * 16));
-      if (__ballot(max(z.x, z.y) >= T::kInf) && ln == 0) bad[i & 1] = i;
+      for (int n = 0; n < PN; n++) {
+        uint4* at = reinterpret_cast<uint4*>(lds + 2 * TB + (i & 1) * TB + (wave * PN + n) * 1024 + ln * 16);
+        uint4 z = *at;
+        const u16x2 most = magnitudes8(0, z);
+        if (__ballot(max(most.x, most.y) >= T::kInf)) {
+#pragma unroll
+          for (int w = 0; w < 4; w++) (&z.x)[w] = finite2<T>((&z.x)[w]);
+          *at = z;
+          bad = 1;
+        }
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (i + 1 < t1) load(a.v, i + 1, page2, v_lds, vo);
-    const bool careful = cut && bad[i & 1] == i;
+    if (i + 1 < t1) {
+      load(a.v, i + 1, next_page, v_lds, vo);
+      if (i + 2 < t1) {
+        next_page = page_at(i + 2);
+        load(a.k, i + 2, next_page, k_lds, ko);
+      }
+    }
     u32x8 p;
-    read_keys(i, 1);
-    read_values(i, 0, 0);
-    __builtin_amdgcn_sched_barrier(0);  // (they are on their way under what follows)
-    products(x1);
-    numerators(x, p);
-    if (careful) {
-      careful_sums(i, 0, p);
-    } else {
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      // (behind the last tile, keys that nobody looks at)
+      float16v &now = y ? x1 : x, &next = y ? x : x1;
+      read_values(i, y, 0);
+      __builtin_amdgcn_sched_barrier(0);  // (they are on their way under what follows)
+      products(next);
+      numerators(now, p);
+      read_keys(i + 1, y);
       sums(0, p);
-      read_values(i, 0, 1);
+      read_values(i, y, 1);
       sums(1, p);
+      if (y == 0 || i + 1 < t1) settle(y ? tile_at(i + 1) : k0 + 32, next);
     }
-    settle(k0 + 32, x1);
-    // M(i)
-    if (i + 1 < t1)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (i + 2 < t1) {
-      page2 = page_at(i + 2);
-      load(a.k, i + 2, page2, k_lds, ko);
+  }
+  if (bad) {
+    // the values left out above, for the rows that see them: weights are above zero, so
+    // they count as they are
+#pragma unroll 1
+    for (int i = t0; i < t1; i++) {
+      const int k0 = tile_at(i);
+      if (!cut(k0)) continue;
+#pragma unroll 1
+      for (int k = k0; k < min(k0 + kK, B.len); k++) {
+        const int page = scalar_int(table, k >> a.b.shift);
+        if ((unsigned)page >= (unsigned)a.b.pages) continue;
+        const bool seen = k <= qpos && (k > qpos - a.window || k < a.sinks);
+        const uint16_t* v = a.v + ((((int64_t)page * a.Hkv + j) << a.b.shift) + (k & ((1 << a.b.shift) - 1))) * D + 4 * h;
+#pragma unroll
+        for (int e = 0; e < D / 32; e++)
+#pragma unroll
+          for (int u = 0; u < 16; u++) {
+            const uint16_t b = v[32 * e + 8 * (u >> 2) + (u & 3)];
+            if (seen && (b & 0x7FFF) >= T::kInf) o[e][u] += T::to_f32(b);
+          }
+      }
     }
-    // (behind the last tile, scores of keys that nobody looks at)
-    read_keys(i + 1, 0);
-    read_values(i, 1, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    products(x);
-    numerators(x1, p);
-    if (careful) {
-      careful_sums(i, 1, p);
-    } else {
-      sums(0, p);
-      read_values(i, 1, 1);
-      sums(1, p);
-    }
-    if (i + 1 < t1) settle(tile_at(i + 1), x);
   }
   l = xlane_level_sum_f32<6>(l);
   if (row > last_row) return;
