@@ -360,12 +360,15 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
       float16v &now = y ? x1 : x, &next = y ? x : x1;
       read_values(i, y, 0);
       __builtin_amdgcn_sched_barrier(0);  // (they are on their way under what follows)
+      // (before the other workgroup's wave while there are products to feed: 2 %)
+      __builtin_amdgcn_s_setprio(1);
       products(next);
       numerators(now, p);
       read_keys(i + 1, y);
       sums(0, p);
       read_values(i, y, 1);
       sums(1, p);
+      __builtin_amdgcn_s_setprio(0);
       if (y == 0 || i + 1 < t1) settle(y ? tile_at(i + 1) : k0 + 32, next);
     }
   }
