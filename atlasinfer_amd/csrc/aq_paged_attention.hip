@@ -31,6 +31,7 @@ struct AttendArgs {
   int few_span, few_spans; // steps a workgroup of the first kernel, workgroups a sequence
   int span, spans;         // tiles a workgroup of the second, workgroups a block
   int slots;               // the larger number of spans
+  int few_eights, many_eights;  // eights of workgroups of both, where they share a launch
   float c;  // |scale| log2(e), above 0: a masked score, -inf, times it stays that
   uint32_t keep, flip;  // for the queries' bits: none for a scale of 0, the sign of a negative one
 };
@@ -162,18 +163,22 @@ __device__ __forceinline__ int few_place(int r, int c) {
 // registers a half before they are needed.  So when everyone comes to a tile's one
 // barrier, its keys and the last tile's values are done with; what takes their places
 // in LDS, the keys of two tiles on and the values of the next, has a tile's time.
+// lds: many_lds<D> bytes, on a multiple of 1024: keys of even and odd tiles, values
+template <int D>
+constexpr int many_lds = 4 * kK * D * 2 + 16;
+
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
+__device__ __forceinline__ void many_block(const AttendArgs& a, int block, int part, uint8_t* lds) {
   constexpr int NC = D / 8;                    // 16-byte pieces of a row
   constexpr int TB = kK * D * 2;               // bytes of a tile of keys, or of values
   constexpr int PN = TB / 1024 / 4;            // 1 KiB loads of each a wave: 16 rows
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * TB];  // keys of even and odd tiles, values
-  __shared__ int bad;  // whether a tile that the mask cuts had an infinity or NaN among its values
+  // whether a tile that the mask cuts had an infinity or NaN among its values
+  volatile int& bad = *reinterpret_cast<volatile int*>(lds + 4 * TB);
   const int t = threadIdx.x, ln = t & 63, c = ln & 31, h = ln >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   // runs of neighbouring items to an XCD (they share keys and values in its L2)
-  const int item = (int)(blockIdx.x & 7) * a.per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= a.per || item >= a.items) return;
+  const int item = (block & 7) * a.per + (block >> 3);
+  if ((block >> 3) >= a.per || item >= a.items) return;
   const int blocks = a.items / a.Hkv;
   const int j = item / blocks, blk = blocks - 1 - item % blocks;  // late blocks (more keys) first
   int blk0;
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   if (seq < 0) return;
   Block B;
   if (!find_block<kK>(a, seq, (blk - blk0) * kQ, kQ, B) || B.n * a.G <= a.few) return;
-  const int t0 = (int)blockIdx.y * a.span, t1 = min(t0 + a.span, B.tiles);
+  const int t0 = part * a.span, t1 = min(t0 + a.span, B.tiles);
   if (t0 >= t1) return;
   if (t == 0) bad = 0;  // (before any wave may set it, which is behind the first barrier)
   const int lo = B.lo, hi = B.hi;
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttendArgs a) {
   if (row > last_row) return;
   const int64_t at = (int64_t)(B.first + tok) * a.H + head;
   if (B.tiles > a.span) {  // one of several spans: sums, maximum and denominator as they are
-    const int64_t slot = at * a.slots + blockIdx.y;
+    const int64_t slot = at * a.slots + part;
     float* pp = a.part + slot * D + 4 * h;
 #pragma unroll
     for (int e = 0; e < D / 32; e++)
@@ -434,23 +439,27 @@ constexpr int kStep = 32;  // keys a wave takes at a time below
 //            order of keys in which the numerators are at hand
 // The next keys are asked for when the scores' products have taken the last ones, the
 // next values when the last ones are in LDS.
+// lds: few_lds<D, NR> bytes, on a multiple of 16
+template <int D, int NR>
+constexpr int few_sums = 4 * NR * 16 * (D + 4) * 4 > 4 * kStep * D * 2 ? 4 * NR * 16 * (D + 4) * 4 : 4 * kStep * D * 2;
+template <int D, int NR>
+constexpr int few_lds = few_sums<D, NR> + 4 * NR * 16 * 8;
+
 template <class T, int D, int NR>
-__global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
+__device__ __forceinline__ void few_block(const AttendArgs& a, int block, int part, uint8_t* lds) {
   constexpr int NW = 4;                 // waves
   constexpr int NC = D / 8;             // 16-byte pieces of a row
   constexpr int RL = 64 / NC;           // rows a load of values
   constexpr int NV = kStep / RL;        // loads of values a step
   constexpr int VB = kStep * D * 2;     // bytes of a step's values
   constexpr int RS = D + 4;             // floats of a row of sums in LDS, so that rows spread over the banks
-  constexpr int SUMS = NW * NR * 16 * RS * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[SUMS > NW * VB ? SUMS : NW * VB];
-  __shared__ float2 ends[NW][NR * 16];
+  float2(*ends)[NR * 16] = reinterpret_cast<float2(*)[NR * 16]>(lds + few_sums<D, NR>);  // of each wave
   const int t = threadIdx.x, ln = t & 63, i16 = ln & 15, g = ln >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int seq = blockIdx.x / a.Hkv, j = blockIdx.x % a.Hkv;
+  const int seq = block / a.Hkv, j = block % a.Hkv;
   Block B;
   if (!find_block<kStep>(a, seq, 0, NR * 16, B) || B.n * a.G > a.few) return;
-  const int t0 = (int)blockIdx.y * a.few_span, t1 = min(t0 + a.few_span, B.tiles);
+  const int t0 = part * a.few_span, t1 = min(t0 + a.few_span, B.tiles);
   if (t0 >= t1) return;
   const int rows = B.n * a.G;
   auto step_at = [&](int i) { return (i < B.na ? i : B.b0 + i - B.na) * kStep; };
@@ -648,7 +657,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
     const int tok = r / a.G, head = j * a.G + r - tok * a.G;
     const int64_t at = (int64_t)(B.first + tok) * a.H + head;
     if (B.tiles > a.few_span) {
-      const int64_t slot = at * a.slots + blockIdx.y;
+      const int64_t slot = at * a.slots + part;
       *reinterpret_cast<float4*>(a.part + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       *reinterpret_cast<float4*>(a.part + slot * D + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
       if (d == 0) ends_of<D>(a)[slot] = make_float2(mx, den);
@@ -659,6 +668,36 @@ __global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
           make_uint4(T::pack(acc[0] * f, acc[1] * f), T::pack(acc[2] * f, acc[3] * f), T::pack(acc[4] * f, acc[5] * f),
                      T::pack(acc[6] * f, acc[7] * f));
     }
+  }
+}
+
+template <class T, int D, int NR>
+__global__ __launch_bounds__(256) void paged_few_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<D, NR>];
+  few_block<T, D, NR>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void paged_many_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[many_lds<D>];
+  many_block<T, D>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// Both in one launch, their workgroups side by side: the first kernel waits for
+// memory, the second for the matrix unit (31 single tokens and a chunk of 1501
+// positions: 74 and 65 us one after the other, 97 together).  Eight workgroups
+// at a time, one an XCD, in the proportion of their numbers.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[many_lds<D> > few_lds<D, 1> ? many_lds<D> : few_lds<D, 1>];
+  const int64_t few = a.few_eights, all = few + a.many_eights, n = blockIdx.x >> 3;
+  const int before = (int)(n * few / all), x = blockIdx.x & 7;
+  if ((int)((n + 1) * few / all) > before) {
+    const int f = before * 8 + x, heads = a.b.S * a.Hkv;
+    if (f < heads * a.few_spans) few_block<T, D, 1>(a, f % heads, f / heads, lds);
+  } else {
+    const int m = (int)(n - before) * 8 + x;
+    many_block<T, D>(a, m % (8 * a.per), m / (8 * a.per), lds);
   }
 }
 
@@ -827,11 +866,14 @@ bool sizes_ok(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t m
 
 template <class T, int D>
 void launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
-  const dim3 few((unsigned)(a.b.S * a.Hkv), (unsigned)p.few_spans);
-  if (p.nr == 1) hipLaunchKernelGGL((paged_few_kernel<T, D, 1>), few, dim3(256), 0, stream, a);
-  if (p.nr == 2) hipLaunchKernelGGL((paged_few_kernel<T, D, 2>), few, dim3(256), 0, stream, a);
-  if (p.many)
-    hipLaunchKernelGGL((paged_attention_kernel<T, D>), dim3((unsigned)(8 * p.per), (unsigned)p.spans), dim3(256), 0, stream, a);
+  const dim3 few((unsigned)(a.b.S * a.Hkv), (unsigned)p.few_spans), many((unsigned)(8 * p.per), (unsigned)p.spans);
+  if (p.nr == 1 && p.many) {
+    hipLaunchKernelGGL((paged_mixed_kernel<T, D>), dim3(8u * (a.few_eights + a.many_eights)), dim3(256), 0, stream, a);
+  } else {
+    if (p.nr == 1) hipLaunchKernelGGL((paged_few_kernel<T, D, 1>), few, dim3(256), 0, stream, a);
+    if (p.nr == 2) hipLaunchKernelGGL((paged_few_kernel<T, D, 2>), few, dim3(256), 0, stream, a);
+    if (p.many) hipLaunchKernelGGL((paged_many_kernel<T, D>), many, dim3(256), 0, stream, a);
+  }
   if (p.few_spans > 1)
     hipLaunchKernelGGL((paged_few_merge_kernel<T, D>), dim3(few.x, (unsigned)p.few_rows), dim3(256), 0, stream, a);
   if (p.spans > 1)
@@ -872,7 +914,7 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   AQ_CHECK_ARG(p.bytes == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", me, (long long)ws_bytes, (long long)p.bytes);
   // (a grid has fewer than 2^32 threads)
-  AQ_CHECK_ARG(p.items <= (1 << 24) / p.spans - 8 && S * Hkv <= (1 << 24) / p.few_spans && T * H <= (1 << 25),
+  AQ_CHECK_ARG(p.items <= (1 << 23) / p.spans - 16 && S * Hkv <= (1 << 23) / p.few_spans - 16 && T * H <= (1 << 25),
                "%s: %lld rows of %lld heads, %lld sequences", me, (long long)T, (long long)H, (long long)S);
   AttendArgs a;
   a.b = paged::Batch{starts, lengths, table, (int)T, (int)S, (int)W, (int)pages, __builtin_ctz((unsigned)page_size),
@@ -897,6 +939,8 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   a.span = (int)p.span;
   a.spans = (int)p.spans;
   a.slots = (int)p.slots;
+  a.few_eights = p.nr ? (int)aq::ceil_div(S * Hkv * p.few_spans, 8) : 0;
+  a.many_eights = (int)(p.per * p.spans);
   a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504f;
   a.keep = scale == 0.0f ? 0u : 0xFFFFFFFFu;
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
