@@ -47,9 +47,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise ValueError(f"token_logprobs: {top} alternatives (0 .. {MAX_TOP}, at most a row's {V})")
     if torch.is_grad_enabled() and logits.requires_grad:
         raise RuntimeError("token_logprobs records no gradients: call it under torch.no_grad()")
-    f32, i64 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.int64, device=dev)
-    out = TokenLogprobs(torch.empty(B, **f32), torch.empty(B, **f32), torch.empty(B, **i64), torch.empty(B, top, **f32),
-                        torch.empty(B, top, **i64))
+    # (allocations are most of a small call: those of known shape and type are the cheapest)
+    logprobs, top_logprobs = torch.empty(B, dtype=torch.float32, device=dev), torch.empty(B, top, dtype=torch.float32, device=dev)
+    out = TokenLogprobs(logprobs, torch.empty_like(logprobs), torch.empty_like(tokens), top_logprobs,
+                        torch.empty(B, top, dtype=torch.int64, device=dev))
     if B == 0:
         return out
     if (logits.stride(1) != 1 and V > 1) or (logits.stride(0) < V and B > 1):

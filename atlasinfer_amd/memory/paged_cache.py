@@ -152,8 +152,8 @@ def _cache(what, cache, batch):
     return k, v, Hkv, P, D
 
 
-def _no_gradients(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradients(what):
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{what} records no gradients: call it under torch.no_grad()")
 
 
@@ -189,7 +189,8 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, cache: Sequence[torch.Tensor],
         R = 2 * freq.numel()
         if freq.dtype != torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or freq.device != dev or R % 16 or not 0 < R <= D:
             _refuse(f"{what}: frequencies must be contiguous float32 [n] on {dev}, n a multiple of 8 up to {D // 2}")
-    _no_gradients(what, q, k, v)
+    if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+        _no_gradients(what)
     if T == 0:
         return q_out
     if q is not None:
@@ -240,18 +241,21 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
         _refuse(f"{what}: out must be contiguous {dtype} {tuple(q.shape)} on {dev}")
     if workspace is not None and not (workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev):
         _refuse(f"{what}: the workspace must be contiguous uint8 on {dev}")
-    _no_gradients(what, q, kc, vc)
+    if q.requires_grad or kc.requires_grad or vc.requires_grad:
+        _no_gradients(what)
     if T == 0:
         return out
-    q = _lib.strided_rows(q)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = _lib.strided_rows(q)
     starts, lengths, S, table, W, max_new, max_length = batch._args
     L = _lib.load()
     if workspace is None:
         size = L.aq_paged_attention_workspace(T, S, H, Hkv, D, max_new, max_length)
         workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    row, head, _ = q.stride()
     with _lib.on_device(dev):
-        _lib.check(L.aq_paged_attention(q.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, *q.stride()[:2],
+        _lib.check(L.aq_paged_attention(q.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, row, head,
                                         kc.data_ptr(), vc.data_ptr(), kc.shape[0], P, starts, lengths, S, table, W, max_new, max_length,
                                         min(window, _INT_MAX), min(sinks, _INT_MAX), scale, ws, size, out.data_ptr(),
                                         _lib.stream_of(dev)), "aq_paged_attention")

@@ -182,3 +182,16 @@ def test_streams_and_graph():
         tokens.add_(100)
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(out, token_logprobs(x, tokens, 8)))
+
+
+def test_python_refusals():
+    x, t = torch.randn(3, 50, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    for args in ((x[0], t), (x.double(), t), (x.long(), t), (x, t.int()), (x, t[:2]), (x, t.cpu()), (x, t, 51), (x, t, -1),
+                 (torch.randn(3, 100, device=DEV), t, 65), (x[:, :0], t), (torch.empty(1, (1 << 18) + 1, device=DEV), t[:1]),
+                 (x, torch.zeros(6, dtype=torch.int64, device=DEV)[::2])):
+        with pytest.raises(ValueError):
+            token_logprobs(*args)
+    with pytest.raises(RuntimeError, match="gradients"):
+        token_logprobs(x.clone().requires_grad_(), t)
+    out = token_logprobs(x[:0], t[:0], 4)
+    assert out.logprobs.shape == (0,) and out.top_tokens.shape == (0, 4)

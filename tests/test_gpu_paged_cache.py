@@ -383,3 +383,47 @@ def test_two_streams_and_graphs():
                 both.append(paged_attention(x, b.cache, batch, scale=0.09, workspace=w))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(both, want))
+
+
+def test_python_refusals():
+    b = R.Batch([3], [20], 2, 64, 16, F16, DEV)
+    batch = _batch(b)
+    q, k, v = b.normal(3, 4, 64).half(), b.normal(3, 2, 64).half(), b.normal(3, 2, 64).half()
+    f = rotary_frequencies(64, device=DEV)[0]
+
+    def store(k=k, v=v, cache=b.cache, batch=batch, **kw):
+        return paged_store(k, v, cache, batch, **kw)
+
+    def attend(q=q, cache=b.cache, batch=batch, **kw):
+        return paged_attention(q, cache, batch, **{"scale": 0.1, **kw})
+    kc, vc = b.cache
+    caches = [(kc, vc[:1]), (kc.float(), vc.float()), (kc, vc.bfloat16()), (kc[:, :, :8].contiguous(), vc[:, :, :8].contiguous()),
+              (kc[..., ::2], vc[..., ::2]), (kc[..., :32].contiguous(), vc[..., :32].contiguous()), (kc.cpu(), vc.cpu())]
+    for c in caches:
+        for f_ in (store, attend):
+            with pytest.raises(ValueError):
+                f_(cache=c)
+    for kw in (dict(k=k[:2]), dict(v=v[:, :1]), dict(k=k.bfloat16()), dict(k=k.cpu()), dict(k=k[0]), dict(q=q[:2]), dict(q=q.float()),
+               dict(q=q[..., :32]), dict(q_out=q), dict(q=q, q_out=q.bfloat16()), dict(q=q, q_out=q), dict(rope=Rotary(f.half())),
+               dict(rope=Rotary(f[:4])), dict(rope=Rotary(f.repeat(2))), dict(rope=Rotary(f.cpu())), dict(rope=Rotary(f[:0]))):
+        with pytest.raises(ValueError):
+            store(**kw)
+    for kw in (dict(q=q[:, :3]), dict(q=q.bfloat16()), dict(q=q[0]), dict(q=q[..., :32]), dict(window=0), dict(sinks=-1),
+               dict(out=q.float()), dict(out=q[:2]), dict(out=q.cpu()), dict(workspace=torch.empty(4, device=DEV)),
+               dict(batch=PagedBatch(b.starts, b.lengths, b.table, 3, 1000))):
+        with pytest.raises(ValueError):
+            attend(**kw)
+    for f_, kw in ((store, dict(k=k.clone().requires_grad_())), (attend, dict(q=q.clone().requires_grad_()))):
+        with pytest.raises(RuntimeError, match="gradients"):
+            f_(**kw)
+        with torch.no_grad():
+            f_(**kw)
+    for bad in ((b.starts.long(), b.lengths, b.table), (b.starts, b.lengths.cpu(), b.table), (b.starts, b.lengths, b.table.long()),
+                (b.starts[::1].repeat(2)[::2], b.lengths, b.table)):
+        with pytest.raises(ValueError):
+            PagedBatch(*bad, 3, 23)
+    for n, x in ((0, 23), (3, 0)):
+        with pytest.raises(ValueError):
+            PagedBatch(b.starts, b.lengths, b.table, n, x)
+    with pytest.raises(AttributeError):
+        batch.max_length = 7
