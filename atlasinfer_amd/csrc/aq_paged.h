@@ -77,6 +77,31 @@ struct Batch {
   int max_new, max_length;
 
   __device__ __forceinline__ int start(int s) const { return min(max(starts[s], 0), T); }
+  __device__ __forceinline__ int scalar_start(int s) const { return min(max(scalar_int(starts, s), 0), T); }
 };
+
+// The last of 0 .. n - 1 with value(s) <= x, -1 if there is none, the values
+// ascending: a wave looks at 64 of them at a time, one look up to 64 of them, two up to
+// 4096, three up to 65535 (a look waits for memory).
+template <class F>
+__device__ __forceinline__ int last_at_most(int n, int x, F value) {
+  const int ln = threadIdx.x & 63;
+  int lo = 0;
+  for (;;) {
+    const int step = (n + 63) >> 6, s = ln * step;
+    const uint64_t mask = __ballot(s < n && value(lo + min(s, n - 1)) <= x);
+    if (!mask) return lo - 1;
+    const int k = 63 - __builtin_clzll(mask);
+    lo = __builtin_amdgcn_readfirstlane(lo + k * step);
+    if (step == 1) return lo;
+    n = min(step, n - k * step);
+  }
+}
+
+// The sequence whose rows hold row t, -1 for none; the same for all lanes.
+__device__ __forceinline__ int sequence_of(const Batch& b, int t) {
+  const int s = last_at_most(b.S, t, [&](int i) { return b.start(i); });
+  return s >= 0 && t < b.scalar_start(s + 1) ? s : -1;
+}
 
 }  // namespace paged

@@ -98,8 +98,8 @@ struct Block {
 // every lane.
 template <int KEYS>
 __device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, int rows, Block& k) {
-  k.first = min(max(scalar_int(a.b.starts, s), 0), a.b.T);
-  k.n = max(min(max(scalar_int(a.b.starts, s + 1), 0), a.b.T) - k.first, 0);
+  k.first = a.b.scalar_start(s);
+  k.n = max(a.b.scalar_start(s + 1) - k.first, 0);
   k.len = scalar_int(a.b.lengths, s);
   k.r0 = r0;
   if (r0 >= k.n * a.G || k.n > k.len || k.n > a.b.max_new || k.len > a.b.max_length) return false;
@@ -113,20 +113,13 @@ __device__ __forceinline__ bool find_block(const AttendArgs& a, int s, int r0, i
   return true;
 }
 
-// The sequence that block `blk` belongs to, -1 for none: sequence s's blocks
-// are starts[s] G / 128 + s and on (as many as its rows can need, or one more).
-__device__ __forceinline__ int find_sequence(const AttendArgs& a, int blk, int ln, int& first) {
-  for (int s0 = 0; s0 < a.b.S; s0 += 64) {
-    const int s = min(s0 + ln, a.b.S - 1);
-    const int f = a.b.start(s) * a.G / kQ + s, e = a.b.start(s + 1) * a.G / kQ + s + 1;
-    const uint64_t hit = __ballot(f <= blk && blk < e && s == s0 + ln);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      first = __builtin_amdgcn_readlane(f, at);
-      return __builtin_amdgcn_readfirstlane(s0 + at);
-    }
-  }
-  return -1;
+// The sequence that block `blk` belongs to, -1 for none, and its first block: sequence
+// s's are starts[s] G / 128 + s and on (as many as its rows can need, or one more).
+__device__ __forceinline__ int find_sequence(const AttendArgs& a, int blk, int& first) {
+  const int s = last_at_most(a.b.S, blk, [&](int i) { return a.b.start(i) * a.G / kQ + i; });
+  if (s < 0 || blk > a.b.scalar_start(s + 1) * a.G / kQ + s) return -1;
+  first = a.b.scalar_start(s) * a.G / kQ + s;
+  return s;
 }
 
 // A tile's rows lie in LDS one after the other, 16-byte pieces permuted within each
@@ -182,7 +175,7 @@ __device__ __forceinline__ void many_block(const AttendArgs& a, int block, int p
   const int blocks = a.items / a.Hkv;
   const int j = item / blocks, blk = blocks - 1 - item % blocks;  // late blocks (more keys) first
   int blk0;
-  const int seq = find_sequence(a, blk, ln, blk0);
+  const int seq = find_sequence(a, blk, blk0);
   if (seq < 0) return;
   Block B;
   if (!find_block<kK>(a, seq, (blk - blk0) * kQ, kQ, B) || B.n * a.G <= a.few) return;
@@ -701,35 +694,6 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(AttendArgs a) {
   }
 }
 
-// The spans of a row (token and head, `at` of them) joined by a wave: lane s has the
-// maximum and denominator of span s (y; there are up to 64).
-template <class T, int D>
-__device__ __forceinline__ void merge_row(const AttendArgs& a, int64_t at, int spans, float2 y) {
-  const int ln = threadIdx.x & 63;
-  if (ln >= spans) y = make_float2(-INFINITY, 0.0f);
-  const float m = wave_group_max_f32<64>(y.x);
-  // a span with scores of -inf only has sums of zero, or the NaN of what it saw
-  const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - m) * a.c);
-  const float l = wave_group_sum_f32<64>(y.y * f);
-  constexpr int E = D / 64;
-  float o[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) o[e] = 0.0f;
-  const float* pp = a.part + at * a.slots * D + ln * E;
-#pragma unroll 8
-  for (int s = 0; s < spans; s++) {
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = fmaf(pp[(int64_t)s * D + e], w, o[e]);
-  }
-  const float inv = l == 0.0f ? NAN : 1.0f / l;
-  uint16_t* op = a.out + at * D + ln * E;
-  if (D == 128)
-    *reinterpret_cast<uint32_t*>(op) = T::pack(o[0] * inv, o[E - 1] * inv);
-  else
-    *op = T::from_f32(o[0] * inv);
-}
-
 // For the first kernel, a workgroup a row: 16 bytes a lane, the spans dealt to
 // groups of D / 4 lanes, whose sums meet in LDS.  Everything is asked for at once,
 // before it is known how many spans there are: what is none is not looked at.
@@ -786,28 +750,51 @@ __global__ __launch_bounds__(256) void paged_few_merge_kernel(AttendArgs a) {
   *reinterpret_cast<uint2*>(a.out + at * D + 4 * d) = make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
 }
 
-// For the second, a wave a row.
+// For the second, a wave a row: 16 bytes a lane, the spans dealt to groups of D / 4
+// lanes; lane s has the maximum and denominator of span s (there are up to 64).
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
   const int ln = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = (int)(at / a.H), head = (int)(at % a.H);
   if (t >= a.b.T) return;
+  constexpr int N = 64 / (D / 4);
+  const int grp = ln / (D / 4), d = ln % (D / 4);
+  const float4* pp = reinterpret_cast<const float4*>(a.part + at * a.slots * D) + d;
   // (read before it is known how many there are: what is none is not looked at)
-  const float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
+  float2 y = ends_of<D>(a)[at * a.slots + min(ln, a.slots - 1)];
   // the row's sequence, and the block that it was in
-  int seq = -1;
-  for (int s0 = 0; s0 < a.b.S && seq < 0; s0 += 64) {
-    const int s = min(s0 + ln, a.b.S - 1);
-    const uint64_t hit = __ballot(a.b.start(s) <= t && t < a.b.start(s + 1) && s == s0 + ln);
-    if (hit) seq = __builtin_amdgcn_readfirstlane(s0 + __builtin_ctzll(hit));
-  }
+  const int seq = sequence_of(a.b, t);
   if (seq < 0) return;
-  const int r = (t - min(max(scalar_int(a.b.starts, seq), 0), a.b.T)) * a.G + head % a.G;
+  const int r = (t - a.b.scalar_start(seq)) * a.G + head % a.G;
   Block B;
   if (!find_block<kK>(a, seq, r / kQ * kQ, kQ, B) || B.n * a.G <= a.few) return;
   const int spans = (B.tiles + a.span - 1) / a.span;
-  if (spans > 1) merge_row<T, D>(a, at, spans, y);
+  if (spans <= 1) return;
+  if (ln >= spans) y = make_float2(-INFINITY, 0.0f);
+  const float m = wave_group_max_f32<64>(y.x);
+  // a span with scores of -inf only has sums of zero, or the NaN of what it saw
+  const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - m) * a.c);
+  const float l = wave_group_sum_f32<64>(y.y * f);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int s = grp; s < spans; s += N) {
+    const float4 x = pp[(int64_t)s * (D / 4)];
+    const float w = __shfl(f, s, 64);
+    o.x = fmaf(x.x, w, o.x);
+    o.y = fmaf(x.y, w, o.y);
+    o.z = fmaf(x.z, w, o.z);
+    o.w = fmaf(x.w, w, o.w);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float& z = (&o.x)[i];
+    if (D == 64) z = xlane_level_sum_f32<5>(z);
+    z = xlane_level_sum_f32<6>(z);
+  }
+  const float inv = l == 0.0f ? NAN : 1.0f / l;
+  if (grp == 0)
+    *reinterpret_cast<uint2*>(a.out + at * D + 4 * d) = make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
 }
 
 // Which kernels run, and how the keys are split: sequences of up to `few` rows by

@@ -27,26 +27,15 @@ struct StoreArgs {
 // elements turn together (half layout: R/2 apart), or two neighbouring pieces.
 template <class T>
 __global__ __launch_bounds__(kThreads) void paged_store_kernel(StoreArgs a) {
-  __shared__ int s_pos, s_page;
   __shared__ float s_cos[64], s_sin[64];
   const int t = blockIdx.x, tid = threadIdx.x;
-  if (tid == 0) s_pos = -1;
-  __syncthreads();
-  // the sequence whose rows hold t (empty ones hold none), by whoever has it
-  for (int s = tid; s < a.b.S; s += kThreads) {
-    const int lo = a.b.start(s), hi = max(a.b.start(s + 1), lo), len = a.b.lengths[s];
-    if (t >= lo && t < hi) {
-      const int p = len - (hi - t);
-      if (len - (hi - lo) >= 0 && hi - lo <= a.b.max_new && len <= a.b.max_length) {
-        const int page = a.b.table[(int64_t)s * a.b.W + (p >> a.b.shift)];
-        s_page = (unsigned)page < (unsigned)a.b.pages ? page : -1;
-        s_pos = p;
-      }
-    }
-  }
-  __syncthreads();
-  const int pos = s_pos;
-  if (pos < 0) return;
+  const int seq = sequence_of(a.b, t);
+  if (seq < 0) return;
+  const int n = a.b.scalar_start(seq + 1) - a.b.scalar_start(seq), len = scalar_int(a.b.lengths, seq);
+  if (n > len || n > a.b.max_new || len > a.b.max_length) return;
+  const int pos = len - (a.b.scalar_start(seq + 1) - t);
+  int page = scalar_int(a.b.table, (int64_t)seq * a.b.W + (pos >> a.b.shift));
+  if ((unsigned)page >= (unsigned)a.b.pages) page = -1;
   if (tid < a.R / 2) {
     // in turns, in 64 bits: an angle of a far position has lost its fraction in 32
     const double u = (double)pos * (double)a.freq[tid] * 0.15915494309189535;
@@ -56,11 +45,11 @@ __global__ __launch_bounds__(kThreads) void paged_store_kernel(StoreArgs a) {
     s_sin[tid] = sn * a.factor;
   }
   __syncthreads();
-  const int page = s_page, slot = pos & ((1 << a.b.shift) - 1);
+  const int slot = pos & ((1 << a.b.shift) - 1);
   const int UH = a.D / 16, RU = a.R / 16;  // units of a head, of its turning part
   const int units = (a.H + 2 * a.Hkv) * UH;
-  for (int n = tid; n < units; n += kThreads) {
-    const int head = n / UH, u = n % UH;
+  for (int i = tid; i < units; i += kThreads) {
+    const int head = i / UH, u = i % UH;
     const uint16_t* src;
     uint16_t* dst;
     if (head < a.H) {

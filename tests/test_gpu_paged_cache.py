@@ -196,6 +196,43 @@ def test_many_sequences():
     _check([1] * 150, [(91 * i) % 400 for i in range(150)], 2, 1, 128, dtype=BF16)
 
 
+def test_thousands_of_sequences():
+    """More sequences than one look at 64 of 64 finds: rows and blocks in their places."""
+    S = 4500
+    news = [(7 * i) % 3 for i in range(S)]
+    news[2000], news[4400] = 40, 150
+    contexts = [(13 * i) % 40 for i in range(S)]
+    b = R.Batch(news, contexts, 1, 64, 16, F16, DEV)
+    q = b.normal(b.T, 2, 64).half()
+    got = paged_attention(q, b.cache, _batch(b), scale=0.125)
+    for i in list(range(0, S, 371)) + [1999, 2000, 2001, 4400, 4498, 4499]:
+        if news[i]:
+            want, bound = R.attend(q[b.first[i]:b.first[i + 1]], b, i, 0.125)
+            assert ((got[b.first[i]:b.first[i + 1]].double() - want).abs() <= bound).all(), i
+    _check_store([(5 * i) % 2 for i in range(S)], [(11 * i) % 30 for i in range(S)], 1, 1, 64, 16, F16, 64, False)
+
+
+def test_shared_and_freed_pages():
+    """Sequences that share the pages of a common beginning; pages that have left the window, given back."""
+    P, n = 16, 64
+    b = R.Batch([1, 30, 2], [100, 80, n], 2, 64, P, F16, DEV)
+    b.table[1, :n // P] = b.table[0, :n // P]
+    b.table[2, :n // P] = b.table[0, :n // P]
+    for i in (1, 2):
+        b.pages[i][:n // P] = b.pages[0][:n // P]
+    q = b.normal(b.T, 4, 64).half()
+    got = paged_attention(q, b.cache, _batch(b), scale=0.1)
+    for i in range(3):
+        want, bound = R.attend(q[b.first[i]:b.first[i + 1]], b, i, 0.1)
+        assert ((got[b.first[i]:b.first[i + 1]].double() - want).abs() <= bound).all()
+    # nothing before position 100 - 39 is seen by any row through a window of 40, but for 3 sinks
+    b = R.Batch([1, 70], [100, 100], 2, 128, P, F16, DEV)
+    q = b.normal(b.T, 4, 128).half()
+    want = paged_attention(q, b.cache, _batch(b), scale=0.1, window=40, sinks=3)
+    b.table[:, 1:61 // P] = torch.tensor([-1, 1 << 30], dtype=torch.int32, device=DEV)
+    assert torch.equal(paged_attention(q, b.cache, _batch(b), scale=0.1, window=40, sinks=3), want)
+
+
 def test_large_scores_and_scales():
     """Peaked rows (keys 30 times as large), a negative scale, and 0, with which every key seen counts alike."""
     for D in (64, 128):
