@@ -6,10 +6,9 @@
 // in one pass, each lane with a maximum of its own: where it grows by d, Z and E so
 // far become Z e^-d and (E - d Z) e^-d.  Lanes, and parts of a row, meet the same way.
 //
-// The alternatives need no sort of the row.  In each wave, the n-th largest of the
-// lanes' maxima is a value that n elements at least reach; the largest of the
-// waves' values cuts the row to a short list (about four times n), which is ranked by
-// counting.
+// The alternatives need no sort of the row.  The n-th largest of the lanes' maxima is
+// a value that n elements at least reach; it cuts the row to a short list (a few more
+// than n), which is ranked by counting.
 #include "aq_common.h"
 
 namespace {
@@ -17,7 +16,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kHeld = 8;   // pieces that a thread keeps (in LDS): 2048 a workgroup
-constexpr int kList = 256;  // places of a wave's list
+constexpr int kList = 576;  // places of a wave's list: all that fewer than 64 lanes have is at most 518
 constexpr int kMaxTop = 64, kMaxParts = 32;
 constexpr int kMaxVocab = 1 << 18;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -142,7 +141,7 @@ struct Shared {
   u64 top[kMaxTop];
   Sums sums[kWaves];
   float largest[kWaves];
-  uint32_t cut[kWaves];
+  uint32_t keys[kThreads];
   int count[kWaves];
   u64 best[kWaves];
 };
@@ -243,22 +242,43 @@ __device__ __forceinline__ int part_top(Shared& s, const Part<FMT>& r, bool ther
   typedef Type<FMT> T;
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t key = has ? key_of(mine) : 0u;
-  // the largest value that n of the wave's lanes reach (0: fewer have any), two bits
-  // at a time; the low bits of 16-bit numbers are all alike
+  // The largest value that n of the lanes reach (0: fewer have any), two bits at a time;
+  // the low bits of 16-bit numbers are all alike.  For more than 8 of all lanes, whose
+  // keys every wave has; up to 8 of each wave by itself, the largest of the waves'
+  // values: a quarter of the work, lists of 4 n (2048 rows of 128256 with n = 5 177 us
+  // so, 186 by all lanes; with n = 20 222 and 202, with n = 64 3140 and 279).
   constexpr int kLowest = FMT == AQ_F32 ? 0 : FMT == AQ_BF16 ? 16 : 12;
-  uint32_t cut = 0;
+  auto highest = [&](auto reach) {
+    uint32_t c = 0;
 #pragma unroll 1
-  for (int bit = 30; bit >= kLowest; bit -= 2) {
-    const uint32_t c1 = cut | 1u << bit, c2 = cut | 2u << bit, c3 = cut | 3u << bit;
-    const int k1 = __popcll(__ballot(key >= c1)), k2 = __popcll(__ballot(key >= c2)), k3 = __popcll(__ballot(key >= c3));
-    cut = k3 >= n ? c3 : k2 >= n ? c2 : k1 >= n ? c1 : cut;
-  }
-  if (cut && !(cut >> 31)) cut |= (1u << kLowest) - 1;
+    for (int bit = 30; bit >= kLowest; bit -= 2) {
+      const uint32_t c1 = c | 1u << bit, c2 = c | 2u << bit, c3 = c | 3u << bit;
+      const int k1 = reach(c1), k2 = reach(c2), k3 = reach(c3);
+      c = k3 >= n ? c3 : k2 >= n ? c2 : k1 >= n ? c1 : c;
+    }
+    return c && !(c >> 31) ? c | ((1u << kLowest) - 1) : c;
+  };
+  uint32_t cut = 0;
   __syncthreads();
-  if ((t & 63) == 0) s.cut[wave] = cut;
-  __syncthreads();
+  if (n <= 8) {
+    cut = highest([&](uint32_t c) { return __popcll(__ballot(key >= c)); });
+    if ((t & 63) == 0) s.keys[wave] = cut;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) cut = max(cut, s.cut[w]);
+    for (int w = 0; w < kWaves; w++) cut = max(cut, s.keys[w]);
+  } else {
+    s.keys[t] = key;
+    __syncthreads();
+    uint32_t keys[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) keys[w] = s.keys[(t & 63) + 64 * w];
+    cut = highest([&](uint32_t c) {
+      int k = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) k += __popcll(__ballot(keys[w] >= c));
+      return k;
+    });
+  }
   // Each wave lists its elements with keys of `low` and above (where it has one); the
   // second time, where very many are equal to the cut, those above it.
   int c = 0, before = 0;

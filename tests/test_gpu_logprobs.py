@@ -195,3 +195,14 @@ def test_python_refusals():
         token_logprobs(x.clone().requires_grad_(), t)
     out = token_logprobs(x[:0], t[:0], 4)
     assert out.logprobs.shape == (0,) and out.top_tokens.shape == (0, 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_fewer_lanes_than_alternatives(dtype):
+    """Rows that fewer threads share than alternatives are asked for, whole and off the 16-byte grid: everything is listed."""
+    x = torch.randn(3, 600, device=DEV).to(dtype)
+    tokens = torch.tensor([0, 99, 63], device=DEV)
+    for V in (64, 255, 256, 263, 300, 503, 504, 511, 512, 517, 518, 519, 526, 540):
+        for skip in (0, 1, 5):
+            _check(x[:, skip:skip + V], tokens, 64)
+            _check(x[:, skip:skip + V], tokens, 9)
