@@ -151,11 +151,17 @@ __device__ __forceinline__ int few_place(int r, int c) {
 //   values   o^T = v^T p^T: the numerators, rounded to 16 bits, are the operand as
 //            they are; the values come out of their rows transposed
 //   sums     of the rounded numerators, so that rounding them does not shift the mean
-// The products of the next half's scores stand beside the exponentials of this one's
-// in the code, so that the matrix unit works under them, and a half's keys are in
+// The products of the next half's scores stand among the exponentials of this one's in
+// the code, so that the matrix unit works under them, and a half's keys are in
 // registers a half before they are needed.  So when everyone comes to a tile's one
 // barrier, its keys and the last tile's values are done with; what takes their places
 // in LDS, the keys of two tiles on and the values of the next, has a tile's time.
+// A prompt of 8192, 32 heads of 128 over 8 key/value heads: 566 to 590 us, 930 to 970
+// TFLOP/s of the two products (the library's fp16 product of 8192^3: 1177), the matrix
+// unit 47 % busy at 1.9 GHz, no bank conflicts.  One half after the other, without the
+// places and the registers ahead, it took 614.  Nothing gained: workgroups of 256 rows,
+// also with four tiles in flight (580 against 590), other proportions of the interleaving
+// (all within 1 %), the loads later in the tile (580 against 570).
 // lds: many_lds<D> bytes, on a multiple of 1024: keys of even and odd tiles, values
 template <int D>
 constexpr int many_lds = 4 * kK * D * 2 + 16;
@@ -219,11 +225,17 @@ __device__ __forceinline__ void many_block(const AttendArgs& a, int block, int p
     ko[n] = k_place<D>(r, pc);  // (the places are their own inverse)
     vo[n] = v_place<D>(r, pc);
   }
+  // The pages of this wave's 16 rows of 64 tiles from p0 on, one a lane (past the last
+  // tile: any): read one by one by the scalar unit they would come at any time among the
+  // answers of LDS, which would have to be waited for all together.
   const int* table = a.b.table + (int64_t)seq * a.b.W;
-  const int last_page = (B.len - 1) >> a.b.shift;
-  auto page_at = [&](int i) {  // of this wave's 16 rows of tile i (past the last: any)
-    return scalar_int(table, min((tile_at(min(i, t1 - 1)) + wave * 16) >> a.b.shift, last_page));
+  int p0, pages;
+  auto read_pages = [&](int i) {
+    p0 = i;
+    pages = table[min((tile_at(min(i + ln, t1 - 1)) + wave * 16) >> a.b.shift, (B.len - 1) >> a.b.shift)];
+    asm volatile("" : "+v"(pages));  // (waited for here)
   };
+  auto page_at = [&](int i) { return __builtin_amdgcn_readlane(pages, i - p0); };
   auto load = [&](const uint16_t* base, int i, int page, uint32_t dst, const int (&off)[PN]) {
     const int k0 = tile_at(i) + wave * 16;
     // rows past the last, and those of a page outside the cache, read as zeros
@@ -307,11 +319,11 @@ __device__ __forceinline__ void many_block(const AttendArgs& a, int block, int p
       o[e] = T::mfma32(u32x4{vr[e][0].x, vr[e][0].y, vr[e][1].x, vr[e][1].y},
                        u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}, o[e]);
   };
-  int page = page_at(t0), next_page = page_at(t0 + 1);
-  load(a.k, t0, page, k_lds, ko);
-  load(a.v, t0, page, v_lds, vo);
+  read_pages(t0);
+  load(a.k, t0, page_at(t0), k_lds, ko);
+  load(a.v, t0, page_at(t0), v_lds, vo);
   if (t0 + 1 < t1) {
-    load(a.k, t0 + 1, next_page, k_lds, ko);
+    load(a.k, t0 + 1, page_at(t0 + 1), k_lds, ko);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PN) : "memory");
   } else {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PN) : "memory");
@@ -343,13 +355,14 @@ __device__ __forceinline__ void many_block(const AttendArgs& a, int block, int p
         }
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), in a form that the compiler takes into account
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     if (i + 1 < t1) {
-      load(a.v, i + 1, next_page, v_lds, vo);
-      if (i + 2 < t1) {
-        next_page = page_at(i + 2);
-        load(a.k, i + 2, next_page, k_lds, ko);
-      }
+      if (i + 2 - p0 >= 64) read_pages(i + 1);
+      load(a.v, i + 1, page_at(i + 1), v_lds, vo);
+      if (i + 2 < t1) load(a.k, i + 2, page_at(i + 2), k_lds, ko);
     }
     u32x8 p;
 #pragma unroll
@@ -362,6 +375,12 @@ __device__ __forceinline__ void many_block(const AttendArgs& a, int block, int p
       __builtin_amdgcn_s_setprio(1);
       products(next);
       numerators(now, p);
+#pragma unroll
+      for (int n = 0; n < D / 16; n++) {  // a product, then 6 (D = 128) of the exponentials' instructions: 3 %
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, 768 / D, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       read_keys(i + 1, y);
       sums(0, p);
       read_values(i, y, 1);
