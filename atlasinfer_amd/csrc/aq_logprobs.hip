@@ -20,9 +20,11 @@ constexpr int kList = 576;  // places of a wave's list: all that fewer than 64 l
 constexpr int kMaxTop = 64, kMaxParts = 32;
 constexpr int kMaxVocab = 1 << 18;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Logits that the pass over a row can weigh; a part whose largest is not between
-// these is looked at again, number by number.
-constexpr float kLow = -1e30f, kHigh = 1e30f;
+// Where the largest logit of a part has to lie for the pass over it, whose exponents are
+// off by the rounding of that times log2(e), 1 at most, until it is put right at the end; a
+// part with another largest (all fp16 ones but infinities lie between) is looked at
+// again, number by number.
+constexpr float kLow = -16777216.0f, kHigh = 16777216.0f;
 
 typedef unsigned long long u64;
 typedef u64 u64x2 __attribute__((ext_vector_type(2)));
@@ -217,8 +219,8 @@ __device__ __forceinline__ int count_above(const u64* list, int n, u64 e) {
   return above + __builtin_amdgcn_mov_dpp(above, 0x4E, 0xF, 0xF, false);  // [2,3,0,1]
 }
 
-// Sums number by number, for parts that the pass over them cannot weigh, or of a
-// token whose logit is not above kLow: e^(x - m) with the largest exactly 1, +inf too.
+// Sums number by number, for parts that the pass over them cannot weigh, or where the
+// token's logit is -inf: e^(x - m) with the largest exactly 1, +inf too.
 template <int FMT>
 __device__ __forceinline__ Sums exact_sums(Shared& s, const Part<FMT>& r, bool there, float own, int token) {
   float m = -INFINITY;
@@ -299,8 +301,8 @@ __device__ __forceinline__ int part_top(Shared& s, const Part<FMT>& r, bool ther
       if (reach) each(s, r, there, list);
     } else {
       // lane by lane of those whose maxima reach it, an element of its pieces a lane
-      // (two lanes at once for numbers of 32 bits): a tenth of the time that every
-      // lane's walk over its own takes
+      // (two lanes at once for numbers of 32 bits): 64 rows of 128256 1.6 us less than
+      // with every lane walking over its own
       if (wave == 0 && r.singles) list(t < r.singles ? r.value(r.single(t)) : -INFINITY, r.single(min(t, r.singles - 1)), t < r.singles);
       constexpr int kAtOnce = 64 / (kHeld * T::E);
       const int ln = t & 63, u = ln / T::E % kHeld, el = ln % T::E, half = ln / (kHeld * T::E);
@@ -429,7 +431,11 @@ __device__ __forceinline__ void write_top(const Args& a, int row, int at, u64 e,
   a.top_logprobs[(int64_t)row * a.top + at] = v.m > -INFINITY ? (x == v.m ? 0.0f : x - v.m) - log_z : NAN;
 }
 
-// One workgroup a part of a row (grid: parts, rows).
+// One workgroup a part of a row (grid: parts, rows).  2048 rows of 128256 fp16: 132 us
+// without alternatives (525 MB at 4.0 TB/s; the library's row maximum takes 126), 203 with 20:
+// memory, and 10 vector instructions an element, an exponential among them.  64 rows:
+// 12.2 and 4.4 for the merge, steps one after the other: the row's loads 2 to 3, the pass
+// 2.5, sums, cut, list and ranks 5.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   typedef Type<FMT> T;
@@ -502,7 +508,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
     for (int i = r.lead + own_piece * T::E; i < token; i++) v.before += r.scalar_value(i) == own;
   const bool has = t < r.singles || r.p0 + t < r.p1;
   const float all = block_max(s, m);
-  if (!(all > kLow && all < kHigh) || !(own > kLow)) {  // (nothing at all, too: it counts as -inf)
+  if (!(all > kLow && all < kHigh) || own == -INFINITY) {  // (nothing at all, too: it counts as -inf)
     v = exact_sums(s, r, there, own, token);
   } else {
     m = all;

@@ -156,8 +156,8 @@ __device__ __forceinline__ int few_place(int r, int c) {
 // registers a half before they are needed.  So when everyone comes to a tile's one
 // barrier, its keys and the last tile's values are done with; what takes their places
 // in LDS, the keys of two tiles on and the values of the next, has a tile's time.
-// A prompt of 8192, 32 heads of 128 over 8 key/value heads: 566 to 590 us, 930 to 970
-// TFLOP/s of the two products (the library's fp16 product of 8192^3: 1177), the matrix
+// A prompt of 8192, 32 heads of 128 over 8 key/value heads: 544 to 590 us, 930 to
+// 1010 TFLOP/s of the two products (the library's fp16 product of 8192^3: 1177), the matrix
 // unit 47 % busy at 1.9 GHz, no bank conflicts.  One half after the other, without the
 // places and the registers ahead, it took 614.  Nothing gained: workgroups of 256 rows,
 // also with four tiles in flight (580 against 590), other proportions of the interleaving
@@ -451,6 +451,12 @@ constexpr int kStep = 32;  // keys a wave takes at a time below
 //            order of keys in which the numerators are at hand
 // The next keys are asked for when the scores' products have taken the last ones, the
 // next values when the last ones are in LDS.
+// Bound by memory: 32 sequences of up to 16384 positions, 8 key/value heads of 128, 1 GB
+// in 182 us (5.5 TB/s; a copy of 2 GiB runs at 4.9); 8 of 4000 131 MB in 22.5; one of 700
+// 5.6, a launch and the chain of loads from the lengths over the pages to the keys.
+// Eight waves a workgroup instead of four took as long or longer (8 of 4000: 30.7 against
+// 27.9 us with the merge of that time), page numbers read ahead into a register, as below,
+// 0.2 us longer for one sequence and the same for many.
 // lds: few_lds<D, NR> bytes, on a multiple of 16
 template <int D, int NR>
 constexpr int few_sums = 4 * NR * 16 * (D + 4) * 4 > 4 * kStep * D * 2 ? 4 * NR * 16 * (D + 4) * 4 : 4 * kStep * D * 2;
@@ -713,8 +719,8 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(AttendArgs a) {
   }
 }
 
-// For the first kernel, a workgroup a row: 16 bytes a lane, the spans dealt to
-// groups of D / 4 lanes, whose sums meet in LDS.  Everything is asked for at once,
+// For the first kernel, a workgroup a row (3 to 5 us, a wave a row took up to 7): 16
+// bytes a lane, the spans dealt to groups of D / 4 lanes, whose sums meet in LDS.  Everything is asked for at once,
 // before it is known how many spans there are: what is none is not looked at.
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_few_merge_kernel(AttendArgs a) {

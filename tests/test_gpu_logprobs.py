@@ -206,3 +206,23 @@ def test_fewer_lanes_than_alternatives(dtype):
         for skip in (0, 1, 5):
             _check(x[:, skip:skip + V], tokens, 64)
             _check(x[:, skip:skip + V], tokens, 9)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1.6e7, 1e8, 1e20, 5e29, 2e30, 1e37])
+def test_large_logits(dtype, size):
+    """Rows of either sign up to the type's range, alone and with ordinary ones; whole rows near one large number."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    for V in (300, 50272):
+        x = torch.randn(8, V, generator=g, device=DEV)
+        x[0] *= size
+        x[1] = x[1].abs() * -size - size
+        x[2, ::7] -= size
+        x[3, V // 3] += size
+        x[4] = x[4] * 3 + size
+        x[5] = x[5] * 3 - size
+        x[6] = torch.where(x[6] > 1, -size, size)
+        x[7, V // 2:] = -size
+        x = x.to(dtype)
+        for n in (0, V // 3, V - 1):
+            _check(x, torch.full((8,), n, device=DEV), min(9, V))
