@@ -433,7 +433,7 @@ __device__ __forceinline__ void write_top(const Args& a, int row, int at, u64 e,
 
 // One workgroup a part of a row (grid: parts, rows).  2048 rows of 128256 fp16: 132 us
 // without alternatives (525 MB at 4.0 TB/s; the library's row maximum takes 126), 203 with 20:
-// memory, and 10 vector instructions an element, an exponential among them.  64 rows:
+// memory, and 9.5 vector instructions an element, an exponential among them.  64 rows:
 // 12.2 and 4.4 for the merge, steps one after the other: the row's loads 2 to 3, the pass
 // 2.5, sums, cut, list and ranks 5.
 template <int FMT>
