@@ -161,6 +161,10 @@ class GraphDecoder:
             raise ValueError("GraphDecoder: pages without a page_size")
         if page_size is not None and kv_bits != 16:
             raise ValueError("GraphDecoder: pages hold fp16 (kv_bits 16)")
+        if page_size is not None and self.kind == "opt":
+            known = model.model.decoder.embed_positions.weight.shape[0] - 2
+            if self.L > known:  # prompts and texts look their positions up in the table
+                raise ValueError(f"GraphDecoder: max_len {self.L} passes the model's {known} positions")
         if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, cfg.vocab_size):
             raise ValueError(f"GraphDecoder: {logprobs} alternatives (0 .. {MAX_TOP})")
         self.paged, self.logprobs = page_size is not None, logprobs

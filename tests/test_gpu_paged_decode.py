@@ -171,3 +171,14 @@ def test_refusals():
             gd.prefill(prompts)
     with pytest.raises(NotImplementedError):
         GraphDecoder(m.float(), 2, 64, page_size=16)
+
+
+def test_positions_past_a_table():
+    """A decoder that would pass the learned positions' table is refused, one that just reaches its end runs."""
+    m = _model("opt", 3, quantize=False)
+    known = m.config.max_position_embeddings
+    with pytest.raises(ValueError, match="positions"):
+        GraphDecoder(m, 1, known + 1, page_size=16)
+    gd = GraphDecoder(m, 1, known, page_size=16)
+    got, = gd.score(_prompts([known]))
+    assert torch.isfinite(got.logprobs).all() and got.logprobs.shape == (known - 1,)
