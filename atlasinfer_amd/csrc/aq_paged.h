@@ -7,7 +7,6 @@
 namespace paged {
 
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
-typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
@@ -26,7 +25,6 @@ typedef __attribute__((address_space(3))) short4v lds_s4;
 struct Half {
   static constexpr uint16_t kInf = 0x7C00;
   static __device__ __forceinline__ float to_f32(uint16_t b) { return (float)bits_to_h(b); }
-  static __device__ __forceinline__ uint16_t from_f32(float x) { return h_to_bits(rn_h(x)); }
   // two numbers to nearest (one conversion)
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{a, b}, half2v));
@@ -46,7 +44,6 @@ struct Half {
 struct Bf16 {
   static constexpr uint16_t kInf = 0x7F80;
   static __device__ __forceinline__ float to_f32(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
-  static __device__ __forceinline__ uint16_t from_f32(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2v{a, b}, bf2v));
   }

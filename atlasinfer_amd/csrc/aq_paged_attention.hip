@@ -29,7 +29,7 @@ struct AttendArgs {
   int H, G, Hkv, window, sinks, items, per;
   int few;                 // sequences of up to so many rows are the first kernel's, the others the second's
   int few_span, few_spans; // steps a workgroup of the first kernel, workgroups a sequence
-  int span, spans;         // tiles a workgroup of the second, workgroups a block
+  int span;                // tiles a workgroup of the second
   int slots;               // the larger number of spans
   int few_eights, many_eights;  // eights of workgroups of both, where they share a launch
   float c;  // |scale| log2(e), above 0: a masked score, -inf, times it stays that
@@ -915,7 +915,7 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
                (long long)S, (long long)max_new, (long long)max_length);
   AQ_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
                "%s: page size %lld (a power of two from 16 to 1024)", me, (long long)page_size);
-  AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W * page_size <= INT32_MAX && max_length <= W * page_size,
+  AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W <= INT32_MAX / page_size && max_length <= W * page_size,
                "%s: %lld pages, %lld of a sequence for %lld positions", me, (long long)pages, (long long)W, (long long)max_length);
   AQ_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %lld, %lld sinks", me, (long long)window, (long long)sinks);
   AQ_CHECK_ARG(q_row % 8 == 0 && q_head % 8 == 0, "%s: strides must be multiples of 8", me);
@@ -949,7 +949,6 @@ extern "C" int aq_paged_attention(const void* q, int dtype, int64_t T, int64_t H
   a.few_span = (int)p.few_span;
   a.few_spans = (int)p.few_spans;
   a.span = (int)p.span;
-  a.spans = (int)p.spans;
   a.slots = (int)p.slots;
   a.few_eights = p.nr ? (int)aq::ceil_div(S * Hkv * p.few_spans, 8) : 0;
   a.many_eights = (int)(p.per * p.spans);

@@ -118,7 +118,7 @@ extern "C" int aq_paged_store(const void* q, const void* k, const void* v, int d
                "%s: sizes out of range (%lld rows, %lld sequences)", me, (long long)T, (long long)S);
   AQ_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
                "%s: page size %lld (a power of two from 16 to 1024)", me, (long long)page_size);
-  AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W * page_size <= INT32_MAX, "%s: %lld pages, %lld of a sequence", me,
+  AQ_CHECK_ARG(pages > 0 && pages <= INT32_MAX && W > 0 && W <= INT32_MAX / page_size, "%s: %lld pages, %lld of a sequence", me,
                (long long)pages, (long long)W);
   AQ_CHECK_ARG(max_new > 0 && max_length > 0 && max_length <= W * page_size, "%s: at most %lld new, %lld positions of a sequence", me,
                (long long)max_new, (long long)max_length);

@@ -164,7 +164,8 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, cache: Sequence[torch.Tensor],
     any strides) to their places in the cache.  ``rope``: keys are turned to their
     positions, over the first ``2 len(frequencies)`` elements (a multiple of 16).
     ``q`` [T, H, D] is turned likewise and returned as [T, H, D] (in ``q_out`` if
-    given; rows that belong to no sequence are not written)."""
+    given, which must overlap neither the inputs nor the cache; rows that belong to no
+    sequence are not written)."""
     what = "paged_store"
     kc, vc, Hkv, P, D = _cache(what, cache, batch)
     dev, dtype = kc.device, kc.dtype
@@ -222,8 +223,8 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
     positions' (``paged_store``) included; [T, H, D].  A row at position p sees the
     keys at or before it that are less than ``window`` positions back (None: all) or
     among the first ``sinks``.  ``workspace`` (uint8, paged_attention_workspace
-    bytes) and ``out``: given, or allocated; rows that belong to no sequence are not
-    written."""
+    bytes) and ``out`` (which must overlap neither q nor the cache): given, or allocated;
+    rows that belong to no sequence are not written."""
     what = "paged_attention"
     kc, vc, Hkv, P, D = _cache(what, cache, batch)
     dev, dtype = kc.device, kc.dtype
@@ -247,6 +248,8 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
         return out
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = _lib.strided_rows(q)
+    if out.data_ptr() == q.data_ptr():
+        _refuse(f"{what}: out must not be q")
     starts, lengths, S, table, W, max_new, max_length = batch._args
     L = _lib.load()
     if workspace is None:

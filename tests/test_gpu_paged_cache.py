@@ -464,3 +464,38 @@ def test_python_refusals():
             PagedBatch(b.starts, b.lengths, b.table, n, x)
     with pytest.raises(AttributeError):
         batch.max_length = 7
+
+
+def test_graphs_that_share_a_workspace():
+    """Two captured attentions of different batches in one workspace, replayed in turns
+    with eager calls in it between them."""
+    P, D, H, Hkv = 16, 128, 8, 2
+    shapes = [([1, 1, 1], [3000, 700, 41]), ([200, 1], [2500, 1200])]
+    bs = [R.Batch(new, length, Hkv, D, P, F16, DEV) for new, length in shapes]
+    batches = [_batch(b) for b in bs]
+    qs = [b.normal(b.T, H, D).half() for b in bs]
+    ws = torch.empty(max(paged_attention_workspace(b.T, H, Hkv, D, x) for b, x in zip(bs, batches)), dtype=torch.uint8, device=DEV)
+    assert ws.numel() > 0
+
+    def attend(i):
+        return paged_attention(qs[i], bs[i].cache, batches[i], scale=0.09, workspace=ws)
+    attend(0), attend(1)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in bs], []
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            outs.append(attend(i))
+    for n in range(4):
+        for i, g in enumerate(graphs):
+            qs[i].normal_()
+            outs[i].zero_()
+            g.replay()
+            attend(1 - i)
+        for i in range(2):
+            assert torch.equal(outs[i], paged_attention(qs[i], bs[i].cache, batches[i], scale=0.09)), (n, i)
+
+
+def test_output_over_its_queries():
+    b = R.Batch([3], [20], 2, 64, 16, F16, DEV)
+    q = b.normal(b.T, 4, 64).half()
+    with pytest.raises(ValueError, match="must not be q"):
+        paged_attention(q, b.cache, _batch(b), scale=0.1, out=q)

@@ -208,3 +208,10 @@ def test_the_reference_turns_and_attends():
             out = torch.softmax(k @ q[i, h].double() * 0.125, 0) @ v
             assert (want[i, h] - out).abs().max() < 1e-12
     assert (bound > 0).all() and (bound < 0.05).all()
+
+
+def test_table_widths_past_64_bits(lib):
+    """A width whose positions do not fit 64 bits is refused as any other that is too large."""
+    for c in (_store(lib), _attend(lib)):
+        c.bad("pages", W=1 << 60)
+        c.bad("pages", W=(1 << 60) + 1)
