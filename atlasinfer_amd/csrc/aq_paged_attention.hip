@@ -802,14 +802,18 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
   const float f = y.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((y.x - m) * a.c);
   const float l = wave_group_sum_f32<64>(y.y * f);
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  // (all lanes stay to the last round: a weight that lies in a lane that has left reads as 0)
 #pragma unroll 2
-  for (int s = grp; s < spans; s += N) {
-    const float4 x = pp[(int64_t)s * (D / 4)];
-    const float w = __shfl(f, s, 64);
-    o.x = fmaf(x.x, w, o.x);
-    o.y = fmaf(x.y, w, o.y);
-    o.z = fmaf(x.z, w, o.z);
-    o.w = fmaf(x.w, w, o.w);
+  for (int s0 = 0; s0 < spans; s0 += N) {
+    const int s = s0 + grp;
+    const float w = __shfl(f, min(s, 63), 64);
+    if (s < spans) {
+      const float4 x = pp[(int64_t)s * (D / 4)];
+      o.x = fmaf(x.x, w, o.x);
+      o.y = fmaf(x.y, w, o.y);
+      o.z = fmaf(x.z, w, o.z);
+      o.w = fmaf(x.w, w, o.w);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) {

@@ -499,3 +499,17 @@ def test_output_over_its_queries():
     q = b.normal(b.T, 4, 64).half()
     with pytest.raises(ValueError, match="must not be q"):
         paged_attention(q, b.cache, _batch(b), scale=0.1, out=q)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("spans", [2, 5, 16, 17, 18, 19, 20, 21, 31, 32, 33, 34, 35, 48, 49, 63, 64])
+def test_every_number_of_spans(D, spans):
+    """Chunks whose keys are split into so many spans of 8 tiles of 64, the last of 7 tiles: none is lost in the
+    merge, whatever rest the number leaves by the spans that it takes at once."""
+    L = 64 * (8 * spans - 1)
+    for n, H, dtype, window in ((33, 1, F16, None), (9, 4, BF16, None), (128, 1, F16, L - 40)):
+        # one sequence and key/value head, more rows than the kernel for few takes: the workspace tells the spans
+        b = R.Batch([n], [L - n], 1, D, 16, dtype, DEV)
+        rows = paged_attention_workspace(n, H, 1, D, _batch(b)) // (n * H * (D + 2) * 4)
+        assert rows == spans
+        _check([n], [L - n], H, 1, D, dtype=dtype, window=window, seed=spans)
