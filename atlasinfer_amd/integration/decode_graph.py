@@ -266,8 +266,13 @@ class GraphDecoder:
         need = [-(-n // P) for n in lengths]
         if all(len(h) >= n for h, n in zip(self._held, need)):
             return
-        if sum(max(0, n - len(h)) for h, n in zip(self._held, need)) > len(self._free):
+        if sum(need) > self.pages:
             raise RuntimeError(f"GraphDecoder: {self.pages} pages of {P} positions are too few")
+        if sum(max(0, n - len(h)) for h, n in zip(self._held, need)) > len(self._free):
+            # what others hold ahead of their positions (nothing is written there yet) goes back
+            for h, n in zip(self._held, need):
+                while len(h) > n:
+                    self._free.append(h.pop())
         for wanted in (need, [-(-min(n + ahead, self.L) // P) for n in lengths]):
             for h, n in zip(self._held, wanted):
                 while len(h) < n and self._free:

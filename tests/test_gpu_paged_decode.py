@@ -182,3 +182,15 @@ def test_positions_past_a_table():
     gd = GraphDecoder(m, 1, known, page_size=16)
     got, = gd.score(_prompts([known]))
     assert torch.isfinite(got.logprobs).all() and got.logprobs.shape == (known - 1,)
+
+
+def test_a_pool_of_the_final_need():
+    """Prompts of uneven lengths end with every page of the pool: pages held ahead by one serve the other."""
+    m = _model("llama", 9)
+    prompts = _prompts([16, 8])
+    want = GraphDecoder(m, 2, 96, page_size=16).generate(prompts, 17)  # 32 and 24 positions in the cache
+    tight = GraphDecoder(m, 2, 96, page_size=16, pages=4)
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(tight.generate(prompts, 17), want))
+    with pytest.raises(RuntimeError, match="pages"):
+        tight.step()

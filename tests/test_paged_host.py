@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import paged_ref as R
+from atlasinfer_amd.integration.decode_graph import GraphDecoder
 from atlasinfer_amd.integration.logprobs import token_logprobs
 from atlasinfer_amd.memory import paged_cache as PC
 from test_decode_operators_host import ODD, P, Call
@@ -215,3 +216,43 @@ def test_table_widths_past_64_bits(lib):
     for c in (_store(lib), _attend(lib)):
         c.bad("pages", W=1 << 60)
         c.bad("pages", W=(1 << 60) + 1)
+
+
+class Pool:
+    """What ``GraphDecoder._reserve`` needs of a decoder, on the CPU."""
+
+    def __init__(self, B, pages, L, P=16):
+        self.B, self.pages, self.L, self.page_size = B, pages, L, P
+        self.table = torch.zeros(B, -(-L // P), dtype=torch.int32)
+        GraphDecoder._release(self)
+
+    def _device(self, values, dtype):
+        return torch.tensor(values, dtype=dtype)
+
+    def check(self, lengths):
+        """Every sequence holds the pages of its positions, none twice, and the table says so."""
+        for h, row, n in zip(self._held, self.table.tolist(), lengths):
+            assert len(h) >= -(-n // self.page_size) and row == h + [0] * (len(row) - len(h))
+        assert sorted(sum(self._held, []) + self._free) == list(range(self.pages))
+
+
+@pytest.mark.parametrize("counts,steps,pages", [([16, 8], 16, 4), ([60, 3, 20], 44, 14), ([1, 1, 1, 1], 47, 12), ([33, 40], 8, 6)])
+def test_pages_held_ahead_go_back(counts, steps, pages):
+    """A pool of just the pages that the sequences end with serves them to the end; a position more is refused,
+    and what they hold stays."""
+    assert sum(-(-(n + steps) // 16) for n in counts) == pages
+    p = Pool(len(counts), pages, 128)
+    GraphDecoder._reserve(p, counts)
+    kept = [[] for _ in counts]
+    for step in range(steps + 1):
+        lengths = [n + step for n in counts]
+        GraphDecoder._reserve(p, lengths, ahead=64)
+        p.check(lengths)
+        for k, h, n in zip(kept, p._held, lengths):  # written pages stay where they are
+            assert h[:len(k)] == k
+            k[:] = h[:-(-n // 16)]
+    before = [list(h) for h in p._held]
+    with pytest.raises(RuntimeError, match="pages"):
+        GraphDecoder._reserve(p, [16 * pages + 1] + lengths[1:], ahead=64)
+    assert p._held == before
+    p.check(lengths)
