@@ -85,8 +85,9 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, scaling: Optional[dic
       they are, blended in between;
     * ``yarn``: divided by ``factor`` below ``beta_slow`` turns over the original
       length, as they are above ``beta_fast``, blended by index in between; the
-      factor of the turned elements is 0.1 ln(factor) + 1 unless
-      ``attention_factor`` gives it.
+      factor of the turned elements is 0.1 ln(factor) + 1, or where both ``mscale`` = a
+      and ``mscale_all_dim`` = b are given (and not 0) (0.1 a ln(factor) + 1) / (0.1 b
+      ln(factor) + 1), unless ``attention_factor`` gives it.
     """
     if rotary <= 0 or rotary % 2:
         _refuse(f"rotary_frequencies: {rotary} elements")
@@ -115,7 +116,12 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, scaling: Optional[dic
         f = f / s * ramp + f * (1 - ramp)
         m = scaling.get("attention_factor")
         if m is None:
-            m = 0.1 * math.log(s) + 1.0 if s > 1 else 1.0
+            a, b = scaling.get("mscale"), scaling.get("mscale_all_dim")
+
+            def size(weight):
+                return 0.1 * weight * math.log(s) + 1.0 if s > 1 else 1.0
+
+            m = size(a) / size(b) if a and b else size(1.0)
     elif kind != "default":
         raise NotImplementedError(f"rotary_frequencies: rope type {kind!r} (default, linear, llama3, yarn supported)")
     return f.float().to(device), float(m)

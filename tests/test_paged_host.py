@@ -256,3 +256,24 @@ def test_pages_held_ahead_go_back(counts, steps, pages):
         GraphDecoder._reserve(p, [16 * pages + 1] + lengths[1:], ahead=64)
     assert p._held == before
     p.check(lengths)
+
+
+@pytest.mark.parametrize("factor", [1.0, 4.0, 40.0])
+@pytest.mark.parametrize("given", [dict(mscale=1.0, mscale_all_dim=1.0), dict(mscale=0.707, mscale_all_dim=0.707),
+                                   dict(mscale=1.0, mscale_all_dim=0.707), dict(mscale=0.707, mscale_all_dim=1.0),
+                                   dict(mscale=2.0), dict(mscale_all_dim=2.0), dict(mscale=0.0, mscale_all_dim=1.0),
+                                   dict(mscale=1.0, mscale_all_dim=0.0), dict(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.7)])
+def test_yarn_with_scales_of_its_factor(factor, given):
+    """The factor of yarn's turned elements where a configuration scales it, against transformers' own."""
+    transformers = pytest.importorskip("transformers")
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    scaling = dict(rope_type="yarn", factor=factor, original_max_position_embeddings=4096, **given)
+    cfg = transformers.LlamaConfig(hidden_size=512, num_attention_heads=4, num_key_value_heads=4,
+                                   max_position_embeddings=int(4096 * factor))
+    cfg.rope_theta = 10000.0
+    cfg.rope_scaling = dict(scaling)
+    if hasattr(cfg, "rope_parameters"):
+        cfg.rope_parameters = {**scaling, "rope_theta": 10000.0}
+    want, m = ROPE_INIT_FUNCTIONS["yarn"](cfg, torch.device("cpu"))
+    got, factor = PC.rotary_frequencies(128, 10000.0, scaling)
+    assert abs(factor - m) <= 1e-6 and torch.allclose(got.double(), want.double(), rtol=2e-6, atol=0)
