@@ -94,15 +94,22 @@ def rotary_frequencies(rotary: int, base: float = 10000.0, scaling: Optional[dic
     f = float(base) ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary)
     m = 1.0
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+
+    def given(key):
+        x = scaling.get(key)
+        if x is None:
+            _refuse(f"rotary_frequencies: rope type {kind!r} without {key}")
+        return x
+
     if kind == "linear":
-        f = f / scaling["factor"]
+        f = f / given("factor")
     elif kind == "llama3":
-        s, low, high = scaling["factor"], scaling["low_freq_factor"], scaling["high_freq_factor"]
-        turns = scaling["original_max_position_embeddings"] * f / (2 * math.pi)
+        s, low, high = given("factor"), given("low_freq_factor"), given("high_freq_factor")
+        turns = given("original_max_position_embeddings") * f / (2 * math.pi)
         keep = ((turns - low) / (high - low)).clamp(0, 1)  # 0: divided, 1: as they are
         f = f * keep + f / s * (1 - keep)
     elif kind == "yarn":
-        s, n = scaling["factor"], scaling["original_max_position_embeddings"]
+        s, n = given("factor"), given("original_max_position_embeddings")
         fast, slow = scaling.get("beta_fast") or 32, scaling.get("beta_slow") or 1
 
         def index(turns):  # the pair that makes so many turns over n positions

@@ -277,3 +277,15 @@ def test_yarn_with_scales_of_its_factor(factor, given):
     want, m = ROPE_INIT_FUNCTIONS["yarn"](cfg, torch.device("cpu"))
     got, factor = PC.rotary_frequencies(128, 10000.0, scaling)
     assert abs(factor - m) <= 1e-6 and torch.allclose(got.double(), want.double(), rtol=2e-6, atol=0)
+
+
+def test_scalings_without_what_they_need():
+    """A scaling that lacks a number, or has None for it, is refused by its name."""
+    whole = dict(linear=dict(factor=2.0), yarn=dict(factor=4.0, original_max_position_embeddings=4096),
+                 llama3=dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192))
+    for kind, numbers in whole.items():
+        PC.rotary_frequencies(64, scaling=dict(rope_type=kind, **numbers))
+        for key in numbers:
+            for rest in ({k: x for k, x in numbers.items() if k != key}, {**numbers, key: None}):
+                with pytest.raises(ValueError, match=f"{kind}.* without {key}"):
+                    PC.rotary_frequencies(64, scaling=dict(rope_type=kind, **rest))
