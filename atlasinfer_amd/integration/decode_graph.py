@@ -188,7 +188,7 @@ class GraphDecoder:
                                  top_p=torch.ones(B, device=dev), min_p=torch.zeros(B, device=dev))
         if logprobs is not None:
             f32, i64 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.long, device=dev)
-            # of the tokens in ``out``, at the same places
+            # of the tokens in ``out``, at the same places; zeros behind them
             self.chosen = TokenLogprobs(torch.zeros(B, L, **f32), torch.zeros(B, L, **f32), torch.zeros(B, L, **i64),
                                         torch.zeros(B, L, logprobs, **f32), torch.zeros(B, L, logprobs, **i64))
         if self.kind == "llama" and not self.paged:
@@ -737,6 +737,9 @@ class GraphDecoder:
             logits = self._own_prefill(input_ids)
             self.pos.fill_(S)
         self.slot.zero_()
+        if self.logprobs is not None:
+            for kept in self.chosen:
+                kept.zero_()
         first = self._choose(logits, self.slot)
         self.tok.copy_(first)
         self.out.zero_()

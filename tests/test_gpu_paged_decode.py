@@ -194,3 +194,18 @@ def test_a_pool_of_the_final_need():
         assert all(torch.equal(a, b) for a, b in zip(tight.generate(prompts, 17), want))
     with pytest.raises(RuntimeError, match="pages"):
         tight.step()
+
+
+@pytest.mark.parametrize("graph", [True, False])
+@pytest.mark.parametrize("paged", [False, True])
+def test_chosen_holds_one_text(graph, paged):
+    """A short text after a longer one, and the first after the steps that come before a capture: nothing of
+    another stands behind its tokens."""
+    m = _model("llama", 4)
+    gd = GraphDecoder(m, 2, 50, graph=graph, logprobs=3, **(dict(page_size=16) if paged else {}))
+    for n in (1, 20, 4):
+        gd.generate(torch.stack(_prompts([6, 6], n)), n)
+        assert (gd.chosen.logprobs[:, :n] < 0).all() and (gd.chosen.entropies[:, :n] > 0).all()
+        assert (gd.chosen.top_logprobs[:, :n] < 0).all()
+        for t in gd.chosen + (gd.out,):
+            assert (t[:, n:] == 0).all()
