@@ -721,6 +721,8 @@ class GraphDecoder:
         if self.paged:
             prompts = self._prompts(input_ids)
             S = max(p.numel() for p in prompts)
+        elif not isinstance(input_ids, torch.Tensor):
+            raise ValueError("prefill: prompts of several lengths need page_size")
         else:
             B, S = input_ids.shape
             if B != self.B or S >= self.L:

@@ -201,3 +201,15 @@ def test_window_prompts_nest_and_keep_to_their_thread(monkeypatch):
     assert ran(a) == (4, 0)
     two.__exit__(None, None, None)
     assert ran(a) is None and a.config._attn_implementation == before
+
+
+def test_lists_of_prompts_need_pages():
+    """Both ways in refuse them in the same words, and the decoder lives on."""
+    gd = GraphDecoder(_model("llama"), batch=2, max_len=20, graph=False)
+    ids = torch.randint(0, 256, (2, 5))
+    want = gd.generate(ids, 6)
+    for call in (gd.prefill, lambda p: gd.generate(p, 3)):
+        for prompts in ([ids[0], ids[1, :3]], list(ids), tuple(ids), ids.tolist()):
+            with pytest.raises(ValueError, match="several lengths need page_size"):
+                call(prompts)
+    assert torch.equal(gd.generate(ids, 6), want)
