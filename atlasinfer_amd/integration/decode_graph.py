@@ -227,6 +227,8 @@ class GraphDecoder:
     def _page_state(self, page_size: int, pages: Optional[int], chunk: int) -> None:
         """The pool of pages, the table of the sequences' and the batch of a step."""
         B, dev = self.B, self.dev
+        if page_size < 1:
+            raise ValueError(f"GraphDecoder: pages of {page_size} positions (a power of two from 16 to 1024)")
         width = -(-self.L // page_size)
         if pages is None:
             pages = B * width

@@ -289,3 +289,11 @@ def test_scalings_without_what_they_need():
             for rest in ({k: x for k, x in numbers.items() if k != key}, {**numbers, key: None}):
                 with pytest.raises(ValueError, match=f"{kind}.* without {key}"):
                     PC.rotary_frequencies(64, scaling=dict(rope_type=kind, **rest))
+
+
+@pytest.mark.parametrize("page_size", [0, -16])
+def test_pages_of_no_positions(page_size):
+    p = Pool(2, 4, 64)
+    p.dev = torch.device("cpu")
+    with pytest.raises(ValueError, match=f"pages of {page_size} positions"):
+        GraphDecoder._page_state(p, page_size, None, 2048)
