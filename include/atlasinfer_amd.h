@@ -573,11 +573,14 @@ int aq_sample(const void* logits, int dtype, int64_t B, int64_t V, int64_t strid
  * aq_paged_attention: query head h of a row at position p sees the keys j <= p of its
  * sequence with p - j < window or j < sinks (window >= max_length: all of them),
  *   out[t, h, :] = softmax(scale q . k) v
- * Scores, softmax and sums in f32, the softmax's numerators rounded to the data's type;
- * scores up to 2^26 in magnitude, for the reason given at aq_window_attention.  What a key
- * or value that a row does not see holds, infinities and NaN included, does not reach
- * its output; a seen value that is not finite makes its element of the output not
- * finite; a row whose seen scores are all -inf answers NaN.
+ * Scores, softmax and sums in f32.  The softmax's numerators are rounded to the data's
+ * type, except for sequences of few rows (new tokens times heads of a key/value head: where
+ * max_new allows no sequence more than 32, or up to 16 in a call of several sequences),
+ * which hold them as two numbers of it.  Scores up to 2^26 in magnitude, for the reason
+ * given at aq_window_attention.  What a key or value that a row does not see holds,
+ * infinities and NaN included, does not reach its output; a seen value that is not finite
+ * makes its element of the output not finite; a row whose seen scores are all -inf
+ * answers NaN.
  *   q   [T, H, D] by strides, multiples of 8; H a multiple of Hkv
  *   out [T, H, D]; q, out and the caches 16-byte aligned
  *   workspace  aq_paged_attention_workspace bytes (may be 0, then NULL will do; -1 for

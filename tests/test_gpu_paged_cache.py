@@ -513,3 +513,47 @@ def test_every_number_of_spans(D, spans):
         rows = paged_attention_workspace(n, H, 1, D, _batch(b)) // (n * H * (D + 2) * 4)
         assert rows == spans
         _check([n], [L - n], H, 1, D, dtype=dtype, window=window, seed=spans)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("news,contexts,H,Hkv", [([1], [1], 4, 4), ([1], [4], 4, 1), ([1, 1, 1], [12, 30, 39], 8, 2), ([5], [3], 6, 2),
+                                                 ([3, 2], [20, 9], 8, 1), ([1, 1], [700, 90], 8, 1), ([40, 1, 3], [5, 17, 9], 4, 2)])
+def test_steps_lose_no_bits_of_their_numerators(D, dtype, news, contexts, H, Hkv):
+    """Sequences of up to 32 rows hold a numerator as two numbers of the type: h^2 of it is lost where the bound
+    of ``attend`` has h, and the rest of that bound stays.  Few keys, small scores: the output's own rounding and
+    the scores' leave room for no more."""
+    b = R.Batch(news, contexts, Hkv, D, 16, dtype, DEV, seed=11)
+    q = b.normal(b.T, H, D).to(dtype)
+    scale = 0.25 * D ** -0.5
+    out = paged_attention(q, b.cache, _batch(b), scale=scale)
+    v = b.cache[1]
+    h = R.HALF[dtype]
+    for i in range(len(news)):
+        if news[i] * H // Hkv > 32:
+            continue
+        rows = q[b.first[i]:b.first[i + 1]]
+        b.cache[1] = v
+        want, bound = R.attend(rows, b, i, scale)
+        b.cache[1] = v.abs()
+        size, _ = R.attend(rows, b, i, scale)
+        tight = bound - 1.01 * (h - h * h) * (size + want.abs())
+        off = (out[b.first[i]:b.first[i + 1]].double() - want).abs()
+        assert (tight > 0).all() and (off <= tight).all(), (i, (off / tight).max())
+
+
+@pytest.mark.parametrize("n", [1, 3, 200])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("key", [0, 101])
+def test_seen_infinities_keep_their_signs(n, dtype, key):
+    """With weights above zero an infinity among the values is what the row answers there, whichever tile it is in:
+    101 lies in one that the mask cuts for n = 3 and 200."""
+    b = R.Batch([n], [101], 1, 64, 16, dtype, DEV)
+    q = b.normal(n, 2, 64).to(dtype)
+    page, slot = int(b.table[0, key // 16]), key % 16
+    b.cache[1][page, 0, slot, 5] = float("inf")
+    b.cache[1][page, 0, slot, 40] = -float("inf")
+    got = paged_attention(q, b.cache, _batch(b), scale=0.1)
+    assert (got[..., 5] == float("inf")).all() and (got[..., 40] == -float("inf")).all()
+    got[..., [5, 40]] = 0.0
+    assert torch.isfinite(got).all()
