@@ -226,3 +226,28 @@ def test_large_logits(dtype, size):
         x = x.to(dtype)
         for n in (0, V // 3, V - 1):
             _check(x, torch.full((8,), n, device=DEV), min(9, V))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [1, 2, 5, 8, 17, 64])
+def test_short_rows_to_the_last_bits(dtype, V):
+    """Rows of one piece a lane, logits of a few units, where the sums' own roundings are few.  Relative to Z, in
+    units of 2^-24: 18 additions (8 a lane, 6 of a wave's lanes, 4 waves), three exponentials of 2^-22 and their
+    products (15), exponents off by 1.5 of the mean distance D from the maximum (D <= log V < 4.2: 7) and 1.5 of a lane's
+    distance, which the lanes near the maximum, e^-y of the sum, weigh by y e^-y <= 1/e: 1, in all
+    below 64, so 2^-18 of log Z.  E has the same on each of its terms and one product more; log and subtractions
+    add 2^-22 of their results."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = (2.0 * torch.randn(400, V, generator=g, device=DEV)).to(dtype)
+    tokens = torch.randint(0, V, (400,), generator=g, device=DEV)
+    got = token_logprobs(x, tokens, min(5, V))
+    y = x.double()
+    d = y - y.amax(1, keepdim=True)
+    z = d.exp().sum(1, keepdim=True)
+    lp, mean = d - z.log(), -(d.exp() / z * d).sum(1)
+    want = lp.gather(1, tokens[:, None])[:, 0]
+    assert ((got.logprobs.double() - want).abs() <= 2.0 ** -18 + 2.0 ** -22 * want.abs()).all()
+    top = torch.sort(lp, dim=1, descending=True, stable=True).values[:, :min(5, V)]
+    assert ((got.top_logprobs.double() - top).abs() <= 2.0 ** -18 + 2.0 ** -22 * top.abs()).all()
+    entropy = z.log()[:, 0] + mean
+    assert ((got.entropies.double() - entropy).abs() <= 2.0 ** -18 * (1 + 2 * mean) + 2.0 ** -22 * entropy).all()
