@@ -259,8 +259,10 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
         _no_gradients(what)
     if T == 0:
         return out
-    if not q.is_contiguous() or q.data_ptr() % 16:
-        q = _lib.strided_rows(q)
+    row, head, last = q.stride()
+    if last != 1 or (row | head) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        row, head, _ = q.stride()
     if out.data_ptr() == q.data_ptr():
         _refuse(f"{what}: out must not be q")
     starts, lengths, S, table, W, max_new, max_length = batch._args
@@ -269,7 +271,6 @@ def paged_attention(q: torch.Tensor, cache: Sequence[torch.Tensor], batch: Paged
         size = L.aq_paged_attention_workspace(T, S, H, Hkv, D, max_new, max_length)
         workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     ws, size = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    row, head, _ = q.stride()
     with _lib.on_device(dev):
         _lib.check(L.aq_paged_attention(q.data_ptr(), _DTYPES[dtype], T, H, Hkv, D, row, head,
                                         kc.data_ptr(), vc.data_ptr(), kc.shape[0], P, starts, lengths, S, table, W, max_new, max_length,

@@ -557,3 +557,16 @@ def test_seen_infinities_keep_their_signs(n, dtype, key):
     assert (got[..., 5] == float("inf")).all() and (got[..., 40] == -float("inf")).all()
     got[..., [5, 40]] = 0.0
     assert torch.isfinite(got).all()
+
+
+def test_one_row_of_an_odd_pitch():
+    """A single row, or a single head, keeps the pitch of the buffer that it is a view of, whatever torch calls it:
+    answered as any other strides are."""
+    b = R.Batch([1], [50], 1, 128, 16, F16, DEV)
+    wide = b.normal(2, 4 * 128 + 7).half()
+    one = torch.as_strided(b.normal(128).half(), (1, 1, 128), (3, 5, 1))
+    for q in (wide[:1, :512].view(1, 4, 128), one):
+        assert q.is_contiguous() and any(s % 8 for s in q.stride())
+        want = paged_attention(q.clone(memory_format=torch.contiguous_format), b.cache, _batch(b), scale=0.1)
+        assert torch.equal(paged_attention(q, b.cache, _batch(b), scale=0.1), want)
+        paged_store(q[:, :1], q[:, :1], b.cache, _batch(b), q=q)
