@@ -431,11 +431,12 @@ __device__ __forceinline__ void write_top(const Args& a, int row, int at, u64 e,
   a.top_logprobs[(int64_t)row * a.top + at] = v.m > -INFINITY ? (x == v.m ? 0.0f : x - v.m) - log_z : NAN;
 }
 
-// One workgroup a part of a row (grid: parts, rows).  2048 rows of 128256 fp16: 132 us
-// without alternatives (525 MB at 4.0 TB/s; the library's row maximum takes 126), 203 with 20:
-// memory, and 9.5 vector instructions an element, an exponential among them.  64 rows:
-// 12.2 and 4.4 for the merge, steps one after the other: the row's loads 2 to 3, the pass
-// 2.5, sums, cut, list and ranks 5.
+// One workgroup a part of a row (grid: parts, rows).  2048 rows of 128256 fp16: 132
+// to 138 us without alternatives (525 MB at 3.9 TB/s; the library's row maximum takes 126), 204
+// with 20, 278 with 64: memory, and 12.6, 18.2 and 23.1 vector instructions an element by
+// counters (9.5 of them the pass, an exponential among these).  As many fp32 logits: 204, 375,
+// 572.  64 rows: 11.9 and 4.1 for the merge, steps one after the other: the row's loads 2
+// to 3, the pass 2.5, sums, cut, list and ranks 5.
 template <int FMT>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   typedef Type<FMT> T;

@@ -159,11 +159,12 @@ __device__ __forceinline__ int few_place(int r, int c) {
 // barrier, its keys and the last tile's values are done with; what takes their places
 // in LDS, the keys of two tiles on and the values of the next, has a tile's time.
 // A prompt of 8192, 32 heads of 128 over 8 key/value heads: 544 to 590 us, 930 to
-// 1010 TFLOP/s of the two products (the library's fp16 product of 8192^3: 1177), the matrix
-// unit 47 % busy at 1.9 GHz, no bank conflicts.  One half after the other, without the
-// places and the registers ahead, it took 614.  Nothing gained: workgroups of 256 rows,
-// also with four tiles in flight (580 against 590), other proportions of the interleaving
-// (all within 1 %), the loads later in the tile (580 against 570).
+// 1010 TFLOP/s of the two products (the library's fp16 product of 8192^3: 1177).  By
+// counters 1.0 M cycles, the matrix unit busy in 53 % of them, the vector unit in 48 %, no bank
+// conflicts; that is 1.8 GHz at 554 us.  One half after the other, without the places and
+// the registers ahead, it took 614.  Nothing gained: workgroups of 256 rows, also with four
+// tiles in flight (580 against 590), other proportions of the interleaving (all within 1 %),
+// the loads later in the tile (580 against 570).
 // lds: many_lds<D> bytes, on a multiple of 1024: keys of even and odd tiles, values
 template <int D>
 constexpr int many_lds = 4 * kK * D * 2 + 16;
@@ -463,8 +464,9 @@ constexpr float kRaise = 7.0f;
 // The next keys are asked for when the scores' products have taken the last ones, the
 // next values when the last ones are in LDS.
 // Bound by memory: 32 sequences of up to 16384 positions, 8 key/value heads of 128, 1 GB
-// in 182 us (5.5 TB/s; a copy of 2 GiB runs at 4.9); 8 of 4000 131 MB in 22.5; one of 700
-// 5.6, a launch and the chain of loads from the lengths over the pages to the keys.
+// in 184 us (5.5 TB/s; a copy of 2 GiB runs at 4.9); 8 of 4000 131 MB in 22.6; one of 700
+// 6.0, a launch and the chain of loads from the lengths over the pages to the keys; 20 rows each
+// of 8 sequences of 4005, with the merge, 32.6 (D = 128: more registers than 256, so one wave a SIMD).
 // Eight waves a workgroup instead of four took as long or longer (8 of 4000: 30.7 against
 // 27.9 us with the merge of that time), page numbers read ahead into a register, as below,
 // 0.2 us longer for one sequence and the same for many.
@@ -866,7 +868,11 @@ Plan plan(int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t max_n
     // are many (256 of 4000 positions 91 us, 96 in two spans each), but for long ones,
     // whose lengths differ more (256 of up to 16384: 220 us, 187 in 8 spans); else 512
     // workgroups (64 of 4000: 26.0, 26.9 with 1024; 8 of 16000 17.4) of a step a wave at
-    // least.
+    // least.  All measured with max_length at the longest sequence.  Spans follow that bound,
+    // so far above the lengths, where a captured step has it, fewer of them hold keys: with
+    // bounds of the length, 32768 and 131072 one sequence of 700 takes 7.5, 12.2 and 12.5 us, of
+    // 2000 7.4, 12.0, 24.0, of 20000 20.3, 22.3, 29.4, 8 of 4000 25.4, 46.0, 46.0, 32 of 8000
+    // 184, 186, 193.
     if (steps <= 12 || pairs > 512) p.few_spans = 1;
     else if (pairs >= 256) p.few_spans = steps <= 160 ? 1 : std::min<int64_t>(aq::ceil_div(steps, 64), 64);
     else p.few_spans = std::min<int64_t>({512 / pairs, aq::ceil_div(steps, 4), 64});
